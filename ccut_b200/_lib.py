@@ -30,7 +30,7 @@ KERNEL_AUTO, KERNEL_TC, KERNEL_MMA = 0, 1, 2
 KERNELS = {"auto": KERNEL_AUTO, "tc": KERNEL_TC, "mma": KERNEL_MMA}
 ROUTING = {"softmax_topk": ROUTE_SOFTMAX_TOPK, "topk_softmax": ROUTE_TOPK_SOFTMAX, "sigmoid_group": ROUTE_SIGMOID_GROUP}
 
-_vp, _sz, _i, _f = C.c_void_p, C.c_size_t, C.c_int, C.c_float
+_vp, _sz, _i, _f, _ll = C.c_void_p, C.c_size_t, C.c_int, C.c_float, C.c_longlong
 
 
 class RouteParams(C.Structure):
@@ -97,6 +97,15 @@ SIGNATURES: dict[str, tuple] = {
     "ccut_mla_attention": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _vp, _i, _vp, _sz, _vp]),
     "ccut_mla_attention_pool": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, C.c_longlong, _i, _f, _vp, _i, _vp,
                                      _sz, _vp]),
+    "ccut_kv4_append": (_i, [_vp, _i, _ll, _ll, _vp, _i, _ll, _ll, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _ll, _i,
+                             _vp]),
+    "ccut_kv4_read": (_i, [_vp] * 6 + [_i, _i, _i, _i, _ll, _i, _vp, _vp, _i, _vp]),
+    "ccut_kv4_attention_workspace_bytes": (_sz, [_i] * 6),
+    "ccut_kv4_attention": (_i, [_vp] * 7 + [_i] * 7 + [_ll, _i, _f, _f, _vp, _i, _vp, _sz, _vp]),
+    "ccut_token_logprobs_workspace_bytes": (_sz, [_i, _i, _i]),
+    "ccut_token_logprobs": (_i, [_vp, _i, _i, _i, _ll, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ccut_lora_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "ccut_lora_add": (_i, [_vp] * 5 + [_i] * 5 + [C.POINTER(_i), _vp, _ll, _vp, _ll, _i, _vp, _sz, _vp]),
     "ccut_moe_ep_forward": (_i, [_vp, C.POINTER(MoeLayerDesc), _i, _i, C.POINTER(RouteParams), _vp, _i, _i, _vp,
                                  _i, _vp, _sz, _vp]),
     "ccut_workspace_status": (_i, [_vp, _vp]),

@@ -1,0 +1,214 @@
+"""4-bit kv caches and the attention that reads them (``ccut_kv4_*``).
+
+A cache row (one position of one kv head) keeps 4-bit codes with one fp16 pair (scale, minimum)
+per 64 features: 36 bytes per 64 features where the bf16 caches keep 128.  ``Kv4Pool`` /
+``Kv4Cache`` stand where ``model.KvPool`` / ``model.KvCache`` do (``MoeDecoder.new_pool(...,
+kv_dtype="int4")``, ``GenericBackend(..., kv_dtype="int4")``, ``[quant] kv_cache_dtype =
+"int4"``).  The reference keeps fp32 arrays (``ccut/models/generic.py:304-345``); there is no
+reference counterpart of the format.
+
+- ``kv4_append(pool, layer, k, v, slots, positions)`` quantizes new rows into the pool;
+- ``kv4_attention(q, pool, layer, slots, starts)`` attends over it, a batch of sequences of
+  different lengths in one call (decode steps and prompt chunks);
+- ``kv4_read(pool, layer, slots, positions)`` gives rows back as the values they stand for.
+
+The tensors are on one CUDA device; the calls run on that device's current stream.  Head dims
+64 and 128.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from ccut_b200 import _lib
+
+__all__ = ["GROUP", "Kv4Cache", "Kv4Pool", "kv4_append", "kv4_attention", "kv4_read"]
+
+GROUP = 64  # features per (scale, minimum) pair
+
+_DTYPES = {torch.bfloat16: _lib.OUT_BF16, torch.float32: _lib.OUT_F32}
+
+
+class Kv4Pool:
+    """The 4-bit caches of up to ``slots`` sequences in one allocation: ``k`` / ``v`` codes
+    ``[slots, layers, kv_heads, max_len, head_dim / 2]`` uint8 and ``k_par`` / ``v_par``
+    ``[slots, layers, kv_heads, max_len, head_dim / 64, 2]`` fp16."""
+
+    def __init__(self, slots: int, layers: int, kv_heads: int, max_len: int, head_dim: int, device="cuda"):
+        if slots <= 0 or layers <= 0 or kv_heads <= 0 or max_len <= 0:
+            raise ValueError("slots, layers, kv_heads and max_len must be positive")
+        if head_dim not in (64, 128):
+            raise NotImplementedError(f"head dim {head_dim} (have 64, 128)")
+        rows = (slots, layers, kv_heads, max_len)
+        self.k = torch.zeros(rows + (head_dim // 2,), dtype=torch.uint8, device=device)
+        self.v = torch.zeros_like(self.k)
+        self.k_par = torch.zeros(rows + (head_dim // GROUP, 2), dtype=torch.float16, device=device)
+        self.v_par = torch.zeros_like(self.k_par)
+        self._shape()
+
+    @classmethod
+    def wrap(cls, k: torch.Tensor, k_par: torch.Tensor, v: torch.Tensor, v_par: torch.Tensor) -> "Kv4Pool":
+        """A pool over existing tensors of the layout above (contiguous, nothing copied)."""
+        if k.dim() != 5 or k.dtype != torch.uint8 or k.shape[4] not in (32, 64):
+            raise ValueError("k must be uint8 [slots, layers, kv_heads, max_len, 32 or 64]")
+        rows = k.shape[:4]
+        par = rows + (k.shape[4] // 32, 2)
+        if v.dtype != torch.uint8 or v.shape != k.shape or k_par.shape != par or v_par.shape != par:
+            raise ValueError("k, v, k_par and v_par must share slots, layers, kv_heads, max_len and head_dim")
+        if k_par.dtype != torch.float16 or v_par.dtype != torch.float16:
+            raise ValueError("k_par and v_par must be fp16")
+        if not (k.is_contiguous() and v.is_contiguous() and k_par.is_contiguous() and v_par.is_contiguous()):
+            raise ValueError("the pool's tensors must be contiguous")
+        if not k.device == v.device == k_par.device == v_par.device:
+            raise ValueError("the pool's tensors must be on one device")
+        p = cls.__new__(cls)
+        p.k, p.k_par, p.v, p.v_par = k, k_par, v, v_par
+        p._shape()
+        return p
+
+    def _shape(self) -> None:
+        self.slots, self.layers, self.kv_heads, self.max_len, half = self.k.shape
+        self.head_dim = 2 * half
+        self.device = self.k.device
+        self.slot_rows = self.layers * self.kv_heads * self.max_len
+
+    def _pointers(self, layer: int):
+        """Device addresses of layer ``layer`` of slot 0: k codes, k params, v codes, v params."""
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"layer {layer} outside the pool's {self.layers}")
+        rows = layer * self.kv_heads * self.max_len
+        c, p = rows * (self.head_dim // 2), rows * (self.head_dim // GROUP) * 4
+        return (self.k.data_ptr() + c, self.k_par.data_ptr() + p, self.v.data_ptr() + c, self.v_par.data_ptr() + p)
+
+    def cache(self, slot: int) -> "Kv4Cache":
+        return Kv4Cache.in_pool(self, slot)
+
+    def bytes_per_position(self) -> int:
+        return self.layers * self.kv_heads * self.head_dim // GROUP * 36 * 2
+
+
+class Kv4Cache:
+    """One sequence's 4-bit cache: slot ``slot`` of ``pool`` (a pool of one slot of its own when
+    made directly), ``length`` positions valid."""
+
+    def __init__(self, layers: int, kv_heads: int, max_len: int, head_dim: int, device="cuda"):
+        self._take(Kv4Pool(1, layers, kv_heads, max_len, head_dim, device), 0)
+
+    @classmethod
+    def in_pool(cls, pool: Kv4Pool, slot: int) -> "Kv4Cache":
+        if not 0 <= slot < pool.slots:
+            raise ValueError(f"slot {slot} outside the pool's {pool.slots}")
+        c = cls.__new__(cls)
+        c._take(pool, slot)
+        return c
+
+    def _take(self, pool: Kv4Pool, slot: int) -> None:
+        self.pool, self.slot, self.max_len, self.length = pool, int(slot), pool.max_len, 0
+
+    def truncate(self, n: int) -> None:
+        """Keep the first ``n`` positions (later ones are overwritten by the next forward)."""
+        if not 0 <= n <= self.length:
+            raise ValueError(f"cannot truncate {self.length} cached positions to {n}")
+        self.length = int(n)
+
+
+def _check_pool(pool, device) -> None:
+    if not isinstance(pool, Kv4Pool):
+        raise ValueError("pool must be a Kv4Pool")
+    if not pool.k.is_cuda:
+        raise ValueError("the 4-bit cache runs on CUDA tensors only")
+    if device != pool.device:
+        raise ValueError(f"tensors on {device} for a pool on {pool.device}")
+
+
+def _index(t: torch.Tensor, n: int, pool: Kv4Pool, name: str) -> torch.Tensor:
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.device != pool.device:
+        raise ValueError(f"{name} must be int32 [{n}] on {pool.device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _rows(x: torch.Tensor, pool: Kv4Pool, name: str) -> torch.Tensor:
+    """x ``[tokens, kv_heads, head_dim]`` bf16 or fp32 with strides the kernel reads in place."""
+    if x.dim() != 3 or x.shape[1] != pool.kv_heads or x.shape[2] != pool.head_dim:
+        raise ValueError(f"{name} must be [tokens, {pool.kv_heads}, {pool.head_dim}], got {tuple(x.shape)}")
+    if x.dtype not in _DTYPES:
+        raise ValueError(f"{name} must be bf16 or fp32")
+    if x.stride(2) != 1 or (x.stride(0) | x.stride(1)) % 8 or x.data_ptr() % 16:
+        x = x.contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
+    return x
+
+
+def kv4_append(pool: Kv4Pool, layer: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
+               positions: torch.Tensor) -> None:
+    """Quantize ``k`` / ``v`` ``[tokens, kv_heads, head_dim]`` (bf16 or fp32, any strides) into rows
+    ``(slots[t], positions[t])`` (int32) of ``layer``.  Pairs outside the pool are skipped; the
+    pairs of one call must differ."""
+    _check_pool(pool, k.device)
+    k, v = _rows(k, pool, "k"), _rows(v, pool, "v")
+    n = k.shape[0]
+    if v.shape[0] != n or v.device != k.device:
+        raise ValueError("k and v must have the same tokens on the same device")
+    slots, positions = _index(slots, n, pool, "slots"), _index(positions, n, pool, "positions")
+    kc, kp, vc, vp = pool._pointers(layer)
+    with torch.cuda.device(pool.device):
+        _lib.call("ccut_kv4_append", k.data_ptr(), _DTYPES[k.dtype], k.stride(0), k.stride(1), v.data_ptr(),
+                  _DTYPES[v.dtype], v.stride(0), v.stride(1), n, pool.kv_heads, pool.head_dim, slots.data_ptr(),
+                  positions.data_ptr(), kc, kp, vc, vp, pool.max_len, pool.slot_rows, pool.slots,
+                  torch.cuda.current_stream().cuda_stream)
+
+
+def kv4_read(pool: Kv4Pool, layer: int, slots: torch.Tensor, positions: torch.Tensor,
+             out_dtype: torch.dtype = torch.float32) -> tuple:
+    """``(k, v)`` ``[tokens, kv_heads, head_dim]`` (fp32 or bf16): the values that rows
+    ``(slots[t], positions[t])`` (int32) of ``layer`` stand for, zeros for pairs outside the pool."""
+    _check_pool(pool, slots.device)
+    n = slots.shape[0] if slots.dim() else 0
+    slots, positions = _index(slots, n, pool, "slots"), _index(positions, n, pool, "positions")
+    if out_dtype not in _DTYPES:
+        raise ValueError("out_dtype must be bf16 or fp32")
+    shape = (n, pool.kv_heads, pool.head_dim)
+    k = torch.empty(shape, dtype=out_dtype, device=pool.device)
+    v = torch.empty(shape, dtype=out_dtype, device=pool.device)
+    kc, kp, vc, vp = pool._pointers(layer)
+    with torch.cuda.device(pool.device):
+        _lib.call("ccut_kv4_read", kc, kp, vc, vp, slots.data_ptr(), positions.data_ptr(), n, pool.kv_heads,
+                  pool.head_dim, pool.max_len, pool.slot_rows, pool.slots, k.data_ptr(), v.data_ptr(),
+                  _DTYPES[out_dtype], torch.cuda.current_stream().cuda_stream)
+    return k, v
+
+
+def kv4_attention(q: torch.Tensor, pool: Kv4Pool, layer: int, slots: torch.Tensor, starts: torch.Tensor,
+                  kv_len: int | None = None, scale: float | None = None, softcap: float | None = None,
+                  out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """q ``[batch, heads, seq, head_dim]`` bf16; batch row b attends over slot ``slots[b]`` of
+    ``layer``, its query i over positions ``<= starts[b] + i`` (int32) -> ``[batch, heads, seq,
+    head_dim]`` (bf16 or fp32).  ``kv_len``: an upper bound of ``starts[b] + seq`` when the host
+    knows one (positions at or past it are not read); default: the pool's ``max_len``."""
+    _check_pool(pool, q.device)
+    if q.dtype != torch.bfloat16 or q.dim() != 4 or q.shape[3] != pool.head_dim:
+        raise ValueError(f"q must be bf16 [batch, heads, seq, {pool.head_dim}]")
+    b, h, s, d = q.shape
+    if h == 0 or h % pool.kv_heads:
+        raise ValueError(f"heads ({h}) must be a positive multiple of kv_heads ({pool.kv_heads})")
+    if out_dtype not in _DTYPES:
+        raise ValueError("out_dtype must be bf16 or fp32")
+    n = pool.max_len if kv_len is None else int(kv_len)
+    if not 0 <= n <= pool.max_len:
+        raise ValueError(f"kv_len {n} outside [0, {pool.max_len}]")
+    slots, starts = _index(slots, b, pool, "slots"), _index(starts, b, pool, "starts")
+    q = q if q.is_contiguous() else q.contiguous()
+    if q.data_ptr() % 16:
+        q = q.clone()
+    out = torch.empty((b, h, s, d), dtype=out_dtype, device=q.device)
+    lib = _lib.load()
+    kc, kp, vc, vp = pool._pointers(layer)
+    with torch.cuda.device(pool.device):
+        nbytes = lib.ccut_kv4_attention_workspace_bytes(b, h, pool.kv_heads, s, n, d)
+        ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=q.device)
+        _lib.call("ccut_kv4_attention", q.data_ptr(), kc, kp, vc, vp, slots.data_ptr(), starts.data_ptr(), b, h,
+                  pool.kv_heads, s, d, pool.max_len, n, pool.slot_rows, pool.slots, float(scale or 0.0),
+                  float(softcap or 0.0), out.data_ptr(), _DTYPES[out_dtype], ws.data_ptr(), ws.numel(),
+                  torch.cuda.current_stream().cuda_stream)
+    return out

@@ -1,0 +1,190 @@
+// kv4.cu -- writing and reading the 4-bit kv cache (format: kv4.cuh).
+//
+// kv4_append_kernel: k and v rows of new tokens (bf16 or fp32, any token / head strides) -> codes and
+// params at (slots[t], positions[t]) of the pool.  Eight lanes hold a group's 64 features (8 each, one
+// or two 16-byte loads), find its minimum and maximum with three shuffles and write one 32-bit word of
+// codes each: 32 contiguous bytes per group.  Bound: HBM for long prompts (each input byte is read
+// once, 36 bytes per group written), launch latency for a decode step.
+// kv4_read_kernel: the fp32 / bf16 values of given rows, one thread per 32-bit word of codes.
+#include "kv4.cuh"
+
+namespace ccut {
+
+template <bool BF16>
+CCUT_DEVICE void load8(const void* base, long long off, float (&x)[8]) {
+  if constexpr (BF16) {
+    const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + off);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  } else {
+    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + off);
+    const float4 a = p[0], b = p[1];
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  }
+}
+
+struct Kv4In {
+  const void* x;
+  long long token_stride, head_stride;  // elements
+  uint8_t* codes;
+  __half2* params;
+};
+
+// blockIdx.y: 0 = k, 1 = v.  Eight consecutive lanes per (token, head, group).
+template <bool K_BF16, bool V_BF16>
+__global__ void __launch_bounds__(256) kv4_append_kernel(Kv4In k, Kv4In v, int tokens, int kv_heads, int groups,
+                                                         const int32_t* __restrict__ slots,
+                                                         const int32_t* __restrict__ positions, int max_len,
+                                                         long long slot_rows, int num_slots) {
+  pdl_wait();
+  pdl_trigger();
+  const long long item = (long long)blockIdx.x * 32 + (threadIdx.x >> 3);
+  const int lane8 = threadIdx.x & 7;
+  const int per_token = kv_heads * groups;
+  if (item >= (long long)tokens * per_token) return;
+  const int t = (int)(item / per_token), hg = (int)(item % per_token), h = hg / groups, g = hg % groups;
+  const int slot = slots[t], pos = positions[t];
+  const bool store = slot >= 0 && slot < num_slots && pos >= 0 && pos < max_len;
+  const unsigned mask = 0xFFu << (threadIdx.x & 24);  // the item's eight lanes
+  const Kv4In in = blockIdx.y ? v : k;
+  float x[8];
+  const long long off = t * in.token_stride + h * in.head_stride + g * kKv4Group + lane8 * 8;
+  if (blockIdx.y) load8<V_BF16>(in.x, off, x);
+  else load8<K_BF16>(in.x, off, x);
+  float lo = x[0], hi = x[0];
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    lo = fminf(lo, x[i]);
+    hi = fmaxf(hi, x[i]);
+    bad |= !(fabsf(x[i]) <= 3.402823466e38f);
+  }
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) {
+    lo = fminf(lo, __shfl_xor_sync(mask, lo, o));
+    hi = fmaxf(hi, __shfl_xor_sync(mask, hi, o));
+  }
+  bad = (__ballot_sync(mask, bad) & mask) != 0;
+  lo = fminf(fmaxf(lo, -65504.f), 65504.f);
+  hi = fminf(fmaxf(hi, -65504.f), 65504.f);
+  __half m = __float2half_rn(lo);
+  const float mf = __half2float(m);
+  __half s = __float2half_rn(fmaxf(__fmul_rn(__fsub_rn(hi, mf), 0.06666667f), 0.f));
+  const float sf = __half2float(s);
+  uint32_t w = 0;
+  if (sf > 0.f && !bad) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float q = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], mf), sf)), 0.f), 15.f);
+      w |= (uint32_t)q << (4 * i);
+    }
+  }
+  if (bad) s = m = __ushort_as_half(0x7FFF);
+  if (!store) return;
+  const size_t row = (size_t)slot * (size_t)slot_rows + (size_t)h * max_len + pos;
+  *reinterpret_cast<uint32_t*>(in.codes + (row * groups + g) * (kKv4Group / 2) + lane8 * 4) = w;
+  if (lane8 == 0) in.params[row * groups + g] = __halves2half2(s, m);
+}
+
+// Values of rows (slots[t], positions[t]): out [tokens, kv_heads, d]; rows outside the pool read zero.
+template <bool OUT_BF16>
+__global__ void __launch_bounds__(256) kv4_read_kernel(const uint8_t* __restrict__ kc, const __half2* __restrict__ kp,
+                                                       const uint8_t* __restrict__ vc, const __half2* __restrict__ vp,
+                                                       const int32_t* __restrict__ slots,
+                                                       const int32_t* __restrict__ positions, int tokens, int kv_heads,
+                                                       int groups, int max_len, long long slot_rows, int num_slots,
+                                                       void* __restrict__ k_out, void* __restrict__ v_out) {
+  pdl_wait();
+  pdl_trigger();
+  const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;  // a word of 8 features
+  const int words = groups * 8, per_token = kv_heads * words;
+  if (idx >= (long long)tokens * per_token) return;
+  const int t = (int)(idx / per_token), hw = (int)(idx % per_token), h = hw / words, w8 = hw % words;
+  const int slot = slots[t], pos = positions[t];
+  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (slot >= 0 && slot < num_slots && pos >= 0 && pos < max_len) {
+    const size_t row = (size_t)slot * (size_t)slot_rows + (size_t)h * max_len + pos;
+    const uint32_t w = reinterpret_cast<const uint32_t*>(blockIdx.y ? vc : kc)[row * words + w8];
+    const float2 sm = __half22float2((blockIdx.y ? vp : kp)[row * groups + w8 / 8]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = kv4_value((w >> (4 * i)) & 15, sm.x, sm.y);
+  }
+  void* out = blockIdx.y ? v_out : k_out;
+  if constexpr (OUT_BF16) {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      u[i] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    reinterpret_cast<uint4*>(out)[idx] = make_uint4(u[0], u[1], u[2], u[3]);
+  } else {
+    float4* o = reinterpret_cast<float4*>(out) + 2 * idx;
+    o[0] = make_float4(x[0], x[1], x[2], x[3]);
+    o[1] = make_float4(x[4], x[5], x[6], x[7]);
+  }
+}
+
+static bool float_dtype(int t) { return t == CCUT_OUT_BF16 || t == CCUT_OUT_F32; }
+
+}  // namespace ccut
+
+using namespace ccut;
+
+extern "C" {
+
+int ccut_kv4_append(const void* k, int k_dtype, long long k_token_stride, long long k_head_stride, const void* v,
+                    int v_dtype, long long v_token_stride, long long v_head_stride, int tokens, int kv_heads,
+                    int head_dim, const int32_t* slots, const int32_t* positions, uint8_t* k_codes,
+                    uint16_t* k_params, uint8_t* v_codes, uint16_t* v_params, int max_len, long long slot_rows,
+                    int num_slots, ccut_stream_t stream) {
+  PdlScope pdl_scope(tokens);
+  if (head_dim != 64 && head_dim != 128) return CCUT_ERR_UNSUPPORTED;
+  if (tokens < 0 || !kv4_shape_ok(kv_heads, head_dim, max_len, slot_rows, num_slots)) return CCUT_ERR_INVALID;
+  if (!float_dtype(k_dtype) || !float_dtype(v_dtype)) return CCUT_ERR_INVALID;
+  if (tokens == 0) return CCUT_OK;
+  if (!k || !v || !slots || !positions || (num_slots > 0 && (!k_codes || !k_params || !v_codes || !v_params)))
+    return CCUT_ERR_INVALID;
+  if ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) % 8) return CCUT_ERR_INVALID;
+  if (misaligned(k, 16) || misaligned(v, 16) || misaligned(k_codes, 16) || misaligned(v_codes, 16) ||
+      misaligned(k_params, head_dim / 16) || misaligned(v_params, head_dim / 16))
+    return CCUT_ERR_INVALID;
+  const int groups = head_dim / kKv4Group;
+  const long long blocks = ((long long)tokens * kv_heads * groups + 31) / 32;
+  if (blocks > 2147483647LL) return CCUT_ERR_UNSUPPORTED;
+  const Kv4In ki{k, k_token_stride, k_head_stride, k_codes, reinterpret_cast<__half2*>(k_params)};
+  const Kv4In vi{v, v_token_stride, v_head_stride, v_codes, reinterpret_cast<__half2*>(v_params)};
+  const bool kb = k_dtype == CCUT_OUT_BF16, vb = v_dtype == CCUT_OUT_BF16;
+  auto kern = kb ? (vb ? kv4_append_kernel<true, true> : kv4_append_kernel<true, false>)
+                 : (vb ? kv4_append_kernel<false, true> : kv4_append_kernel<false, false>);
+  return launch_k(kern, dim3((unsigned)blocks, 2), dim3(256), 0, stream, ki, vi, tokens, kv_heads, groups, slots,
+                  positions, max_len, slot_rows, num_slots);
+}
+
+int ccut_kv4_read(const uint8_t* k_codes, const uint16_t* k_params, const uint8_t* v_codes, const uint16_t* v_params,
+                  const int32_t* slots, const int32_t* positions, int tokens, int kv_heads, int head_dim, int max_len,
+                  long long slot_rows, int num_slots, void* k_out, void* v_out, int out_dtype, ccut_stream_t stream) {
+  PdlScope pdl_scope(tokens);
+  if (head_dim != 64 && head_dim != 128) return CCUT_ERR_UNSUPPORTED;
+  if (tokens < 0 || !kv4_shape_ok(kv_heads, head_dim, max_len, slot_rows, num_slots) || !float_dtype(out_dtype))
+    return CCUT_ERR_INVALID;
+  if (tokens == 0) return CCUT_OK;
+  if (!k_out || !v_out || !slots || !positions || (num_slots > 0 && (!k_codes || !k_params || !v_codes || !v_params)))
+    return CCUT_ERR_INVALID;
+  if (misaligned(k_out, 16) || misaligned(v_out, 16) || misaligned(k_codes, 16) || misaligned(v_codes, 16) ||
+      misaligned(k_params, head_dim / 16) || misaligned(v_params, head_dim / 16))
+    return CCUT_ERR_INVALID;
+  const int groups = head_dim / kKv4Group;
+  const long long blocks = ((long long)tokens * kv_heads * groups * 8 + 255) / 256;
+  if (blocks > 2147483647LL) return CCUT_ERR_UNSUPPORTED;
+  auto kern = out_dtype == CCUT_OUT_BF16 ? kv4_read_kernel<true> : kv4_read_kernel<false>;
+  return launch_k(kern, dim3((unsigned)blocks, 2), dim3(256), 0, stream, k_codes,
+                  reinterpret_cast<const __half2*>(k_params), v_codes, reinterpret_cast<const __half2*>(v_params),
+                  slots, positions, tokens, kv_heads, groups, max_len, slot_rows, num_slots, k_out, v_out);
+}
+
+}  // extern "C"

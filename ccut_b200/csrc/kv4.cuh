@@ -1,0 +1,32 @@
+// kv4.cuh -- the 4-bit kv cache format shared by its writer, its reader and the attention kernels.
+//
+// A cache row is one (slot, kv head, position): row = slot * slot_rows + head * max_len + position.
+// Codes: head_dim / 2 bytes per row, byte j holds feature 2 j (low nibble) and 2 j + 1 (high nibble).
+// Params: head_dim / 64 pairs (scale s, minimum m) of fp16 per row, one pair per group of 64 features;
+// the value of code q is q s + m.  One pair per 64 features keeps the params at 4 of 36 bytes, and
+// 64 features are four k16 steps of an MMA, so a group's scale can be applied to the fp32 product of
+// the codes instead of to every code.
+//
+// Rounding: m = fp16(min) and s = fp16(fl32(max - m) * fl32(1/15)) to the nearest (two roundings of
+// 2^-11; the codes are chosen with the rounded pair, so they only move the grid), q = the nearest of
+// 0..15, ties to even.  Values beyond +-65504 saturate there, so s <= 8734 and q s + m stays in fp16's
+// range.  A group that holds a NaN or an infinity gets s = m = NaN and reads back NaN.
+#pragma once
+
+#include "host.cuh"
+
+namespace ccut {
+
+constexpr int kKv4Group = 64;
+
+// The value of code q under the pair (s, m): q * s has at most 15 significant bits, so the fma rounds once.
+CCUT_DEVICE float kv4_value(uint32_t q, float s, float m) { return fmaf((float)q, s, m); }
+
+// Host-side shape checks shared by the entry points.
+inline bool kv4_shape_ok(int kv_heads, int head_dim, int max_len, long long slot_rows, int num_slots) {
+  return kv_heads > 0 && (head_dim == 64 || head_dim == 128) && max_len > 0 && num_slots >= 0 &&
+         slot_rows >= (long long)kv_heads * max_len;
+}
+inline bool misaligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a != 0; }
+
+}  // namespace ccut

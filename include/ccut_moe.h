@@ -325,6 +325,85 @@ CCUT_API int ccut_mla_attention_pool(const float* q, const uint16_t* kv_pool, co
                                      int rope_dim, long long slot_stride, int num_slots, float scale, void* out,
                                      int out_dtype, void* workspace, size_t ws_bytes, ccut_stream_t stream);
 
+/* ---- 4-bit kv cache (no reference counterpart: the reference's cache is fp32 arrays,
+ * ccut/models/generic.py:304-345; its kv_cache_dtype setting, ccut/config.py:91-108, names the
+ * choice) -------------------------------------------------------------------------------- */
+/* Cache row r = slot * slot_rows + kv_head * max_len + position holds one position of one kv head:
+ * codes, head_dim / 2 bytes at r * head_dim / 2 (byte j: feature 2j in the low nibble, 2j + 1 in
+ * the high one); params, head_dim / 64 pairs (scale s, minimum m) of fp16 bit patterns, one pair
+ * per group of 64 features.  The value of code q is q * s + m.  slot_rows >= kv_heads * max_len is
+ * the distance of two slots in rows; head_dim is 64 or 128.  Codes are 16-byte, params
+ * head_dim / 16-byte aligned.  A pool of one slot is one sequence's cache. */
+/* Quantizes k / v of `tokens` tokens into rows (slots[t], positions[t]) (int32, device); a pair
+ * outside the pool writes nothing.  k, v: bf16 or fp32 (CCUT_OUT_*, each its own), feature f of
+ * head h of token t at t * token_stride + h * head_stride + f (elements, strides multiples of 8,
+ * 16-byte aligned base).  Per group m = fp16(min), s = fp16((max - m) * fl(1/15)), q = (x - m) / s
+ * to the nearest, ties to even (0 when s is 0), values clamped to +-65504 first; a group with a
+ * NaN or an infinity reads back NaN.  The pairs of one call must differ: of two tokens for the
+ * same row, which one's codes and which one's params stay is not defined. */
+CCUT_API int ccut_kv4_append(const void* k, int k_dtype, long long k_token_stride, long long k_head_stride,
+                             const void* v, int v_dtype, long long v_token_stride, long long v_head_stride,
+                             int tokens, int kv_heads, int head_dim, const int32_t* slots,
+                             const int32_t* positions, uint8_t* k_codes, uint16_t* k_params, uint8_t* v_codes,
+                             uint16_t* v_params, int max_len, long long slot_rows, int num_slots,
+                             ccut_stream_t stream);
+/* The values of rows (slots[t], positions[t]): k_out, v_out [tokens, kv_heads, head_dim] bf16 or
+ * fp32 (out_dtype), 16-byte aligned; a pair outside the pool reads zeros. */
+CCUT_API int ccut_kv4_read(const uint8_t* k_codes, const uint16_t* k_params, const uint8_t* v_codes,
+                           const uint16_t* v_params, const int32_t* slots, const int32_t* positions, int tokens,
+                           int kv_heads, int head_dim, int max_len, long long slot_rows, int num_slots, void* k_out,
+                           void* v_out, int out_dtype, ccut_stream_t stream);
+/* ccut_gqa_attention_pool over a 4-bit pool: q bf16 [batch, heads, seq, head_dim], out the same
+ * shape in out_dtype; batch row b reads slot slots[b], its query i sees positions <= starts[b] + i
+ * and < kv_len (kv_len <= max_len bounds what any row sees: pass the longest length when the host
+ * knows it, else max_len).  A slot outside [0, num_slots) or a negative start gives zero rows;
+ * what a query does not see never reaches its row, whatever is stored there.  scale <= 0 means
+ * 1/sqrt(head_dim); softcap > 0 as in ccut_gqa_attention.  q, out and workspace are 16-byte
+ * aligned. */
+CCUT_API size_t ccut_kv4_attention_workspace_bytes(int batch, int heads, int kv_heads, int seq, int kv_len,
+                                                   int head_dim);
+CCUT_API int ccut_kv4_attention(const uint16_t* q, const uint8_t* k_codes, const uint16_t* k_params,
+                                const uint8_t* v_codes, const uint16_t* v_params, const int32_t* slots,
+                                const int32_t* starts, int batch, int heads, int kv_heads, int seq, int head_dim,
+                                int max_len, int kv_len, long long slot_rows, int num_slots, float scale,
+                                float softcap, void* out, int out_dtype, void* workspace, size_t ws_bytes,
+                                ccut_stream_t stream);
+
+/* ---- log probabilities of given tokens (no reference counterpart: the reference's engine answers
+ * with token ids only, ccut/engine.py:335-352) ------------------------------------------------ */
+/* Per row of logits [rows, vocab] (bf16 or fp32, rows ld elements apart) and its token (int32,
+ * device): logprob = log softmax(row)[token], entropy of softmax(row) (both in nats), rank = 1 +
+ * the number of logits that come before the token's in the order (value descending, index
+ * ascending), and the first top_n of that order with their log probabilities (top_ids,
+ * top_logprobs [rows, top_n]).  Logits of -inf take part with probability 0.  A token outside
+ * [0, vocab) gets logprob NaN and rank 0.  A row with a NaN, with +inf or with nothing but -inf
+ * has NaN log probabilities and entropy; in the order a NaN comes after -inf.
+ * top_n <= min(vocab, CCUT_MAX_TOP_LOGPROBS). */
+#define CCUT_MAX_TOP_LOGPROBS 32
+CCUT_API size_t ccut_token_logprobs_workspace_bytes(int rows, int vocab, int top_n);
+CCUT_API int ccut_token_logprobs(const void* logits, int dtype, int rows, int vocab, long long ld,
+                                 const int32_t* tokens, int top_n, float* logprob, float* entropy, int32_t* rank,
+                                 int32_t* top_ids, float* top_logprobs, void* workspace, size_t ws_bytes,
+                                 ccut_stream_t stream);
+
+/* ---- low-rank adapters (no reference counterpart) -------------------------------------------- */
+/* out[t] = base[t] + scales[i] * B_i A_i x[t] with i = ids[t] (int32, device), for a projection
+ * whose outputs are `slices` parts side by side (widths: host ints, multiples of 8), each with an
+ * adapter of its own: a bf16 [adapters, slices * rank, inputs], b bf16 [adapters, sum(widths),
+ * rank], scales fp32 [adapters]; outputs of slice j take rank rows j * rank .. of a.  x bf16
+ * [tokens, inputs]; base, out [tokens, sum(widths)] bf16 or fp32 (dtype) with rows base_ld / out_ld
+ * elements apart (multiples of 8); out may be base.  A row whose id is outside [0, adapters) is
+ * copied from base; nothing of another adapter reaches a row.  rank is a multiple of 16, slices *
+ * rank <= 256, inputs a multiple of 8; x, a, b, base, out and workspace 16-byte aligned.  The sums
+ * over the inputs and the ranks are fp32, added to base before the one rounding to dtype.  Tokens
+ * of one adapter next to each other read its weights once per 16. */
+#define CCUT_LORA_MAX_SLICES 4
+CCUT_API size_t ccut_lora_workspace_bytes(int tokens, int inputs, int rank, int slices);
+CCUT_API int ccut_lora_add(const uint16_t* x, const uint16_t* a, const uint16_t* b, const float* scales,
+                           const int32_t* ids, int tokens, int inputs, int rank, int adapters, int slices,
+                           const int* widths, const void* base, long long base_ld, void* out, long long out_ld,
+                           int dtype, void* workspace, size_t ws_bytes, ccut_stream_t stream);
+
 /* ---- diagnostics ------------------------------------------------------------------- */
 /* Device-side status word kept at the start of every workspace: a kernel whose bounded
  * wait expired stores CCUT_ERR_TIMEOUT there instead of hanging.  Reads it (synchronises
