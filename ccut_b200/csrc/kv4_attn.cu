@@ -10,18 +10,21 @@
 // - No dequantization.  A nibble masked in place is an fp16 subnormal: bits 0-3 hold c 2^-24, bits
 //   4-7 hold c 2^-20 (16 times as much).  One AND makes an operand pair, exact; the powers of two go
 //   into q (odd features divided by 16) and into the output.  The MMA multiplies the codes, and the
-//   group's scale and minimum are applied in fp32 to the products:
-//   x = sum_g s_g (q_g . c_g) + m_g (sum q_g),  o = sum_j (p_j s_jg) c_j + (sum_j p_j m_jg).
+//   group's scale and minimum are applied to the products:
+//   x = sum_g s_g (q_g . c_g) + m_g (sum q_g),  o = sum_j (p_j s_jg) c_j + (sum_j p_j m_jg),
+//   the minima of k by one more MMA (their fp16 pairs times sum q_g in two fp16 parts).
 // - Positions are the M of m16n8k16, the query rows of a kv head the N: 8 rows take half the MMAs
 //   they would take as the M.  The order of the k index is free, so lanes load their operands straight
 //   from global memory (8 bytes of 8 rows of k, 4 bytes of 4 rows of v a lane, full 32-byte sectors),
 //   no shared memory, and the scores' accumulators become the second product's operand by movmatrix.
 // - The running maximum moves only when a score passes it by 2^8 (one vote a tile instead of
 //   six shuffles a row pair): probabilities stay below 2^8, and fp16's range has room for that.
-// Roundings to fp16: q, scaled to its row's largest element (2^-20 of it at least is kept); p s_v,
-// scaled by the power of two R that brings the largest v scale seen so far to [1/2, 1) (11 bits, and
-// 2^-25 of the largest absolutely; with fp32 output a second fp16 part keeps 22).  Everything else,
-// running maximum, sums and outputs, is fp32.
+// - Tiles that every row sees in whole run without bounds or mask tests, four pointers advancing by
+//   constant strides; the few others (the last tile, the diagonal of a query block) run a checked copy.
+// Roundings to fp16: q, scaled to its row's largest element (2^-35 of it is kept), and sum q_g (2^-15
+// of the largest element); p s_v, scaled by the power of two R that brings the largest v scale seen so
+// far to [1/2, 1) (11 bits, and 2^-25 of the largest absolutely; with fp32 output a second fp16 part
+// keeps 22).  Everything else, running maximum, sums and outputs, is fp32.
 #include <math.h>
 
 #include "kv4.cuh"
@@ -47,7 +50,7 @@ struct Kv4AttnArgs {
 
 constexpr int kKv4Warps = 4;
 constexpr int kKv4Tile = 16;           // positions per warp step
-constexpr int kKv4Short = 32;          // query rows per kv head up to which the short kernel runs
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 CCUT_DEVICE uint32_t movmatrix_trans(uint32_t a) {
@@ -64,7 +67,10 @@ CCUT_DEVICE uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-CCUT_DEVICE float2 unpack_f16(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+CCUT_DEVICE __half2 as_half2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
+CCUT_DEVICE float2 unpack_f16(uint32_t u) { return __half22float2(as_half2(u)); }
+CCUT_DEVICE float low_f16(uint32_t u) { return __low2float(as_half2(u)); }
+CCUT_DEVICE float high_f16(uint32_t u) { return __high2float(as_half2(u)); }
 CCUT_DEVICE float pow2f(int e) { return __int_as_float((e + 127) << 23); }
 CCUT_DEVICE int exponent_of(float x) { return (int)((__float_as_uint(x) >> 23) & 255) - 127; }
 
@@ -102,10 +108,9 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_attn_kernel(Kv4AttnArgs a)
   const size_t row_base = valid ? (size_t)slot * (size_t)a.slot_rows + (size_t)kvh * a.max_len : 0;
 
   // ---- the query rows as B fragments (row n = g of n-tile nt; features t * 16 .. of each group) ----
-  uint32_t qf[NT][G][4][2];
-  float fr[NT][2], qs[NT][G][2];  // columns 2t, 2t + 1: factor of the code products, scaled sums of q
-  int lim[NT][2];                 // last visible position
-  const float xs = a.scale * kLog2e;
+  uint32_t qf[NT][G][4][2], qm[NT];  // qm: sum q_g of the groups, high parts in lanes t = 0, the rest in t = 1
+  float fr[NT][2];                   // columns 2t, 2t + 1: factor of the products
+  int lim[NT][2];                    // last visible position
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int r = r0 + nt * 8 + g;
@@ -134,7 +139,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_attn_kernel(Kv4AttnArgs a)
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     const int e = min(max(exponent_of(mx), -90), 90);  // |q| 2^-e in [1, 2)
-    const float f = pow2f(-e);
+    const float f = pow2f(14 - e);                     // the operand in [2^14, 2^15)
 #pragma unroll
     for (int gr = 0; gr < G; ++gr)
 #pragma unroll
@@ -145,25 +150,26 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_attn_kernel(Kv4AttnArgs a)
           qf[nt][gr][w * 2 + h][0] = pack_f16(d[0] * f, d[4] * f);
           qf[nt][gr][w * 2 + h][1] = pack_f16(d[1] * (f * 0.0625f), d[5] * (f * 0.0625f));
         }
-    const float back = pow2f(24 + e) * xs;
+    // operand pair of the minima: (m of group 0, of group 1), or with one group the row's (s, m)
+    const float s0 = G == 2 ? sum[0] * pow2f(-10 - e) : 0.f, s1 = sum[G - 1] * pow2f(-10 - e);
+    const uint32_t hi = pack_f16(s0, s1);
+    const float2 hf = unpack_f16(hi);
+    qm[nt] = t == 0 ? hi : t == 1 ? pack_f16(s0 - hf.x, s1 - hf.y) : 0u;
+    const float back = pow2f(10 + e) * (a.scale * kLog2e);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const int from = (2 * t + c) * 4;  // a lane that holds row 2t + c
-      fr[nt][c] = __shfl_sync(0xffffffffu, back, from);
-#pragma unroll
-      for (int gr = 0; gr < G; ++gr) qs[nt][gr][c] = __shfl_sync(0xffffffffu, sum[gr], from) * xs;
+      fr[nt][c] = __shfl_sync(0xffffffffu, back, (2 * t + c) * 4);  // a lane that holds row 2t + c
       lim[nt][c] = start + (r0 + nt * 8 + 2 * t + c) / grp;
     }
   }
 
-  float m[NT][2], mu[NT][2], l[NT][2], am[NT][G][2], o[NT][D / 16][4], R[G];
-#pragma unroll
-  for (int gr = 0; gr < G; ++gr) R[gr] = pow2f(30);
+  float m[NT][2], l[NT][2], am[NT][G][2], o[NT][D / 16][4], R = 1.f;
+  __half r_inv = __ushort_as_half(0);  // 1 / R; 0 before the first tile
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      m[nt][c] = -INFINITY, mu[nt][c] = 0.f, l[nt][c] = 0.f;
+      m[nt][c] = -INFINITY, l[nt][c] = 0.f;
 #pragma unroll
       for (int gr = 0; gr < G; ++gr) am[nt][gr][c] = 0.f;
     }
@@ -173,56 +179,59 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_attn_kernel(Kv4AttnArgs a)
       for (int i = 0; i < 4; ++i) o[nt][mt][i] = 0.f;
   }
 
-  const uint8_t* kc = a.kc + row_base * (D / 2) + t * 8;
-  const uint8_t* vc = a.vc + row_base * (D / 2) + g * 4;
-  const uint32_t* kp = reinterpret_cast<const uint32_t*>(a.kp) + row_base * G;
-  const uint32_t* vp = reinterpret_cast<const uint32_t*>(a.vp) + row_base * G;
-  const int ntiles = k1 > k0 ? (k1 - k0 + kKv4Tile - 1) / kKv4Tile : 0;
+  // lane addresses at position k0
+  const uint8_t* kc = a.kc + (row_base + k0 + g) * (D / 2) + t * 8;
+  const uint8_t* vc = a.vc + (row_base + k0 + 2 * t) * (D / 2) + g * 4;
+  const uint8_t* kp = reinterpret_cast<const uint8_t*>(a.kp) + (row_base + k0 + g) * (4 * G);
+  const uint8_t* vp = reinterpret_cast<const uint8_t*>(a.vp) + (row_base + k0 + g) * (4 * G);
 
-  auto load = [&](Kv4Tile<G>& x, int tile) {  // rows at or past k1 come as zeros
-    const int p0 = k0 + tile * kKv4Tile;
+  // the tile at the lane addresses; kChecked: `left` positions from its first, the others come as zeros
+  auto load = [&](Kv4Tile<G>& x, auto checked, int left) {
+    constexpr bool kChecked = decltype(checked)::value;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int p = p0 + g + 8 * h;
-      const bool in = p < k1;
+      const bool in = !kChecked || g + 8 * h < left;
 #pragma unroll
-      for (int gr = 0; gr < G; ++gr) {
-        x.k[h][gr] = make_uint2(0, 0);
-        x.kp[h][gr] = 0, x.vp[h][gr] = 0;
-        if (in) {
-          x.k[h][gr] = __ldg(reinterpret_cast<const uint2*>(kc + (size_t)p * (D / 2) + gr * 32));
-        }
-      }
-      if (in) {
-        if constexpr (G == 2) {
-          const uint2 uk = __ldg(reinterpret_cast<const uint2*>(kp + (size_t)p * G));
-          const uint2 uv = __ldg(reinterpret_cast<const uint2*>(vp + (size_t)p * G));
-          x.kp[h][0] = uk.x, x.kp[h][G - 1] = uk.y, x.vp[h][0] = uv.x, x.vp[h][G - 1] = uv.y;
-        } else {
-          x.kp[h][0] = __ldg(kp + p);
-          x.vp[h][0] = __ldg(vp + p);
-        }
+      for (int gr = 0; gr < G; ++gr)
+        x.k[h][gr] = in ? __ldg(reinterpret_cast<const uint2*>(kc + h * 8 * (D / 2) + gr * 32)) : make_uint2(0, 0);
+      if constexpr (G == 2) {
+        const uint2 uk = in ? __ldg(reinterpret_cast<const uint2*>(kp + h * 64)) : make_uint2(0, 0);
+        const uint2 uv = in ? __ldg(reinterpret_cast<const uint2*>(vp + h * 64)) : make_uint2(0, 0);
+        x.kp[h][0] = uk.x, x.kp[h][G - 1] = uk.y, x.vp[h][0] = uv.x, x.vp[h][G - 1] = uv.y;
+      } else {
+        x.kp[h][0] = in ? __ldg(reinterpret_cast<const uint32_t*>(kp + h * 32)) : 0u;
+        x.vp[h][0] = in ? __ldg(reinterpret_cast<const uint32_t*>(vp + h * 32)) : 0u;
       }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int p = p0 + 2 * t + (i & 1) + 8 * (i >> 1);
+      const int p = (i & 1) + 8 * (i >> 1);
+      const bool in = !kChecked || 2 * t + p < left;
 #pragma unroll
-      for (int gr = 0; gr < G; ++gr) {
-        x.v[i][gr] = 0;
-        if (p < k1) x.v[i][gr] = __ldg(reinterpret_cast<const uint32_t*>(vc + (size_t)p * (D / 2) + gr * 32));
-      }
+      for (int gr = 0; gr < G; ++gr)
+        x.v[i][gr] = in ? __ldg(reinterpret_cast<const uint32_t*>(vc + p * (D / 2) + gr * 32)) : 0u;
     }
+  };
+  auto advance = [&](int tiles) {
+    kc += (long long)tiles * (kKv4Tile * (D / 2));
+    vc += (long long)tiles * (kKv4Tile * (D / 2));
+    kp += (long long)tiles * (kKv4Tile * 4 * G);
+    vp += (long long)tiles * (kKv4Tile * 4 * G);
   };
 
   auto step = [&](const Kv4Tile<G>& x, int p0, auto masked_tag) {
     constexpr bool kMasked = decltype(masked_tag)::value;
     float sc[NT][4];
-    float2 sk[2][G];
+    {
+      const uint32_t f[4] = {G == 2 ? __byte_perm(x.kp[0][0], x.kp[0][G - 1], 0x7632) : x.kp[0][0],
+                             G == 2 ? __byte_perm(x.kp[1][0], x.kp[1][G - 1], 0x7632) : x.kp[1][0], 0u, 0u};
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+      for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-      for (int gr = 0; gr < G; ++gr) sk[h][gr] = unpack_f16(x.kp[h][gr]);
+        for (int i = 0; i < 4; ++i) sc[nt][i] = 0.f;
+        mma_16816<false>(sc[nt], f, qm[nt], 0u);
+      }
+    }
 #pragma unroll
     for (int gr = 0; gr < G; ++gr) {
       float c4[NT][4];
@@ -240,13 +249,11 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_attn_kernel(Kv4AttnArgs a)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) mma_16816<false>(c4[nt], f, qf[nt][gr][w * 2 + h][0], qf[nt][gr][w * 2 + h][1]);
         }
+      const float s[2] = {low_f16(x.kp[0][gr]), low_f16(x.kp[1][gr])};
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {  // i: row g + 8 (i >> 1), column 2t + (i & 1)
-          const float y = fmaf(sk[i >> 1][gr].x * fr[nt][i & 1], c4[nt][i], sk[i >> 1][gr].y * qs[nt][gr][i & 1]);
-          sc[nt][i] = gr ? sc[nt][i] + y : y;
-        }
+        for (int i = 0; i < 4; ++i) sc[nt][i] = fmaf(s[i >> 1], c4[nt][i], sc[nt][i]);  // row g + 8 (i >> 1), column 2t + (i & 1)
     }
     bool vis[NT][4];
     bool need = false;
@@ -254,6 +261,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_attn_kernel(Kv4AttnArgs a)
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
+        sc[nt][i] *= fr[nt][i & 1];
         if (a.softcap > 0.f) sc[nt][i] = tanhf(sc[nt][i] * (1.f / kLog2e) / a.softcap) * (a.softcap * kLog2e);
         if constexpr (kMasked) {
           const int p = p0 + g + 8 * (i >> 1);
@@ -262,14 +270,9 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_attn_kernel(Kv4AttnArgs a)
         }
         need |= sc[nt][i] > m[nt][i & 1] + 8.f;
       }
-    float2 sv[2][G];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int gr = 0; gr < G; ++gr) {
-        sv[h][gr] = unpack_f16(x.vp[h][gr]);
-        need |= sv[h][gr].x * R[gr] > 1.f;
-      }
+    __half2 top = __hmax2(as_half2(x.vp[0][0]), as_half2(x.vp[1][0]));
+    if constexpr (G == 2) top = __hmax2(top, __hmax2(as_half2(x.vp[0][G - 1]), as_half2(x.vp[1][G - 1])));
+    need |= __hgt(__low2half(top), r_inv);
     if (__any_sync(0xffffffffu, need)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -281,65 +284,64 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_attn_kernel(Kv4AttnArgs a)
           v = fmaxf(v, m[nt][c]);
           const float al = v == -INFINITY ? 1.f : ex2(m[nt][c] - v);
           m[nt][c] = v;
-          mu[nt][c] = v == -INFINITY ? 0.f : v;
           l[nt][c] *= al;
 #pragma unroll
           for (int gr = 0; gr < G; ++gr) am[nt][gr][c] *= al;
 #pragma unroll
           for (int mt = 0; mt < D / 16; ++mt) o[nt][mt][c] *= al, o[nt][mt][c + 2] *= al;
         }
+      float v = __low2float(top);
 #pragma unroll
-      for (int gr = 0; gr < G; ++gr) {
-        float v = fmaxf(sv[0][gr].x, sv[1][gr].x);
+      for (int s = 4; s < 32; s <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, s));
+      v = fminf(v, 65504.f);
+      if (v > __half2float(r_inv)) {
+        const float r = pow2f(-exponent_of(v) - 1), f = r / R;
+        R = r;
+        r_inv = __float2half_rn(1.f / r);
 #pragma unroll
-        for (int s = 4; s < 32; s <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, s));
-        v = fminf(v, 65504.f);
-        if (v * R[gr] > 1.f) {
-          const float r = pow2f(-exponent_of(v) - 1), f = r / R[gr];
-          R[gr] = r;
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int mt = 0; mt < D / 16; ++mt)
 #pragma unroll
-            for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) o[nt][gr * 4 + mt][i] *= f;
-        }
+            for (int i = 0; i < 4; ++i) o[nt][mt][i] *= f;
       }
     }
-    uint32_t wb[NT][G][2], wl[NT][G][2];  // p s_v R as the B operand: high part, and the rest
+    float p[NT][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float p[4];
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        p[i] = ex2(sc[nt][i] - mu[nt][i & 1]);
-        l[nt][i & 1] += p[i];
+        p[nt][i] = ex2(sc[nt][i] - m[nt][i & 1]);
+        if constexpr (kMasked) p[nt][i] = vis[nt][i] ? p[nt][i] : 0.f;  // a row that saw nothing yet has m = -inf
+        l[nt][i & 1] += p[nt][i];
       }
 #pragma unroll
-      for (int gr = 0; gr < G; ++gr) {
+    for (int gr = 0; gr < G; ++gr) {
+      const float sr[2] = {low_f16(x.vp[0][gr]) * R, low_f16(x.vp[1][gr]) * R};
+      const float mv[2] = {high_f16(x.vp[0][gr]), high_f16(x.vp[1][gr])};
+      uint32_t wb[NT][2], wl[NT][2];  // p s_v R as the B operand: high part, and the rest
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
         float w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          w[i] = p[i] * (sv[i >> 1][gr].x * R[gr]);
-          float y = p[i] * sv[i >> 1][gr].y;
+          w[i] = p[nt][i] * sr[i >> 1];
           if constexpr (kMasked) {  // 0 * NaN stays out
             w[i] = vis[nt][i] ? w[i] : 0.f;
-            y = vis[nt][i] ? y : 0.f;
+            am[nt][gr][i & 1] += vis[nt][i] ? p[nt][i] * mv[i >> 1] : 0.f;
+          } else {
+            am[nt][gr][i & 1] = fmaf(p[nt][i], mv[i >> 1], am[nt][gr][i & 1]);
           }
-          am[nt][gr][i & 1] += y;
         }
         const uint32_t h0 = pack_f16(w[0], w[1]), h1 = pack_f16(w[2], w[3]);
-        wb[nt][gr][0] = movmatrix_trans(h0);
-        wb[nt][gr][1] = movmatrix_trans(h1);
+        wb[nt][0] = movmatrix_trans(h0);
+        wb[nt][1] = movmatrix_trans(h1);
         if constexpr (!OUT_BF16) {
           const float2 b0 = unpack_f16(h0), b1 = unpack_f16(h1);
-          wl[nt][gr][0] = movmatrix_trans(pack_f16(w[0] - b0.x, w[1] - b0.y));
-          wl[nt][gr][1] = movmatrix_trans(pack_f16(w[2] - b1.x, w[3] - b1.y));
+          wl[nt][0] = movmatrix_trans(pack_f16(w[0] - b0.x, w[1] - b0.y));
+          wl[nt][1] = movmatrix_trans(pack_f16(w[2] - b1.x, w[3] - b1.y));
         }
       }
-    }
-#pragma unroll
-    for (int gr = 0; gr < G; ++gr)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const uint32_t sel = half ? 0x7632 : 0x5410;
@@ -350,22 +352,41 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_attn_kernel(Kv4AttnArgs a)
           const uint32_t f[4] = {u0 & M0, u0 & M1, u1 & M0, u1 & M1};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            mma_16816<false>(o[nt][gr * 4 + half * 2 + h], f, wb[nt][gr][0], wb[nt][gr][1]);
-            if constexpr (!OUT_BF16) mma_16816<false>(o[nt][gr * 4 + half * 2 + h], f, wl[nt][gr][0], wl[nt][gr][1]);
+            mma_16816<false>(o[nt][gr * 4 + half * 2 + h], f, wb[nt][0], wb[nt][1]);
+            if constexpr (!OUT_BF16) mma_16816<false>(o[nt][gr * 4 + half * 2 + h], f, wl[nt][0], wl[nt][1]);
           }
         }
       }
+    }
   };
 
-  const int all_see = start + r0 / grp;  // last position every row of this CTA sees
-  Kv4Tile<G> next;
-  if (warp < ntiles) load(next, warp);
-  for (int j = warp; j < ntiles; j += kKv4Warps) {
-    const Kv4Tile<G> cur = next;
-    if (j + kKv4Warps < ntiles) load(next, j + kKv4Warps);
+  // tiles of this warp: j, j + 4, ..; the first `whole` of the split are seen in whole by every row
+  const int ntiles = k1 > k0 ? (k1 - k0 + kKv4Tile - 1) / kKv4Tile : 0;
+  const int whole = k1 > k0 ? max(0, min(k1, start + r0 / grp + 1) - k0) / kKv4Tile : 0;
+  int j = warp;
+  advance(warp);
+  if (j < whole) {
+    Kv4Tile<G> x, y;
+    load(x, std::false_type{}, 0);
+    while (true) {  // one tile in flight while the other is worked on
+      advance(kKv4Warps);
+      if (j + kKv4Warps < whole) load(y, std::false_type{}, 0);
+      step(x, 0, std::false_type{});
+      j += kKv4Warps;
+      if (j >= whole) break;
+      advance(kKv4Warps);
+      if (j + kKv4Warps < whole) load(x, std::false_type{}, 0);
+      step(y, 0, std::false_type{});
+      j += kKv4Warps;
+      if (j >= whole) break;
+    }
+  }
+  for (; j < ntiles; j += kKv4Warps) {
+    Kv4Tile<G> x;
     const int p0 = k0 + j * kKv4Tile;
-    if (p0 + kKv4Tile <= k1 && p0 + kKv4Tile - 1 <= all_see) step(cur, p0, std::false_type{});
-    else step(cur, p0, std::true_type{});
+    load(x, std::true_type{}, k1 - p0);
+    advance(kKv4Warps);
+    step(x, p0, std::true_type{});
   }
 
   // ---- join the warps: rows 2t + c of n-tile nt, features 8 g + {0..7} of each group -----------------
@@ -383,7 +404,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_attn_kernel(Kv4AttnArgs a)
       if (g == 0) sm_m[warp][n] = m[nt][c], sm_l[warp][n] = l[nt][c];
 #pragma unroll
       for (int gr = 0; gr < G; ++gr) {
-        const float u = pow2f(20) / R[gr];
+        const float u = pow2f(20) / R;
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) {
           float* d = &sm_o[warp][n][gr * kKv4Group + g * 8 + mt * 2];
