@@ -21,6 +21,12 @@
 //   six shuffles a row pair): probabilities stay below 2^8, and fp16's range has room for that.
 // - Tiles that every row sees in whole run without bounds or mask tests, four pointers advancing by
 //   constant strides; the few others (the last tile, the diagonal of a query block) run a checked copy.
+// - Work is cut evenly whatever the lengths: the blocks of 64 positions of all (sequence, tile of query
+//   rows, kv head) units form one line, found from starts on the device, and each CTA of one resident
+//   round takes an equal span of it.  A unit inside one span is finished there; of the others a span
+//   leaves at most two partial results (the first and the last of its units), which a second kernel joins.
+//   Equal chunks per sequence cost a prologue, a reduction and a partial result every chunk instead
+//   (64 sequences of 3001..8191 positions: 66 us at the best chunk).
 // Roundings to fp16: q, scaled to its row's largest element (2^-35 of it is kept), and sum q_g (2^-15
 // of the largest element); p s_v, scaled by the power of two R that brings the largest v scale seen so
 // far to [1/2, 1) (11 bits, and 2^-25 of the largest absolutely; with fp32 output a second fp16 part
@@ -43,13 +49,15 @@ struct Kv4AttnArgs {
   long long slot_rows;
   float scale, softcap;
   void* out;
-  float2* ml;   // [rows][splits] running maximum (log2 units) and sum of a split
-  float* acc;   // [rows][splits][d] its unnormalised output
-  int chunk, splits;  // positions per split
+  int batch, row_tiles;  // row_tiles: tiles of 8 or 16 query rows per kv head
+  int ctas;              // grid of the attention kernel
+  float2* ml;            // [ctas][2][rows of a tile] running maximum (log2 units) and sum of a partial unit
+  float* acc;            // [ctas][2][rows of a tile][d] its unnormalised output
 };
 
 constexpr int kKv4Warps = 4;
-constexpr int kKv4Tile = 16;           // positions per warp step
+constexpr int kKv4Tile = 16;                      // positions per warp step
+constexpr int kKv4Block = kKv4Warps * kKv4Tile;   // positions per block of work
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -84,8 +92,51 @@ struct Kv4Tile {
   uint32_t kp[2][G], vp[2][G];
 };
 
+// The line of work: sequence b has blocks(b) blocks of 64 positions in each of its units, at least one (a
+// unit that sees nothing still writes its zeros).
+CCUT_DEVICE int kv4_seen(const Kv4AttnArgs& a, int b) {  // positions its last query sees
+  const int slot = a.slots[b], start = a.starts[b];
+  return slot >= 0 && slot < a.num_slots && start >= 0 ? min(a.kv_len, min(start, a.kv_len) + a.seq) : 0;
+}
+CCUT_DEVICE int kv4_blocks(int seen) { return max(1, (seen + kKv4Block - 1) / kKv4Block); }
+// Whole warp.  Blocks of all sequences (times units: the length of the line).
+CCUT_DEVICE long long kv4_total(const Kv4AttnArgs& a, int lane) {
+  unsigned n = 0;  // kv_len / 64 x batch fits: both are bounded at launch
+  for (int b = lane; b < a.batch; b += 32) n += kv4_blocks(kv4_seen(a, b));
+  return (long long)__reduce_add_sync(0xffffffffu, n) * a.kv_heads * a.row_tiles;
+}
+// Whole warp.  The sequence at place `at` of the line, and the place of its first block.
+CCUT_DEVICE int kv4_find(const Kv4AttnArgs& a, int lane, long long at, long long& first) {
+  const long long units = (long long)a.kv_heads * a.row_tiles;
+  long long base = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 32) {
+    const int n = b0 + lane < a.batch ? kv4_blocks(kv4_seen(a, b0 + lane)) : 0;
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += v;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, base + sum * units > at);
+    if (past) {
+      const int w = __ffs(past) - 1;
+      first = base + (long long)__shfl_sync(0xffffffffu, sum - n, w) * units;
+      return b0 + w;
+    }
+    base += (long long)__shfl_sync(0xffffffffu, sum, 31) * units;
+  }
+  first = base;
+  return a.batch;  // not reached for places on the line
+}
+// First place of span i of n, and the span that holds a place.
+CCUT_DEVICE long long kv4_span(long long total, int n, int i) { return total * i / n; }
+CCUT_DEVICE int kv4_span_of(long long total, int n, long long at) { return (int)(((at + 1) * n - 1) / total); }
+
+template <int D, int NT>
+constexpr int kKv4Resident = D == 64 ? (NT == 1 ? 5 : 3) : (NT == 1 ? 3 : 2);  // CTAs per SM, by registers
+
 template <int D, int NT, bool OUT_BF16>
-__global__ void __launch_bounds__(kKv4Warps * 32) kv4_attn_kernel(Kv4AttnArgs a) {
+__global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_kernel(Kv4AttnArgs a) {
   pdl_wait();
   pdl_trigger();
   constexpr int G = D / kKv4Group;
@@ -95,17 +146,27 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_attn_kernel(Kv4AttnArgs a)
   __shared__ float sm_m[kKv4Warps][kRows], sm_l[kKv4Warps][kRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int grp = a.heads / a.kv_heads, nrows = grp * a.seq;
-  const int b = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads;
-  const int r0 = blockIdx.x * kRows;
-  const int slot = a.slots[b];
-  int start = min(a.starts[b], a.kv_len);
-  const bool valid = slot >= 0 && slot < a.num_slots && start >= 0;
+  const long long total = kv4_total(a, lane);
+  const int spans = (int)min((long long)a.ctas, total);
+  if ((int)blockIdx.x >= spans) return;
+  const long long begin = kv4_span(total, spans, blockIdx.x), end = kv4_span(total, spans, blockIdx.x + 1);
+  long long first;
+  int b = kv4_find(a, lane, begin, first);
+  long long at = begin;
+
+  while (at < end) {
+  const int seen = kv4_seen(a, b), nblocks = kv4_blocks(seen);
+  const int unit = (int)((at - first) / nblocks), block0 = (int)((at - first) % nblocks);
+  const int block1 = (int)min((long long)nblocks, block0 + (end - at));
+  const bool whole_unit = block0 == 0 && block1 == nblocks;
+  const int part = blockIdx.x * 2 + (at != begin);
+  const int kvh = unit % a.kv_heads, r0 = unit / a.kv_heads * kRows;
+  const int start = min(a.starts[b], a.kv_len);
   const int last_row = min(nrows, r0 + kRows) - 1;
-  const int k0 = blockIdx.z * a.chunk;
-  // positions any row of this CTA sees in this split
-  int k1 = valid ? min(min(a.kv_len, k0 + a.chunk), start + last_row / grp + 1) : 0;
-  if (a.splits > 1 && k1 <= k0) return;  // the merge kernel does not read a split that sees nothing
-  const size_t row_base = valid ? (size_t)slot * (size_t)a.slot_rows + (size_t)kvh * a.max_len : 0;
+  const int k0 = block0 * kKv4Block;
+  // positions any row of this tile sees in this segment
+  const int k1 = seen > 0 ? min(min(seen, block1 * kKv4Block), start + last_row / grp + 1) : 0;
+  const size_t row_base = seen > 0 ? (size_t)a.slots[b] * (size_t)a.slot_rows + (size_t)kvh * a.max_len : 0;
 
   // ---- the query rows as B fragments (row n = g of n-tile nt; features t * 16 .. of each group) ----
   uint32_t qf[NT][G][4][2], qm[NT];  // qm: sum q_g of the groups, high parts in lanes t = 0, the rest in t = 1
@@ -185,8 +246,9 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_attn_kernel(Kv4AttnArgs a)
   const uint8_t* kp = reinterpret_cast<const uint8_t*>(a.kp) + (row_base + k0 + g) * (4 * G);
   const uint8_t* vp = reinterpret_cast<const uint8_t*>(a.vp) + (row_base + k0 + g) * (4 * G);
 
-  // the tile at the lane addresses; kChecked: `left` positions from its first, the others come as zeros
-  auto load = [&](Kv4Tile<G>& x, auto checked, int left) {
+  // the k / v half of a tile at the lane addresses, which then move on to the warp's next tile; kChecked:
+  // `left` positions from the tile's first, the others come as zeros
+  auto load_k = [&](Kv4Tile<G>& x, auto checked, int left) {
     constexpr bool kChecked = decltype(checked)::value;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -195,14 +257,17 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_attn_kernel(Kv4AttnArgs a)
       for (int gr = 0; gr < G; ++gr)
         x.k[h][gr] = in ? __ldg(reinterpret_cast<const uint2*>(kc + h * 8 * (D / 2) + gr * 32)) : make_uint2(0, 0);
       if constexpr (G == 2) {
-        const uint2 uk = in ? __ldg(reinterpret_cast<const uint2*>(kp + h * 64)) : make_uint2(0, 0);
-        const uint2 uv = in ? __ldg(reinterpret_cast<const uint2*>(vp + h * 64)) : make_uint2(0, 0);
-        x.kp[h][0] = uk.x, x.kp[h][G - 1] = uk.y, x.vp[h][0] = uv.x, x.vp[h][G - 1] = uv.y;
+        const uint2 u = in ? __ldg(reinterpret_cast<const uint2*>(kp + h * 64)) : make_uint2(0, 0);
+        x.kp[h][0] = u.x, x.kp[h][G - 1] = u.y;
       } else {
         x.kp[h][0] = in ? __ldg(reinterpret_cast<const uint32_t*>(kp + h * 32)) : 0u;
-        x.vp[h][0] = in ? __ldg(reinterpret_cast<const uint32_t*>(vp + h * 32)) : 0u;
       }
     }
+    kc += kKv4Warps * kKv4Tile * (D / 2);
+    kp += kKv4Warps * kKv4Tile * 4 * G;
+  };
+  auto load_v = [&](Kv4Tile<G>& x, auto checked, int left) {
+    constexpr bool kChecked = decltype(checked)::value;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int p = (i & 1) + 8 * (i >> 1);
@@ -211,15 +276,22 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_attn_kernel(Kv4AttnArgs a)
       for (int gr = 0; gr < G; ++gr)
         x.v[i][gr] = in ? __ldg(reinterpret_cast<const uint32_t*>(vc + p * (D / 2) + gr * 32)) : 0u;
     }
-  };
-  auto advance = [&](int tiles) {
-    kc += (long long)tiles * (kKv4Tile * (D / 2));
-    vc += (long long)tiles * (kKv4Tile * (D / 2));
-    kp += (long long)tiles * (kKv4Tile * 4 * G);
-    vp += (long long)tiles * (kKv4Tile * 4 * G);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bool in = !kChecked || g + 8 * h < left;
+      if constexpr (G == 2) {
+        const uint2 u = in ? __ldg(reinterpret_cast<const uint2*>(vp + h * 64)) : make_uint2(0, 0);
+        x.vp[h][0] = u.x, x.vp[h][G - 1] = u.y;
+      } else {
+        x.vp[h][0] = in ? __ldg(reinterpret_cast<const uint32_t*>(vp + h * 32)) : 0u;
+      }
+    }
+    vc += kKv4Warps * kKv4Tile * (D / 2);
+    vp += kKv4Warps * kKv4Tile * 4 * G;
   };
 
-  auto step = [&](const Kv4Tile<G>& x, int p0, auto masked_tag) {
+  // one tile; `more`: the tile two steps on is loaded into x, each half as soon as x's own is used up
+  auto step = [&](Kv4Tile<G>& x, int p0, auto masked_tag, bool more) {
     constexpr bool kMasked = decltype(masked_tag)::value;
     float sc[NT][4];
     {
@@ -255,6 +327,8 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_attn_kernel(Kv4AttnArgs a)
 #pragma unroll
         for (int i = 0; i < 4; ++i) sc[nt][i] = fmaf(s[i >> 1], c4[nt][i], sc[nt][i]);  // row g + 8 (i >> 1), column 2t + (i & 1)
     }
+    if constexpr (!kMasked)
+      if (more) load_k(x, std::false_type{}, 0);
     bool vis[NT][4];
     bool need = false;
 #pragma unroll
@@ -358,25 +432,31 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_attn_kernel(Kv4AttnArgs a)
         }
       }
     }
+    if constexpr (!kMasked)
+      if (more) load_v(x, std::false_type{}, 0);
   };
 
   // tiles of this warp: j, j + 4, ..; the first `whole` of the split are seen in whole by every row
   const int ntiles = k1 > k0 ? (k1 - k0 + kKv4Tile - 1) / kKv4Tile : 0;
   const int whole = k1 > k0 ? max(0, min(k1, start + r0 / grp + 1) - k0) / kKv4Tile : 0;
   int j = warp;
-  advance(warp);
+  kc += warp * kKv4Tile * (D / 2);
+  vc += warp * kKv4Tile * (D / 2);
+  kp += warp * kKv4Tile * 4 * G;
+  vp += warp * kKv4Tile * 4 * G;
   if (j < whole) {
     Kv4Tile<G> x, y;
-    load(x, std::false_type{}, 0);
-    while (true) {  // one tile in flight while the other is worked on
-      advance(kKv4Warps);
-      if (j + kKv4Warps < whole) load(y, std::false_type{}, 0);
-      step(x, 0, std::false_type{});
+    load_k(x, std::false_type{}, 0);
+    load_v(x, std::false_type{}, 0);
+    if (j + kKv4Warps < whole) {
+      load_k(y, std::false_type{}, 0);
+      load_v(y, std::false_type{}, 0);
+    }
+    while (true) {
+      step(x, 0, std::false_type{}, j + 2 * kKv4Warps < whole);
       j += kKv4Warps;
       if (j >= whole) break;
-      advance(kKv4Warps);
-      if (j + kKv4Warps < whole) load(x, std::false_type{}, 0);
-      step(y, 0, std::false_type{});
+      step(y, 0, std::false_type{}, j + 2 * kKv4Warps < whole);
       j += kKv4Warps;
       if (j >= whole) break;
     }
@@ -384,9 +464,9 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_attn_kernel(Kv4AttnArgs a)
   for (; j < ntiles; j += kKv4Warps) {
     Kv4Tile<G> x;
     const int p0 = k0 + j * kKv4Tile;
-    load(x, std::true_type{}, k1 - p0);
-    advance(kKv4Warps);
-    step(x, p0, std::true_type{});
+    load_k(x, std::true_type{}, k1 - p0);
+    load_v(x, std::true_type{}, k1 - p0);
+    step(x, p0, std::true_type{}, false);
   }
 
   // ---- join the warps: rows 2t + c of n-tile nt, features 8 g + {0..7} of each group -----------------
@@ -427,46 +507,69 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_attn_kernel(Kv4AttnArgs a)
       L = fmaf(sm_l[w][n], f, L);
       v = fmaf(sm_o[w][n][d], f, v);
     }
-    const size_t row = ((size_t)b * a.heads + kvh * grp + r % grp) * a.seq + r / grp;
-    if (a.splits > 1) {
-      if (d == 0) a.ml[row * a.splits + blockIdx.z] = make_float2(M, L);
-      a.acc[(row * a.splits + blockIdx.z) * D + d] = v;
+    if (!whole_unit) {
+      if (d == 0) a.ml[part * kRows + n] = make_float2(M, L);
+      a.acc[((size_t)part * kRows + n) * D + d] = v;
     } else {
+      const size_t row = ((size_t)b * a.heads + kvh * grp + r % grp) * a.seq + r / grp;
       v = L == 0.f ? 0.f : v / L;
       if constexpr (OUT_BF16) static_cast<__nv_bfloat16*>(a.out)[row * D + d] = __float2bfloat16_rn(v);
       else static_cast<float*>(a.out)[row * D + d] = v;
     }
   }
+  at += block1 - block0;
+  if (at < end) {
+    if (at >= first + (long long)nblocks * a.kv_heads * a.row_tiles) {
+      first = at;
+      ++b;
+    }
+    __syncthreads();  // the join's shared memory is used again
+  }
+  }
 }
 
-// Merge of the splits of one query row per CTA: warp w takes splits w, w + 4, .., each lane D / 32 features;
-// the four sums are added in warp order.
-template <int D, bool OUT_BF16>
-__global__ void __launch_bounds__(128) kv4_merge_kernel(Kv4AttnArgs a) {
+// Joins the partial results of one query row per CTA (none: the row was finished by its span): warp w takes
+// spans w, w + 8, .. of the row's unit, each lane D / 32 features; the eight sums are added in warp order.
+template <int D, int NT, bool OUT_BF16>
+__global__ void __launch_bounds__(256) kv4_merge_kernel(Kv4AttnArgs a) {
   pdl_wait();
   pdl_trigger();
-  constexpr int E = D / 32;
-  __shared__ float so[4][D], sl[4];
+  constexpr int E = D / 32, kRows = 8 * NT;
+  __shared__ float so[8][D], sl[8];
   const long long row = blockIdx.x;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int i = (int)(row % a.seq), b = (int)(row / a.seq / a.heads);
-  const int slot = a.slots[b], start = min(a.starts[b], a.kv_len);
-  // the splits that the CTA of this row had work in: up to the last row of the row's tile
-  const int n = slot >= 0 && slot < a.num_slots && start >= 0 ? min(a.kv_len, start + i + 1) : 0;
-  const int splits = (n + a.chunk - 1) / a.chunk;
-  const float2* ml = a.ml + row * a.splits;
+  const int i = (int)(row % a.seq), b = (int)(row / a.seq / a.heads), h = (int)(row / a.seq % a.heads);
+  const int grp = a.heads / a.kv_heads, r = i * grp + h % grp;
+  unsigned all = 0, before = 0;
+  for (int j = lane; j < a.batch; j += 32) {
+    const int n = kv4_blocks(kv4_seen(a, j));
+    all += n;
+    before += j < b ? n : 0;
+  }
+  const long long units = (long long)a.kv_heads * a.row_tiles;
+  const long long total = __reduce_add_sync(0xffffffffu, all) * units;
+  const int nblocks = kv4_blocks(kv4_seen(a, b));
+  const long long first = __reduce_add_sync(0xffffffffu, before) * units +
+                          ((long long)(r / kRows) * a.kv_heads + h / grp) * nblocks;
+  const int spans = (int)min((long long)a.ctas, total);
+  const int c0 = kv4_span_of(total, spans, first), c1 = kv4_span_of(total, spans, first + nblocks - 1);
+  if (c0 == c1) return;
+  // in span c0 the unit comes after others (partial result 1) unless it begins the span; in the rest it begins it
+  const bool late = kv4_span(total, spans, c0) < first;
+  const float2* ml = a.ml + r % kRows;
   float M = -INFINITY;
-  for (int s = lane; s < splits; s += 32) M = fmaxf(M, ml[s].x);
+  for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, ml[(2 * c + (late && c == c0)) * kRows].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
   const float Mu = M == -INFINITY ? 0.f : M;
   float L = 0.f, v[E] = {};
 #pragma unroll 4
-  for (int s = warp; s < splits; s += 4) {
-    const float2 x = ml[s];
+  for (int c = c0 + warp; c <= c1; c += 8) {
+    const int part = 2 * c + (late && c == c0);
+    const float2 x = ml[part * kRows];
     const float f = ex2(x.x - Mu);
     L = fmaf(x.y, f, L);
-    const float* p = a.acc + (row * a.splits + s) * D + lane * E;
+    const float* p = a.acc + ((size_t)part * kRows + r % kRows) * D + lane * E;
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = fmaf(p[e], f, v[e]);
   }
@@ -476,35 +579,37 @@ __global__ void __launch_bounds__(128) kv4_merge_kernel(Kv4AttnArgs a) {
   __syncthreads();
   if (threadIdx.x < D) {
     const int d = threadIdx.x;
-    L = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-    const float s = (so[0][d] + so[1][d]) + (so[2][d] + so[3][d]);
+    float s = 0.f;
+    L = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) L += sl[w], s += so[w][d];
     const float y = L == 0.f ? 0.f : s / L;
     if constexpr (OUT_BF16) static_cast<__nv_bfloat16*>(a.out)[row * D + d] = __float2bfloat16_rn(y);
     else static_cast<float*>(a.out)[row * D + d] = y;
   }
 }
 
-// Positions per split.  Enough CTAs for four rounds of four CTAs an SM, so that uneven lengths and the
-// last round cost little, and at least one tile per warp; no split where the rows fill the GPU.
-static int kv4_chunk(int batch, int heads, int kv_heads, int seq, int kv_len) {
-  const long rows = (long)(heads / kv_heads) * seq, per = rows <= 8 ? 8 : 16;
-  const long units = (long)batch * kv_heads * ((rows + per - 1) / per);
-  const long target = 4L * 4 * 148, least = kKv4Warps * kKv4Tile;
-  if (kv_len <= least || units >= target / 2) return kv_len > 0 ? kv_len : 1;
-  long chunk = (units * kv_len + target - 1) / target;
-  chunk = (chunk + least - 1) / least * least;
-  return (int)(chunk < kv_len ? chunk : kv_len);
+// Query rows per tile: 8 where a kv head has no more, else 16.
+static int kv4_rows(int heads, int kv_heads, int seq) { return (long)(heads / kv_heads) * seq <= 8 ? 8 : 16; }
+static long long kv4_row_tiles(int heads, int kv_heads, int seq) {
+  const long long rows = (long long)(heads / kv_heads) * seq, per = kv4_rows(heads, kv_heads, seq);
+  return (rows + per - 1) / per;
+}
+// One resident round, or one block each where there are fewer.
+static int kv4_ctas(int batch, int heads, int kv_heads, int seq, int kv_len, int head_dim) {
+  const bool one = kv4_rows(heads, kv_heads, seq) == 8;
+  const int most = 148 * (head_dim == 64 ? (one ? kKv4Resident<64, 1> : kKv4Resident<64, 2>)
+                                         : (one ? kKv4Resident<128, 1> : kKv4Resident<128, 2>));
+  const long long blocks = kv_len > 0 ? (kv_len + kKv4Block - 1) / kKv4Block : 1;
+  const long long n = kv4_row_tiles(heads, kv_heads, seq) * kv_heads * batch;
+  return n >= most || n * blocks >= most ? most : (int)(n * blocks);
 }
 
-template <int D, bool OB>
-static int run_kv4_attention(Kv4AttnArgs a, int batch, cudaStream_t st) {
-  const long rows = (long)(a.heads / a.kv_heads) * a.seq;
-  const int per = rows <= 8 ? 8 : 16;
-  const dim3 grid((unsigned)((rows + per - 1) / per), batch * a.kv_heads, a.splits);
-  auto kern = per == 8 ? kv4_attn_kernel<D, 1, OB> : kv4_attn_kernel<D, 2, OB>;
-  int rc = launch_k(kern, grid, dim3(kKv4Warps * 32), 0, st, a);
-  if (rc || a.splits == 1) return rc;
-  return launch_k(kv4_merge_kernel<D, OB>, dim3((unsigned)((long)batch * a.heads * a.seq)), dim3(128), 0, st, a);
+template <int D, int NT, bool OB>
+static int run_kv4_attention(const Kv4AttnArgs& a, cudaStream_t st) {
+  int rc = launch_k(kv4_attn_kernel<D, NT, OB>, dim3(a.ctas), dim3(kKv4Warps * 32), 0, st, a);
+  if (rc || a.kv_len <= kKv4Block) return rc;  // one block a unit: no unit is cut
+  return launch_k(kv4_merge_kernel<D, NT, OB>, dim3((unsigned)((long)a.batch * a.heads * a.seq)), dim3(256), 0, st, a);
 }
 
 }  // namespace ccut
@@ -517,11 +622,9 @@ size_t ccut_kv4_attention_workspace_bytes(int batch, int heads, int kv_heads, in
   if (batch < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || seq < 0 || kv_len < 0 ||
       (head_dim != 64 && head_dim != 128))
     return 0;
-  if (batch == 0 || seq == 0 || kv_len == 0) return 256;
-  const int chunk = kv4_chunk(batch, heads, kv_heads, seq, kv_len);
-  const size_t sp = (kv_len + chunk - 1) / chunk;
-  if (sp <= 1) return 256;
-  return 256 + sp * batch * heads * seq * (head_dim + 2) * sizeof(float);
+  if (batch == 0 || seq == 0 || kv_len <= kKv4Block) return 256;
+  return 256 + (size_t)kv4_ctas(batch, heads, kv_heads, seq, kv_len, head_dim) * 2 * kv4_rows(heads, kv_heads, seq) *
+                   (head_dim + 2) * sizeof(float);
 }
 
 int ccut_kv4_attention(const uint16_t* q, const uint8_t* k_codes, const uint16_t* k_params, const uint8_t* v_codes,
@@ -541,24 +644,29 @@ int ccut_kv4_attention(const uint16_t* q, const uint8_t* k_codes, const uint16_t
   if (misaligned(q, 16) || misaligned(k_codes, 16) || misaligned(v_codes, 16) || misaligned(k_params, head_dim / 16) ||
       misaligned(v_params, head_dim / 16) || misaligned(out, 16) || misaligned(workspace, 16))
     return CCUT_ERR_INVALID;
-  const long long rows = (long long)batch * heads * seq;
-  if (rows > 2147483647LL || (long long)batch * kv_heads > 65535) return CCUT_ERR_UNSUPPORTED;
+  // rows in a grid; blocks of all sequences in 32 bits
+  if ((long long)batch * heads * seq > 2147483647LL ||
+      (long long)batch * ((long long)kv_len / kKv4Block + 1) > 2147483647LL)
+    return CCUT_ERR_UNSUPPORTED;
   const size_t need = ccut_kv4_attention_workspace_bytes(batch, heads, kv_heads, seq, kv_len, head_dim);
   if (need > 256 && (!workspace || ws_bytes < need)) return CCUT_ERR_WORKSPACE;
   if (!(scale > 0.f)) scale = 1.f / sqrtf((float)head_dim);
-  const int chunk = kv4_chunk(batch, heads, kv_heads, seq, kv_len);
   Kv4AttnArgs a{q, k_codes, reinterpret_cast<const __half2*>(k_params), v_codes,
                 reinterpret_cast<const __half2*>(v_params), slots, starts, heads, kv_heads, seq, max_len, kv_len,
-                num_slots, slot_rows, scale, softcap, out, nullptr, nullptr, chunk,
-                kv_len > 0 ? (kv_len + chunk - 1) / chunk : 1};
-  if (a.splits > 1) {
+                num_slots, slot_rows, scale, softcap, out, batch, (int)kv4_row_tiles(heads, kv_heads, seq),
+                kv4_ctas(batch, heads, kv_heads, seq, kv_len, head_dim), nullptr, nullptr};
+  const int rows = kv4_rows(heads, kv_heads, seq);
+  if (need > 256) {
     a.ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + 256);
-    a.acc = reinterpret_cast<float*>(a.ml + (size_t)rows * a.splits);
+    a.acc = reinterpret_cast<float*>(a.ml + (size_t)a.ctas * 2 * rows);
   }
-  const bool ob = out_dtype == CCUT_OUT_BF16;
-  if (head_dim == 128)
-    return ob ? run_kv4_attention<128, true>(a, batch, stream) : run_kv4_attention<128, false>(a, batch, stream);
-  return ob ? run_kv4_attention<64, true>(a, batch, stream) : run_kv4_attention<64, false>(a, batch, stream);
+  const bool ob = out_dtype == CCUT_OUT_BF16, d128 = head_dim == 128;
+  if (rows == 8) {
+    if (d128) return ob ? run_kv4_attention<128, 1, true>(a, stream) : run_kv4_attention<128, 1, false>(a, stream);
+    return ob ? run_kv4_attention<64, 1, true>(a, stream) : run_kv4_attention<64, 1, false>(a, stream);
+  }
+  if (d128) return ob ? run_kv4_attention<128, 2, true>(a, stream) : run_kv4_attention<128, 2, false>(a, stream);
+  return ob ? run_kv4_attention<64, 2, true>(a, stream) : run_kv4_attention<64, 2, false>(a, stream);
 }
 
 }  // extern "C"
