@@ -14,13 +14,17 @@
 //   x = sum_g s_g (q_g . c_g) + m_g (sum q_g),  o = sum_j (p_j s_jg) c_j + (sum_j p_j m_jg),
 //   the minima of k by one more MMA (their fp16 pairs times sum q_g in two fp16 parts).
 // - Positions are the M of m16n8k16, the query rows of a kv head the N: 8 rows take half the MMAs
-//   they would take as the M.  The order of the k index is free, so lanes load their operands straight
-//   from global memory (8 bytes of 8 rows of k, 4 bytes of 4 rows of v a lane, full 32-byte sectors),
-//   no shared memory, and the scores' accumulators become the second product's operand by movmatrix.
+//   they would take as the M.  The order of the k index is free, so a lane's operands are the next
+//   bytes of a cache row (no ldmatrix), and the scores' accumulators become the second product's operand
+//   by movmatrix.
+// - Each warp streams its own tiles of 16 positions through a four-deep cp.async ring, with no barrier
+//   between warps; 32-byte units are placed so that the reads of both operands touch every bank once.
+//   (Prefetching into registers instead took 168 of them, three CTAs an SM, and 67 us where this takes
+//   TIME_RING.)
 // - The running maximum moves only when a score passes it by 2^8 (one vote a tile instead of
 //   six shuffles a row pair): probabilities stay below 2^8, and fp16's range has room for that.
-// - Tiles that every row sees in whole run without bounds or mask tests, four pointers advancing by
-//   constant strides; the few others (the last tile, the diagonal of a query block) run a checked copy.
+// - Tiles that every row sees in whole run without mask tests; the few others (the last tile, the diagonal
+//   of a query block) run a masked copy.
 // - Work is cut evenly whatever the lengths: the blocks of 64 positions of all (sequence, tile of query
 //   rows, kv head) units form one line, found from starts on the device, and each CTA of one resident
 //   round takes an equal span of it.  A unit inside one span is finished there; of the others a span
@@ -82,15 +86,40 @@ CCUT_DEVICE float high_f16(uint32_t u) { return __high2float(as_half2(u)); }
 CCUT_DEVICE float pow2f(int e) { return __int_as_float((e + 127) << 23); }
 CCUT_DEVICE int exponent_of(float x) { return (int)((__float_as_uint(x) >> 23) & 255) - 127; }
 
-// One 16-position tile of a warp as it comes from memory: lane (g, t) holds of k 16 features (8 bytes) per
-// group of rows g and g + 8, of v 8 features (4 bytes) per group of rows 2t, 2t + 1, 2t + 8, 2t + 9,
-// and the (scale, minimum) pairs of rows g and g + 8.
-template <int G>
-struct Kv4Tile {
-  uint2 k[2][G];
-  uint32_t v[4][G];
-  uint32_t kp[2][G], vp[2][G];
+// A warp's 16 positions in shared memory: k codes, v codes (32-byte units, see the placements), then the
+// (scale, minimum) pairs of k and of v.
+template <int D>
+struct Kv4Stage {
+  static constexpr int kCodes = kKv4Tile * D / 2, kParams = kKv4Tile * D / 16;
+  static constexpr int kBytes = 2 * kCodes + 2 * kParams;
 };
+constexpr int kKv4Stages = 4;
+// Row i of the MMAs' M (scores) and k (values) index is position kv4_row(i) of the tile: lane t then reads v at
+// positions t, t + 4, t + 8, t + 12, four different bank groups for the four t.
+CCUT_DEVICE int kv4_row(int i) { return ((i >> 1) & 3) + 4 * (i & 1) + (i & 8); }
+// Byte offset of 32-byte unit `gr` (its group) of position r: lanes that read one unit each of positions
+// {0, 1, 2, 3}, {4, .., 7} (v) or {0, 4, 1, 5}, {2, 6, 3, 7} (k, half a warp) meet every bank once.
+template <int D>
+CCUT_DEVICE int kv4_unit(int r, int gr) {
+  if constexpr (D == 128) return r * 64 + ((gr ^ (((r >> 1) ^ (r >> 2)) & 1)) * 32);
+  else return (r ^ ((r >> 1) & 2)) * 32;
+}
+// cp.async of N (16, 8 or 4) bytes to shared address `to`; kChecked: zeros when !in
+template <int N, bool kChecked>
+CCUT_DEVICE void copy_in(uint32_t to, const uint8_t* from, bool in) {
+  if constexpr (N == 16) {
+    if constexpr (kChecked)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(in ? 16 : 0) : "memory");
+    else
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+  } else {
+    if constexpr (kChecked)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(to), "l"(from), "r"(in ? N : 0), "n"(N)
+                   : "memory");
+    else
+      asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(N) : "memory");
+  }
+}
 
 // The line of work: sequence b has blocks(b) blocks of 64 positions in each of its units, at least one (a
 // unit that sees nothing still writes its zeros).
@@ -133,7 +162,7 @@ CCUT_DEVICE long long kv4_span(long long total, int n, int i) { return total * i
 CCUT_DEVICE int kv4_span_of(long long total, int n, long long at) { return (int)(((at + 1) * n - 1) / total); }
 
 template <int D, int NT>
-constexpr int kKv4Resident = D == 64 ? (NT == 1 ? 5 : 3) : (NT == 1 ? 3 : 2);  // CTAs per SM, by registers
+constexpr int kKv4Resident = D == 64 ? (NT == 1 ? 6 : 4) : (NT == 1 ? 4 : 2);  // CTAs per SM, by registers
 
 template <int D, int NT, bool OUT_BF16>
 __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_kernel(Kv4AttnArgs a) {
@@ -142,7 +171,10 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
   constexpr int G = D / kKv4Group;
   constexpr int kRows = 8 * NT;
   constexpr uint32_t M0 = 0x000F000Fu, M1 = 0x00F000F0u;
-  __shared__ float sm_o[kKv4Warps][kRows][D + 4];
+  using St = Kv4Stage<D>;
+  constexpr int kRing = kKv4Warps * kKv4Stages * St::kBytes, kJoin = kKv4Warps * kRows * (D + 4) * 4;
+  __shared__ __align__(16) uint8_t smem[kRing > kJoin ? kRing : kJoin];  // the ring, then the warps' outputs
+  float(*sm_o)[kRows][D + 4] = reinterpret_cast<float(*)[kRows][D + 4]>(smem);
   __shared__ float sm_m[kKv4Warps][kRows], sm_l[kKv4Warps][kRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int grp = a.heads / a.kv_heads, nrows = grp * a.seq;
@@ -240,63 +272,61 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
       for (int i = 0; i < 4; ++i) o[nt][mt][i] = 0.f;
   }
 
-  // lane addresses at position k0
-  const uint8_t* kc = a.kc + (row_base + k0 + g) * (D / 2) + t * 8;
-  const uint8_t* vc = a.vc + (row_base + k0 + 2 * t) * (D / 2) + g * 4;
-  const uint8_t* kp = reinterpret_cast<const uint8_t*>(a.kp) + (row_base + k0 + g) * (4 * G);
-  const uint8_t* vp = reinterpret_cast<const uint8_t*>(a.vp) + (row_base + k0 + g) * (4 * G);
+  // This lane's part of a tile: 16-byte chunks `lane` and, of 128 features, `lane` + 32 (8 positions further)
+  // of the codes, and position lane % 16's pair(s) of k or of v.  The addresses move from one tile of
+  // the warp to its next; positions at or past k1 come as zeros.
+  const uint8_t* ring = smem + warp * kKv4Stages * St::kBytes;
+  constexpr int kPer = D / 32;  // chunks per position
+  const int cr = lane / kPer, first_tile = (k0 + warp * kKv4Tile);
+  const uint32_t to_codes = smem_u32(ring) + kv4_unit<D>(cr, lane % kPer >> 1) + (lane & 1) * 16;
+  const uint32_t to_params = smem_u32(ring) + 2 * St::kCodes + lane * (D / 16);
+  const uint8_t* kc = a.kc + (row_base + first_tile) * (D / 2) + lane * 16;
+  const uint8_t* vc = a.vc + (row_base + first_tile) * (D / 2) + lane * 16;
+  const uint8_t* pp =
+      reinterpret_cast<const uint8_t*>(lane < 16 ? a.kp : a.vp) + (row_base + first_tile + (lane & 15)) * (D / 16);
+  auto copy_tile = [&](uint32_t stage, int left, auto checked) {
+    constexpr bool kC = decltype(checked)::value;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      const bool in = cr + 8 * i < left;
 
-  // the k / v half of a tile at the lane addresses, which then move on to the warp's next tile; kChecked:
-  // `left` positions from the tile's first, the others come as zeros
-  auto load_k = [&](Kv4Tile<G>& x, auto checked, int left) {
-    constexpr bool kChecked = decltype(checked)::value;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const bool in = !kChecked || g + 8 * h < left;
-#pragma unroll
-      for (int gr = 0; gr < G; ++gr)
-        x.k[h][gr] = in ? __ldg(reinterpret_cast<const uint2*>(kc + h * 8 * (D / 2) + gr * 32)) : make_uint2(0, 0);
-      if constexpr (G == 2) {
-        const uint2 u = in ? __ldg(reinterpret_cast<const uint2*>(kp + h * 64)) : make_uint2(0, 0);
-        x.kp[h][0] = u.x, x.kp[h][G - 1] = u.y;
-      } else {
-        x.kp[h][0] = in ? __ldg(reinterpret_cast<const uint32_t*>(kp + h * 32)) : 0u;
-      }
+      copy_in<16, kC>(to_codes + stage + i * 512, kC && !in ? a.kc : kc + i * 512, in);
+      copy_in<16, kC>(to_codes + stage + St::kCodes + i * 512, kC && !in ? a.vc : vc + i * 512, in);
     }
-    kc += kKv4Warps * kKv4Tile * (D / 2);
-    kp += kKv4Warps * kKv4Tile * 4 * G;
+    const bool in = (lane & 15) < left;
+    copy_in<D / 16, kC>(to_params + stage, kC && !in ? reinterpret_cast<const uint8_t*>(a.kp) : pp, in);
+    kc += kKv4Block * (D / 2);
+    vc += kKv4Block * (D / 2);
+    pp += kKv4Block * (D / 16);
   };
-  auto load_v = [&](Kv4Tile<G>& x, auto checked, int left) {
-    constexpr bool kChecked = decltype(checked)::value;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int p = (i & 1) + 8 * (i >> 1);
-      const bool in = !kChecked || 2 * t + p < left;
-#pragma unroll
-      for (int gr = 0; gr < G; ++gr)
-        x.v[i][gr] = in ? __ldg(reinterpret_cast<const uint32_t*>(vc + p * (D / 2) + gr * 32)) : 0u;
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const bool in = !kChecked || g + 8 * h < left;
-      if constexpr (G == 2) {
-        const uint2 u = in ? __ldg(reinterpret_cast<const uint2*>(vp + h * 64)) : make_uint2(0, 0);
-        x.vp[h][0] = u.x, x.vp[h][G - 1] = u.y;
-      } else {
-        x.vp[h][0] = in ? __ldg(reinterpret_cast<const uint32_t*>(vp + h * 32)) : 0u;
-      }
-    }
-    vc += kKv4Warps * kKv4Tile * (D / 2);
-    vp += kKv4Warps * kKv4Tile * 4 * G;
+  auto issue = [&](int tile, int stage) {
+    const int left = k1 - k0 - tile * kKv4Tile;
+    if (left >= kKv4Tile) copy_tile(stage * St::kBytes, left, std::false_type{});
+    else copy_tile(stage * St::kBytes, left, std::true_type{});
   };
+  const int kr = kv4_row(g);                          // this lane's score rows: positions kr and kr + 8
+  const int k_unit[2] = {kv4_unit<D>(kr, 0) + t * 8, kv4_unit<D>(kr, 1) + t * 8};
+  const int v_unit[2][2] = {{kv4_unit<D>(t, 0) + g * 4, kv4_unit<D>(t, 1) + g * 4},
+                            {kv4_unit<D>(t + 4, 0) + g * 4, kv4_unit<D>(t + 4, 1) + g * 4}};
 
-  // one tile; `more`: the tile two steps on is loaded into x, each half as soon as x's own is used up
-  auto step = [&](Kv4Tile<G>& x, int p0, auto masked_tag, bool more) {
+  auto step = [&](const uint8_t* st, int p0, auto masked_tag) {
     constexpr bool kMasked = decltype(masked_tag)::value;
+    uint32_t kpw[2][G], vpw[2][G];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint8_t* p = st + 2 * St::kCodes + (kr + 8 * h) * (D / 16);
+      if constexpr (G == 2) {
+        const uint2 uk = *reinterpret_cast<const uint2*>(p), uv = *reinterpret_cast<const uint2*>(p + St::kParams);
+        kpw[h][0] = uk.x, kpw[h][G - 1] = uk.y, vpw[h][0] = uv.x, vpw[h][G - 1] = uv.y;
+      } else {
+        kpw[h][0] = *reinterpret_cast<const uint32_t*>(p);
+        vpw[h][0] = *reinterpret_cast<const uint32_t*>(p + St::kParams);
+      }
+    }
     float sc[NT][4];
     {
-      const uint32_t f[4] = {G == 2 ? __byte_perm(x.kp[0][0], x.kp[0][G - 1], 0x7632) : x.kp[0][0],
-                             G == 2 ? __byte_perm(x.kp[1][0], x.kp[1][G - 1], 0x7632) : x.kp[1][0], 0u, 0u};
+      const uint32_t f[4] = {G == 2 ? __byte_perm(kpw[0][0], kpw[0][G - 1], 0x7632) : kpw[0][0],
+                             G == 2 ? __byte_perm(kpw[1][0], kpw[1][G - 1], 0x7632) : kpw[1][0], 0u, 0u};
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -311,7 +341,9 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) c4[nt][i] = 0.f;
-      const uint32_t w0[2] = {x.k[0][gr].x, x.k[0][gr].y}, w1[2] = {x.k[1][gr].x, x.k[1][gr].y};
+      const uint2 ka = *reinterpret_cast<const uint2*>(st + k_unit[gr]);
+      const uint2 kb = *reinterpret_cast<const uint2*>(st + k_unit[gr] + 8 * (D / 2));
+      const uint32_t w0[2] = {ka.x, ka.y}, w1[2] = {kb.x, kb.y};
 #pragma unroll
       for (int w = 0; w < 2; ++w)
 #pragma unroll
@@ -321,14 +353,12 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) mma_16816<false>(c4[nt], f, qf[nt][gr][w * 2 + h][0], qf[nt][gr][w * 2 + h][1]);
         }
-      const float s[2] = {low_f16(x.kp[0][gr]), low_f16(x.kp[1][gr])};
+      const float s[2] = {low_f16(kpw[0][gr]), low_f16(kpw[1][gr])};
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) sc[nt][i] = fmaf(s[i >> 1], c4[nt][i], sc[nt][i]);  // row g + 8 (i >> 1), column 2t + (i & 1)
     }
-    if constexpr (!kMasked)
-      if (more) load_k(x, std::false_type{}, 0);
     bool vis[NT][4];
     bool need = false;
 #pragma unroll
@@ -338,14 +368,14 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
         sc[nt][i] *= fr[nt][i & 1];
         if (a.softcap > 0.f) sc[nt][i] = tanhf(sc[nt][i] * (1.f / kLog2e) / a.softcap) * (a.softcap * kLog2e);
         if constexpr (kMasked) {
-          const int p = p0 + g + 8 * (i >> 1);
+          const int p = p0 + kr + 8 * (i >> 1);
           vis[nt][i] = p < k1 && p <= lim[nt][i & 1];
           if (!vis[nt][i]) sc[nt][i] = -INFINITY;
         }
         need |= sc[nt][i] > m[nt][i & 1] + 8.f;
       }
-    __half2 top = __hmax2(as_half2(x.vp[0][0]), as_half2(x.vp[1][0]));
-    if constexpr (G == 2) top = __hmax2(top, __hmax2(as_half2(x.vp[0][G - 1]), as_half2(x.vp[1][G - 1])));
+    __half2 top = __hmax2(as_half2(vpw[0][0]), as_half2(vpw[1][0]));
+    if constexpr (G == 2) top = __hmax2(top, __hmax2(as_half2(vpw[0][G - 1]), as_half2(vpw[1][G - 1])));
     need |= __hgt(__low2half(top), r_inv);
     if (__any_sync(0xffffffffu, need)) {
 #pragma unroll
@@ -391,8 +421,8 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
       }
 #pragma unroll
     for (int gr = 0; gr < G; ++gr) {
-      const float sr[2] = {low_f16(x.vp[0][gr]) * R, low_f16(x.vp[1][gr]) * R};
-      const float mv[2] = {high_f16(x.vp[0][gr]), high_f16(x.vp[1][gr])};
+      const float sr[2] = {low_f16(vpw[0][gr]) * R, low_f16(vpw[1][gr]) * R};
+      const float mv[2] = {high_f16(vpw[0][gr]), high_f16(vpw[1][gr])};
       uint32_t wb[NT][2], wl[NT][2];  // p s_v R as the B operand: high part, and the rest
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -416,10 +446,14 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
           wl[nt][1] = movmatrix_trans(pack_f16(w[2] - b1.x, w[3] - b1.y));
         }
       }
+      uint32_t v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)  // positions t, t + 4, t + 8, t + 12: k indices 2t, 2t + 1, 2t + 8, 2t + 9
+        v[i] = *reinterpret_cast<const uint32_t*>(st + St::kCodes + v_unit[i & 1][gr] + (i >> 1) * 8 * (D / 2));
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const uint32_t sel = half ? 0x7632 : 0x5410;
-        const uint32_t p01 = __byte_perm(x.v[0][gr], x.v[1][gr], sel), p23 = __byte_perm(x.v[2][gr], x.v[3][gr], sel);
+        const uint32_t p01 = __byte_perm(v[0], v[1], sel), p23 = __byte_perm(v[2], v[3], sel);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t u0 = p01 >> (8 * h), u1 = p23 >> (8 * h);
@@ -432,42 +466,29 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
         }
       }
     }
-    if constexpr (!kMasked)
-      if (more) load_v(x, std::false_type{}, 0);
   };
 
-  // tiles of this warp: j, j + 4, ..; the first `whole` of the split are seen in whole by every row
+  // tiles of this warp: warp, warp + 4, ..; the first `whole` of the segment are seen in whole by every row.
+  // One commit group per tile (empty past the end), so that wait_group always means "this tile has landed".
   const int ntiles = k1 > k0 ? (k1 - k0 + kKv4Tile - 1) / kKv4Tile : 0;
   const int whole = k1 > k0 ? max(0, min(k1, start + r0 / grp + 1) - k0) / kKv4Tile : 0;
-  int j = warp;
-  kc += warp * kKv4Tile * (D / 2);
-  vc += warp * kKv4Tile * (D / 2);
-  kp += warp * kKv4Tile * 4 * G;
-  vp += warp * kKv4Tile * 4 * G;
-  if (j < whole) {
-    Kv4Tile<G> x, y;
-    load_k(x, std::false_type{}, 0);
-    load_v(x, std::false_type{}, 0);
-    if (j + kKv4Warps < whole) {
-      load_k(y, std::false_type{}, 0);
-      load_v(y, std::false_type{}, 0);
-    }
-    while (true) {
-      step(x, 0, std::false_type{}, j + 2 * kKv4Warps < whole);
-      j += kKv4Warps;
-      if (j >= whole) break;
-      step(y, 0, std::false_type{}, j + 2 * kKv4Warps < whole);
-      j += kKv4Warps;
-      if (j >= whole) break;
-    }
+#pragma unroll
+  for (int i = 0; i < kKv4Stages - 1; ++i) {
+    if (warp + i * kKv4Warps < ntiles) issue(warp + i * kKv4Warps, i);
+    cp_async_commit();
   }
-  for (; j < ntiles; j += kKv4Warps) {
-    Kv4Tile<G> x;
-    const int p0 = k0 + j * kKv4Tile;
-    load_k(x, std::true_type{}, k1 - p0);
-    load_v(x, std::true_type{}, k1 - p0);
-    step(x, p0, std::true_type{}, false);
+  for (int j = warp, i = 0; j < ntiles; j += kKv4Warps, ++i) {
+    cp_async_wait<kKv4Stages - 2>();
+    __syncwarp();  // every lane's copies of this tile have landed, every lane is done with the tile before
+    const int jn = j + (kKv4Stages - 1) * kKv4Warps;
+    if (jn < ntiles) issue(jn, (i + kKv4Stages - 1) % kKv4Stages);
+    cp_async_commit();
+    const uint8_t* st = ring + i % kKv4Stages * St::kBytes;
+    if (j < whole) step(st, 0, std::false_type{});
+    else step(st, k0 + j * kKv4Tile, std::true_type{});
   }
+  cp_async_wait<0>();
+  __syncthreads();  // the warps' outputs take the ring's place
 
   // ---- join the warps: rows 2t + c of n-tile nt, features 8 g + {0..7} of each group -----------------
 #pragma unroll
