@@ -25,7 +25,7 @@
 //   six shuffles a row pair): probabilities stay below 2^8, and fp16's range has room for that.
 // - Tiles that every row sees in whole run without mask tests; the few others (the last tile, the diagonal
 //   of a query block) run a masked copy.
-// - Work is cut evenly whatever the lengths: the blocks of 64 positions of all (sequence, tile of query
+// - Work is cut evenly whatever the lengths: the blocks of 128 or 64 positions of all (sequence, tile of query
 //   rows, kv head) units form one line, found from starts on the device, and each CTA of one resident
 //   round takes an equal span of it.  A unit inside one span is finished there; of the others a span
 //   leaves at most two partial results (the first and the last of its units), which a second kernel joins.
@@ -60,8 +60,12 @@ struct Kv4AttnArgs {
 };
 
 constexpr int kKv4Warps = 4;
-constexpr int kKv4Tile = 16;                      // positions per warp step
-constexpr int kKv4Block = kKv4Warps * kKv4Tile;   // positions per block of work
+// Positions per warp step: 32 with one n-tile (two independent chains of MMAs and one vote a step), 16 with two
+// (the registers hold no more).
+template <int NT>
+constexpr int kKv4Tile = NT == 1 ? 32 : 16;
+template <int NT>
+constexpr int kKv4Block = kKv4Warps * kKv4Tile<NT>;  // positions per block of work
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -86,15 +90,20 @@ CCUT_DEVICE float high_f16(uint32_t u) { return __high2float(as_half2(u)); }
 CCUT_DEVICE float pow2f(int e) { return __int_as_float((e + 127) << 23); }
 CCUT_DEVICE int exponent_of(float x) { return (int)((__float_as_uint(x) >> 23) & 255) - 127; }
 
-// A warp's 16 positions in shared memory: k codes, v codes (32-byte units, see the placements), then the
-// (scale, minimum) pairs of k and of v.
-template <int D>
+// A warp's tile in shared memory: k codes, v codes (32-byte units, see the placements), then the (scale,
+// minimum) pairs of k and of v.
+template <int D, int NT>
 struct Kv4Stage {
-  static constexpr int kCodes = kKv4Tile * D / 2, kParams = kKv4Tile * D / 16;
+  static constexpr int kCodes = kKv4Tile<NT> * D / 2, kParams = kKv4Tile<NT> * D / 16;
   static constexpr int kBytes = 2 * kCodes + 2 * kParams;
 };
-constexpr int kKv4Stages = 4;
-// Row i of the MMAs' M (scores) and k (values) index is position kv4_row(i) of the tile: lane t then reads v at
+template <int NT>
+constexpr int kKv4Stages = NT == 1 ? 3 : 4;
+template <int D, int NT>
+constexpr int kKv4Smem = kKv4Warps * (kKv4Stages<NT> * Kv4Stage<D, NT>::kBytes > 8 * NT * (D + 4) * 4
+                                          ? kKv4Stages<NT> * Kv4Stage<D, NT>::kBytes
+                                          : 8 * NT * (D + 4) * 4);
+// Row i of the MMAs' M (scores) and k (values) index is position kv4_row(i) of its 16: lane t then reads v at
 // positions t, t + 4, t + 8, t + 12, four different bank groups for the four t.
 CCUT_DEVICE int kv4_row(int i) { return ((i >> 1) & 3) + 4 * (i & 1) + (i & 8); }
 // Byte offset of 32-byte unit `gr` (its group) of position r: lanes that read one unit each of positions
@@ -121,25 +130,30 @@ CCUT_DEVICE void copy_in(uint32_t to, const uint8_t* from, bool in) {
   }
 }
 
-// The line of work: sequence b has blocks(b) blocks of 64 positions in each of its units, at least one (a
+// The line of work: sequence b has kv4_blocks blocks of positions in each of its units, at least one (a
 // unit that sees nothing still writes its zeros).
 CCUT_DEVICE int kv4_seen(const Kv4AttnArgs& a, int b) {  // positions its last query sees
   const int slot = a.slots[b], start = a.starts[b];
   return slot >= 0 && slot < a.num_slots && start >= 0 ? min(a.kv_len, min(start, a.kv_len) + a.seq) : 0;
 }
-CCUT_DEVICE int kv4_blocks(int seen) { return max(1, (seen + kKv4Block - 1) / kKv4Block); }
+template <int NT>
+CCUT_DEVICE int kv4_blocks(int seen) {
+  return max(1, (seen + kKv4Block<NT> - 1) / kKv4Block<NT>);
+}
 // Whole warp.  Blocks of all sequences (times units: the length of the line).
+template <int NT>
 CCUT_DEVICE long long kv4_total(const Kv4AttnArgs& a, int lane) {
-  unsigned n = 0;  // kv_len / 64 x batch fits: both are bounded at launch
-  for (int b = lane; b < a.batch; b += 32) n += kv4_blocks(kv4_seen(a, b));
+  unsigned n = 0;  // fits: kv_len / 64 x batch is bounded at launch
+  for (int b = lane; b < a.batch; b += 32) n += kv4_blocks<NT>(kv4_seen(a, b));
   return (long long)__reduce_add_sync(0xffffffffu, n) * a.kv_heads * a.row_tiles;
 }
 // Whole warp.  The sequence at place `at` of the line, and the place of its first block.
+template <int NT>
 CCUT_DEVICE int kv4_find(const Kv4AttnArgs& a, int lane, long long at, long long& first) {
   const long long units = (long long)a.kv_heads * a.row_tiles;
   long long base = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 32) {
-    const int n = b0 + lane < a.batch ? kv4_blocks(kv4_seen(a, b0 + lane)) : 0;
+    const int n = b0 + lane < a.batch ? kv4_blocks<NT>(kv4_seen(a, b0 + lane)) : 0;
     int sum = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -162,7 +176,7 @@ CCUT_DEVICE long long kv4_span(long long total, int n, int i) { return total * i
 CCUT_DEVICE int kv4_span_of(long long total, int n, long long at) { return (int)(((at + 1) * n - 1) / total); }
 
 template <int D, int NT>
-constexpr int kKv4Resident = D == 64 ? (NT == 1 ? 6 : 4) : (NT == 1 ? 4 : 2);  // CTAs per SM, by registers
+constexpr int kKv4Resident = D == 64 ? (NT == 1 ? 5 : 4) : (NT == 1 ? 3 : 2);  // CTAs per SM, by registers
 
 template <int D, int NT, bool OUT_BF16>
 __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_kernel(Kv4AttnArgs a) {
@@ -171,23 +185,23 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
   constexpr int G = D / kKv4Group;
   constexpr int kRows = 8 * NT;
   constexpr uint32_t M0 = 0x000F000Fu, M1 = 0x00F000F0u;
-  using St = Kv4Stage<D>;
-  constexpr int kRing = kKv4Warps * kKv4Stages * St::kBytes, kJoin = kKv4Warps * kRows * (D + 4) * 4;
-  __shared__ __align__(16) uint8_t smem[kRing > kJoin ? kRing : kJoin];  // the ring, then the warps' outputs
+  using St = Kv4Stage<D, NT>;
+  constexpr int kTile = kKv4Tile<NT>, kBlock = kKv4Block<NT>, kStages = kKv4Stages<NT>, U = kTile / 16;
+  extern __shared__ __align__(16) uint8_t smem[];  // the rings, then the warps' outputs
   float(*sm_o)[kRows][D + 4] = reinterpret_cast<float(*)[kRows][D + 4]>(smem);
   __shared__ float sm_m[kKv4Warps][kRows], sm_l[kKv4Warps][kRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int grp = a.heads / a.kv_heads, nrows = grp * a.seq;
-  const long long total = kv4_total(a, lane);
+  const long long total = kv4_total<NT>(a, lane);
   const int spans = (int)min((long long)a.ctas, total);
   if ((int)blockIdx.x >= spans) return;
   const long long begin = kv4_span(total, spans, blockIdx.x), end = kv4_span(total, spans, blockIdx.x + 1);
   long long first;
-  int b = kv4_find(a, lane, begin, first);
+  int b = kv4_find<NT>(a, lane, begin, first);
   long long at = begin;
 
   while (at < end) {
-  const int seen = kv4_seen(a, b), nblocks = kv4_blocks(seen);
+  const int seen = kv4_seen(a, b), nblocks = kv4_blocks<NT>(seen);
   const int unit = (int)((at - first) / nblocks), block0 = (int)((at - first) % nblocks);
   const int block1 = (int)min((long long)nblocks, block0 + (end - at));
   const bool whole_unit = block0 == 0 && block1 == nblocks;
@@ -195,9 +209,9 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
   const int kvh = unit % a.kv_heads, r0 = unit / a.kv_heads * kRows;
   const int start = min(a.starts[b], a.kv_len);
   const int last_row = min(nrows, r0 + kRows) - 1;
-  const int k0 = block0 * kKv4Block;
+  const int k0 = block0 * kBlock;
   // positions any row of this tile sees in this segment
-  const int k1 = seen > 0 ? min(min(seen, block1 * kKv4Block), start + last_row / grp + 1) : 0;
+  const int k1 = seen > 0 ? min(min(seen, block1 * kBlock), start + last_row / grp + 1) : 0;
   const size_t row_base = seen > 0 ? (size_t)a.slots[b] * (size_t)a.slot_rows + (size_t)kvh * a.max_len : 0;
 
   // ---- the query rows as B fragments (row n = g of n-tile nt; features t * 16 .. of each group) ----
@@ -272,36 +286,38 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
       for (int i = 0; i < 4; ++i) o[nt][mt][i] = 0.f;
   }
 
-  // This lane's part of a tile: 16-byte chunks `lane` and, of 128 features, `lane` + 32 (8 positions further)
-  // of the codes, and position lane % 16's pair(s) of k or of v.  The addresses move from one tile of
-  // the warp to its next; positions at or past k1 come as zeros.
-  const uint8_t* ring = smem + warp * kKv4Stages * St::kBytes;
-  constexpr int kPer = D / 32;  // chunks per position
-  const int cr = lane / kPer, first_tile = (k0 + warp * kKv4Tile);
+  // This lane's part of a tile: 16-byte chunks lane, lane + 32, .. of the codes, and a position's pair(s):
+  // with 32 positions of k and then of v, with 16 of k (lanes 0-15) or of v.  The addresses move from
+  // one tile of the warp to its next; positions at or past k1 come as zeros.
+  const uint8_t* ring = smem + warp * kStages * St::kBytes;
+  constexpr int kPer = D / 32, kStepRows = 32 / kPer;  // chunks per position, positions per 32 chunks
+  const int cr = lane / kPer, first_tile = k0 + warp * kTile, prow = U == 2 ? lane : lane & 15;
   const uint32_t to_codes = smem_u32(ring) + kv4_unit<D>(cr, lane % kPer >> 1) + (lane & 1) * 16;
   const uint32_t to_params = smem_u32(ring) + 2 * St::kCodes + lane * (D / 16);
   const uint8_t* kc = a.kc + (row_base + first_tile) * (D / 2) + lane * 16;
   const uint8_t* vc = a.vc + (row_base + first_tile) * (D / 2) + lane * 16;
-  const uint8_t* pp =
-      reinterpret_cast<const uint8_t*>(lane < 16 ? a.kp : a.vp) + (row_base + first_tile + (lane & 15)) * (D / 16);
+  const uint8_t* kp = reinterpret_cast<const uint8_t*>(U == 2 || lane < 16 ? a.kp : a.vp) + (row_base + first_tile + prow) * (D / 16);
+  const uint8_t* vp = reinterpret_cast<const uint8_t*>(a.vp) + (row_base + first_tile + prow) * (D / 16);  // U == 2
   auto copy_tile = [&](uint32_t stage, int left, auto checked) {
-    constexpr bool kC = decltype(checked)::value;
+    constexpr bool kC = decltype(checked)::value;  // a position past the end is not touched, nor is its address formed
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
-      const bool in = cr + 8 * i < left;
-
+    for (int i = 0; i < St::kCodes / 512; ++i) {
+      const bool in = cr + kStepRows * i < left;
       copy_in<16, kC>(to_codes + stage + i * 512, kC && !in ? a.kc : kc + i * 512, in);
       copy_in<16, kC>(to_codes + stage + St::kCodes + i * 512, kC && !in ? a.vc : vc + i * 512, in);
     }
-    const bool in = (lane & 15) < left;
-    copy_in<D / 16, kC>(to_params + stage, kC && !in ? reinterpret_cast<const uint8_t*>(a.kp) : pp, in);
-    kc += kKv4Block * (D / 2);
-    vc += kKv4Block * (D / 2);
-    pp += kKv4Block * (D / 16);
+    const bool in = prow < left;
+    copy_in<D / 16, kC>(to_params + stage, kC && !in ? reinterpret_cast<const uint8_t*>(a.kp) : kp, in);
+    if constexpr (U == 2)
+      copy_in<D / 16, kC>(to_params + stage + St::kParams, kC && !in ? reinterpret_cast<const uint8_t*>(a.vp) : vp, in);
+    kc += kBlock * (D / 2);
+    vc += kBlock * (D / 2);
+    kp += kBlock * (D / 16);
+    if constexpr (U == 2) vp += kBlock * (D / 16);
   };
   auto issue = [&](int tile, int stage) {
-    const int left = k1 - k0 - tile * kKv4Tile;
-    if (left >= kKv4Tile) copy_tile(stage * St::kBytes, left, std::false_type{});
+    const int left = k1 - k0 - tile * kTile;
+    if (left >= kTile) copy_tile(stage * St::kBytes, left, std::false_type{});
     else copy_tile(stage * St::kBytes, left, std::true_type{});
   };
   const int kr = kv4_row(g);                          // this lane's score rows: positions kr and kr + 8
@@ -311,78 +327,88 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
 
   auto step = [&](const uint8_t* st, int p0, auto masked_tag) {
     constexpr bool kMasked = decltype(masked_tag)::value;
-    uint32_t kpw[2][G], vpw[2][G];
+    float sc[U][NT][4];  // element i: row g + 8 (i >> 1), column 2t + (i & 1)
+    bool vis[U][NT][4];
+    uint32_t vpw[U][2][G];
+    bool need = false;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint8_t* p = st + 2 * St::kCodes + (kr + 8 * h) * (D / 16);
-      if constexpr (G == 2) {
-        const uint2 uk = *reinterpret_cast<const uint2*>(p), uv = *reinterpret_cast<const uint2*>(p + St::kParams);
-        kpw[h][0] = uk.x, kpw[h][G - 1] = uk.y, vpw[h][0] = uv.x, vpw[h][G - 1] = uv.y;
-      } else {
-        kpw[h][0] = *reinterpret_cast<const uint32_t*>(p);
-        vpw[h][0] = *reinterpret_cast<const uint32_t*>(p + St::kParams);
+    for (int u = 0; u < U; ++u) {
+      uint32_t kpw[2][G];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* p = st + 2 * St::kCodes + (16 * u + 8 * h + kr) * (D / 16);
+        if constexpr (G == 2) {
+          const uint2 uk = *reinterpret_cast<const uint2*>(p), uv = *reinterpret_cast<const uint2*>(p + St::kParams);
+          kpw[h][0] = uk.x, kpw[h][G - 1] = uk.y, vpw[u][h][0] = uv.x, vpw[u][h][G - 1] = uv.y;
+        } else {
+          kpw[h][0] = *reinterpret_cast<const uint32_t*>(p);
+          vpw[u][h][0] = *reinterpret_cast<const uint32_t*>(p + St::kParams);
+        }
       }
-    }
-    float sc[NT][4];
-    {
-      const uint32_t f[4] = {G == 2 ? __byte_perm(kpw[0][0], kpw[0][G - 1], 0x7632) : kpw[0][0],
-                             G == 2 ? __byte_perm(kpw[1][0], kpw[1][G - 1], 0x7632) : kpw[1][0], 0u, 0u};
+      const uint32_t fm[4] = {G == 2 ? __byte_perm(kpw[0][0], kpw[0][G - 1], 0x7632) : kpw[0][0],
+                              G == 2 ? __byte_perm(kpw[1][0], kpw[1][G - 1], 0x7632) : kpw[1][0], 0u, 0u};
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[nt][i] = 0.f;
-        mma_16816<false>(sc[nt], f, qm[nt], 0u);
+        for (int i = 0; i < 4; ++i) sc[u][nt][i] = 0.f;
+        mma_16816<false>(sc[u][nt], fm, qm[nt], 0u);
       }
-    }
 #pragma unroll
-    for (int gr = 0; gr < G; ++gr) {
-      float c4[NT][4];
+      for (int gr = 0; gr < G; ++gr) {
+        float c4[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) c4[nt][i] = 0.f;
+        const uint2 ka = *reinterpret_cast<const uint2*>(st + k_unit[gr] + u * 16 * (D / 2));
+        const uint2 kb = *reinterpret_cast<const uint2*>(st + k_unit[gr] + (u * 16 + 8) * (D / 2));
+        const uint32_t w0[2] = {ka.x, ka.y}, w1[2] = {kb.x, kb.y};
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t u0 = w0[w] >> (8 * h), u1 = w1[w] >> (8 * h);
+            const uint32_t f[4] = {u0 & M0, u1 & M0, u0 & M1, u1 & M1};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma_16816<false>(c4[nt], f, qf[nt][gr][w * 2 + h][0], qf[nt][gr][w * 2 + h][1]);
+          }
+        const float s[2] = {low_f16(kpw[0][gr]), low_f16(kpw[1][gr])};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[u][nt][i] = fmaf(s[i >> 1], c4[nt][i], sc[u][nt][i]);
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c4[nt][i] = 0.f;
-      const uint2 ka = *reinterpret_cast<const uint2*>(st + k_unit[gr]);
-      const uint2 kb = *reinterpret_cast<const uint2*>(st + k_unit[gr] + 8 * (D / 2));
-      const uint32_t w0[2] = {ka.x, ka.y}, w1[2] = {kb.x, kb.y};
-#pragma unroll
-      for (int w = 0; w < 2; ++w)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t u0 = w0[w] >> (8 * h), u1 = w1[w] >> (8 * h);
-          const uint32_t f[4] = {u0 & M0, u1 & M0, u0 & M1, u1 & M1};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_16816<false>(c4[nt], f, qf[nt][gr][w * 2 + h][0], qf[nt][gr][w * 2 + h][1]);
+        for (int i = 0; i < 4; ++i) {
+          float& x = sc[u][nt][i];
+          x *= fr[nt][i & 1];
+          if (a.softcap > 0.f) x = tanhf(x * (1.f / kLog2e) / a.softcap) * (a.softcap * kLog2e);
+          if constexpr (kMasked) {
+            const int p = p0 + 16 * u + kr + 8 * (i >> 1);
+            vis[u][nt][i] = p < k1 && p <= lim[nt][i & 1];
+            if (!vis[u][nt][i]) x = -INFINITY;
+          }
+          need |= x > m[nt][i & 1] + 8.f;
         }
-      const float s[2] = {low_f16(kpw[0][gr]), low_f16(kpw[1][gr])};
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sc[nt][i] = fmaf(s[i >> 1], c4[nt][i], sc[nt][i]);  // row g + 8 (i >> 1), column 2t + (i & 1)
     }
-    bool vis[NT][4];
-    bool need = false;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        sc[nt][i] *= fr[nt][i & 1];
-        if (a.softcap > 0.f) sc[nt][i] = tanhf(sc[nt][i] * (1.f / kLog2e) / a.softcap) * (a.softcap * kLog2e);
-        if constexpr (kMasked) {
-          const int p = p0 + kr + 8 * (i >> 1);
-          vis[nt][i] = p < k1 && p <= lim[nt][i & 1];
-          if (!vis[nt][i]) sc[nt][i] = -INFINITY;
-        }
-        need |= sc[nt][i] > m[nt][i & 1] + 8.f;
-      }
-    __half2 top = __hmax2(as_half2(vpw[0][0]), as_half2(vpw[1][0]));
-    if constexpr (G == 2) top = __hmax2(top, __hmax2(as_half2(vpw[0][G - 1]), as_half2(vpw[1][G - 1])));
+    __half2 top = __hmax2(as_half2(vpw[0][0][0]), as_half2(vpw[0][1][0]));
+    if constexpr (G == 2) top = __hmax2(top, __hmax2(as_half2(vpw[0][0][G - 1]), as_half2(vpw[0][1][G - 1])));
+    if constexpr (U == 2) {
+      top = __hmax2(top, __hmax2(as_half2(vpw[U - 1][0][0]), as_half2(vpw[U - 1][1][0])));
+      if constexpr (G == 2)
+        top = __hmax2(top, __hmax2(as_half2(vpw[U - 1][0][G - 1]), as_half2(vpw[U - 1][1][G - 1])));
+    }
     need |= __hgt(__low2half(top), r_inv);
     if (__any_sync(0xffffffffu, need)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float v = fmaxf(sc[nt][c], sc[nt][c + 2]);
+          float v = fmaxf(sc[0][nt][c], sc[0][nt][c + 2]);
+          if constexpr (U == 2) v = fmaxf(v, fmaxf(sc[U - 1][nt][c], sc[U - 1][nt][c + 2]));
 #pragma unroll
           for (int s = 4; s < 32; s <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, s));
           v = fmaxf(v, m[nt][c]);
@@ -410,58 +436,62 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
             for (int i = 0; i < 4; ++i) o[nt][mt][i] *= f;
       }
     }
-    float p[NT][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int u = 0; u < U; ++u) {
+      float p[NT][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        p[nt][i] = ex2(sc[nt][i] - m[nt][i & 1]);
-        if constexpr (kMasked) p[nt][i] = vis[nt][i] ? p[nt][i] : 0.f;  // a row that saw nothing yet has m = -inf
-        l[nt][i & 1] += p[nt][i];
-      }
-#pragma unroll
-    for (int gr = 0; gr < G; ++gr) {
-      const float sr[2] = {low_f16(vpw[0][gr]) * R, low_f16(vpw[1][gr]) * R};
-      const float mv[2] = {high_f16(vpw[0][gr]), high_f16(vpw[1][gr])};
-      uint32_t wb[NT][2], wl[NT][2];  // p s_v R as the B operand: high part, and the rest
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float w[4];
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          w[i] = p[nt][i] * sr[i >> 1];
-          if constexpr (kMasked) {  // 0 * NaN stays out
-            w[i] = vis[nt][i] ? w[i] : 0.f;
-            am[nt][gr][i & 1] += vis[nt][i] ? p[nt][i] * mv[i >> 1] : 0.f;
-          } else {
-            am[nt][gr][i & 1] = fmaf(p[nt][i], mv[i >> 1], am[nt][gr][i & 1]);
+          p[nt][i] = ex2(sc[u][nt][i] - m[nt][i & 1]);
+          if constexpr (kMasked) p[nt][i] = vis[u][nt][i] ? p[nt][i] : 0.f;  // a row that saw nothing yet has m = -inf
+          l[nt][i & 1] += p[nt][i];
+        }
+#pragma unroll
+      for (int gr = 0; gr < G; ++gr) {
+        const float sr[2] = {low_f16(vpw[u][0][gr]) * R, low_f16(vpw[u][1][gr]) * R};
+        const float mv[2] = {high_f16(vpw[u][0][gr]), high_f16(vpw[u][1][gr])};
+        uint32_t wb[NT][2], wl[NT][2];  // p s_v R as the B operand: high part, and the rest
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            w[i] = p[nt][i] * sr[i >> 1];
+            if constexpr (kMasked) {  // 0 * NaN stays out
+              w[i] = vis[u][nt][i] ? w[i] : 0.f;
+              am[nt][gr][i & 1] += vis[u][nt][i] ? p[nt][i] * mv[i >> 1] : 0.f;
+            } else {
+              am[nt][gr][i & 1] = fmaf(p[nt][i], mv[i >> 1], am[nt][gr][i & 1]);
+            }
+          }
+          const uint32_t h0 = pack_f16(w[0], w[1]), h1 = pack_f16(w[2], w[3]);
+          wb[nt][0] = movmatrix_trans(h0);
+          wb[nt][1] = movmatrix_trans(h1);
+          if constexpr (!OUT_BF16) {
+            const float2 b0 = unpack_f16(h0), b1 = unpack_f16(h1);
+            wl[nt][0] = movmatrix_trans(pack_f16(w[0] - b0.x, w[1] - b0.y));
+            wl[nt][1] = movmatrix_trans(pack_f16(w[2] - b1.x, w[3] - b1.y));
           }
         }
-        const uint32_t h0 = pack_f16(w[0], w[1]), h1 = pack_f16(w[2], w[3]);
-        wb[nt][0] = movmatrix_trans(h0);
-        wb[nt][1] = movmatrix_trans(h1);
-        if constexpr (!OUT_BF16) {
-          const float2 b0 = unpack_f16(h0), b1 = unpack_f16(h1);
-          wl[nt][0] = movmatrix_trans(pack_f16(w[0] - b0.x, w[1] - b0.y));
-          wl[nt][1] = movmatrix_trans(pack_f16(w[2] - b1.x, w[3] - b1.y));
-        }
-      }
-      uint32_t v[4];
+        uint32_t v[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)  // positions t, t + 4, t + 8, t + 12: k indices 2t, 2t + 1, 2t + 8, 2t + 9
-        v[i] = *reinterpret_cast<const uint32_t*>(st + St::kCodes + v_unit[i & 1][gr] + (i >> 1) * 8 * (D / 2));
+        for (int i = 0; i < 4; ++i)  // positions t, t + 4, t + 8, t + 12: k indices 2t, 2t + 1, 2t + 8, 2t + 9
+          v[i] = *reinterpret_cast<const uint32_t*>(st + St::kCodes + v_unit[i & 1][gr] +
+                                                    (u * 16 + (i >> 1) * 8) * (D / 2));
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t sel = half ? 0x7632 : 0x5410;
-        const uint32_t p01 = __byte_perm(v[0], v[1], sel), p23 = __byte_perm(v[2], v[3], sel);
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t sel = half ? 0x7632 : 0x5410;
+          const uint32_t p01 = __byte_perm(v[0], v[1], sel), p23 = __byte_perm(v[2], v[3], sel);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t u0 = p01 >> (8 * h), u1 = p23 >> (8 * h);
-          const uint32_t f[4] = {u0 & M0, u0 & M1, u1 & M0, u1 & M1};
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t u0 = p01 >> (8 * h), u1 = p23 >> (8 * h);
+            const uint32_t f[4] = {u0 & M0, u0 & M1, u1 & M0, u1 & M1};
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma_16816<false>(o[nt][gr * 4 + half * 2 + h], f, wb[nt][0], wb[nt][1]);
-            if constexpr (!OUT_BF16) mma_16816<false>(o[nt][gr * 4 + half * 2 + h], f, wl[nt][0], wl[nt][1]);
+            for (int nt = 0; nt < NT; ++nt) {
+              mma_16816<false>(o[nt][gr * 4 + half * 2 + h], f, wb[nt][0], wb[nt][1]);
+              if constexpr (!OUT_BF16) mma_16816<false>(o[nt][gr * 4 + half * 2 + h], f, wl[nt][0], wl[nt][1]);
+            }
           }
         }
       }
@@ -470,22 +500,22 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
 
   // tiles of this warp: warp, warp + 4, ..; the first `whole` of the segment are seen in whole by every row.
   // One commit group per tile (empty past the end), so that wait_group always means "this tile has landed".
-  const int ntiles = k1 > k0 ? (k1 - k0 + kKv4Tile - 1) / kKv4Tile : 0;
-  const int whole = k1 > k0 ? max(0, min(k1, start + r0 / grp + 1) - k0) / kKv4Tile : 0;
+  const int ntiles = k1 > k0 ? (k1 - k0 + kTile - 1) / kTile : 0;
+  const int whole = k1 > k0 ? max(0, min(k1, start + r0 / grp + 1) - k0) / kTile : 0;
 #pragma unroll
-  for (int i = 0; i < kKv4Stages - 1; ++i) {
+  for (int i = 0; i < kStages - 1; ++i) {
     if (warp + i * kKv4Warps < ntiles) issue(warp + i * kKv4Warps, i);
     cp_async_commit();
   }
   for (int j = warp, i = 0; j < ntiles; j += kKv4Warps, ++i) {
-    cp_async_wait<kKv4Stages - 2>();
+    cp_async_wait<kStages - 2>();
     __syncwarp();  // every lane's copies of this tile have landed, every lane is done with the tile before
-    const int jn = j + (kKv4Stages - 1) * kKv4Warps;
-    if (jn < ntiles) issue(jn, (i + kKv4Stages - 1) % kKv4Stages);
+    const int jn = j + (kStages - 1) * kKv4Warps;
+    if (jn < ntiles) issue(jn, (i + kStages - 1) % kStages);
     cp_async_commit();
-    const uint8_t* st = ring + i % kKv4Stages * St::kBytes;
+    const uint8_t* st = ring + i % kStages * St::kBytes;
     if (j < whole) step(st, 0, std::false_type{});
-    else step(st, k0 + j * kKv4Tile, std::true_type{});
+    else step(st, k0 + j * kTile, std::true_type{});
   }
   cp_async_wait<0>();
   __syncthreads();  // the warps' outputs take the ring's place
@@ -563,13 +593,13 @@ __global__ void __launch_bounds__(256) kv4_merge_kernel(Kv4AttnArgs a) {
   const int grp = a.heads / a.kv_heads, r = i * grp + h % grp;
   unsigned all = 0, before = 0;
   for (int j = lane; j < a.batch; j += 32) {
-    const int n = kv4_blocks(kv4_seen(a, j));
+    const int n = kv4_blocks<NT>(kv4_seen(a, j));
     all += n;
     before += j < b ? n : 0;
   }
   const long long units = (long long)a.kv_heads * a.row_tiles;
   const long long total = __reduce_add_sync(0xffffffffu, all) * units;
-  const int nblocks = kv4_blocks(kv4_seen(a, b));
+  const int nblocks = kv4_blocks<NT>(kv4_seen(a, b));
   const long long first = __reduce_add_sync(0xffffffffu, before) * units +
                           ((long long)(r / kRows) * a.kv_heads + h / grp) * nblocks;
   const int spans = (int)min((long long)a.ctas, total);
@@ -612,6 +642,7 @@ __global__ void __launch_bounds__(256) kv4_merge_kernel(Kv4AttnArgs a) {
 
 // Query rows per tile: 8 where a kv head has no more, else 16.
 static int kv4_rows(int heads, int kv_heads, int seq) { return (long)(heads / kv_heads) * seq <= 8 ? 8 : 16; }
+static int kv4_block(int rows) { return rows == 8 ? kKv4Block<1> : kKv4Block<2>; }
 static long long kv4_row_tiles(int heads, int kv_heads, int seq) {
   const long long rows = (long long)(heads / kv_heads) * seq, per = kv4_rows(heads, kv_heads, seq);
   return (rows + per - 1) / per;
@@ -621,15 +652,19 @@ static int kv4_ctas(int batch, int heads, int kv_heads, int seq, int kv_len, int
   const bool one = kv4_rows(heads, kv_heads, seq) == 8;
   const int most = 148 * (head_dim == 64 ? (one ? kKv4Resident<64, 1> : kKv4Resident<64, 2>)
                                          : (one ? kKv4Resident<128, 1> : kKv4Resident<128, 2>));
-  const long long blocks = kv_len > 0 ? (kv_len + kKv4Block - 1) / kKv4Block : 1;
+  const int block = kv4_block(one ? 8 : 16);
+  const long long blocks = kv_len > 0 ? (kv_len + block - 1) / block : 1;
   const long long n = kv4_row_tiles(heads, kv_heads, seq) * kv_heads * batch;
   return n >= most || n * blocks >= most ? most : (int)(n * blocks);
 }
 
 template <int D, int NT, bool OB>
 static int run_kv4_attention(const Kv4AttnArgs& a, cudaStream_t st) {
-  int rc = launch_k(kv4_attn_kernel<D, NT, OB>, dim3(a.ctas), dim3(kKv4Warps * 32), 0, st, a);
-  if (rc || a.kv_len <= kKv4Block) return rc;  // one block a unit: no unit is cut
+  static std::atomic<uint64_t> smem_set{0};  // devices with the limit raised
+  int rc = ensure_smem_limit(kv4_attn_kernel<D, NT, OB>, kKv4Smem<D, NT>, smem_set);
+  if (rc) return rc;
+  rc = launch_k(kv4_attn_kernel<D, NT, OB>, dim3(a.ctas), dim3(kKv4Warps * 32), kKv4Smem<D, NT>, st, a);
+  if (rc || a.kv_len <= kKv4Block<NT>) return rc;  // one block a unit: no unit is cut
   return launch_k(kv4_merge_kernel<D, NT, OB>, dim3((unsigned)((long)a.batch * a.heads * a.seq)), dim3(256), 0, st, a);
 }
 
@@ -643,7 +678,7 @@ size_t ccut_kv4_attention_workspace_bytes(int batch, int heads, int kv_heads, in
   if (batch < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || seq < 0 || kv_len < 0 ||
       (head_dim != 64 && head_dim != 128))
     return 0;
-  if (batch == 0 || seq == 0 || kv_len <= kKv4Block) return 256;
+  if (batch == 0 || seq == 0 || kv_len <= kv4_block(kv4_rows(heads, kv_heads, seq))) return 256;
   return 256 + (size_t)kv4_ctas(batch, heads, kv_heads, seq, kv_len, head_dim) * 2 * kv4_rows(heads, kv_heads, seq) *
                    (head_dim + 2) * sizeof(float);
 }
@@ -667,7 +702,7 @@ int ccut_kv4_attention(const uint16_t* q, const uint8_t* k_codes, const uint16_t
     return CCUT_ERR_INVALID;
   // rows in a grid; blocks of all sequences in 32 bits
   if ((long long)batch * heads * seq > 2147483647LL ||
-      (long long)batch * ((long long)kv_len / kKv4Block + 1) > 2147483647LL)
+      (long long)batch * ((long long)kv_len / kKv4Block<2> + 1) > 2147483647LL)
     return CCUT_ERR_UNSUPPORTED;
   const size_t need = ccut_kv4_attention_workspace_bytes(batch, heads, kv_heads, seq, kv_len, head_dim);
   if (need > 256 && (!workspace || ws_bytes < need)) return CCUT_ERR_WORKSPACE;
