@@ -130,6 +130,18 @@ CCUT_DEVICE void copy_in(uint32_t to, const uint8_t* from, bool in) {
   }
 }
 
+// Four features of an output row.
+template <bool OUT_BF16>
+CCUT_DEVICE void kv4_store(void* out, long long at, const float4& v) {
+  if constexpr (OUT_BF16) {
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+  } else {
+    *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = v;
+  }
+}
+
 // The line of work: sequence b has kv4_blocks blocks of positions in each of its units, at least one (a
 // unit that sees nothing still writes its zeros).
 CCUT_DEVICE int kv4_seen(const Kv4AttnArgs& a, int b) {  // positions its last query sees
@@ -140,20 +152,21 @@ template <int NT>
 CCUT_DEVICE int kv4_blocks(int seen) {
   return max(1, (seen + kKv4Block<NT> - 1) / kKv4Block<NT>);
 }
-// Whole warp.  Blocks of all sequences (times units: the length of the line).
+// Whole warp.  Length of the line.  `mine`: blocks of sequence `lane`, for kv4_find.
 template <int NT>
-CCUT_DEVICE long long kv4_total(const Kv4AttnArgs& a, int lane) {
-  unsigned n = 0;  // fits: kv_len / 64 x batch is bounded at launch
-  for (int b = lane; b < a.batch; b += 32) n += kv4_blocks<NT>(kv4_seen(a, b));
-  return (long long)__reduce_add_sync(0xffffffffu, n) * a.kv_heads * a.row_tiles;
+CCUT_DEVICE int kv4_total(const Kv4AttnArgs& a, int lane, int& mine) {
+  mine = lane < a.batch ? kv4_blocks<NT>(kv4_seen(a, lane)) : 0;
+  unsigned n = mine;  // no overflow: the line is bounded at launch
+  for (int b = lane + 32; b < a.batch; b += 32) n += kv4_blocks<NT>(kv4_seen(a, b));
+  return (int)__reduce_add_sync(0xffffffffu, n) * a.kv_heads * a.row_tiles;
 }
 // Whole warp.  The sequence at place `at` of the line, and the place of its first block.
 template <int NT>
-CCUT_DEVICE int kv4_find(const Kv4AttnArgs& a, int lane, long long at, long long& first) {
-  const long long units = (long long)a.kv_heads * a.row_tiles;
-  long long base = 0;
+CCUT_DEVICE int kv4_find(const Kv4AttnArgs& a, int lane, int mine, int at, int& first) {
+  const int units = a.kv_heads * a.row_tiles;
+  int base = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 32) {
-    const int n = b0 + lane < a.batch ? kv4_blocks<NT>(kv4_seen(a, b0 + lane)) : 0;
+    const int n = b0 == 0 ? mine : b0 + lane < a.batch ? kv4_blocks<NT>(kv4_seen(a, b0 + lane)) : 0;
     int sum = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -163,17 +176,20 @@ CCUT_DEVICE int kv4_find(const Kv4AttnArgs& a, int lane, long long at, long long
     const unsigned past = __ballot_sync(0xffffffffu, base + sum * units > at);
     if (past) {
       const int w = __ffs(past) - 1;
-      first = base + (long long)__shfl_sync(0xffffffffu, sum - n, w) * units;
+      first = base + __shfl_sync(0xffffffffu, sum - n, w) * units;
       return b0 + w;
     }
-    base += (long long)__shfl_sync(0xffffffffu, sum, 31) * units;
+    base += __shfl_sync(0xffffffffu, sum, 31) * units;
   }
   first = base;
   return a.batch;  // not reached for places on the line
 }
-// First place of span i of n, and the span that holds a place.
-CCUT_DEVICE long long kv4_span(long long total, int n, int i) { return total * i / n; }
-CCUT_DEVICE int kv4_span_of(long long total, int n, long long at) { return (int)(((at + 1) * n - 1) / total); }
+// The line in n spans, the first total % n of them one longer: where span i begins, and the span of a place.
+CCUT_DEVICE int kv4_span(int total, int n, int i) { return i * (total / n) + min(i, total % n); }
+CCUT_DEVICE int kv4_span_of(int total, int n, int at) {
+  const int per = total / n, cut = (total % n) * (per + 1);
+  return at < cut ? at / (per + 1) : total % n + (at - cut) / per;
+}
 
 template <int D, int NT>
 constexpr int kKv4Resident = D == 64 ? (NT == 1 ? 5 : 4) : (NT == 1 ? 3 : 2);  // CTAs per SM, by registers
@@ -189,21 +205,21 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
   constexpr int kTile = kKv4Tile<NT>, kBlock = kKv4Block<NT>, kStages = kKv4Stages<NT>, U = kTile / 16;
   extern __shared__ __align__(16) uint8_t smem[];  // the rings, then the warps' outputs
   float(*sm_o)[kRows][D + 4] = reinterpret_cast<float(*)[kRows][D + 4]>(smem);
-  __shared__ float sm_m[kKv4Warps][kRows], sm_l[kKv4Warps][kRows];
+  __shared__ float sm_m[kKv4Warps][kRows], sm_l[kKv4Warps][kRows], sm_f[kKv4Warps][kRows];
+  __shared__ long long sm_at[kRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int grp = a.heads / a.kv_heads, nrows = grp * a.seq;
-  const long long total = kv4_total<NT>(a, lane);
-  const int spans = (int)min((long long)a.ctas, total);
+  int mine, first;
+  const int total = kv4_total<NT>(a, lane, mine), spans = min(a.ctas, total);
   if ((int)blockIdx.x >= spans) return;
-  const long long begin = kv4_span(total, spans, blockIdx.x), end = kv4_span(total, spans, blockIdx.x + 1);
-  long long first;
-  int b = kv4_find<NT>(a, lane, begin, first);
-  long long at = begin;
+  const int begin = kv4_span(total, spans, blockIdx.x), end = kv4_span(total, spans, blockIdx.x + 1);
+  int b = kv4_find<NT>(a, lane, mine, begin, first);
+  int at = begin;
 
   while (at < end) {
   const int seen = kv4_seen(a, b), nblocks = kv4_blocks<NT>(seen);
-  const int unit = (int)((at - first) / nblocks), block0 = (int)((at - first) % nblocks);
-  const int block1 = (int)min((long long)nblocks, block0 + (end - at));
+  const int unit = (at - first) / nblocks, block0 = (at - first) % nblocks;
+  const int block1 = min(nblocks, block0 + (end - at));
   const bool whole_unit = block0 == 0 && block1 == nblocks;
   const int part = blockIdx.x * 2 + (at != begin);
   const int kvh = unit % a.kv_heads, r0 = unit / a.kv_heads * kRows;
@@ -545,32 +561,42 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
       }
     }
   __syncthreads();
-  for (int idx = threadIdx.x; idx < kRows * D; idx += kKv4Warps * 32) {
-    const int n = idx / D, d = idx % D, r = r0 + n;
-    if (r >= nrows) continue;
-    float M = -INFINITY, L = 0.f, v = 0.f;
+  if (threadIdx.x < kRows) {  // each warp's factor for row n, and where the row goes (-1: past the last)
+    const int n = threadIdx.x, r = r0 + n;
+    float M = -INFINITY, L = 0.f, f[kKv4Warps];
 #pragma unroll
     for (int w = 0; w < kKv4Warps; ++w) M = fmaxf(M, sm_m[w][n]);
-    const float Mu = M == -INFINITY ? 0.f : M;
 #pragma unroll
     for (int w = 0; w < kKv4Warps; ++w) {
-      const float f = ex2(sm_m[w][n] - Mu);  // 0 for a warp that saw nothing
-      L = fmaf(sm_l[w][n], f, L);
-      v = fmaf(sm_o[w][n][d], f, v);
+      f[w] = ex2(sm_m[w][n] - (M == -INFINITY ? 0.f : M));  // 0 for a warp that saw nothing
+      L = fmaf(sm_l[w][n], f[w], L);
     }
-    if (!whole_unit) {
-      if (d == 0) a.ml[part * kRows + n] = make_float2(M, L);
-      a.acc[((size_t)part * kRows + n) * D + d] = v;
-    } else {
-      const size_t row = ((size_t)b * a.heads + kvh * grp + r % grp) * a.seq + r / grp;
-      v = L == 0.f ? 0.f : v / L;
-      if constexpr (OUT_BF16) static_cast<__nv_bfloat16*>(a.out)[row * D + d] = __float2bfloat16_rn(v);
-      else static_cast<float*>(a.out)[row * D + d] = v;
+    if (!whole_unit) a.ml[part * kRows + n] = make_float2(M, L);
+    const float inv = !whole_unit ? 1.f : L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+    for (int w = 0; w < kKv4Warps; ++w) sm_f[w][n] = f[w] * inv;
+    sm_at[n] = r >= nrows    ? -1
+               : !whole_unit ? (long long)part * kRows + n
+                             : ((long long)b * a.heads + kvh * grp + r % grp) * a.seq + r / grp;
+  }
+  __syncthreads();
+  for (int idx = threadIdx.x; idx < kRows * D / 4; idx += kKv4Warps * 32) {
+    const int n = idx / (D / 4), d = idx % (D / 4) * 4;
+    const long long row = sm_at[n];
+    if (row < 0) continue;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kKv4Warps; ++w) {
+      const float f = sm_f[w][n];
+      const float4 x = *reinterpret_cast<const float4*>(&sm_o[w][n][d]);
+      v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y), v.z = fmaf(x.z, f, v.z), v.w = fmaf(x.w, f, v.w);
     }
+    if (!whole_unit) *reinterpret_cast<float4*>(a.acc + row * D + d) = v;
+    else kv4_store<OUT_BF16>(a.out, row * D + d, v);
   }
   at += block1 - block0;
   if (at < end) {
-    if (at >= first + (long long)nblocks * a.kv_heads * a.row_tiles) {
+    if (at >= first + nblocks * a.kv_heads * a.row_tiles) {
       first = at;
       ++b;
     }
@@ -579,17 +605,19 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
   }
 }
 
-// Joins the partial results of one query row per CTA (none: the row was finished by its span): warp w takes
-// spans w, w + 8, .. of the row's unit, each lane D / 32 features; the eight sums are added in warp order.
-template <int D, int NT, bool OUT_BF16>
-__global__ void __launch_bounds__(256) kv4_merge_kernel(Kv4AttnArgs a) {
-  pdl_wait();
-  pdl_trigger();
-  constexpr int E = D / 32, kRows = 8 * NT;
+// Joins the partial results of a query row (none: the row was finished by its span).  W warps a row, eight
+// warps a CTA: warp w of a row takes spans w, w + W, .. of the row's unit, each lane D / 32 features; the W
+// sums are added in warp order.  The line is looked up before the wait for the attention kernel: slots and
+// starts were there before that began.
+template <int D, int NT, int W, bool OUT_BF16>
+__global__ void __launch_bounds__(256) kv4_merge_kernel(Kv4AttnArgs a, long long rows) {
+  constexpr int E = D / 32, kRows = 8 * NT, kPer = 8 / W;
   __shared__ float so[8][D], sl[8];
-  const long long row = blockIdx.x;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int i = (int)(row % a.seq), b = (int)(row / a.seq / a.heads), h = (int)(row / a.seq % a.heads);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w = warp % W;
+  const long long row = (long long)blockIdx.x * kPer + warp / W;
+  const bool live = row < rows;
+  int b = 0, h = 0, i = 0;
+  if (live) i = (int)(row % a.seq), b = (int)(row / a.seq / a.heads), h = (int)(row / a.seq % a.heads);
   const int grp = a.heads / a.kv_heads, r = i * grp + h % grp;
   unsigned all = 0, before = 0;
   for (int j = lane; j < a.batch; j += 32) {
@@ -597,46 +625,62 @@ __global__ void __launch_bounds__(256) kv4_merge_kernel(Kv4AttnArgs a) {
     all += n;
     before += j < b ? n : 0;
   }
-  const long long units = (long long)a.kv_heads * a.row_tiles;
-  const long long total = __reduce_add_sync(0xffffffffu, all) * units;
+  const int units = a.kv_heads * a.row_tiles;
+  const int total = (int)__reduce_add_sync(0xffffffffu, all) * units;
   const int nblocks = kv4_blocks<NT>(kv4_seen(a, b));
-  const long long first = __reduce_add_sync(0xffffffffu, before) * units +
-                          ((long long)(r / kRows) * a.kv_heads + h / grp) * nblocks;
-  const int spans = (int)min((long long)a.ctas, total);
+  const int first = (int)__reduce_add_sync(0xffffffffu, before) * units + (r / kRows * a.kv_heads + h / grp) * nblocks;
+  const int spans = min(a.ctas, total);
   const int c0 = kv4_span_of(total, spans, first), c1 = kv4_span_of(total, spans, first + nblocks - 1);
-  if (c0 == c1) return;
   // in span c0 the unit comes after others (partial result 1) unless it begins the span; in the rest it begins it
-  const bool late = kv4_span(total, spans, c0) < first;
+  const int late = kv4_span(total, spans, c0) < first ? 1 : 0;
+  pdl_wait();
+  pdl_trigger();
+  if (!live || c0 == c1) return;  // the same for every warp of a row; with W == 8 for the whole CTA
   const float2* ml = a.ml + r % kRows;
   float M = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, ml[(2 * c + (late && c == c0)) * kRows].x);
+  for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, ml[(2 * c + (c == c0 ? late : 0)) * kRows].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
   const float Mu = M == -INFINITY ? 0.f : M;
   float L = 0.f, v[E] = {};
-#pragma unroll 4
-  for (int c = c0 + warp; c <= c1; c += 8) {
-    const int part = 2 * c + (late && c == c0);
-    const float2 x = ml[part * kRows];
+#pragma unroll 8
+  for (int c = c0 + w; c <= c1; c += W) {
+    const int part = (2 * c + (c == c0 ? late : 0)) * kRows;
+    const float2 x = ml[part];
     const float f = ex2(x.x - Mu);
     L = fmaf(x.y, f, L);
-    const float* p = a.acc + ((size_t)part * kRows + r % kRows) * D + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = fmaf(p[e], f, v[e]);
+    const float* p = a.acc + ((size_t)part + r % kRows) * D + lane * E;
+    if constexpr (E == 4) {
+      const float4 y = *reinterpret_cast<const float4*>(p);
+      v[0] = fmaf(y.x, f, v[0]), v[1] = fmaf(y.y, f, v[1]), v[E - 2] = fmaf(y.z, f, v[E - 2]);
+      v[E - 1] = fmaf(y.w, f, v[E - 1]);
+    } else {
+      const float2 y = *reinterpret_cast<const float2*>(p);
+      v[0] = fmaf(y.x, f, v[0]), v[1] = fmaf(y.y, f, v[1]);
+    }
   }
+  if constexpr (W > 1) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) so[warp][lane * E + e] = v[e];
-  if (lane == 0) sl[warp] = L;
-  __syncthreads();
-  if (threadIdx.x < D) {
-    const int d = threadIdx.x;
-    float s = 0.f;
+    for (int e = 0; e < E; ++e) so[warp][lane * E + e] = v[e];
+    if (lane == 0) sl[warp] = L;
+    __syncthreads();
+    if (warp != 0) return;
     L = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) L += sl[w], s += so[w][d];
-    const float y = L == 0.f ? 0.f : s / L;
-    if constexpr (OUT_BF16) static_cast<__nv_bfloat16*>(a.out)[row * D + d] = __float2bfloat16_rn(y);
-    else static_cast<float*>(a.out)[row * D + d] = y;
+    for (int e = 0; e < E; ++e) v[e] = 0.f;
+#pragma unroll
+    for (int x = 0; x < W; ++x) {
+      L += sl[x];
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] += so[x][lane * E + e];
+    }
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float y = v[e] * inv;
+    if constexpr (OUT_BF16) static_cast<__nv_bfloat16*>(a.out)[row * D + lane * E + e] = __float2bfloat16_rn(y);
+    else static_cast<float*>(a.out)[row * D + lane * E + e] = y;
   }
 }
 
@@ -665,7 +709,11 @@ static int run_kv4_attention(const Kv4AttnArgs& a, cudaStream_t st) {
   if (rc) return rc;
   rc = launch_k(kv4_attn_kernel<D, NT, OB>, dim3(a.ctas), dim3(kKv4Warps * 32), kKv4Smem<D, NT>, st, a);
   if (rc || a.kv_len <= kKv4Block<NT>) return rc;  // one block a unit: no unit is cut
-  return launch_k(kv4_merge_kernel<D, NT, OB>, dim3((unsigned)((long)a.batch * a.heads * a.seq)), dim3(256), 0, st, a);
+  // a warp per row where few spans share a unit, else a CTA
+  const long long rows = (long long)a.batch * a.heads * a.seq, units = (long long)a.batch * a.kv_heads * a.row_tiles;
+  if (a.ctas <= 8 * units)
+    return launch_k(kv4_merge_kernel<D, NT, 1, OB>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, a, rows);
+  return launch_k(kv4_merge_kernel<D, NT, 8, OB>, dim3((unsigned)rows), dim3(256), 0, st, a, rows);
 }
 
 }  // namespace ccut
@@ -700,10 +748,9 @@ int ccut_kv4_attention(const uint16_t* q, const uint8_t* k_codes, const uint16_t
   if (misaligned(q, 16) || misaligned(k_codes, 16) || misaligned(v_codes, 16) || misaligned(k_params, head_dim / 16) ||
       misaligned(v_params, head_dim / 16) || misaligned(out, 16) || misaligned(workspace, 16))
     return CCUT_ERR_INVALID;
-  // rows in a grid; blocks of all sequences in 32 bits
-  if ((long long)batch * heads * seq > 2147483647LL ||
-      (long long)batch * ((long long)kv_len / kKv4Block<2> + 1) > 2147483647LL)
-    return CCUT_ERR_UNSUPPORTED;
+  // rows in a grid; the line of work in 32 bits
+  const double line = (double)batch * kv_heads * kv4_row_tiles(heads, kv_heads, seq) * (kv_len / kKv4Block<2> + 1);
+  if ((double)batch * heads * seq > 2147483647.0 || line > 2147483647.0) return CCUT_ERR_UNSUPPORTED;
   const size_t need = ccut_kv4_attention_workspace_bytes(batch, heads, kv_heads, seq, kv_len, head_dim);
   if (need > 256 && (!workspace || ws_bytes < need)) return CCUT_ERR_WORKSPACE;
   if (!(scale > 0.f)) scale = 1.f / sqrtf((float)head_dim);
