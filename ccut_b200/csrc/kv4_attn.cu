@@ -605,14 +605,15 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
   }
 }
 
-// Joins the partial results of a query row (none: the row was finished by its span).  W warps a row, eight
-// warps a CTA: warp w of a row takes spans w, w + W, .. of the row's unit, each lane D / 32 features; the W
+// Joins the partial results of a query row (none: the row was finished by its span).  W warps a row, at least
+// eight a CTA: warp w of a row takes spans w, w + W, .. of the row's unit, each lane D / 32 features; the W
 // sums are added in warp order.  The line is looked up before the wait for the attention kernel: slots and
 // starts were there before that began.
 template <int D, int NT, int W, bool OUT_BF16>
-__global__ void __launch_bounds__(256) kv4_merge_kernel(Kv4AttnArgs a, long long rows) {
-  constexpr int E = D / 32, kRows = 8 * NT, kPer = 8 / W;
-  __shared__ float so[8][D], sl[8];
+__global__ void __launch_bounds__(W > 8 ? W * 32 : 256) kv4_merge_kernel(Kv4AttnArgs a, long long rows) {
+  constexpr int E = D / 32, kRows = 8 * NT, kPer = W > 8 ? 1 : 8 / W;
+  __shared__ float so[W][D];
+  __shared__ float2 sl[W];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w = warp % W;
   const long long row = (long long)blockIdx.x * kPer + warp / W;
   const bool live = row < rows;
@@ -635,44 +636,44 @@ __global__ void __launch_bounds__(256) kv4_merge_kernel(Kv4AttnArgs a, long long
   const int late = kv4_span(total, spans, c0) < first ? 1 : 0;
   pdl_wait();
   pdl_trigger();
-  if (!live || c0 == c1) return;  // the same for every warp of a row; with W == 8 for the whole CTA
-  const float2* ml = a.ml + r % kRows;
-  float M = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, ml[(2 * c + (c == c0 ? late : 0)) * kRows].x);
+  if (!live || c0 == c1) return;  // the same for every warp of a row; with one row a CTA for the whole CTA
+  // one pass with a running maximum: no load waits for another
+  float M = -INFINITY, L = 0.f, v[E] = {};
+  auto take = [&](float m2, float l2, const float(&x)[E]) {
+    const float top = fmaxf(M, m2), base = top == -INFINITY ? 0.f : top;
+    const float f = ex2(M - base), f2 = ex2(m2 - base);
+    M = top;
+    L = fmaf(L, f, l2 * f2);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  const float Mu = M == -INFINITY ? 0.f : M;
-  float L = 0.f, v[E] = {};
+    for (int e = 0; e < E; ++e) v[e] = fmaf(v[e], f, x[e] * f2);
+  };
 #pragma unroll 8
   for (int c = c0 + w; c <= c1; c += W) {
-    const int part = (2 * c + (c == c0 ? late : 0)) * kRows;
-    const float2 x = ml[part];
-    const float f = ex2(x.x - Mu);
-    L = fmaf(x.y, f, L);
-    const float* p = a.acc + ((size_t)part + r % kRows) * D + lane * E;
+    const size_t part = (size_t)(2 * c + (c == c0 ? late : 0)) * kRows + r % kRows;
+    const float2 ml = a.ml[part];
+    const float* p = a.acc + part * D + lane * E;
+    float x[E];
     if constexpr (E == 4) {
       const float4 y = *reinterpret_cast<const float4*>(p);
-      v[0] = fmaf(y.x, f, v[0]), v[1] = fmaf(y.y, f, v[1]), v[E - 2] = fmaf(y.z, f, v[E - 2]);
-      v[E - 1] = fmaf(y.w, f, v[E - 1]);
+      x[0] = y.x, x[1] = y.y, x[E - 2] = y.z, x[E - 1] = y.w;
     } else {
       const float2 y = *reinterpret_cast<const float2*>(p);
-      v[0] = fmaf(y.x, f, v[0]), v[1] = fmaf(y.y, f, v[1]);
+      x[0] = y.x, x[1] = y.y;
     }
+    take(ml.x, ml.y, x);
   }
   if constexpr (W > 1) {
 #pragma unroll
     for (int e = 0; e < E; ++e) so[warp][lane * E + e] = v[e];
-    if (lane == 0) sl[warp] = L;
+    if (lane == 0) sl[warp] = make_float2(M, L);
     __syncthreads();
     if (warp != 0) return;
-    L = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = 0.f;
+    for (int x = 1; x < W; ++x) {
+      float y[E];
 #pragma unroll
-    for (int x = 0; x < W; ++x) {
-      L += sl[x];
-#pragma unroll
-      for (int e = 0; e < E; ++e) v[e] += so[x][lane * E + e];
+      for (int e = 0; e < E; ++e) y[e] = so[x][lane * E + e];
+      take(sl[x].x, sl[x].y, y);
     }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
@@ -691,7 +692,9 @@ static long long kv4_row_tiles(int heads, int kv_heads, int seq) {
   const long long rows = (long long)(heads / kv_heads) * seq, per = kv4_rows(heads, kv_heads, seq);
   return (rows + per - 1) / per;
 }
-// One resident round, or one block each where there are fewer.
+// One resident round, or one block each where there are fewer; a unit in at most about kKv4Parts parts, whose
+// joining would else take longer than the shorter spans save.
+constexpr int kKv4Parts = 128;
 static int kv4_ctas(int batch, int heads, int kv_heads, int seq, int kv_len, int head_dim) {
   const bool one = kv4_rows(heads, kv_heads, seq) == 8;
   const int most = 148 * (head_dim == 64 ? (one ? kKv4Resident<64, 1> : kKv4Resident<64, 2>)
@@ -699,7 +702,8 @@ static int kv4_ctas(int batch, int heads, int kv_heads, int seq, int kv_len, int
   const int block = kv4_block(one ? 8 : 16);
   const long long blocks = kv_len > 0 ? (kv_len + block - 1) / block : 1;
   const long long n = kv4_row_tiles(heads, kv_heads, seq) * kv_heads * batch;
-  return n >= most || n * blocks >= most ? most : (int)(n * blocks);
+  const long long ctas = n * (blocks < kKv4Parts ? blocks : kKv4Parts);
+  return n >= most || ctas >= most ? most : (int)ctas;
 }
 
 template <int D, int NT, bool OB>
@@ -713,7 +717,7 @@ static int run_kv4_attention(const Kv4AttnArgs& a, cudaStream_t st) {
   const long long rows = (long long)a.batch * a.heads * a.seq, units = (long long)a.batch * a.kv_heads * a.row_tiles;
   if (a.ctas <= 8 * units)
     return launch_k(kv4_merge_kernel<D, NT, 1, OB>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, a, rows);
-  return launch_k(kv4_merge_kernel<D, NT, 8, OB>, dim3((unsigned)rows), dim3(256), 0, st, a, rows);
+  return launch_k(kv4_merge_kernel<D, NT, 16, OB>, dim3((unsigned)rows), dim3(512), 0, st, a, rows);
 }
 
 }  // namespace ccut
