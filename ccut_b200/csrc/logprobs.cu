@@ -1,21 +1,48 @@
 // logprobs.cu -- log probability, entropy and rank of given tokens, and the top alternatives.
 //
-// Per row x of vocab logits and its token t, in fp32 (natural logarithms):
-//   logZ = m + log sum_v e^(x_v - m), m = max x;  logprob = x_t - logZ;
-//   entropy = log sum_v e^(x_v - m) - (sum_v e^(x_v - m) (x_v - m)) / sum_v e^(x_v - m);
-//   rank = 1 + #{v: x_v > x_t} + #{v < t: x_v = x_t};
-//   top n by descending value, ties to the lowest index, with their log probabilities.
+// Per row x of vocab logits and its token t (natural logarithms, fp32 sums):
+//   m = max x,  S = sum_v e^(x_v - m),  W = sum_v e^(x_v - m) (x_v - m),
+//   logprob = x_t - m - log S,  entropy = log S - W / S,
+//   rank = 1 + #{v: x_v > x_t} + #{v < t: x_v = x_t},
+//   top n by (value descending, index ascending) with their log probabilities.
+//
+// Bound: HBM, each logit read once.  A warp streams a contiguous part of a row in rounds of 512 logits
+// (16 a lane, the next round's loads in flight): about eight instructions a logit, so that the reading
+// stays in front.
+// - m moves once a round of a lane: the 16 logits' maximum first, then one exponential each; S and W are
+//   packed pairs (fma.rn.f32x2).  A lane that finds a new maximum rescales S and W, W by
+//   e^d (W + S d), d = m_old - m_new.
+// - rank: x >= x_t counts before t, x >= the next float above x_t behind it; only the round that holds t
+//   compares indices.
+// - Top n: each warp keeps its 32 best as 64-bit keys (order of the value, then of the index) sorted
+//   over its lanes.  One vote a round asks whether any lane's maximum reaches the n-th best; if so the
+//   logits that do are collected, and every 32 of them are sorted and merged in (bitonic, 20 exchanges).
+//   The first bar is the n-th largest of the first round's 32 lane maxima: at least n logits reach it.
+// Few rows are cut into up to 8 warps x several CTAs each, joined in shared memory and then by a second kernel;
+// many rows take fewer warps each, since every warp has to find its own best from the start.
 #include <math.h>
 
 #include "host.cuh"
 
 namespace ccut {
 
-template <bool BF16>
-CCUT_DEVICE float logit(const void* x, size_t i) {
-  if constexpr (BF16) return __uint_as_float((uint32_t) static_cast<const uint16_t*>(x)[i] << 16);
-  else return static_cast<const float*>(x)[i];
-}
+constexpr int kLpWarps = 8;
+constexpr int kLpRound = 512;    // logits a warp takes in a round
+constexpr float kL2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+typedef unsigned long long u64;
+
+struct LpArgs {
+  const void* x;
+  int vocab;
+  long long ld, rows;
+  const int32_t* tokens;
+  int top_n, wpr, ctas;  // warps per row in a CTA; CTAs per row
+  float *logprob, *entropy;
+  int32_t *rank, *top_ids;
+  float* top_lp;
+  float4* stats;  // [rows][ctas] m, S, W (in log2 units), count as int bits
+  u64* lists;     // [rows][ctas][32]
+};
 
 // The order of logits as integers: descending value is descending key, -0 equals +0, NaN comes last.
 CCUT_DEVICE int order_key(float x) {
@@ -23,95 +50,373 @@ CCUT_DEVICE int order_key(float x) {
   const int b = __float_as_int(x + 0.f);
   return b < 0 ? b ^ 0x7FFFFFFF : b;
 }
+CCUT_DEVICE u64 entry_of(float x, int i) {  // 0 is no entry
+  return ((u64)((uint32_t)order_key(x) ^ 0x80000000u) << 32) | (0xFFFFFFFFu - (uint32_t)i);
+}
+CCUT_DEVICE float entry_value(u64 e) {
+  const int k = (int)((uint32_t)(e >> 32) ^ 0x80000000u);
+  return k == -0x7FFFFFFF - 1 ? __int_as_float(0x7FFFFFFF) : __int_as_float(k < 0 ? k ^ 0x7FFFFFFF : k);
+}
+CCUT_DEVICE int entry_index(u64 e) { return (int)(0xFFFFFFFFu - (uint32_t)e); }
 
-CCUT_DEVICE float block_max(float v, float* red) {
+// Sorted over the lanes, descending: exchanges at distance j of the bitonic network; `up`: this lane's pair ascends.
+template <class T>
+CCUT_DEVICE T exchange(T v, int j, bool up, int lane) {
+  const T o = __shfl_xor_sync(0xffffffffu, v, j);
+  const bool low = (lane & j) == 0;          // the lane that keeps the larger when descending
+  return (low != up) == (v > o) ? v : o;
+}
+template <class T>
+CCUT_DEVICE T sort32(T v, int lane) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[0];
-  for (int w = 1; w < (int)blockDim.x / 32; ++w) v = fmaxf(v, red[w]);
+  for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+    for (int j = k >> 1; j > 0; j >>= 1) v = exchange(v, j, k < 32 && (lane & k) != 0, lane);
   return v;
 }
-CCUT_DEVICE float block_sum(float v, float* red) {
+// The 32 largest of two descending lists, descending.
+CCUT_DEVICE u64 merge32(u64 a, u64 b, int lane) {
+  const u64 r = __shfl_sync(0xffffffffu, b, 31 - lane);
+  u64 v = a > r ? a : r;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[0];
-  for (int w = 1; w < (int)blockDim.x / 32; ++w) v += red[w];
+  for (int j = 16; j > 0; j >>= 1) v = exchange(v, j, false, lane);
   return v;
 }
 
-// One CTA per row: a pass for the maximum, one for the sums and the rank, one per alternative.
+CCUT_DEVICE float lp_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+CCUT_DEVICE u64 pair(float a, float b) {
+  u64 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+CCUT_DEVICE void unpair(u64 p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+CCUT_DEVICE u64 add2(u64 a, u64 b) {
+  u64 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+CCUT_DEVICE u64 mul2(u64 a, u64 b) {
+  u64 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+CCUT_DEVICE u64 fma2(u64 a, u64 b, u64 c) {
+  u64 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+CCUT_DEVICE float max_nan(float a, float b) {  // NaN when either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 template <bool BF16>
-__global__ void __launch_bounds__(256) logprobs_simple_kernel(const void* __restrict__ logits, int vocab, long long ld,
-                                                              const int32_t* __restrict__ tokens, int top_n,
-                                                              float* __restrict__ logprob, float* __restrict__ entropy,
-                                                              int32_t* __restrict__ rank, int32_t* __restrict__ top_ids,
-                                                              float* __restrict__ top_lp) {
+CCUT_DEVICE float logit(const void* x, long long i) {
+  if constexpr (BF16) return __uint_as_float((uint32_t) static_cast<const uint16_t*>(x)[i] << 16);
+  else return static_cast<const float*>(x)[i];
+}
+
+// Maximum, S and W (log2 units) of a set of logits.
+struct LpSum {
+  float m = -INFINITY, s = 0.f, w = 0.f;
+  CCUT_DEVICE void move(float to) {  // to >= m
+    const float d = m == -INFINITY ? 0.f : (m - to) * kL2e, f = m == -INFINITY ? 0.f : lp_ex2(d);
+    w = f * fmaf(s, fmaxf(d, -1000.f), w);  // f is 0 long before the bound
+    s *= f;
+    m = to;
+  }
+  CCUT_DEVICE void join(LpSum o) {
+    if (o.m > m) move(o.m);
+    else if (m > o.m) o.move(m);
+    s += o.s;
+    w += o.w;
+  }
+};
+
+// The answers of a row from its joined state (one warp).
+template <bool BF16, bool TOP>
+CCUT_DEVICE void lp_finish(const LpArgs& a, long long row, const LpSum& sum, int count, u64 list, int lane) {
+  const float log_s = logf(sum.s);
+  if (lane == 0) {
+    const int t = a.tokens[row];
+    const bool has = t >= 0 && t < a.vocab;
+    const char* base = static_cast<const char*>(a.x) + row * a.ld * (BF16 ? 2 : 4);
+    a.logprob[row] = has ? (logit<BF16>(base, t) - sum.m) - log_s : __int_as_float(0x7FFFFFFF);
+    a.entropy[row] = log_s - sum.w * kLn2 / sum.s;
+    a.rank[row] = has ? count + 1 : 0;
+  }
+  if constexpr (TOP) {
+    if (lane < a.top_n) {
+      a.top_ids[row * a.top_n + lane] = entry_index(list);
+      a.top_lp[row * a.top_n + lane] = (entry_value(list) - sum.m) - log_s;
+    }
+  }
+}
+
+template <bool TOP>
+struct LpWarp {  // a warp's state; pending: 64 entries of shared memory
+  LpSum sum;
+  int count = 0;  // of the rank, per lane
+  u64 list = 0, bar = 0;
+  float bar_value = -INFINITY;  // logits below it are not among the best
+  int pend = 0, head = 0;
+  bool first = true;
+  u64* pending;
+
+  CCUT_DEVICE void flush(int n, int top_n, int lane) {  // the oldest n <= 32 pending entries
+    __syncwarp();
+    u64 e = lane < n ? pending[(head + lane) & 63] : 0;
+    __syncwarp();
+    list = merge32(list, sort32(e, lane), lane);
+    head += n;
+    pend -= n;
+    const u64 nth = __shfl_sync(0xffffffffu, list, top_n - 1);
+    if (nth > bar) {
+      bar = nth;
+      bar_value = entry_value(nth);
+    }
+  }
+
+  // One round: 16 logits a lane; index(i) of logit i; kChecked: those with !valid(i) do not exist.
+  template <bool kChecked, class Index, class Valid>
+  CCUT_DEVICE void round(const float (&x)[16], Index index, Valid valid, int begin, int end, int t, float xt, float above,
+                         int top_n, int lane) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (!kChecked || valid(i)) top = fmaxf(top, x[i]);
+    if (top > sum.m) sum.move(top);
+    const float mu = sum.m == -INFINITY ? 0.f : sum.m;
+    const u64 neg = pair(-mu, -mu), scale = pair(kL2e, kL2e);
+    u64 s2 = 0, w2 = 0;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      u64 d = mul2(add2(pair(x[i], x[i + 1]), neg), scale);
+      float a, b;
+      unpair(d, a, b);
+      a = max_nan(a, -1000.f);  // e^a is 0 there, and 0 * -inf is not
+      b = max_nan(b, -1000.f);
+      if constexpr (kChecked) {
+        a = valid(i) ? a : -1000.f;
+        b = valid(i + 1) ? b : -1000.f;
+      }
+      const u64 e = pair(lp_ex2(a), lp_ex2(b));
+      s2 = add2(s2, e);
+      w2 = fma2(e, pair(a, b), w2);
+    }
+    float a, b;
+    unpair(s2, a, b);
+    sum.s += a + b;
+    unpair(w2, a, b);
+    sum.w += a + b;
+    if (!kChecked && (end <= t || begin > t)) {
+      const float bound = begin > t ? above : xt;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) count += x[i] >= bound;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (!kChecked || valid(i)) count += x[i] >= (index(i) < t ? xt : above) && index(i) != t;
+    }
+    if constexpr (TOP) {
+      if (first) {
+        first = false;
+        const float nth = __shfl_sync(0xffffffffu, sort32(top, lane), top_n - 1);
+        if (nth > -INFINITY) {
+          bar = entry_of(nth, -1) & ~0xFFFFFFFFull;  // every logit of this value passes
+          bar_value = nth;
+        }
+      }
+      if (__any_sync(0xffffffffu, !(top < bar_value))) {
+        uint32_t reach = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) reach |= (!kChecked || valid(i)) && !(x[i] < bar_value) ? 1u << i : 0u;
+        while (__any_sync(0xffffffffu, reach != 0)) {  // one logit a lane at a time
+          const int i = reach ? __ffs(reach) - 1 : 0;
+          float v = x[0];
+#pragma unroll
+          for (int j = 1; j < 16; ++j) v = j == i ? x[j] : v;  // registers have no index
+          const u64 e = reach ? entry_of(v, index(i)) : 0;
+          reach &= reach - 1;
+          const unsigned pass = __ballot_sync(0xffffffffu, e > bar);
+          if (e > bar) pending[(head + pend + __popc(pass & ((1u << lane) - 1))) & 63] = e;
+          pend += __popc(pass);
+          if (pend >= 32) flush(32, top_n, lane);
+        }
+      }
+    }
+  }
+};
+
+template <bool BF16, bool TOP>
+__global__ void __launch_bounds__(kLpWarps * 32, 3) logprobs_kernel(LpArgs a) {
   pdl_wait();
   pdl_trigger();
-  __shared__ float red[8];
-  __shared__ int redi[8], redk[8];
-  const size_t base = (size_t)blockIdx.x * (size_t)ld;
-  const int t = tokens[blockIdx.x];
-  const bool ok = t >= 0 && t < vocab;
-  const float xt = ok ? logit<BF16>(logits, base + t) : 0.f;
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < vocab; i += 256) m = fmaxf(m, logit<BF16>(logits, base + i));
-  m = block_max(m, red);
-  float s = 0.f, w = 0.f;
-  int r = 0;
-  const int kt = order_key(xt);
-  for (int i = threadIdx.x; i < vocab; i += 256) {
-    const float x = logit<BF16>(logits, base + i), e = expf(x - m);
-    s += e;
-    if (e > 0.f) w = fmaf(e, x - m, w);
-    const int k = order_key(x);
-    r += k > kt || (k == kt && i < t);
-  }
-  s = block_sum(s, red);
-  w = block_sum(w, red);
-  r = __reduce_add_sync(0xffffffffu, r);
-  if ((threadIdx.x & 31) == 0) redi[threadIdx.x >> 5] = r;
-  __syncthreads();
-  r = 0;
-  for (int o = 0; o < 8; ++o) r += redi[o];
-  __syncthreads();
-  const float lz = logf(s);
-  if (threadIdx.x == 0) {
-    logprob[blockIdx.x] = ok ? (xt - m) - lz : __int_as_float(0x7FFFFFFF);
-    entropy[blockIdx.x] = lz - w / s;
-    rank[blockIdx.x] = ok ? 1 + r : 0;
-  }
-  int lastk = 0x7FFFFFFF, lasti = -1;
-  for (int j = 0; j < top_n; ++j) {  // the first entry after (lastk, lasti) in the order
-    int bk = -0x7FFFFFFF - 1, bi = 0x7FFFFFFF;
-    for (int i = threadIdx.x; i < vocab; i += 256) {
-      const int k = order_key(logit<BF16>(logits, base + i));
-      if (!(k < lastk || (k == lastk && i > lasti))) continue;
-      if (k > bk || (k == bk && i < bi)) bk = k, bi = i;
-    }
+  __shared__ u64 pending[TOP ? kLpWarps : 1][TOP ? 64 : 1];
+  __shared__ u64 lists[TOP ? kLpWarps : 1][TOP ? 32 : 1];
+  __shared__ float4 stats[kLpWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rows_per_cta = kLpWarps / a.wpr;
+  const long long row = (long long)(blockIdx.x / a.ctas) * rows_per_cta + warp / a.wpr;
+  const int cta = blockIdx.x % a.ctas, part = cta * a.wpr + warp % a.wpr, parts = a.ctas * a.wpr;
+  const bool live = row < a.rows;
+  LpWarp<TOP> st;
+  st.pending = pending[TOP ? warp : 0];
+  if (live) {
+    constexpr int kVec = BF16 ? 8 : 4;  // logits per 16 bytes
+    const char* base = static_cast<const char*>(a.x) + row * a.ld * (BF16 ? 2 : 4);
+    const int t = a.tokens[row];
+    const bool has = t >= 0 && t < a.vocab;
+    const float xt = has ? logit<BF16>(base, t) : __int_as_float(0x7FFFFFFF);  // no token: nothing counts
+    // the least float above xt: x > xt is x >= above (x_t = +inf: nothing is above, NaN compares false)
+    const int kt = order_key(xt) + 1;
+    const float above = isnan(xt) || xt == INFINITY ? __int_as_float(0x7FFFFFFF) : __int_as_float(kt < 0 ? kt ^ 0x7FFFFFFF : kt);
+    const int lead = min(a.vocab, (int)((16 - (reinterpret_cast<uintptr_t>(base) & 15)) & 15) / (BF16 ? 2 : 4));
+    const int whole = (a.vocab - lead) / kLpRound;  // rounds of aligned 16-byte vectors
+    const int r0 = (int)((long long)whole * part / parts), r1 = (int)((long long)whole * (part + 1) / parts);
+    const uint4* src = reinterpret_cast<const uint4*>(base + (size_t)lead * (BF16 ? 2 : 4)) + lane;
+    constexpr int kLoads = 16 / kVec;
+    uint4 next[kLoads];
+    auto fetch = [&](int r) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const int ok2 = __shfl_xor_sync(0xffffffffu, bk, o), oi = __shfl_xor_sync(0xffffffffu, bi, o);
-      if (ok2 > bk || (ok2 == bk && oi < bi)) bk = ok2, bi = oi;
+      for (int j = 0; j < kLoads; ++j) next[j] = __ldcs(src + (size_t)r * (kLpRound / kVec) + j * 32);
+    };
+    if (r0 < r1) fetch(r0);
+    for (int r = r0; r < r1; ++r) {
+      float x[16];
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const uint32_t w[4] = {next[j].x, next[j].y, next[j].z, next[j].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (BF16) {
+            x[j * 8 + 2 * e] = __uint_as_float(w[e] << 16);
+            x[j * 8 + 2 * e + 1] = __uint_as_float(w[e] & 0xFFFF0000u);
+          } else {
+            x[j * 4 + e] = __uint_as_float(w[e]);
+          }
+        }
+      }
+      if (r + 1 < r1) fetch(r + 1);
+      const int begin = lead + r * kLpRound;
+      st.template round<false>(
+          x, [&](int i) { return begin + i / kVec * (32 * kVec) + lane * kVec + i % kVec; }, [](int) { return true; },
+          begin, begin + kLpRound, t, xt, above, a.top_n, lane);
     }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) redk[threadIdx.x >> 5] = bk, redi[threadIdx.x >> 5] = bi;
-    __syncthreads();
-    for (int o = 0; o < 8; ++o)
-      if (redk[o] > bk || (redk[o] == bk && redi[o] < bi)) bk = redk[o], bi = redi[o];
-    lastk = bk;
-    lasti = bi;
-    if (threadIdx.x == 0) {
-      top_ids[(size_t)blockIdx.x * top_n + j] = bi;
-      top_lp[(size_t)blockIdx.x * top_n + j] = (logit<BF16>(logits, base + bi) - m) - lz;
+    if (part == parts - 1) {  // what the vectors leave: the tail, then the head
+      for (int side = 0; side < 2; ++side) {
+        const int begin = side ? 0 : lead + whole * kLpRound, end = side ? lead : a.vocab;
+        if (begin >= end) continue;
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int v = begin + i * 32 + lane;
+          x[i] = v < end ? logit<BF16>(base, v) : 0.f;
+        }
+        st.template round<true>(
+            x, [&](int i) { return begin + i * 32 + lane; }, [&](int i) { return begin + i * 32 + lane < end; }, begin,
+            end, t, xt, above, a.top_n, lane);
+      }
+    }
+    if (has && isnan(xt)) {  // NaN is last in the order: everything else is before it, and NaN of lower index
+      st.count = 0;
+      const int v0 = part == 0 ? 0 : lead + r0 * kLpRound, v1 = part == parts - 1 ? a.vocab : lead + r1 * kLpRound;
+      for (int v = v0 + lane; v < v1; v += 32) st.count += !isnan(logit<BF16>(base, v)) || v < t;
     }
   }
+  if constexpr (TOP)
+    if (st.pend > 0) st.flush(st.pend, a.top_n, lane);  // fewer than 32
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    LpSum y;
+    y.m = __shfl_xor_sync(0xffffffffu, st.sum.m, o);
+    y.s = __shfl_xor_sync(0xffffffffu, st.sum.s, o);
+    y.w = __shfl_xor_sync(0xffffffffu, st.sum.w, o);
+    st.sum.join(y);
+  }
+  int count = __reduce_add_sync(0xffffffffu, st.count);
+  if (a.wpr > 1) {
+    if (lane == 0) stats[warp] = make_float4(st.sum.m, st.sum.s, st.sum.w, __int_as_float(count));
+    if constexpr (TOP) lists[warp][lane] = st.list;
+    __syncthreads();
+    if (warp % a.wpr) return;
+    for (int w = 1; w < a.wpr; ++w) {
+      const float4 y = stats[warp + w];
+      LpSum s;
+      s.m = y.x, s.s = y.y, s.w = y.z;
+      st.sum.join(s);
+      count += __float_as_int(y.w);
+      if constexpr (TOP) st.list = merge32(st.list, lists[warp + w][lane], lane);
+    }
+  }
+  if (!live) return;
+  if (a.ctas > 1) {
+    if (lane == 0) a.stats[row * a.ctas + cta] = make_float4(st.sum.m, st.sum.s, st.sum.w, __int_as_float(count));
+    if constexpr (TOP) a.lists[(row * a.ctas + cta) * 32 + lane] = st.list;
+    return;
+  }
+  lp_finish<BF16, TOP>(a, row, st.sum, count, st.list, lane);
+}
+
+// Joins the CTAs' parts of a row: one CTA per row, warp w takes parts w, w + 8, ..
+template <bool BF16, bool TOP>
+__global__ void __launch_bounds__(kLpWarps * 32) logprobs_join_kernel(LpArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ u64 lists[TOP ? kLpWarps : 1][TOP ? 32 : 1];
+  __shared__ float4 stats[kLpWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long row = blockIdx.x;
+  LpSum sum;
+  int count = 0;
+  u64 list = 0;
+#pragma unroll 4
+  for (int c = warp; c < a.ctas; c += kLpWarps) {
+    const float4 y = a.stats[row * a.ctas + c];
+    LpSum s;
+    s.m = y.x, s.s = y.y, s.w = y.z;
+    sum.join(s);
+    count += __float_as_int(y.w);
+    if constexpr (TOP) list = merge32(list, a.lists[(row * a.ctas + c) * 32 + lane], lane);
+  }
+  if (lane == 0) stats[warp] = make_float4(sum.m, sum.s, sum.w, __int_as_float(count));
+  if constexpr (TOP) lists[warp][lane] = list;
+  __syncthreads();
+  if (warp) return;
+  for (int w = 1; w < kLpWarps; ++w) {
+    const float4 y = stats[w];
+    LpSum s;
+    s.m = y.x, s.s = y.y, s.w = y.z;
+    sum.join(s);
+    count += __float_as_int(y.w);
+    if constexpr (TOP) list = merge32(list, lists[w][lane], lane);
+  }
+  lp_finish<BF16, TOP>(a, row, sum, count, list, lane);
+}
+
+// Warps per row and CTAs per row: at least 16 warps an SM, a round of logits or more for each warp.
+static void lp_split(long long rows, int vocab, int& wpr, int& ctas) {
+  const long long want = 148LL * 16;
+  wpr = rows >= 2 * want ? 1 : rows >= want ? 2 : rows >= want / 2 ? 4 : 8;
+  ctas = 1;
+  if (rows * wpr < want) {
+    long long c = want / (rows * wpr), most = vocab / (2 * kLpRound * wpr);
+    if (c > most) c = most;
+    ctas = c < 1 ? 1 : (int)c;
+  }
+}
+
+template <bool BF16, bool TOP>
+static int run_logprobs(const LpArgs& a, cudaStream_t st) {
+  const long long groups = (a.rows + kLpWarps / a.wpr - 1) / (kLpWarps / a.wpr);
+  int rc = launch_k(logprobs_kernel<BF16, TOP>, dim3((unsigned)(groups * a.ctas)), dim3(kLpWarps * 32), 0, st, a);
+  if (rc || a.ctas == 1) return rc;
+  return launch_k(logprobs_join_kernel<BF16, TOP>, dim3((unsigned)a.rows), dim3(kLpWarps * 32), 0, st, a);
 }
 
 }  // namespace ccut
@@ -122,7 +427,9 @@ extern "C" {
 
 size_t ccut_token_logprobs_workspace_bytes(int rows, int vocab, int top_n) {
   if (rows < 0 || vocab <= 0 || top_n < 0) return 0;
-  return 256;
+  int wpr, ctas;
+  lp_split(rows > 0 ? rows : 1, vocab, wpr, ctas);
+  return ctas > 1 ? 256 + (size_t)rows * ctas * (sizeof(float4) + 32 * sizeof(u64)) : 256;
 }
 
 int ccut_token_logprobs(const void* logits, int dtype, int rows, int vocab, long long ld, const int32_t* tokens,
@@ -135,10 +442,18 @@ int ccut_token_logprobs(const void* logits, int dtype, int rows, int vocab, long
   if (rows == 0) return CCUT_OK;
   if (!logits || !tokens || !logprob || !entropy || !rank || (top_n > 0 && (!top_ids || !top_logprobs)))
     return CCUT_ERR_INVALID;
-  if (ws_bytes < ccut_token_logprobs_workspace_bytes(rows, vocab, top_n) || !workspace) return CCUT_ERR_WORKSPACE;
-  auto kern = dtype == CCUT_OUT_BF16 ? logprobs_simple_kernel<true> : logprobs_simple_kernel<false>;
-  return launch_k(kern, dim3(rows), dim3(256), 0, stream, logits, vocab, ld, tokens, top_n, logprob, entropy, rank,
-                  top_ids, top_logprobs);
+  if (reinterpret_cast<uintptr_t>(logits) % (dtype == CCUT_OUT_BF16 ? 2 : 4)) return CCUT_ERR_INVALID;
+  if (vocab > 2147483647 - 2 * kLpRound) return CCUT_ERR_UNSUPPORTED;
+  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 ||
+      ws_bytes < ccut_token_logprobs_workspace_bytes(rows, vocab, top_n))
+    return CCUT_ERR_WORKSPACE;
+  LpArgs a{logits, vocab, ld, rows, tokens, top_n, 1, 1, logprob, entropy, rank, top_ids, top_logprobs, nullptr, nullptr};
+  lp_split(rows, vocab, a.wpr, a.ctas);
+  a.stats = reinterpret_cast<float4*>(static_cast<uint8_t*>(workspace) + 256);
+  a.lists = reinterpret_cast<u64*>(a.stats + (size_t)rows * a.ctas);
+  if (dtype == CCUT_OUT_BF16)
+    return top_n ? run_logprobs<true, true>(a, stream) : run_logprobs<true, false>(a, stream);
+  return top_n ? run_logprobs<false, true>(a, stream) : run_logprobs<false, false>(a, stream);
 }
 
 }  // extern "C"
