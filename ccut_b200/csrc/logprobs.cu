@@ -16,8 +16,9 @@
 //   compares indices.
 // - Top n: each warp keeps its 32 best as 64-bit keys (order of the value, then of the index) sorted
 //   over its lanes.  One vote a round asks whether any lane's maximum reaches the n-th best; if so the
-//   logits that do are collected, and every 32 of them are sorted and merged in (bitonic, 20 exchanges).
-//   The first bar is the n-th largest of the first round's 32 lane maxima: at least n logits reach it.
+//   logits that do are inserted one by one, each by a vote for its place and one shift of the lanes.
+//   The first list is the first round's 32 lane maxima.
+//   Warps of one row publish their ceil(n / warps)-th best; the least of these is a bar for all.
 // Few rows are cut into up to 8 warps x several CTAs each, joined in shared memory and then by a second kernel;
 // many rows take fewer warps each, since every warp has to find its own best from the start.
 #include <math.h>
@@ -115,6 +116,12 @@ CCUT_DEVICE float max_nan(float a, float b) {  // NaN when either is
   return r;
 }
 
+CCUT_DEVICE float at_least(float a, float b) {  // 1 or 0
+  float r;
+  asm("set.ge.f32.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 template <bool BF16>
 CCUT_DEVICE float logit(const void* x, long long i) {
   if constexpr (BF16) return __uint_as_float((uint32_t) static_cast<const uint16_t*>(x)[i] << 16);
@@ -158,27 +165,57 @@ CCUT_DEVICE void lp_finish(const LpArgs& a, long long row, const LpSum& sum, int
   }
 }
 
+// Joins the states of each `n` (a power of two) consecutive warps into the first of them, pairwise.  Whole CTA.
+template <bool TOP, class Stats, class Lists>
+CCUT_DEVICE void lp_tree(LpSum& sum, int& count, u64& list, Stats& stats, Lists& lists, int warp, int lane, int n) {
+  for (int s = 1; s < n; s <<= 1) {
+    if (warp % (2 * s) == s) {
+      if (lane == 0) stats[warp] = make_float4(sum.m, sum.s, sum.w, __int_as_float(count));
+      if constexpr (TOP) lists[warp][lane] = list;
+    }
+    __syncthreads();
+    if (warp % (2 * s) == 0) {
+      const float4 y = stats[warp + s];
+      LpSum o;
+      o.m = y.x, o.s = y.y, o.w = y.z;
+      sum.join(o);
+      count += __float_as_int(y.w);
+      if constexpr (TOP) list = merge32(list, lists[warp + s][lane], lane);
+    }
+  }
+}
+
 template <bool TOP>
-struct LpWarp {  // a warp's state; pending: 64 entries of shared memory
+struct LpWarp {  // a warp's state
   LpSum sum;
   int count = 0;  // of the rank, per lane
   u64 list = 0, bar = 0;
   float bar_value = -INFINITY;  // logits below it are not among the best
-  int pend = 0, head = 0;
   bool first = true;
-  u64* pending;
+  volatile float *row_bar, *mine;  // shared memory: the row's warps' published values, this warp's
+  int share;                       // ceil(top_n / warps of the row in this CTA)
 
-  CCUT_DEVICE void flush(int n, int top_n, int lane) {  // the oldest n <= 32 pending entries
-    __syncwarp();
-    u64 e = lane < n ? pending[(head + lane) & 63] : 0;
-    __syncwarp();
-    list = merge32(list, sort32(e, lane), lane);
-    head += n;
-    pend -= n;
+  CCUT_DEVICE void insert(u64 e, int lane) {  // e the same in every lane
+    const int at = __popc(__ballot_sync(0xffffffffu, list > e));
+    const u64 before = __shfl_up_sync(0xffffffffu, list, 1);
+    list = lane < at ? list : lane == at ? e : before;
+  }
+  CCUT_DEVICE void raise(int top_n, int lane) {
     const u64 nth = __shfl_sync(0xffffffffu, list, top_n - 1);
     if (nth > bar) {
       bar = nth;
       bar_value = entry_value(nth);
+    }
+    if (lane == share - 1 && list) mine[0] = entry_value(list);
+  }
+  // At least `share` logits of each of the row's `wpr` warps here reach its published value: at least top_n reach
+  // the least of them.
+  CCUT_DEVICE void look(int wpr) {
+    float least = row_bar[0];
+    for (int w = 1; w < wpr; ++w) least = fminf(least, row_bar[w]);
+    if (least > bar_value) {
+      bar_value = least;
+      bar = entry_of(least, -1) & ~0xFFFFFFFFull;  // every logit of this value passes
     }
   }
 
@@ -186,29 +223,37 @@ struct LpWarp {  // a warp's state; pending: 64 entries of shared memory
   template <bool kChecked, class Index, class Valid>
   CCUT_DEVICE void round(const float (&x)[16], Index index, Valid valid, int begin, int end, int t, float xt, float above,
                          int top_n, int lane) {
-    float top = -INFINITY;
+    float top = -INFINITY, low = INFINITY;
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      if (!kChecked || valid(i)) top = fmaxf(top, x[i]);
+      if (!kChecked || valid(i)) top = fmaxf(top, x[i]), low = fminf(low, x[i]);
     if (top > sum.m) sum.move(top);
     const float mu = sum.m == -INFINITY ? 0.f : sum.m;
     const u64 neg = pair(-mu, -mu), scale = pair(kL2e, kL2e);
     u64 s2 = 0, w2 = 0;
+    auto terms = [&](auto far_tag) {  // kFar: logits so low that e^a is 0, where 0 * -inf is not
+      constexpr bool kFar = decltype(far_tag)::value;
 #pragma unroll
-    for (int i = 0; i < 16; i += 2) {
-      u64 d = mul2(add2(pair(x[i], x[i + 1]), neg), scale);
-      float a, b;
-      unpair(d, a, b);
-      a = max_nan(a, -1000.f);  // e^a is 0 there, and 0 * -inf is not
-      b = max_nan(b, -1000.f);
-      if constexpr (kChecked) {
-        a = valid(i) ? a : -1000.f;
-        b = valid(i + 1) ? b : -1000.f;
+      for (int i = 0; i < 16; i += 2) {
+        u64 d = mul2(add2(pair(x[i], x[i + 1]), neg), scale);
+        float a, b;
+        unpair(d, a, b);
+        if constexpr (kFar) {
+          a = max_nan(a, -1000.f);
+          b = max_nan(b, -1000.f);
+          if constexpr (kChecked) {
+            a = valid(i) ? a : -1000.f;
+            b = valid(i + 1) ? b : -1000.f;
+          }
+          d = pair(a, b);
+        }
+        const u64 e = pair(lp_ex2(a), lp_ex2(b));
+        s2 = add2(s2, e);
+        w2 = fma2(e, d, w2);
       }
-      const u64 e = pair(lp_ex2(a), lp_ex2(b));
-      s2 = add2(s2, e);
-      w2 = fma2(e, pair(a, b), w2);
-    }
+    };
+    if (kChecked || __any_sync(0xffffffffu, low - mu < -600.f)) terms(std::true_type{});
+    else terms(std::false_type{});
     float a, b;
     unpair(s2, a, b);
     sum.s += a + b;
@@ -216,26 +261,31 @@ struct LpWarp {  // a warp's state; pending: 64 entries of shared memory
     sum.w += a + b;
     if (!kChecked && (end <= t || begin > t)) {
       const float bound = begin > t ? above : xt;
+      u64 n2 = 0;  // counted as floats: the adds take the pipe that has room
 #pragma unroll
-      for (int i = 0; i < 16; ++i) count += x[i] >= bound;
+      for (int i = 0; i < 16; i += 2) n2 = add2(n2, pair(at_least(x[i], bound), at_least(x[i + 1], bound)));
+      unpair(n2, a, b);
+      count += (int)(a + b);
     } else {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         if (!kChecked || valid(i)) count += x[i] >= (index(i) < t ? xt : above) && index(i) != t;
     }
     if constexpr (TOP) {
-      if (first) {
+      int taken = 16;
+      if (first) {  // the lanes' maxima are the first list
         first = false;
-        const float nth = __shfl_sync(0xffffffffu, sort32(top, lane), top_n - 1);
-        if (nth > -INFINITY) {
-          bar = entry_of(nth, -1) & ~0xFFFFFFFFull;  // every logit of this value passes
-          bar_value = nth;
-        }
+#pragma unroll
+        for (int i = 15; i >= 0; --i)
+          if ((!kChecked || valid(i)) && x[i] == top) taken = i;
+        list = sort32(taken < 16 ? entry_of(top, index(taken)) : 0ull, lane);
+        raise(top_n, lane);
       }
       if (__any_sync(0xffffffffu, !(top < bar_value))) {
-        uint32_t reach = 0;
+        uint32_t reach = 0;  // this lane's logits that may be among the best
 #pragma unroll
         for (int i = 0; i < 16; ++i) reach |= (!kChecked || valid(i)) && !(x[i] < bar_value) ? 1u << i : 0u;
+        reach &= ~(1u << taken);
         while (__any_sync(0xffffffffu, reach != 0)) {  // one logit a lane at a time
           const int i = reach ? __ffs(reach) - 1 : 0;
           float v = x[0];
@@ -243,10 +293,9 @@ struct LpWarp {  // a warp's state; pending: 64 entries of shared memory
           for (int j = 1; j < 16; ++j) v = j == i ? x[j] : v;  // registers have no index
           const u64 e = reach ? entry_of(v, index(i)) : 0;
           reach &= reach - 1;
-          const unsigned pass = __ballot_sync(0xffffffffu, e > bar);
-          if (e > bar) pending[(head + pend + __popc(pass & ((1u << lane) - 1))) & 63] = e;
-          pend += __popc(pass);
-          if (pend >= 32) flush(32, top_n, lane);
+          unsigned pass = __ballot_sync(0xffffffffu, e > bar);
+          for (; pass; pass &= pass - 1) insert(__shfl_sync(0xffffffffu, e, __ffs(pass) - 1), lane);
+          raise(top_n, lane);
         }
       }
     }
@@ -257,7 +306,7 @@ template <bool BF16, bool TOP>
 __global__ void __launch_bounds__(kLpWarps * 32, 3) logprobs_kernel(LpArgs a) {
   pdl_wait();
   pdl_trigger();
-  __shared__ u64 pending[TOP ? kLpWarps : 1][TOP ? 64 : 1];
+  __shared__ float bars[kLpWarps];
   __shared__ u64 lists[TOP ? kLpWarps : 1][TOP ? 32 : 1];
   __shared__ float4 stats[kLpWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -266,7 +315,13 @@ __global__ void __launch_bounds__(kLpWarps * 32, 3) logprobs_kernel(LpArgs a) {
   const int cta = blockIdx.x % a.ctas, part = cta * a.wpr + warp % a.wpr, parts = a.ctas * a.wpr;
   const bool live = row < a.rows;
   LpWarp<TOP> st;
-  st.pending = pending[TOP ? warp : 0];
+  st.row_bar = bars + warp / a.wpr * a.wpr;
+  st.mine = &bars[warp];
+  st.share = (a.top_n + a.wpr - 1) / a.wpr;
+  if constexpr (TOP) {
+    if (lane == 0) bars[warp] = -INFINITY;
+    __syncthreads();
+  }
   if (live) {
     constexpr int kVec = BF16 ? 8 : 4;  // logits per 16 bytes
     const char* base = static_cast<const char*>(a.x) + row * a.ld * (BF16 ? 2 : 4);
@@ -303,6 +358,7 @@ __global__ void __launch_bounds__(kLpWarps * 32, 3) logprobs_kernel(LpArgs a) {
         }
       }
       if (r + 1 < r1) fetch(r + 1);
+      if constexpr (TOP) st.look(a.wpr);
       const int begin = lead + r * kLpRound;
       st.template round<false>(
           x, [&](int i) { return begin + i / kVec * (32 * kVec) + lane * kVec + i % kVec; }, [](int) { return true; },
@@ -329,8 +385,6 @@ __global__ void __launch_bounds__(kLpWarps * 32, 3) logprobs_kernel(LpArgs a) {
       for (int v = v0 + lane; v < v1; v += 32) st.count += !isnan(logit<BF16>(base, v)) || v < t;
     }
   }
-  if constexpr (TOP)
-    if (st.pend > 0) st.flush(st.pend, a.top_n, lane);  // fewer than 32
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     LpSum y;
@@ -341,18 +395,8 @@ __global__ void __launch_bounds__(kLpWarps * 32, 3) logprobs_kernel(LpArgs a) {
   }
   int count = __reduce_add_sync(0xffffffffu, st.count);
   if (a.wpr > 1) {
-    if (lane == 0) stats[warp] = make_float4(st.sum.m, st.sum.s, st.sum.w, __int_as_float(count));
-    if constexpr (TOP) lists[warp][lane] = st.list;
-    __syncthreads();
+    lp_tree<TOP>(st.sum, count, st.list, stats, lists, warp, lane, a.wpr);
     if (warp % a.wpr) return;
-    for (int w = 1; w < a.wpr; ++w) {
-      const float4 y = stats[warp + w];
-      LpSum s;
-      s.m = y.x, s.s = y.y, s.w = y.z;
-      st.sum.join(s);
-      count += __float_as_int(y.w);
-      if constexpr (TOP) st.list = merge32(st.list, lists[warp + w][lane], lane);
-    }
   }
   if (!live) return;
   if (a.ctas > 1) {
@@ -384,25 +428,18 @@ __global__ void __launch_bounds__(kLpWarps * 32) logprobs_join_kernel(LpArgs a) 
     count += __float_as_int(y.w);
     if constexpr (TOP) list = merge32(list, a.lists[(row * a.ctas + c) * 32 + lane], lane);
   }
-  if (lane == 0) stats[warp] = make_float4(sum.m, sum.s, sum.w, __int_as_float(count));
-  if constexpr (TOP) lists[warp][lane] = list;
-  __syncthreads();
+  lp_tree<TOP>(sum, count, list, stats, lists, warp, lane, kLpWarps);
   if (warp) return;
-  for (int w = 1; w < kLpWarps; ++w) {
-    const float4 y = stats[w];
-    LpSum s;
-    s.m = y.x, s.s = y.y, s.w = y.z;
-    sum.join(s);
-    count += __float_as_int(y.w);
-    if constexpr (TOP) list = merge32(list, lists[w][lane], lane);
-  }
   lp_finish<BF16, TOP>(a, row, sum, count, list, lane);
 }
 
-// Warps per row and CTAs per row: at least 16 warps an SM, a round of logits or more for each warp.
-static void lp_split(long long rows, int vocab, int& wpr, int& ctas) {
+// Warps per row and CTAs per row.  At least 16 warps an SM, two rounds of logits or more for each.  With
+// alternatives many rows take fewer warps each (2047 rows of 102400, top 20: 193 us with 8 warps a row, 171
+// with 4, 176 with 1); without, eight keep the last round of CTAs short (136 us; 146 with 4).
+static void lp_split(long long rows, int vocab, int top_n, int& wpr, int& ctas) {
   const long long want = 148LL * 16;
-  wpr = rows >= 2 * want ? 1 : rows >= want ? 2 : rows >= want / 2 ? 4 : 8;
+  wpr = top_n == 0 ? 8 : rows >= 2 * want ? 1 : rows >= want ? 2 : rows >= want / 2 ? 4 : 8;
+  while (wpr > 1 && vocab < 2 * kLpRound * wpr) wpr /= 2;
   ctas = 1;
   if (rows * wpr < want) {
     long long c = want / (rows * wpr), most = vocab / (2 * kLpRound * wpr);
@@ -428,7 +465,7 @@ extern "C" {
 size_t ccut_token_logprobs_workspace_bytes(int rows, int vocab, int top_n) {
   if (rows < 0 || vocab <= 0 || top_n < 0) return 0;
   int wpr, ctas;
-  lp_split(rows > 0 ? rows : 1, vocab, wpr, ctas);
+  lp_split(rows > 0 ? rows : 1, vocab, top_n, wpr, ctas);
   return ctas > 1 ? 256 + (size_t)rows * ctas * (sizeof(float4) + 32 * sizeof(u64)) : 256;
 }
 
@@ -448,7 +485,7 @@ int ccut_token_logprobs(const void* logits, int dtype, int rows, int vocab, long
       ws_bytes < ccut_token_logprobs_workspace_bytes(rows, vocab, top_n))
     return CCUT_ERR_WORKSPACE;
   LpArgs a{logits, vocab, ld, rows, tokens, top_n, 1, 1, logprob, entropy, rank, top_ids, top_logprobs, nullptr, nullptr};
-  lp_split(rows, vocab, a.wpr, a.ctas);
+  lp_split(rows, vocab, top_n, a.wpr, a.ctas);
   a.stats = reinterpret_cast<float4*>(static_cast<uint8_t*>(workspace) + 256);
   a.lists = reinterpret_cast<u64*>(a.stats + (size_t)rows * a.ctas);
   if (dtype == CCUT_OUT_BF16)
