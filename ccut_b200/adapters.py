@@ -114,7 +114,7 @@ class LoraBank:
         ids = ids if ids.is_contiguous() else ids.contiguous()
         lib = _lib.load()
         with torch.cuda.device(self.device):
-            nbytes = lib.ccut_lora_workspace_bytes(n, self.inputs, self.rank, len(self.widths))
+            nbytes = lib.ccut_lora_workspace_bytes(n, self.inputs, self.rank, len(self.widths), self.adapters)
             ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=self.device)
             _lib.call("ccut_lora_add", x.data_ptr(), self.a.data_ptr(), self.b.data_ptr(), self.scales.data_ptr(),
                       ids.data_ptr(), n, self.inputs, self.rank, self.adapters, len(self.widths), self._widths,

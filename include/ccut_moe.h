@@ -392,13 +392,14 @@ CCUT_API int ccut_token_logprobs(const void* logits, int dtype, int rows, int vo
  * adapter of its own: a bf16 [adapters, slices * rank, inputs], b bf16 [adapters, sum(widths),
  * rank], scales fp32 [adapters]; outputs of slice j take rank rows j * rank .. of a.  x bf16
  * [tokens, inputs]; base, out [tokens, sum(widths)] bf16 or fp32 (dtype) with rows base_ld / out_ld
- * elements apart (multiples of 8); out may be base.  A row whose id is outside [0, adapters) is
+ * elements apart (multiples of 8); out may be base (with its stride).  A row whose id is outside [0, adapters) is
  * copied from base; nothing of another adapter reaches a row.  rank is a multiple of 16, slices *
  * rank <= 256, inputs a multiple of 8; x, a, b, base, out and workspace 16-byte aligned.  The sums
- * over the inputs and the ranks are fp32, added to base before the one rounding to dtype.  Tokens
- * of one adapter next to each other read its weights once per 16. */
+ * over the inputs and the ranks are fp32, added to base before the one rounding to dtype.  Up to
+ * 256 tokens, an adapter's weights are read once per 16 of its tokens; above that, tokens of one
+ * adapter are best next to each other (the weights are read once per 16 neighbours). */
 #define CCUT_LORA_MAX_SLICES 4
-CCUT_API size_t ccut_lora_workspace_bytes(int tokens, int inputs, int rank, int slices);
+CCUT_API size_t ccut_lora_workspace_bytes(int tokens, int inputs, int rank, int slices, int adapters);
 CCUT_API int ccut_lora_add(const uint16_t* x, const uint16_t* a, const uint16_t* b, const float* scales,
                            const int32_t* ids, int tokens, int inputs, int rank, int adapters, int slices,
                            const int* widths, const void* base, long long base_ld, void* out, long long out_ld,
