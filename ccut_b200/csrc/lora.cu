@@ -4,21 +4,26 @@
 // where j(o) is the slice (q, k or v of a fused projection, say) that output o belongs to; a row whose
 // id is outside [0, adapters) keeps its base.
 //
-// Two launches: lora_shrink_kernel writes partial products h[split, t, slices * rank] of the rows with their
-// adapters' A, split over the inputs; lora_expand_kernel sums h in split order, scales it, multiplies by B
-// and adds the base.  Both give a warp 16 tokens, the M of m16n8k16 bf16 MMAs, in one of two ways:
+// Two launches: a shrink kernel gives h[t, slices * rank] = A x of the rows with their adapters (in parts over
+// the inputs), lora_expand_* scales h, multiplies by B and adds the base.  Products are m16n8k16 bf16 MMAs
+// with 16 tokens as the M, in one of two ways:
 // - Up to kLoraGroupTokens tokens (a decode step), a CTA takes up to 16 tokens of ONE adapter, wherever they
 //   are in the batch: every CTA sorts the few ids itself (each token's rank among its own), so that an
-//   adapter's weights are read once however the requests mix, and all adapters at the same time.  Its four
-//   warps split the inputs, then the outputs.  Bound: latency (two launches, three dependent loads each).
-// - More tokens (prompts): a warp takes 16 neighbours and loops over their distinct adapters (one, inside a
-//   prompt); the four warps of a CTA share its weights through the L1.  A row takes the result of its own
-//   adapter by selection, so nothing of another request's adapter (a NaN weight, say) reaches it.  Bound: HBM
-//   (x, base and out).
-// Operands come straight from global memory: the order of the k index of an MMA is free, so a lane's operand
-// registers are 16 consecutive bytes of a row of x or A (8 of B).  The outputs of two n-tiles interleave so
-// that a lane holds four neighbours.
+//   adapter's weights are read once however the requests mix, and all adapters at the same time.  Bound:
+//   latency.  The four warps split the inputs; operands come straight from global memory (the order of
+//   the k index of an MMA is free: a lane's operand registers are 16 consecutive bytes of a row of x or A).
+//   The expand kernel looks its unit up and fetches B and base before it waits for the shrink kernel.
+//   64 tokens, 16 adapters of rank 16, 2048 inputs, 5120 outputs: TIME_STEP.
+// - More tokens (prompts): a CTA takes 64 neighbours and loops over their distinct adapters (one, inside a
+//   prompt).  A row takes the result of its own adapter by selection, so nothing of another request's
+//   adapter (a NaN weight, say) reaches it.  x and A stream through a cp.async ring; the inputs are split
+//   over a cluster of up to 8 CTAs whose sums meet in distributed shared memory, in rank order.  Bound: HBM (x, base
+//   and out).  4093 tokens, rank 64, 4096 inputs, 2048 bf16 outputs: TIME_PROMPT.
+// The outputs of two n-tiles interleave so that a lane holds four neighbours.
+#include <type_traits>
+
 #include "host.cuh"
+#include "tc.cuh"
 
 namespace ccut {
 
@@ -27,8 +32,10 @@ constexpr int kLoraWarps = 4;
 constexpr int kLoraMaxRanks = 256;  // slices * rank
 constexpr int kLoraGroupTokens = 256;
 constexpr int kLoraRankTiles = 8;   // n-tiles of 8 rank rows a warp keeps
-constexpr int kLoraOutputs = 512;   // outputs per CTA of the expand kernel (prompts)
-constexpr int kLoraGroupOutputs = 256;
+constexpr int kLoraRows = kLoraTile * kLoraWarps;  // tokens per CTA (prompts)
+constexpr int kLoraStep = 64;       // inputs per stage of the ring
+constexpr int kLoraStages = 3;
+constexpr int kLoraOutputs = 128;   // outputs per CTA of the expand kernels
 
 struct LoraArgs {
   const uint16_t* x;
@@ -113,113 +120,209 @@ CCUT_DEVICE bool lora_group(const LoraArgs& p, int u, LoraTile& tile, int* ids, 
   return true;
 }
 
-// Whole warp: the tile of 16 neighbours from token t0.
-CCUT_DEVICE void lora_neighbours(const LoraArgs& p, int t0, LoraTile& tile) {
-  const int lane = threadIdx.x & 31, t = t0 + lane;
-  const int id = lane < kLoraTile && t < p.tokens ? lora_id(p, t) : -1;
-  const unsigned same = __match_any_sync(0xffffffffu, id);
-  const bool first = id >= 0 && (same & ((1u << lane) - 1)) == 0;
-  const unsigned firsts = __ballot_sync(0xffffffffu, first);
-  if (lane < kLoraTile) {
-    tile.rows[lane] = t < p.tokens ? t : -1;
-    tile.ids[lane] = id;
-    if (first) tile.uniq[__popc(firsts & ((1u << lane) - 1))] = id;
+// 64 neighbours and the adapters among them.
+struct LoraRows {
+  int ids[kLoraRows];   // -1: none, or past the last token
+  int uniq[kLoraRows], n;
+};
+// Whole CTA.
+CCUT_DEVICE void lora_neighbours(const LoraArgs& p, int t0, LoraRows& rows) {
+  const int tid = threadIdx.x;
+  if (tid < kLoraRows) rows.ids[tid] = t0 + tid < p.tokens ? lora_id(p, t0 + tid) : -1;
+  __syncthreads();
+  if (tid < 32) {  // first of their kind, in order
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < kLoraRows; k += 32) {
+      const int id = rows.ids[k + tid];
+      const unsigned same = __match_any_sync(0xffffffffu, id);  // every lane takes part
+      bool first = id >= 0 && (same & ((1u << tid) - 1)) == 0;
+      if (k > 0)
+        for (int i = 0; i < n; ++i) first &= rows.uniq[i] != id;
+      const unsigned m = __ballot_sync(0xffffffffu, first);
+      if (first) rows.uniq[n + __popc(m & ((1u << tid) - 1))] = id;
+      n += __popc(m);
+      __syncwarp();
+    }
+    if (tid == 0) rows.n = n;
   }
-  if (lane == 0) tile.n = __popc(firsts);
-  __syncwarp();
+  __syncthreads();
 }
 
-// Grid (units or tiles of 64 tokens, splits, blocks of 64 rank rows).
-template <bool GROUP>
-__global__ void __launch_bounds__(kLoraWarps * 32) lora_shrink_kernel(const __grid_constant__ LoraArgs p) {
+// Decode steps.  Grid (units, splits, blocks of 64 rank rows).
+__global__ void __launch_bounds__(kLoraWarps * 32) lora_shrink_group_kernel(const __grid_constant__ LoraArgs p) {
   pdl_wait();
   pdl_trigger();
-  __shared__ LoraTile tiles[GROUP ? 1 : kLoraWarps];
-  __shared__ __align__(16) int ids[GROUP ? kLoraGroupTokens : 4];
-  __shared__ int counts[GROUP ? kLoraGroupTokens / 32 : 1];
-  __shared__ float red[GROUP ? kLoraWarps - 1 : 1][GROUP ? 32 : 1][kLoraRankTiles * 4 + 1];
+  __shared__ LoraTile tile;
+  __shared__ __align__(16) int ids[kLoraGroupTokens];
+  __shared__ int counts[kLoraGroupTokens / 32];
+  __shared__ float red[kLoraWarps - 1][32][kLoraRankTiles * 4 + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int R = p.slices * p.rank, r0 = blockIdx.z * kLoraRankTiles * 8;
   const int nz = min(kLoraRankTiles, (R - r0) / 8);
-  LoraTile& tile = tiles[GROUP ? 0 : warp];
-  int k0 = blockIdx.y * p.k_per_split, k1 = min(p.inputs, k0 + p.k_per_split);
-  if constexpr (GROUP) {
-    if (!lora_group(p, blockIdx.x, tile, ids, counts)) return;
-    if (tile.uniq[0] < 0) return;
-    const int per = p.k_per_split / kLoraWarps;  // a multiple of 32
-    k0 += warp * per;
-    k1 = min(k1, k0 + per);
-  } else {
-    lora_neighbours(p, (blockIdx.x * kLoraWarps + warp) * kLoraTile, tile);
-  }
+  if (!lora_group(p, blockIdx.x, tile, ids, counts)) return;
+  const int a = tile.uniq[0];
+  if (a < 0) return;
+  const int per = p.k_per_split / kLoraWarps;  // a multiple of 32
+  const int k0 = blockIdx.y * p.k_per_split + warp * per, k1 = min(p.inputs, k0 + per);
   const int row0 = tile.rows[g], row1 = tile.rows[g + 8];
   const uint16_t* x0 = p.x + (size_t)max(row0, 0) * p.inputs;
   const uint16_t* x1 = p.x + (size_t)max(row1, 0) * p.inputs;
+  const uint16_t* ar = p.a + ((size_t)a * R + r0 + g) * p.inputs;
   const uint4 zero = make_uint4(0, 0, 0, 0);
-  float keep[kLoraRankTiles][4];
+  float acc[kLoraRankTiles][4];
 #pragma unroll
   for (int n = 0; n < kLoraRankTiles; ++n)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) keep[n][i] = 0.f;
-  for (int u = 0; u < (GROUP ? 1 : tile.n); ++u) {
-    const int a = tile.uniq[u];
-    const uint16_t* ar = p.a + ((size_t)a * R + r0 + g) * p.inputs;
-    float acc[kLoraRankTiles][4];
+    for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+  // 32 inputs a step: lane t holds inputs k + 8 t .. + 7 of its rows
+#pragma unroll 2
+  for (int k = k0; k < k1; k += 32) {
+    const int kk = k + 8 * t;
+    const bool in = kk < k1;
+    const uint4 v0 = in && row0 >= 0 ? __ldg(reinterpret_cast<const uint4*>(x0 + kk)) : zero;
+    const uint4 v1 = in && row1 >= 0 ? __ldg(reinterpret_cast<const uint4*>(x1 + kk)) : zero;
+    uint4 w[kLoraRankTiles];
+#pragma unroll
+    for (int n = 0; n < kLoraRankTiles; ++n)
+      w[n] = in && n < nz ? __ldg(reinterpret_cast<const uint4*>(ar + (size_t)n * 8 * p.inputs + kk)) : zero;
+    const uint32_t f0[4] = {v0.x, v1.x, v0.y, v1.y}, f1[4] = {v0.z, v1.z, v0.w, v1.w};
+#pragma unroll
+    for (int n = 0; n < kLoraRankTiles; ++n)
+      if (n < nz) {
+        mma_16816<true>(acc[n], f0, w[n].x, w[n].y);
+        mma_16816<true>(acc[n], f1, w[n].z, w[n].w);
+      }
+  }
+  if (warp > 0) {  // the warps' sums, in warp order
 #pragma unroll
     for (int n = 0; n < kLoraRankTiles; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
-    // 32 inputs a step: lane t holds inputs k + 8 t .. + 7 of its rows
-#pragma unroll 2
-    for (int k = k0; k < k1; k += 32) {
-      const int kk = k + 8 * t;
-      const bool in = kk < k1;
-      const uint4 v0 = in && row0 >= 0 ? __ldg(reinterpret_cast<const uint4*>(x0 + kk)) : zero;
-      const uint4 v1 = in && row1 >= 0 ? __ldg(reinterpret_cast<const uint4*>(x1 + kk)) : zero;
-      uint4 w[kLoraRankTiles];
-#pragma unroll
-      for (int n = 0; n < kLoraRankTiles; ++n)
-        w[n] = in && n < nz ? __ldg(reinterpret_cast<const uint4*>(ar + (size_t)n * 8 * p.inputs + kk)) : zero;
-      const uint32_t f0[4] = {v0.x, v1.x, v0.y, v1.y}, f1[4] = {v0.z, v1.z, v0.w, v1.w};
-#pragma unroll
-      for (int n = 0; n < kLoraRankTiles; ++n)
-        if (n < nz) {
-          mma_16816<true>(acc[n], f0, w[n].x, w[n].y);
-          mma_16816<true>(acc[n], f1, w[n].z, w[n].w);
-        }
-    }
-    const bool own0 = GROUP || tile.ids[g] == a, own1 = GROUP || tile.ids[g + 8] == a;
-#pragma unroll
-    for (int n = 0; n < kLoraRankTiles; ++n) {
-      keep[n][0] = own0 ? acc[n][0] : keep[n][0];
-      keep[n][1] = own0 ? acc[n][1] : keep[n][1];
-      keep[n][2] = own1 ? acc[n][2] : keep[n][2];
-      keep[n][3] = own1 ? acc[n][3] : keep[n][3];
-    }
+      for (int i = 0; i < 4; ++i) red[warp - 1][lane][n * 4 + i] = acc[n][i];
   }
-  if constexpr (GROUP) {  // the warps' sums, in warp order
-    if (warp > 0) {
+  __syncthreads();
+  if (warp > 0) return;
 #pragma unroll
-      for (int n = 0; n < kLoraRankTiles; ++n)
+  for (int w = 0; w < kLoraWarps - 1; ++w)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) red[warp - 1][lane][n * 4 + i] = keep[n][i];
-    }
-    __syncthreads();
-    if (warp > 0) return;
+    for (int n = 0; n < kLoraRankTiles; ++n)
 #pragma unroll
-    for (int w = 0; w < kLoraWarps - 1; ++w)
-#pragma unroll
-      for (int n = 0; n < kLoraRankTiles; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) keep[n][i] += red[w][lane][n * 4 + i];
-  }
+      for (int i = 0; i < 4; ++i) acc[n][i] += red[w][lane][n * 4 + i];
   float* h = p.part + (size_t)blockIdx.y * p.tokens * R + r0 + 2 * t;
 #pragma unroll
   for (int n = 0; n < kLoraRankTiles; ++n)
     if (n < nz) {
-      if (row0 >= 0) *reinterpret_cast<float2*>(h + (size_t)row0 * R + n * 8) = make_float2(keep[n][0], keep[n][1]);
-      if (row1 >= 0) *reinterpret_cast<float2*>(h + (size_t)row1 * R + n * 8) = make_float2(keep[n][2], keep[n][3]);
+      if (row0 >= 0) *reinterpret_cast<float2*>(h + (size_t)row0 * R + n * 8) = make_float2(acc[n][0], acc[n][1]);
+      if (row1 >= 0) *reinterpret_cast<float2*>(h + (size_t)row1 * R + n * 8) = make_float2(acc[n][2], acc[n][3]);
     }
+}
+
+// Byte offset of 16-byte chunk c of row r in a tile of 128-byte rows: ldmatrix reads 8 rows of one chunk without
+// meeting a bank twice.
+CCUT_DEVICE int lora_chunk(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
+CCUT_DEVICE float4 ld_cluster(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// Prompts.  Grid (tiles of 64 tokens, splits, blocks of 64 rank rows), the splits of a tile in one cluster.
+constexpr int kLoraStageBytes = 2 * kLoraRows * kLoraStep * 2;  // x and A, 64 rows of 128 bytes each
+__global__ void __launch_bounds__(kLoraWarps * 32) lora_shrink_kernel(const __grid_constant__ LoraArgs p) {
+  pdl_wait();
+  pdl_trigger();
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ LoraRows rows;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int R = p.slices * p.rank, r0 = blockIdx.z * kLoraRankTiles * 8;
+  const int nz = min(kLoraRankTiles, (R - r0) / 8), t0 = blockIdx.x * kLoraRows;
+  lora_neighbours(p, t0, rows);
+  const int k0 = blockIdx.y * p.k_per_split, k1 = min(p.inputs, k0 + p.k_per_split);
+  const int steps = k1 > k0 ? (k1 - k0 + kLoraStep - 1) / kLoraStep : 0, total = steps * rows.n;
+  // copies of a stage: thread -> chunks of rows tid / 8, + 16, + 32, + 48
+  const int cr = threadIdx.x >> 3, cc = threadIdx.x & 7;
+  auto issue = [&](int s) {
+    uint8_t* st = ring + s % kLoraStages * kLoraStageBytes;
+    const int k = k0 + s % steps * kLoraStep + cc * 8;
+    const uint16_t* ar = p.a + ((size_t)rows.uniq[s / steps] * R + r0) * p.inputs;
+#pragma unroll
+    for (int i = 0; i < kLoraRows / 16; ++i) {
+      const int r = cr + 16 * i;
+      const bool xin = k < k1 && t0 + r < p.tokens, win = k < k1 && r < nz * 8;
+      cp_async16(st + lora_chunk(r, cc), xin ? p.x + (size_t)(t0 + r) * p.inputs + k : p.x, xin);
+      cp_async16(st + kLoraRows * 128 + lora_chunk(r, cc), win ? ar + (size_t)r * p.inputs + k : p.x, win);
+    }
+  };
+  float keep[kLoraRankTiles][4], acc[kLoraRankTiles][4];
+#pragma unroll
+  for (int n = 0; n < kLoraRankTiles; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) keep[n][i] = 0.f, acc[n][i] = 0.f;
+  const int id0 = rows.ids[warp * kLoraTile + g], id1 = rows.ids[warp * kLoraTile + g + 8];
+#pragma unroll
+  for (int i = 0; i < kLoraStages - 1; ++i) {
+    if (i < total) issue(i);
+    cp_async_commit();
+  }
+  for (int s = 0; s < total; ++s) {
+    cp_async_wait<kLoraStages - 2>();
+    __syncthreads();  // everyone's copies of this stage have landed, everyone is done with the stage before
+    if (s + kLoraStages - 1 < total) issue(s + kLoraStages - 1);
+    cp_async_commit();
+    const uint8_t* st = ring + s % kLoraStages * kLoraStageBytes;
+#pragma unroll
+    for (int kk = 0; kk < kLoraStep / 16; ++kk) {
+      uint32_t f[4];
+      ldmatrix_x4(f[0], f[1], f[2], f[3], st + lora_chunk(warp * kLoraTile + (lane & 15), kk * 2 + (lane >> 4)));
+#pragma unroll
+      for (int n = 0; n < kLoraRankTiles; n += 2)
+        if (n < nz) {
+          uint32_t b0, b1, b2, b3;
+          ldmatrix_x4(b0, b1, b2, b3,
+                      st + kLoraRows * 128 + lora_chunk(n * 8 + (lane & 7) + (lane >> 4) * 8, kk * 2 + (lane >> 3 & 1)));
+          mma_16816<true>(acc[n], f, b0, b1);
+          mma_16816<true>(acc[n + 1], f, b2, b3);
+        }
+    }
+    if (s % steps == steps - 1) {  // the last of an adapter: its rows take the sums
+      const int a = rows.uniq[s / steps];
+#pragma unroll
+      for (int n = 0; n < kLoraRankTiles; ++n) {
+        keep[n][0] = id0 == a ? acc[n][0] : keep[n][0];
+        keep[n][1] = id0 == a ? acc[n][1] : keep[n][1];
+        keep[n][2] = id1 == a ? acc[n][2] : keep[n][2];
+        keep[n][3] = id1 == a ? acc[n][3] : keep[n][3];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+      }
+    }
+  }
+  cp_async_wait<0>();
+  __syncthreads();
+  // sums of this CTA in its shared memory, [64 tokens][64 rank rows + 4], then each CTA of the cluster adds up its
+  // share of the tokens over all, in rank order
+  constexpr int kLd = kLoraRankTiles * 8 + 4;
+  float* sums = reinterpret_cast<float*>(ring);
+#pragma unroll
+  for (int n = 0; n < kLoraRankTiles; ++n) {
+    float* d = sums + (warp * kLoraTile + g) * kLd + n * 8 + 2 * t;
+    d[0] = keep[n][0], d[1] = keep[n][1];
+    d[8 * kLd] = keep[n][2], d[8 * kLd + 1] = keep[n][3];
+  }
+  __syncthreads();
+  tc::cluster_sync();
+  const int share = kLoraRows / p.splits;
+  for (int i = threadIdx.x; i < share * (nz * 2); i += kLoraWarps * 32) {
+    const int r = blockIdx.y * share + i / (nz * 2), c = i % (nz * 2) * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < p.splits; ++s) {
+      const float4 y = ld_cluster(tc::mapa(sums + r * kLd + c, s));
+      v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
+    }
+    if (t0 + r < p.tokens) *reinterpret_cast<float4*>(p.part + (size_t)(t0 + r) * R + r0 + c) = v;
+  }
+  __syncthreads();
+  tc::cluster_sync();  // no CTA leaves while its sums are read
 }
 
 // (bf16(a), bf16(b)) and what is left of each, packed low = a
@@ -230,126 +333,258 @@ CCUT_DEVICE uint32_t take_bf16x2(float& a, float& b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Four outputs of a row: base plus d (has: the row has an adapter).
+// Four neighbouring values of a row of base (or out).
 template <bool BF16>
-CCUT_DEVICE void lora_write(const LoraArgs& p, int row, int o, const float (&d)[4], bool has) {
-  const size_t bi = (size_t)row * p.base_ld + o, oi = (size_t)row * p.out_ld + o;
-  if constexpr (BF16) {
-    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.base) + bi);
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(__uint_as_float(u.x << 16) + d[0], __uint_as_float(u.x & 0xFFFF0000u) + d[1]);
-    const __nv_bfloat162 hi = __floats2bfloat162_rn(__uint_as_float(u.y << 16) + d[2], __uint_as_float(u.y & 0xFFFF0000u) + d[3]);
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + oi) =
-        has ? make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi)) : u;
-  } else {
-    const float4 u = *reinterpret_cast<const float4*>(static_cast<const float*>(p.base) + bi);
-    *reinterpret_cast<float4*>(static_cast<float*>(p.out) + oi) =
-        has ? make_float4(u.x + d[0], u.y + d[1], u.z + d[2], u.w + d[3]) : u;
+struct LoraFour {
+  using Raw = typename std::conditional<BF16, uint2, float4>::type;
+  static CCUT_DEVICE Raw load(const void* p, size_t at) {
+    if constexpr (BF16) return *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + at);
+    else return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+  }
+  static CCUT_DEVICE void store(void* p, size_t at, const Raw& v) {
+    if constexpr (BF16) *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + at) = v;
+    else *reinterpret_cast<float4*>(static_cast<float*>(p) + at) = v;
+  }
+  static CCUT_DEVICE Raw add(const Raw& u, float a, float b, float c, float d) {  // the one rounding
+    if constexpr (BF16) {
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(__uint_as_float(u.x << 16) + a, __uint_as_float(u.x & 0xFFFF0000u) + b);
+      const __nv_bfloat162 hi = __floats2bfloat162_rn(__uint_as_float(u.y << 16) + c, __uint_as_float(u.y & 0xFFFF0000u) + d);
+      return make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    } else {
+      return make_float4(u.x + a, u.y + b, u.z + c, u.w + d);
+    }
+  }
+};
+
+// h enters the MMAs as bf16 parts whose sum keeps 16 (two parts, bf16 output) or 24 (three, fp32 output)
+// significant bits, kept as planes [part][rows][R + 8] in shared memory.
+template <int kParts>
+CCUT_DEVICE void lora_keep(uint16_t* planes, size_t plane, size_t at, float4 v) {
+#pragma unroll
+  for (int part = 0; part < kParts; ++part) {
+    const uint32_t lo = take_bf16x2(v.x, v.y), hi = take_bf16x2(v.z, v.w);
+    *reinterpret_cast<uint2*>(planes + part * plane + at) = make_uint2(lo, hi);
+  }
+}
+// Operand parts of rank columns `at` .. + 3 of rows g (h0) and g + 8.
+template <int kParts>
+CCUT_DEVICE void lora_operands(const uint16_t* h0, size_t plane, int ld, uint32_t (&f)[kParts][4]) {
+#pragma unroll
+  for (int part = 0; part < kParts; ++part) {
+    const uint2 u = *reinterpret_cast<const uint2*>(h0 + part * plane);
+    const uint2 v = *reinterpret_cast<const uint2*>(h0 + part * plane + 8 * ld);
+    f[part][0] = u.x, f[part][1] = v.x, f[part][2] = u.y, f[part][3] = v.y;
   }
 }
 
-// Grid (units or tiles of 64 tokens, blocks of outputs).  h enters the MMAs as bf16 parts whose sum keeps 16
-// (two parts, bf16 output) or 24 (three, fp32 output) significant bits.  KR: rank / 16 when h's operands
-// stay in registers for all outputs of a slice, 0 for other ranks.
-template <bool GROUP, int KR, bool OUT_BF16>
+// Slice of output o.
+CCUT_DEVICE int lora_slice(const LoraArgs& p, int o) {
+  int j = 0;
+#pragma unroll
+  for (int i = 0; i < CCUT_LORA_MAX_SLICES - 1; ++i) j += i + 1 < p.slices && o >= p.ends[i];
+  return j;
+}
+
+// Decode steps.  Grid (units, blocks of 128 outputs): warp w takes 32 outputs, in blocks of 8 x 2 (columns n of
+// n-tile i: output 4 (n / 2) + 2 i + n % 2 of 16; slices end at multiples of 8, so a block of 16 has one or two).
+template <bool OUT_BF16>
+__global__ void __launch_bounds__(kLoraWarps * 32) lora_expand_group_kernel(const __grid_constant__ LoraArgs p) {
+  constexpr int kParts = OUT_BF16 ? 2 : 3, kBlocks = kLoraOutputs / kLoraWarps / 16, kFetch = 2;
+  using Four = LoraFour<OUT_BF16>;
+  __shared__ LoraTile tile;
+  __shared__ __align__(16) int ids[kLoraGroupTokens];
+  __shared__ int counts[kLoraGroupTokens / 32];
+  extern __shared__ __align__(16) uint16_t hs[];  // [parts][16][R + 8]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int R = p.slices * p.rank, ld = R + 8;
+  const size_t plane = (size_t)kLoraTile * ld;
+  const int o0 = blockIdx.y * kLoraOutputs + warp * (kLoraOutputs / kLoraWarps);
+  const bool unit = lora_group(p, blockIdx.x, tile, ids, counts);
+  const int a = unit ? tile.uniq[0] : -1;
+  const int row0 = unit ? tile.rows[g] : -1, row1 = unit ? tile.rows[g + 8] : -1;
+  // base, and the first two k steps of B, while the shrink kernel still runs
+  typename Four::Raw base[kBlocks][2];
+  uint2 w[kBlocks][2][kFetch];
+  const int steps = p.rank / 16;
+#pragma unroll
+  for (int q = 0; q < kBlocks; ++q) {
+    const int o = o0 + q * 16 + 4 * t, oc = o0 + q * 16 + (g >> 1) * 4 + (g & 1);
+    if (o < p.outputs) {
+      if (row0 >= 0) base[q][0] = Four::load(p.base, (size_t)row0 * p.base_ld + o);
+      if (row1 >= 0) base[q][1] = Four::load(p.base, (size_t)row1 * p.base_ld + o);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 0; k < kFetch; ++k)
+        w[q][i][k] = a >= 0 && oc + 2 * i < p.outputs && k < steps
+                         ? __ldg(reinterpret_cast<const uint2*>(p.b + ((size_t)a * p.outputs + oc + 2 * i) * p.rank + 16 * k + 4 * t))
+                         : make_uint2(0, 0);
+  }
+  pdl_wait();
+  pdl_trigger();
+  if (!unit) return;
+  if (a >= 0) {
+    const float scale = p.scales[a];
+    for (int i = threadIdx.x; i < kLoraTile * R / 4; i += kLoraWarps * 32) {
+      const int r = i / (R / 4), c = i % (R / 4) * 4, row = tile.rows[r];
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row >= 0) {
+#pragma unroll 8
+        for (int s = 0; s < p.splits; ++s) {
+          const float4 y = *reinterpret_cast<const float4*>(p.part + ((size_t)s * p.tokens + row) * R + c);
+          v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
+        }
+        v.x *= scale, v.y *= scale, v.z *= scale, v.w *= scale;
+      }
+      lora_keep<kParts>(hs, plane, r * ld + c, v);
+    }
+    __syncthreads();
+  } else if (p.base == p.out) {
+    return;  // in place: rows without an adapter stay
+  }
+#pragma unroll
+  for (int q = 0; q < kBlocks; ++q) {
+    const int o = o0 + q * 16;
+    if (o >= p.outputs) break;
+    float d[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    if (a >= 0) {
+      // both halves of the block (8 outputs, lanes t < 2 and t >= 2) share a slice, or each has its own
+      const int j0 = lora_slice(p, o), j1 = o + 8 < p.outputs ? lora_slice(p, o + 8) : j0;
+      const int oc = o + (g >> 1) * 4 + (g & 1);
+      for (int j = j0; j <= j1; ++j) {
+        float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        for (int k = 0; k < steps; ++k) {
+          uint32_t f[kParts][4];
+          lora_operands<kParts>(hs + g * ld + j * p.rank + 16 * k + 4 * t, plane, ld, f);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint2 b = make_uint2(0, 0);
+            if (k == 0) b = w[q][i][0];
+            else if (k == 1) b = w[q][i][1];
+            else if (oc + 2 * i < p.outputs)
+              b = __ldg(reinterpret_cast<const uint2*>(p.b + ((size_t)a * p.outputs + oc + 2 * i) * p.rank + 16 * k + 4 * t));
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) mma_16816<true>(acc[i], f[part], b.x, b.y);
+          }
+        }
+        const bool mine = (t < 2 ? j0 : j1) == j;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) d[i][e] = mine ? acc[i][e] : d[i][e];
+      }
+    }
+    if (o + 4 * t < p.outputs) {
+      const bool has = a >= 0;
+      if (row0 >= 0)
+        Four::store(p.out, (size_t)row0 * p.out_ld + o + 4 * t,
+                    has ? Four::add(base[q][0], d[0][0], d[0][1], d[1][0], d[1][1]) : base[q][0]);
+      if (row1 >= 0)
+        Four::store(p.out, (size_t)row1 * p.out_ld + o + 4 * t,
+                    has ? Four::add(base[q][1], d[0][2], d[0][3], d[1][2], d[1][3]) : base[q][1]);
+    }
+  }
+}
+
+// Prompts.  Grid (tiles of 64 tokens, blocks of 128 outputs): base and the adapter's rows of B are on their way while
+// h is read; warp w has tokens 16 w .. and all the outputs.
+template <bool OUT_BF16>
 __global__ void __launch_bounds__(kLoraWarps * 32) lora_expand_kernel(const __grid_constant__ LoraArgs p) {
   pdl_wait();
   pdl_trigger();
-  constexpr int kParts = OUT_BF16 ? 2 : 3;
-  __shared__ LoraTile tiles[GROUP ? 1 : kLoraWarps];
-  __shared__ __align__(16) int ids[GROUP ? kLoraGroupTokens : 4];
-  __shared__ int counts[GROUP ? kLoraGroupTokens / 32 : 1];
-  extern __shared__ __align__(16) float hs_all[];  // [1 or 4][16][R + 4]
+  constexpr int kParts = OUT_BF16 ? 2 : 3, kBlocks = kLoraOutputs / 16;
+  using Four = LoraFour<OUT_BF16>;
+  __shared__ LoraRows rows;
+  extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int R = p.slices * p.rank, ld = R + 4;
-  LoraTile& tile = tiles[GROUP ? 0 : warp];
-  float* hs = hs_all + (GROUP ? 0 : warp * kLoraTile * ld);
-  if constexpr (GROUP) {
-    if (!lora_group(p, blockIdx.x, tile, ids, counts)) return;
-    tile.n = tile.uniq[0] >= 0 ? 1 : 0;  // the same from every thread
-  } else {
-    lora_neighbours(p, (blockIdx.x * kLoraWarps + warp) * kLoraTile, tile);
+  const int R = p.slices * p.rank, ld = R + 8, steps = p.rank / 16;
+  const int bld = p.rank * 2 + 16;  // bytes per row of B
+  const size_t plane = (size_t)kLoraRows * ld;
+  uint16_t* hs = reinterpret_cast<uint16_t*>(smem);  // [parts][64][R + 8]
+  uint8_t* bs = smem + kParts * plane * 2;           // [128][rank] bf16
+  const int t0 = blockIdx.x * kLoraRows, o0 = blockIdx.y * kLoraOutputs, width = min(kLoraOutputs, p.outputs - o0);
+  lora_neighbours(p, t0, rows);
+  auto fetch_b = [&](int a) {
+    for (int i = threadIdx.x; i < width * (p.rank / 8); i += kLoraWarps * 32) {
+      const int r = i / (p.rank / 8), c = i % (p.rank / 8);
+      cp_async16(bs + r * bld + c * 16, p.b + ((size_t)a * p.outputs + o0 + r) * p.rank + c * 8, true);
+    }
+    cp_async_commit();
+  };
+  if (rows.n > 0) fetch_b(rows.uniq[0]);
+  const int row0 = t0 + warp * kLoraTile + g, row1 = row0 + 8;
+  const int id0 = rows.ids[warp * kLoraTile + g], id1 = rows.ids[warp * kLoraTile + g + 8];
+  const bool in0 = row0 < p.tokens, in1 = row1 < p.tokens;
+  typename Four::Raw base[kBlocks][2];
+#pragma unroll
+  for (int q = 0; q < kBlocks; ++q) {
+    const int o = o0 + q * 16 + 4 * t;
+    if (o < p.outputs) {
+      if (in0) base[q][0] = Four::load(p.base, (size_t)row0 * p.base_ld + o);
+      if (in1) base[q][1] = Four::load(p.base, (size_t)row1 * p.base_ld + o);
+    }
   }
-  if (p.base == p.out && tile.n == 0 && GROUP) return;  // in place: rows without an adapter stay
-  for (int i = GROUP ? threadIdx.x : lane; i < kLoraTile * R / 4; i += GROUP ? kLoraWarps * 32 : 32) {
-    const int r = i / (R / 4), c = i % (R / 4) * 4, row = tile.rows[r], id = tile.ids[r];
+  // this warp's 16 rows of h, scaled
+#pragma unroll 4
+  for (int i = lane; i < kLoraTile * R / 4; i += 32) {
+    const int r = warp * kLoraTile + i / (R / 4), c = i % (R / 4) * 4, id = rows.ids[r];
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (id >= 0) {
-#pragma unroll 8
-      for (int s = 0; s < p.splits; ++s) {
-        const float4 y = *reinterpret_cast<const float4*>(p.part + ((size_t)s * p.tokens + row) * R + c);
-        v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
-      }
+      v = *reinterpret_cast<const float4*>(p.part + (size_t)(t0 + r) * R + c);
       const float f = p.scales[id];
       v.x *= f, v.y *= f, v.z *= f, v.w *= f;
     }
-    *reinterpret_cast<float4*>(hs + r * ld + c) = v;
+    lora_keep<kParts>(hs, plane, r * ld + c, v);
   }
-  if constexpr (GROUP) __syncthreads();
-  else __syncwarp();
-  const int row0 = tile.rows[g], row1 = tile.rows[g + 8];
-  const bool has0 = tile.ids[g] >= 0, has1 = tile.ids[g + 8] >= 0;
-  // this warp's outputs, slice by slice
-  constexpr int kWide = GROUP ? kLoraGroupOutputs / kLoraWarps : kLoraOutputs;
-  const int o0 = GROUP ? blockIdx.y * kLoraGroupOutputs + warp * kWide : blockIdx.y * kWide;
-  const int o1 = min(p.outputs, o0 + kWide);
-  for (int j = 0; j < p.slices; ++j) {
-    const int from = max(o0, j ? p.ends[j - 1] : 0), to = min(o1, p.ends[j]);
-    if (from >= to) continue;
-    uint32_t hf[KR ? KR : 1][kParts][4];
-    auto operands = [&](int k, uint32_t(&f)[kParts][4]) {  // of rank columns 16 k ..: lane t takes 16 k + 4 t .. + 3
-      const float* h0 = hs + g * ld + j * p.rank + 16 * k + 4 * t;
-      float4 v0 = *reinterpret_cast<const float4*>(h0), v1 = *reinterpret_cast<const float4*>(h0 + 8 * ld);
+  for (int u = 0; u < rows.n; ++u) {
+    const int a = rows.uniq[u];
+    cp_async_wait<0>();
+    __syncthreads();
+    if (__any_sync(0xffffffffu, id0 == a || id1 == a)) {
 #pragma unroll
-      for (int part = 0; part < kParts; ++part) {
-        f[part][0] = take_bf16x2(v0.x, v0.y);
-        f[part][1] = take_bf16x2(v1.x, v1.y);
-        f[part][2] = take_bf16x2(v0.z, v0.w);
-        f[part][3] = take_bf16x2(v1.z, v1.w);
-      }
-    };
+      for (int q = 0; q < kBlocks; ++q) {
+        const int o = o0 + q * 16;
+        if (o >= p.outputs) break;
+        float d[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        const int j0 = lora_slice(p, o), j1 = o + 8 < p.outputs ? lora_slice(p, o + 8) : j0;
+        const int oc = q * 16 + (g >> 1) * 4 + (g & 1);
+        for (int j = j0; j <= j1; ++j) {
+          float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+          for (int k = 0; k < steps; ++k) {
+            uint32_t f[kParts][4];
+            lora_operands<kParts>(hs + (warp * kLoraTile + g) * ld + j * p.rank + 16 * k + 4 * t, plane, ld, f);
 #pragma unroll
-    for (int k = 0; k < KR; ++k) operands(k, hf[k]);
-#pragma unroll 2
-    for (int o = from; o < to; o += 16) {
-      // n-tile i, column n is output o + 4 (n / 2) + 2 i + n % 2: lane t gets outputs o + 4 t .. + 3
-      float keep[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-      const int oc = o + (g >> 1) * 4 + (g & 1);
-      for (int u = 0; u < tile.n; ++u) {
-        const int a = tile.uniq[u];
-        const uint16_t* br = p.b + ((size_t)a * p.outputs + oc) * p.rank + 4 * t;
-        float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-        auto product = [&](int k, const uint32_t(&f)[kParts][4]) {
+            for (int i = 0; i < 2; ++i) {
+              const uint2 b = oc + 2 * i < width
+                                  ? *reinterpret_cast<const uint2*>(bs + (oc + 2 * i) * bld + 32 * k + 8 * t)
+                                  : make_uint2(0, 0);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint2 w = oc + 2 * i < to ? __ldg(reinterpret_cast<const uint2*>(br + (size_t)2 * i * p.rank + 16 * k)) : make_uint2(0, 0);
-#pragma unroll
-            for (int part = 0; part < kParts; ++part) mma_16816<true>(acc[i], f[part], w.x, w.y);
+              for (int part = 0; part < kParts; ++part) mma_16816<true>(acc[i], f[part], b.x, b.y);
+            }
           }
-        };
-        if constexpr (KR > 0) {
+          const bool mine = (t < 2 ? j0 : j1) == j;
 #pragma unroll
-          for (int k = 0; k < KR; ++k) product(k, hf[k]);
-        } else {
-          for (int k = 0; k < p.rank / 16; ++k) {
-            operands(k, hf[0]);
-            product(k, hf[0]);
-          }
-        }
-        const bool own0 = GROUP || tile.ids[g] == a, own1 = GROUP || tile.ids[g + 8] == a;
+          for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          keep[i][0] = own0 ? acc[i][0] : keep[i][0];
-          keep[i][1] = own0 ? acc[i][1] : keep[i][1];
-          keep[i][2] = own1 ? acc[i][2] : keep[i][2];
-          keep[i][3] = own1 ? acc[i][3] : keep[i][3];
+            for (int e = 0; e < 4; ++e) d[i][e] = mine ? acc[i][e] : d[i][e];
         }
+        if (id0 == a) base[q][0] = Four::add(base[q][0], d[0][0], d[0][1], d[1][0], d[1][1]);
+        if (id1 == a) base[q][1] = Four::add(base[q][1], d[0][2], d[0][3], d[1][2], d[1][3]);
       }
-      if (o + 4 * t < to) {
-        const float d0[4] = {keep[0][0], keep[0][1], keep[1][0], keep[1][1]};
-        const float d1[4] = {keep[0][2], keep[0][3], keep[1][2], keep[1][3]};
-        if (row0 >= 0) lora_write<OUT_BF16>(p, row0, o + 4 * t, d0, has0);
-        if (row1 >= 0) lora_write<OUT_BF16>(p, row1, o + 4 * t, d1, has1);
-      }
+    }
+    if (u + 1 < rows.n) {
+      __syncthreads();  // B is replaced
+      fetch_b(rows.uniq[u + 1]);
+    }
+  }
+  const bool copy = p.base != p.out;  // in place, rows without an adapter stay
+#pragma unroll
+  for (int q = 0; q < kBlocks; ++q) {
+    const int o = o0 + q * 16 + 4 * t;
+    if (o < p.outputs) {
+      if (in0 && (copy || id0 >= 0)) Four::store(p.out, (size_t)row0 * p.out_ld + o, base[q][0]);
+      if (in1 && (copy || id1 >= 0)) Four::store(p.out, (size_t)row1 * p.out_ld + o, base[q][1]);
     }
   }
 }
@@ -359,38 +594,69 @@ static int lora_units(int tokens, int adapters) {
   const long n = (long)adapters + 1 + tokens / kLoraTile;
   return (int)(n < tokens ? n : tokens);
 }
-// Splits of the inputs: two CTAs an SM for a decode step, four for prompts (whose loads in flight are what
-// reads x fast), at least 128 inputs each.
+// Inputs per split: whole steps of each warp of a decode step's CTA, whole stages for prompts.
+static int lora_per_split(int inputs, int splits, bool group) {
+  const int step = group ? 32 * kLoraWarps : kLoraStep;
+  return ((inputs + splits - 1) / splits + step - 1) / step * step;
+}
+// Splits of the inputs: two CTAs an SM for a decode step (at most 16, at least 128 inputs each); for prompts a
+// cluster of 1, 2, 4 or 8 (at least one stage each).
 static int lora_splits(int tokens, int inputs, int ranks, int adapters) {
   const bool group = tokens <= kLoraGroupTokens;
   const long z = (ranks + 8 * kLoraRankTiles - 1) / (8 * kLoraRankTiles);
-  const long base = (group ? lora_units(tokens, adapters) : (tokens + 63) / 64) * z;
-  long sp = base > 0 ? ((group ? 2L : 4L) * 148 + base - 1) / base : 1;
-  const long most = (inputs + 127) / 128;
-  if (sp > most) sp = most;
+  const long base = (group ? lora_units(tokens, adapters) : (tokens + kLoraRows - 1) / kLoraRows) * z;
+  if (!group) {
+    int sp = 8;
+    while (sp > 1 && (base * sp > 4 * 148 || inputs < sp * kLoraStep)) sp /= 2;
+    return sp;
+  }
+  long sp = base > 0 ? (2L * 148 + base - 1) / base : 1;
   if (sp > 16) sp = 16;
-  return sp < 1 ? 1 : (int)sp;
+  const int per = lora_per_split(inputs, (int)(sp < 1 ? 1 : sp), true);
+  return (inputs + per - 1) / per;
+}
+// Parts of h that the workspace holds.
+static int lora_parts(int tokens, int inputs, int ranks, int adapters) {
+  return tokens <= kLoraGroupTokens ? lora_splits(tokens, inputs, ranks, adapters) : 1;
 }
 
-template <bool GROUP, bool OB>
-static int run_lora(const LoraArgs& p, cudaStream_t st) {
+template <bool OB>
+static int run_lora_group(const LoraArgs& p, cudaStream_t st) {
   const int R = p.rank * p.slices;
-  const unsigned units = GROUP ? lora_units(p.tokens, p.adapters) : (p.tokens + 63) / 64;
-  const unsigned z = (R + 8 * kLoraRankTiles - 1) / (8 * kLoraRankTiles);
-  const dim3 block(kLoraWarps * 32);
-  int rc = launch_k(lora_shrink_kernel<GROUP>, dim3(units, p.splits, z), block, 0, st, p);
+  const unsigned units = lora_units(p.tokens, p.adapters), z = (R + 8 * kLoraRankTiles - 1) / (8 * kLoraRankTiles);
+  int rc = launch_k(lora_shrink_group_kernel, dim3(units, p.splits, z), dim3(kLoraWarps * 32), 0, st, p);
   if (rc) return rc;
-  const int wide = GROUP ? kLoraGroupOutputs : kLoraOutputs;
-  const size_t smem = (size_t)(GROUP ? 1 : kLoraWarps) * kLoraTile * (R + 4) * sizeof(float);
-  auto kern = p.rank == 16   ? lora_expand_kernel<GROUP, 1, OB>
-              : p.rank == 32 ? lora_expand_kernel<GROUP, 2, OB>
-              : p.rank == 64 ? lora_expand_kernel<GROUP, 4, OB>
-                             : lora_expand_kernel<GROUP, 0, OB>;
-  static std::atomic<uint64_t> smem_set[4];  // per kernel: devices with the limit raised
-  const size_t most = (size_t)(GROUP ? 1 : kLoraWarps) * kLoraTile * (kLoraMaxRanks + 4) * sizeof(float);
-  rc = ensure_smem_limit(kern, most, smem_set[p.rank == 16 ? 0 : p.rank == 32 ? 1 : p.rank == 64 ? 2 : 3]);
+  return launch_k(lora_expand_group_kernel<OB>, dim3(units, (p.outputs + kLoraOutputs - 1) / kLoraOutputs),
+                  dim3(kLoraWarps * 32), (size_t)(OB ? 2 : 3) * kLoraTile * (R + 8) * 2, st, p);
+}
+
+template <bool OB>
+static int run_lora_prompt(const LoraArgs& p, cudaStream_t st) {
+  const int R = p.rank * p.slices;
+  const unsigned tiles = (p.tokens + kLoraRows - 1) / kLoraRows, z = (R + 8 * kLoraRankTiles - 1) / (8 * kLoraRankTiles);
+  constexpr size_t ring = (size_t)kLoraStages * kLoraStageBytes;
+  static_assert(ring >= (size_t)kLoraRows * (kLoraRankTiles * 8 + 4) * 4, "the sums take the ring's place");
+  static std::atomic<uint64_t> shrink_set{0}, expand_set{0};  // devices with the limit raised
+  int rc = ensure_smem_limit(lora_shrink_kernel, ring, shrink_set);
   if (rc) return rc;
-  return launch_k(kern, dim3(units, (unsigned)((p.outputs + wide - 1) / wide)), block, smem, st, p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(tiles, p.splits, z);
+  cfg.blockDim = dim3(kLoraWarps * 32);
+  cfg.dynamicSmemBytes = ring;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = p.splits;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, lora_shrink_kernel, p) != cudaSuccess) return CCUT_ERR_CUDA;
+  auto smem = [](size_t R, size_t rank) { return (OB ? 2 : 3) * kLoraRows * (R + 8) * 2 + kLoraOutputs * (rank * 2 + 16); };
+  rc = ensure_smem_limit(lora_expand_kernel<OB>, smem(kLoraMaxRanks, kLoraMaxRanks), expand_set);
+  if (rc) return rc;
+  return launch_k(lora_expand_kernel<OB>, dim3(tiles, (p.outputs + kLoraOutputs - 1) / kLoraOutputs),
+                  dim3(kLoraWarps * 32), smem(R, p.rank), st, p);
 }
 
 }  // namespace ccut
@@ -402,7 +668,7 @@ extern "C" {
 size_t ccut_lora_workspace_bytes(int tokens, int inputs, int rank, int slices, int adapters) {
   if (tokens < 0 || inputs <= 0 || rank <= 0 || slices <= 0 || adapters < 0 || (long)rank * slices > kLoraMaxRanks)
     return 0;
-  return 256 + (size_t)lora_splits(tokens, inputs, rank * slices, adapters) * tokens * rank * slices * sizeof(float);
+  return 256 + (size_t)lora_parts(tokens, inputs, rank * slices, adapters) * tokens * rank * slices * sizeof(float);
 }
 
 int ccut_lora_add(const uint16_t* x, const uint16_t* a, const uint16_t* b, const float* scales, const int32_t* ids,
@@ -437,12 +703,11 @@ int ccut_lora_add(const uint16_t* x, const uint16_t* a, const uint16_t* b, const
   p.base = base, p.base_ld = base_ld, p.out = out, p.out_ld = out_ld;
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 256);
   p.splits = lora_splits(tokens, inputs, R, adapters);
-  const int step = tokens <= kLoraGroupTokens ? 32 * kLoraWarps : 32;  // each warp takes whole steps of 32
-  p.k_per_split = ((inputs + p.splits - 1) / p.splits + step - 1) / step * step;
-  if ((o + kLoraGroupOutputs - 1) / kLoraGroupOutputs > 65535) return CCUT_ERR_UNSUPPORTED;
+  p.k_per_split = lora_per_split(inputs, p.splits, tokens <= kLoraGroupTokens);
+  if ((o + kLoraOutputs - 1) / kLoraOutputs > 65535) return CCUT_ERR_UNSUPPORTED;
   const bool ob = dtype == CCUT_OUT_BF16;
-  if (tokens <= kLoraGroupTokens) return ob ? run_lora<true, true>(p, stream) : run_lora<true, false>(p, stream);
-  return ob ? run_lora<false, true>(p, stream) : run_lora<false, false>(p, stream);
+  if (tokens <= kLoraGroupTokens) return ob ? run_lora_group<true>(p, stream) : run_lora_group<false>(p, stream);
+  return ob ? run_lora_prompt<true>(p, stream) : run_lora_prompt<false>(p, stream);
 }
 
 }  // extern "C"
