@@ -357,7 +357,10 @@ struct LoraFour {
 };
 
 // h enters the MMAs as bf16 parts whose sum keeps 16 (two parts, bf16 output) or 24 (three, fp32 output)
-// significant bits, kept as planes [part][rows][R + 8] in shared memory.
+// significant bits, kept as planes [part][rows][lora_ld(R)] in shared memory.
+// Rows of the planes and of B are an odd multiple of 32 bytes apart: the 8 bytes of 4 lanes x 4 rows that half a
+// warp reads meet every bank once.
+__host__ __device__ constexpr int lora_ld(int n) { return n % 32 ? n : n + 16; }  // n a multiple of 16 elements
 template <int kParts>
 CCUT_DEVICE void lora_keep(uint16_t* planes, size_t plane, size_t at, float4 v) {
 #pragma unroll
@@ -394,9 +397,9 @@ __global__ void __launch_bounds__(kLoraWarps * 32) lora_expand_group_kernel(cons
   __shared__ LoraTile tile;
   __shared__ __align__(16) int ids[kLoraGroupTokens];
   __shared__ int counts[kLoraGroupTokens / 32];
-  extern __shared__ __align__(16) uint16_t hs[];  // [parts][16][R + 8]
+  extern __shared__ __align__(16) uint16_t hs[];  // [parts][16][lora_ld(R)]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int R = p.slices * p.rank, ld = R + 8;
+  const int R = p.slices * p.rank, ld = lora_ld(R);
   const size_t plane = (size_t)kLoraTile * ld;
   const int o0 = blockIdx.y * kLoraOutputs + warp * (kLoraOutputs / kLoraWarps);
   const bool unit = lora_group(p, blockIdx.x, tile, ids, counts);
@@ -487,10 +490,15 @@ __global__ void __launch_bounds__(kLoraWarps * 32) lora_expand_group_kernel(cons
   }
 }
 
-// Prompts.  Grid (tiles of 64 tokens, blocks of 128 outputs): base and the adapter's rows of B are on their way while
-// h is read; warp w has tokens 16 w .. and all the outputs.
-template <bool OUT_BF16>
-__global__ void __launch_bounds__(kLoraWarps * 32) lora_expand_kernel(const __grid_constant__ LoraArgs p) {
+// Where output r of a block lies in shared memory: column n of n-tile i at 16-block + 8 i + n.
+CCUT_DEVICE int lora_place(int r) { return (r & ~15) + ((r >> 1) & 1) * 8 + ((r >> 2) & 3) * 2 + (r & 1); }
+
+// Prompts.  Grid (tiles of 64 tokens, blocks of 128 outputs): base and h are on their way while the adapters are
+// looked up, the adapter's rows of B next; warp w has tokens 16 w .. and all the outputs.  KR: rank / 16, or
+// 0 for any.
+template <int KR, bool OUT_BF16>
+__global__ void __launch_bounds__(kLoraWarps * 32, OUT_BF16 ? 4 : 3)
+    lora_expand_kernel(const __grid_constant__ LoraArgs p) {
   pdl_wait();
   pdl_trigger();
   constexpr int kParts = OUT_BF16 ? 2 : 3, kBlocks = kLoraOutputs / 16;
@@ -498,44 +506,59 @@ __global__ void __launch_bounds__(kLoraWarps * 32) lora_expand_kernel(const __gr
   __shared__ LoraRows rows;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int R = p.slices * p.rank, ld = R + 8, steps = p.rank / 16;
-  const int bld = p.rank * 2 + 16;  // bytes per row of B
+  const int R = p.slices * p.rank, ld = lora_ld(R), steps = KR ? KR : p.rank / 16;
+  const int bld = lora_ld(p.rank) * 2;  // bytes per row of B
   const size_t plane = (size_t)kLoraRows * ld;
-  uint16_t* hs = reinterpret_cast<uint16_t*>(smem);  // [parts][64][R + 8]
+  uint16_t* hs = reinterpret_cast<uint16_t*>(smem);  // [parts][64][lora_ld(R)]
   uint8_t* bs = smem + kParts * plane * 2;           // [128][rank] bf16
+  // base, then out: [64][128], moved 16 bytes a lane, whole lines at a time
+  constexpr int kSize = OUT_BF16 ? 2 : 4, kOld = kLoraOutputs * kSize + 16 * kSize, kChunks = kLoraOutputs * kSize / 16;
+  uint8_t* os = bs + kLoraOutputs * bld;
   const int t0 = blockIdx.x * kLoraRows, o0 = blockIdx.y * kLoraOutputs, width = min(kLoraOutputs, p.outputs - o0);
+  const int row0 = t0 + warp * kLoraTile + g, row1 = row0 + 8;
+  const bool in0 = row0 < p.tokens, in1 = row1 < p.tokens;
+  // h of rows g and g + 8, columns 4 t + 16 c .. + 3 (rows without an adapter are zeros there)
+  constexpr int kBatch = 4;
+  float4 h[2][kBatch];
+  auto load_h = [&](int c0) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int c = 0; c < kBatch; ++c)
+        h[i][c] = (i ? in1 : in0) && (c0 + c) * 16 < R
+                      ? *reinterpret_cast<const float4*>(p.part + (size_t)(i ? row1 : row0) * R + (c0 + c) * 16 + 4 * t)
+                      : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  load_h(0);
+  const int chunks = width * kSize / 16;  // widths are multiples of 8: whole chunks
+  for (int i = threadIdx.x; i < kLoraRows * kChunks; i += kLoraWarps * 32) {
+    const int r = i / kChunks, c = i % kChunks;
+    if (c < chunks && t0 + r < p.tokens)
+      cp_async16(os + r * kOld + c * 16, static_cast<const uint8_t*>(p.base) + ((t0 + r) * (size_t)p.base_ld + o0) * kSize + c * 16, true);
+  }
+  cp_async_commit();
   lora_neighbours(p, t0, rows);
   auto fetch_b = [&](int a) {
-    for (int i = threadIdx.x; i < width * (p.rank / 8); i += kLoraWarps * 32) {
-      const int r = i / (p.rank / 8), c = i % (p.rank / 8);
-      cp_async16(bs + r * bld + c * 16, p.b + ((size_t)a * p.outputs + o0 + r) * p.rank + c * 8, true);
-    }
+    const uint16_t* src = p.b + ((size_t)a * p.outputs + o0) * p.rank;
+    for (int r = threadIdx.x >> 3; r < width; r += kLoraWarps * 4)
+      for (int c = threadIdx.x & 7; c < p.rank / 8; c += 8)
+        cp_async16(bs + lora_place(r) * bld + c * 16, src + (size_t)r * p.rank + c * 8, true);
     cp_async_commit();
   };
   if (rows.n > 0) fetch_b(rows.uniq[0]);
-  const int row0 = t0 + warp * kLoraTile + g, row1 = row0 + 8;
   const int id0 = rows.ids[warp * kLoraTile + g], id1 = rows.ids[warp * kLoraTile + g + 8];
-  const bool in0 = row0 < p.tokens, in1 = row1 < p.tokens;
-  typename Four::Raw base[kBlocks][2];
+  const float f0 = id0 >= 0 ? p.scales[id0] : 0.f, f1 = id1 >= 0 ? p.scales[id1] : 0.f;
+  for (int c0 = 0; c0 * 16 < R; c0 += kBatch) {
+    if (c0 > 0) load_h(c0);
 #pragma unroll
-  for (int q = 0; q < kBlocks; ++q) {
-    const int o = o0 + q * 16 + 4 * t;
-    if (o < p.outputs) {
-      if (in0) base[q][0] = Four::load(p.base, (size_t)row0 * p.base_ld + o);
-      if (in1) base[q][1] = Four::load(p.base, (size_t)row1 * p.base_ld + o);
-    }
-  }
-  // this warp's 16 rows of h, scaled
-#pragma unroll 4
-  for (int i = lane; i < kLoraTile * R / 4; i += 32) {
-    const int r = warp * kLoraTile + i / (R / 4), c = i % (R / 4) * 4, id = rows.ids[r];
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (id >= 0) {
-      v = *reinterpret_cast<const float4*>(p.part + (size_t)(t0 + r) * R + c);
-      const float f = p.scales[id];
-      v.x *= f, v.y *= f, v.z *= f, v.w *= f;
-    }
-    lora_keep<kParts>(hs, plane, r * ld + c, v);
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int c = 0; c < kBatch; ++c)
+        if ((c0 + c) * 16 < R) {
+          const float f = i ? f1 : f0;
+          const float4 v = make_float4(h[i][c].x * f, h[i][c].y * f, h[i][c].z * f, h[i][c].w * f);
+          lora_keep<kParts>(hs, plane, (warp * kLoraTile + g + 8 * i) * ld + (c0 + c) * 16 + 4 * t, v);
+        }
   }
   for (int u = 0; u < rows.n; ++u) {
     const int a = rows.uniq[u];
@@ -548,17 +571,17 @@ __global__ void __launch_bounds__(kLoraWarps * 32) lora_expand_kernel(const __gr
         if (o >= p.outputs) break;
         float d[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
         const int j0 = lora_slice(p, o), j1 = o + 8 < p.outputs ? lora_slice(p, o + 8) : j0;
-        const int oc = q * 16 + (g >> 1) * 4 + (g & 1);
+        const uint8_t* br = bs + (q * 16 + g) * bld + 8 * t;
         for (int j = j0; j <= j1; ++j) {
           float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+          const uint16_t* hr = hs + (warp * kLoraTile + g) * ld + j * p.rank + 4 * t;
+#pragma unroll KR ? KR : 1
           for (int k = 0; k < steps; ++k) {
             uint32_t f[kParts][4];
-            lora_operands<kParts>(hs + (warp * kLoraTile + g) * ld + j * p.rank + 16 * k + 4 * t, plane, ld, f);
+            lora_operands<kParts>(hr + 16 * k, plane, ld, f);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint2 b = oc + 2 * i < width
-                                  ? *reinterpret_cast<const uint2*>(bs + (oc + 2 * i) * bld + 32 * k + 8 * t)
-                                  : make_uint2(0, 0);
+            for (int i = 0; i < 2; ++i) {  // a column past the last output is not written, whatever it holds
+              const uint2 b = *reinterpret_cast<const uint2*>(br + i * 8 * bld + 32 * k);
 #pragma unroll
               for (int part = 0; part < kParts; ++part) mma_16816<true>(acc[i], f[part], b.x, b.y);
             }
@@ -569,8 +592,12 @@ __global__ void __launch_bounds__(kLoraWarps * 32) lora_expand_kernel(const __gr
 #pragma unroll
             for (int e = 0; e < 4; ++e) d[i][e] = mine ? acc[i][e] : d[i][e];
         }
-        if (id0 == a) base[q][0] = Four::add(base[q][0], d[0][0], d[0][1], d[1][0], d[1][1]);
-        if (id1 == a) base[q][1] = Four::add(base[q][1], d[0][2], d[0][3], d[1][2], d[1][3]);
+        if (q * 16 + 4 * t < width) {
+          uint8_t* w = os + (warp * kLoraTile + g) * kOld + (q * 16 + 4 * t) * kSize;
+          if (id0 == a) Four::store(w, 0, Four::add(Four::load(w, 0), d[0][0], d[0][1], d[1][0], d[1][1]));
+          w += 8 * kOld;
+          if (id1 == a) Four::store(w, 0, Four::add(Four::load(w, 0), d[0][2], d[0][3], d[1][2], d[1][3]));
+        }
       }
     }
     if (u + 1 < rows.n) {
@@ -578,14 +605,14 @@ __global__ void __launch_bounds__(kLoraWarps * 32) lora_expand_kernel(const __gr
       fetch_b(rows.uniq[u + 1]);
     }
   }
+  cp_async_wait<0>();
+  __syncthreads();
   const bool copy = p.base != p.out;  // in place, rows without an adapter stay
-#pragma unroll
-  for (int q = 0; q < kBlocks; ++q) {
-    const int o = o0 + q * 16 + 4 * t;
-    if (o < p.outputs) {
-      if (in0 && (copy || id0 >= 0)) Four::store(p.out, (size_t)row0 * p.out_ld + o, base[q][0]);
-      if (in1 && (copy || id1 >= 0)) Four::store(p.out, (size_t)row1 * p.out_ld + o, base[q][1]);
-    }
+  for (int i = threadIdx.x; i < kLoraRows * kChunks; i += kLoraWarps * 32) {
+    const int r = i / kChunks, c = i % kChunks;
+    if (c < chunks && t0 + r < p.tokens && (copy || rows.ids[r] >= 0))
+      *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + ((t0 + r) * (size_t)p.out_ld + o0) * kSize + c * 16) =
+          *reinterpret_cast<const uint4*>(os + r * kOld + c * 16);
   }
 }
 
@@ -627,7 +654,7 @@ static int run_lora_group(const LoraArgs& p, cudaStream_t st) {
   int rc = launch_k(lora_shrink_group_kernel, dim3(units, p.splits, z), dim3(kLoraWarps * 32), 0, st, p);
   if (rc) return rc;
   return launch_k(lora_expand_group_kernel<OB>, dim3(units, (p.outputs + kLoraOutputs - 1) / kLoraOutputs),
-                  dim3(kLoraWarps * 32), (size_t)(OB ? 2 : 3) * kLoraTile * (R + 8) * 2, st, p);
+                  dim3(kLoraWarps * 32), (size_t)(OB ? 2 : 3) * kLoraTile * lora_ld(R) * 2, st, p);
 }
 
 template <bool OB>
@@ -636,7 +663,7 @@ static int run_lora_prompt(const LoraArgs& p, cudaStream_t st) {
   const unsigned tiles = (p.tokens + kLoraRows - 1) / kLoraRows, z = (R + 8 * kLoraRankTiles - 1) / (8 * kLoraRankTiles);
   constexpr size_t ring = (size_t)kLoraStages * kLoraStageBytes;
   static_assert(ring >= (size_t)kLoraRows * (kLoraRankTiles * 8 + 4) * 4, "the sums take the ring's place");
-  static std::atomic<uint64_t> shrink_set{0}, expand_set{0};  // devices with the limit raised
+  static std::atomic<uint64_t> shrink_set{0}, expand_set[4];  // per kernel: devices with the limit raised
   int rc = ensure_smem_limit(lora_shrink_kernel, ring, shrink_set);
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -652,11 +679,19 @@ static int run_lora_prompt(const LoraArgs& p, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, lora_shrink_kernel, p) != cudaSuccess) return CCUT_ERR_CUDA;
-  auto smem = [](size_t R, size_t rank) { return (OB ? 2 : 3) * kLoraRows * (R + 8) * 2 + kLoraOutputs * (rank * 2 + 16); };
-  rc = ensure_smem_limit(lora_expand_kernel<OB>, smem(kLoraMaxRanks, kLoraMaxRanks), expand_set);
+  auto smem = [](size_t R, size_t rank) {
+    return (size_t)(OB ? 2 : 3) * kLoraRows * lora_ld((int)R) * 2 + kLoraOutputs * lora_ld((int)rank) * 2 +
+           kLoraRows * (kLoraOutputs + 16) * (OB ? 2 : 4);
+  };
+  auto kern = p.rank == 16   ? lora_expand_kernel<1, OB>
+              : p.rank == 32 ? lora_expand_kernel<2, OB>
+              : p.rank == 64 ? lora_expand_kernel<4, OB>
+                             : lora_expand_kernel<0, OB>;
+  rc = ensure_smem_limit(kern, smem(kLoraMaxRanks, kLoraMaxRanks),
+                         expand_set[p.rank == 16 ? 0 : p.rank == 32 ? 1 : p.rank == 64 ? 2 : 3]);
   if (rc) return rc;
-  return launch_k(lora_expand_kernel<OB>, dim3(tiles, (p.outputs + kLoraOutputs - 1) / kLoraOutputs),
-                  dim3(kLoraWarps * 32), smem(R, p.rank), st, p);
+  return launch_k(kern, dim3(tiles, (p.outputs + kLoraOutputs - 1) / kLoraOutputs), dim3(kLoraWarps * 32),
+                  smem(R, p.rank), st, p);
 }
 
 }  // namespace ccut
