@@ -220,6 +220,9 @@ __global__ void __launch_bounds__(kLoraWarps * 32) lora_shrink_group_kernel(cons
 // Byte offset of 16-byte chunk c of row r in a tile of 128-byte rows: ldmatrix reads 8 rows of one chunk without
 // meeting a bank twice.
 CCUT_DEVICE int lora_chunk(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
+CCUT_DEVICE void lora_copy(uint32_t to, const void* from, bool in) {  // 16 bytes, zeros when !in
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(in ? 16 : 0) : "memory");
+}
 CCUT_DEVICE float4 ld_cluster(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
@@ -239,19 +242,29 @@ __global__ void __launch_bounds__(kLoraWarps * 32) lora_shrink_kernel(const __gr
   lora_neighbours(p, t0, rows);
   const int k0 = blockIdx.y * p.k_per_split, k1 = min(p.inputs, k0 + p.k_per_split);
   const int steps = k1 > k0 ? (k1 - k0 + kLoraStep - 1) / kLoraStep : 0, total = steps * rows.n;
-  // copies of a stage: thread -> chunks of rows tid / 8, + 16, + 32, + 48
+  // copies of a stage: thread -> 16-byte chunk tid % 8 of rows tid / 8, + 16, + 32, + 48 of x and of A; the
+  // addresses move from stage to stage and back at the next adapter
   const int cr = threadIdx.x >> 3, cc = threadIdx.x & 7;
-  auto issue = [&](int s) {
-    uint8_t* st = ring + s % kLoraStages * kLoraStageBytes;
-    const int k = k0 + s % steps * kLoraStep + cc * 8;
-    const uint16_t* ar = p.a + ((size_t)rows.uniq[s / steps] * R + r0) * p.inputs;
+  const int first_k = k0 + cc * 8;
+  const uint16_t* xa = p.x + (size_t)min(t0 + cr, p.tokens - 1) * p.inputs;
+  const size_t hop = (size_t)16 * p.inputs;
+  int fetch_step = 0, fetch_adapter = 0, fetch_stage = 0, fetch_k = first_k;
+  const uint16_t* wa = nullptr;
+  const int xrows = (p.tokens - t0 - cr + 15) / 16, wrows = (nz * 8 - cr + 15) / 16;  // of the four, those that exist
+  const uint32_t to = smem_u32(ring) + lora_chunk(cr, cc);  // rows 16 apart: the same place, 2048 bytes on
+  auto issue = [&]() {
+    if (fetch_step == 0) wa = p.a + ((size_t)rows.uniq[fetch_adapter] * R + r0 + min(cr, nz * 8 - 1)) * p.inputs;
+    const bool in = fetch_k < k1;
+    const uint32_t st = to + fetch_stage * kLoraStageBytes;
 #pragma unroll
     for (int i = 0; i < kLoraRows / 16; ++i) {
-      const int r = cr + 16 * i;
-      const bool xin = k < k1 && t0 + r < p.tokens, win = k < k1 && r < nz * 8;
-      cp_async16(st + lora_chunk(r, cc), xin ? p.x + (size_t)(t0 + r) * p.inputs + k : p.x, xin);
-      cp_async16(st + kLoraRows * 128 + lora_chunk(r, cc), win ? ar + (size_t)r * p.inputs + k : p.x, win);
+      const bool xin = in && i < xrows, win = in && i < wrows;
+      lora_copy(st + i * 2048, xin ? xa + i * hop + fetch_k : p.x, xin);
+      lora_copy(st + kLoraRows * 128 + i * 2048, win ? wa + i * hop + fetch_k : p.x, win);
     }
+    fetch_k += kLoraStep;
+    if (++fetch_stage == kLoraStages) fetch_stage = 0;
+    if (++fetch_step == steps) fetch_step = 0, ++fetch_adapter, fetch_k = first_k;
   };
   float keep[kLoraRankTiles][4], acc[kLoraRankTiles][4];
 #pragma unroll
@@ -261,15 +274,17 @@ __global__ void __launch_bounds__(kLoraWarps * 32) lora_shrink_kernel(const __gr
   const int id0 = rows.ids[warp * kLoraTile + g], id1 = rows.ids[warp * kLoraTile + g + 8];
 #pragma unroll
   for (int i = 0; i < kLoraStages - 1; ++i) {
-    if (i < total) issue(i);
+    if (i < total) issue();
     cp_async_commit();
   }
+  int step = 0, adapter = 0, stage = 0;
   for (int s = 0; s < total; ++s) {
     cp_async_wait<kLoraStages - 2>();
     __syncthreads();  // everyone's copies of this stage have landed, everyone is done with the stage before
-    if (s + kLoraStages - 1 < total) issue(s + kLoraStages - 1);
+    if (s + kLoraStages - 1 < total) issue();
     cp_async_commit();
-    const uint8_t* st = ring + s % kLoraStages * kLoraStageBytes;
+    const uint8_t* st = ring + stage * kLoraStageBytes;
+    if (++stage == kLoraStages) stage = 0;
 #pragma unroll
     for (int kk = 0; kk < kLoraStep / 16; ++kk) {
       uint32_t f[4];
@@ -284,8 +299,9 @@ __global__ void __launch_bounds__(kLoraWarps * 32) lora_shrink_kernel(const __gr
           mma_16816<true>(acc[n + 1], f, b2, b3);
         }
     }
-    if (s % steps == steps - 1) {  // the last of an adapter: its rows take the sums
-      const int a = rows.uniq[s / steps];
+    if (++step == steps) {  // the last of an adapter: its rows take the sums
+      const int a = rows.uniq[adapter++];
+      step = 0;
 #pragma unroll
       for (int n = 0; n < kLoraRankTiles; ++n) {
         keep[n][0] = id0 == a ? acc[n][0] : keep[n][0];
@@ -530,19 +546,28 @@ __global__ void __launch_bounds__(kLoraWarps * 32, OUT_BF16 ? 4 : 3)
                       : make_float4(0.f, 0.f, 0.f, 0.f);
   };
   load_h(0);
-  const int chunks = width * kSize / 16;  // widths are multiples of 8: whole chunks
-  for (int i = threadIdx.x; i < kLoraRows * kChunks; i += kLoraWarps * 32) {
-    const int r = i / kChunks, c = i % kChunks;
-    if (c < chunks && t0 + r < p.tokens)
-      cp_async16(os + r * kOld + c * 16, static_cast<const uint8_t*>(p.base) + ((t0 + r) * (size_t)p.base_ld + o0) * kSize + c * 16, true);
+  constexpr int kHop = kLoraWarps * 32 / kChunks;  // rows that the CTA moves at a time
+  const int mr = threadIdx.x / kChunks, mc = threadIdx.x % kChunks;
+  const bool mine = mc < width * kSize / 16;  // widths are multiples of 8: whole chunks
+  const int mrows = mine ? min(kLoraRows, p.tokens - t0) : 0;
+  {
+    const uint8_t* from = static_cast<const uint8_t*>(p.base) + ((size_t)(t0 + mr) * p.base_ld + o0) * kSize + mc * 16;
+    const size_t hop = (size_t)kHop * p.base_ld * kSize;
+    const uint32_t to = smem_u32(os) + mr * kOld + mc * 16;
+#pragma unroll
+    for (int r = 0; r < kLoraRows; r += kHop)
+      if (r + mr < mrows) lora_copy(to + r * kOld, from + r / kHop * hop, true);
   }
   cp_async_commit();
   lora_neighbours(p, t0, rows);
   auto fetch_b = [&](int a) {
-    const uint16_t* src = p.b + ((size_t)a * p.outputs + o0) * p.rank;
-    for (int r = threadIdx.x >> 3; r < width; r += kLoraWarps * 4)
-      for (int c = threadIdx.x & 7; c < p.rank / 8; c += 8)
-        cp_async16(bs + lora_place(r) * bld + c * 16, src + (size_t)r * p.rank + c * 8, true);
+    const int br = threadIdx.x >> 3, bc = threadIdx.x & 7;
+    const uint16_t* from = p.b + ((size_t)a * p.outputs + o0 + br) * p.rank + bc * 8;
+    const uint32_t to = smem_u32(bs) + lora_place(br) * bld + bc * 16;
+#pragma unroll
+    for (int r = 0; r < kLoraOutputs; r += 16)
+      if (r + br < width)
+        for (int c = 0; c < p.rank / 8 - bc; c += 8) lora_copy(to + r * bld + c * 16, from + (size_t)r * p.rank + c * 8, true);
     cp_async_commit();
   };
   if (rows.n > 0) fetch_b(rows.uniq[0]);
@@ -592,7 +617,7 @@ __global__ void __launch_bounds__(kLoraWarps * 32, OUT_BF16 ? 4 : 3)
 #pragma unroll
             for (int e = 0; e < 4; ++e) d[i][e] = mine ? acc[i][e] : d[i][e];
         }
-        if (q * 16 + 4 * t < width) {
+        if (q * 16 + 4 * t < width) {  // the one place where an output is changed
           uint8_t* w = os + (warp * kLoraTile + g) * kOld + (q * 16 + 4 * t) * kSize;
           if (id0 == a) Four::store(w, 0, Four::add(Four::load(w, 0), d[0][0], d[0][1], d[1][0], d[1][1]));
           w += 8 * kOld;
@@ -608,12 +633,12 @@ __global__ void __launch_bounds__(kLoraWarps * 32, OUT_BF16 ? 4 : 3)
   cp_async_wait<0>();
   __syncthreads();
   const bool copy = p.base != p.out;  // in place, rows without an adapter stay
-  for (int i = threadIdx.x; i < kLoraRows * kChunks; i += kLoraWarps * 32) {
-    const int r = i / kChunks, c = i % kChunks;
-    if (c < chunks && t0 + r < p.tokens && (copy || rows.ids[r] >= 0))
-      *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + ((t0 + r) * (size_t)p.out_ld + o0) * kSize + c * 16) =
-          *reinterpret_cast<const uint4*>(os + r * kOld + c * 16);
-  }
+  uint8_t* out = static_cast<uint8_t*>(p.out) + ((size_t)(t0 + mr) * p.out_ld + o0) * kSize + mc * 16;
+  const size_t hop = (size_t)kHop * p.out_ld * kSize;
+#pragma unroll
+  for (int r = 0; r < kLoraRows; r += kHop)
+    if (r + mr < mrows && (copy || rows.ids[r + mr] >= 0))
+      *reinterpret_cast<uint4*>(out + r / kHop * hop) = *reinterpret_cast<const uint4*>(os + (r + mr) * kOld + mc * 16);
 }
 
 // Units of a decode step at most: one per adapter in use, one more per 16 tokens, tokens without one.
