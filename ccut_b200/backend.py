@@ -20,6 +20,12 @@ one token id back (errors evict that request).  ``GenericBackend`` answers that 
 (the loop of ``_backend_step`` as one call): the requests' new ids run through one decoder
 pass per prefill chunk, so their MoE blocks see all the step's tokens together.
 
+``sampling_params["adapter"]`` names the request's low-rank adapter (an index into the layers' banks; None or
+absent: none); a cache serves only requests of the adapter it was computed with.  ``generate_step`` and
+``generate_batch`` with ``logprobs=n`` also answer each token's log probability, its rank, the entropy and the
+``n`` best alternatives (``ccut_b200.logprobs``, on the logits before temperature and filters); ``score``
+answers them for the tokens of a given text.
+
 ``generate`` and ``forward_step`` give the interface of the reference's fallback backend
 (``L1Backend``, ``ccut/models/backend_transformers.py:31-124``), which the engine uses when a
 backend has no ``generate_step``: ``forward_step(input_ids, past)`` returns the logits of the
@@ -34,6 +40,7 @@ from typing import Any, Callable
 import numpy as np
 import torch
 
+from ccut_b200.logprobs import token_logprobs
 from ccut_b200.model import KvCache, MoeDecoder
 from ccut_b200.sampling import sample
 
@@ -54,6 +61,7 @@ class _Seq:
     def __init__(self, cache: KvCache):
         self.cache = cache
         self.ids: list[int] = []
+        self.adapter: int | None = None  # the adapter the cached positions were computed with
 
 
 class GenericBackend:
@@ -62,13 +70,15 @@ class GenericBackend:
     tier = "L0"
 
     def __init__(self, model: MoeDecoder, max_seqs: int = 4, max_len: int = 4096, prefill_chunk: int = 4096,
-                 seed: int = 0, eos_token_id: int | None = None, pool: bool = False):
+                 seed: int = 0, eos_token_id: int | None = None, pool: bool = False, kv_dtype: str | None = None):
         """``pool``: keep the sequence caches in one ``KvPool``, so that a decode step of several
-        requests (``generate_batch``) runs one attention launch per layer."""
+        requests (``generate_batch``) runs one attention launch per layer.  ``kv_dtype``: ``"bf16"``,
+        ``"int4"`` (4-bit caches, ``blocks.attn_kv4``) or None (the model's ``kv_dtype``)."""
         if max_seqs < 1 or max_len < 1 or prefill_chunk < 1:
             raise ValueError("max_seqs, max_len and prefill_chunk must be positive")
         self.model = model
-        self._pool = model.new_pool(max_seqs, max_len) if pool else None
+        self._cache_args = {} if kv_dtype is None else {"kv_dtype": kv_dtype}
+        self._pool = model.new_pool(max_seqs, max_len, **self._cache_args) if pool else None
         self.max_seqs, self.max_len, self.prefill_chunk = int(max_seqs), int(max_len), int(prefill_chunk)
         self.eos_token_id = eos_token_id
         self._seqs: list[_Seq] = []  # least recently used first
@@ -77,11 +87,12 @@ class GenericBackend:
         self.tokens_run = 0  # positions the decoder computed (prefix reuse skips the rest)
 
     # ---- sequence caches ---------------------------------------------------------------
-    def _acquire(self, ids: list[int], taken: list) -> tuple[_Seq, int]:
-        """The cache to run ``ids`` in (not one of ``taken``) and how many of its positions stay."""
+    def _acquire(self, ids: list[int], taken: list, adapter: int | None = None) -> tuple[_Seq, int]:
+        """The cache to run ``ids`` in (not one of ``taken``) and how many of its positions stay: those
+        of a common prefix computed with the same adapter."""
         best, best_p = None, 0
         for s in self._seqs:
-            if any(s is t for t in taken):
+            if any(s is t for t in taken) or s.adapter != adapter:
                 continue
             p = common_prefix(s.ids, ids)
             if p > best_p:
@@ -91,7 +102,7 @@ class GenericBackend:
             reuse = 0
             if len(self._seqs) < self.max_seqs:
                 cache = (self._pool.cache(len(self._seqs)) if self._pool is not None
-                         else self.model.new_cache(self.max_len))
+                         else self.model.new_cache(self.max_len, **self._cache_args))
                 best = _Seq(cache)
             else:
                 free = [s for s in self._seqs if not any(s is t for t in taken)]
@@ -101,6 +112,7 @@ class GenericBackend:
         if any(best is s for s in self._seqs):
             self._seqs.remove(best)
         self._seqs.append(best)
+        best.adapter = adapter
         return best, reuse
 
     def _check(self, input_ids) -> list[int]:
@@ -111,15 +123,22 @@ class GenericBackend:
             raise ValueError(f"{len(ids)} ids exceed the backend's max_len of {self.max_len}")
         return ids
 
-    def logits_batch(self, id_lists) -> list:
+    def logits_batch(self, id_lists, adapters=None) -> list:
         """fp32 logits ``[vocab]`` of the last id of every list, the lists run together: each
         call of the decoder takes the next ``prefill_chunk`` ids (at most) of every list that
-        has ids left, so decoding sequences share their MoE passes."""
+        has ids left, so decoding sequences share their MoE passes.  ``adapters``: the adapter of
+        every list (or None), default none."""
         lists = [self._check(ids) for ids in id_lists]
+        adapters = [None] * len(lists) if adapters is None else list(adapters)
+        if len(adapters) != len(lists):
+            raise ValueError(f"{len(adapters)} adapters for {len(lists)} id lists")
+        for a in adapters:
+            if a is not None:
+                self.model._adapter(a)  # refused before any cache is taken
         seqs: list[_Seq] = []
         pos: list[int] = []
-        for ids in lists:
-            seq, reuse = self._acquire(ids, seqs)
+        for ids, adapter in zip(lists, adapters):
+            seq, reuse = self._acquire(ids, seqs, adapter)
             seq.cache.truncate(min(reuse, seq.cache.length))
             seq.ids = ids[: seq.cache.length]
             seqs.append(seq)
@@ -131,7 +150,8 @@ class GenericBackend:
                 return out
             ends = [min(len(lists[j]), pos[j] + self.prefill_chunk) for j in todo]
             logits = self.model.forward_batch(
-                [(lists[j][pos[j]: e], seqs[j].cache, pos[j]) for j, e in zip(todo, ends)])
+                [(lists[j][pos[j]: e], seqs[j].cache, pos[j]) + (() if adapters[j] is None else (adapters[j],))
+                 for j, e in zip(todo, ends)])
             for j, e, lg in zip(todo, ends, logits):
                 self.tokens_run += e - pos[j]
                 seqs[j].ids = lists[j][:e]
@@ -139,20 +159,57 @@ class GenericBackend:
                 if e == len(lists[j]):
                     out[j] = lg
 
-    def logits_for(self, input_ids) -> torch.Tensor:
+    def logits_for(self, input_ids, adapter: int | None = None) -> torch.Tensor:
         """fp32 logits ``[vocab]`` of the last of ``input_ids`` (runs what no cache holds)."""
-        return self.logits_batch([input_ids])[0]
+        return self.logits_batch([input_ids], [adapter])[0]
 
     # ---- Engine interface ----------------------------------------------------------------
-    def generate_step(self, input_ids, sampling_params: dict | None = None) -> int:
-        return sample(self.logits_for(input_ids), sampling_params, self._gen)
+    def generate_step(self, input_ids, sampling_params: dict | None = None, logprobs: int | None = None):
+        """The next token id; with ``logprobs`` = n, ``(id, answer)`` as ``generate_batch``."""
+        if logprobs is not None:
+            return self.generate_batch([(input_ids, sampling_params)], logprobs)[0]
+        return sample(self.logits_for(input_ids, (sampling_params or {}).get("adapter")), sampling_params, self._gen)
 
-    def generate_batch(self, requests) -> list[int]:
+    def generate_batch(self, requests, logprobs: int | None = None) -> list:
         """``requests`` = ``[(input_ids, sampling_params), ...]``, one per scheduled request of an
-        engine step (at most ``max_seqs``): the next token of each, from one batched pass."""
+        engine step (at most ``max_seqs``): the next token of each, from one batched pass.  With
+        ``logprobs`` = n, ``(token, answer)`` of each, ``answer`` a dict of the token's ``logprob``
+        and ``rank``, the distribution's ``entropy`` (nats) and the n best ``top`` as ``(id,
+        logprob)``, from the logits before temperature and filters."""
         requests = list(requests)
-        logits = self.logits_batch([r[0] for r in requests])
-        return [sample(lg, r[1], self._gen) for lg, r in zip(logits, requests)]
+        logits = self.logits_batch([r[0] for r in requests], [(r[1] or {}).get("adapter") for r in requests])
+        tokens = [sample(lg, r[1], self._gen) for lg, r in zip(logits, requests)]
+        if logprobs is None:
+            return tokens
+        if not requests:
+            return []
+        return list(zip(tokens, self._answers(torch.stack([lg.reshape(-1) for lg in logits]), tokens, int(logprobs))))
+
+    @staticmethod
+    def _answers(logits: torch.Tensor, tokens, top_n: int) -> list:
+        r = token_logprobs(logits, torch.as_tensor(tokens, dtype=torch.int32).to(logits.device), top_n)
+        lp, ent, rank = r.logprob.tolist(), r.entropy.tolist(), r.rank.tolist()
+        ids, tops = r.top_ids.tolist(), r.top_logprobs.tolist()
+        return [{"logprob": lp[i], "rank": rank[i], "entropy": ent[i], "top": list(zip(ids[i], tops[i]))}
+                for i in range(len(lp))]
+
+    def score(self, input_ids, top_n: int = 0, adapter: int | None = None) -> list:
+        """The answers (as ``generate_batch``) for ``input_ids[1:]``, each given the ids before it.  Runs in
+        a cache of its own, ``min(prefill_chunk, 1024)`` positions at a time (the logits of one chunk are
+        held at once)."""
+        ids = self._check(input_ids)
+        out: list = []
+        if len(ids) < 2:
+            return out
+        cache = self.model.new_cache(len(ids) - 1, **self._cache_args)
+        step = min(self.prefill_chunk, 1024)
+        for c0 in range(0, len(ids) - 1, step):
+            c1 = min(len(ids) - 1, c0 + step)
+            extra = {} if adapter is None else {"adapter": adapter}
+            logits = self.model.forward(ids[c0:c1], cache, c0, all_logits=True, **extra)
+            self.tokens_run += c1 - c0
+            out += self._answers(logits, ids[c0 + 1: c1 + 1], int(top_n))
+        return out
 
     # ---- L1Backend interface -------------------------------------------------------------
     def forward_step(self, input_ids, past: Any = None) -> tuple[torch.Tensor, KvCache]:
@@ -162,7 +219,7 @@ class GenericBackend:
         ids = [int(t) for t in input_ids]
         if not ids:
             raise ValueError("forward_step needs at least one input id")
-        cache = past if past is not None else self.model.new_cache(self.max_len)
+        cache = past if past is not None else self.model.new_cache(self.max_len, **self._cache_args)
         if len(ids) > cache.max_len:
             raise ValueError(f"{len(ids)} ids exceed the cache's max_len of {cache.max_len}")
         start = min(cache.length, len(ids) - 1)

@@ -734,7 +734,8 @@ def load_decoder(model_dir: str | Path, device="cuda", kernel: str = "auto", nam
     kept as bf16 for cuBLAS.  RoPE from ``rope_theta`` / ``rope_scaling``: the reference's
     ``build_rope`` table (``rope_table``: none, linear, dynamic, its own yarn), whose attention
     factor the reference's layer does not apply, and neither does this decoder.  ``app_config``: the engine's config (``[experts]`` / ``[quant]``,
-    ``ccut_b200.config``), checked against the checkpoint before anything is uploaded.
+    ``ccut_b200.config``), checked against the checkpoint before anything is uploaded; its
+    ``kv_cache_dtype`` is what the decoder's caches are made as.
 
     MLA checkpoints (DeepSeek-V2 / V3) give ``MlaDecoderLayer`` layers: ``kv_a_proj_with_mqa``
     (576 outputs, not a multiple of the 128 the quantized-projection kernel tiles by) and
@@ -749,12 +750,15 @@ def load_decoder(model_dir: str | Path, device="cuda", kernel: str = "auto", nam
     from ccut_b200.model import DecoderLayer, MlaDecoderLayer, MoeDecoder, rope_table, yarn_rope_table
     from ccut_b200.quant import QuantLinear, dequantize, pad_out_channels
 
+    kv_dtype = "bf16"
     if app_config is not None:  # the engine's [experts] / [quant] settings, checked before any upload
         from ccut_b200.config import resolve
 
-        resolve(app_config, CheckpointReader(model_dir).config)
+        kv_dtype = resolve(app_config, CheckpointReader(model_dir).config)["kv_cache_dtype"]
     w = load_decoder_weights(model_dir, names)
     spec = w["spec"]
+    if spec.mla and kv_dtype != "bf16":
+        raise NotImplementedError(f"kv_cache_dtype = {kv_dtype!r} for a model with multi-head latent attention")
     scaling_type = "none"
     if spec.mla and spec.rope_scaling and spec.rope_scaling["type"] == "yarn":
         inv_freq, f = yarn_rope_table(spec.head_dim, spec.rope_theta, spec.rope_scaling)
@@ -809,6 +813,8 @@ def load_decoder(model_dir: str | Path, device="cuda", kernel: str = "auto", nam
         q, k, v, o = (dense(lay[p], *dims[p]) for p in "qkvo")
         layers.append(DecoderLayer(lay["ln1"], q, k, v, o, lay["ln2"], ffn, lay["q_norm"], lay["k_norm"],
                                    heads=spec.heads, kv_heads=spec.kv_heads, head_dim=d, device=device))
-    return MoeDecoder(w["embed"], layers, w["final_norm"], w["lm_head"], inv_freq=inv_freq,
-                      attention_factor=attn_factor, scaling_type=scaling_type, eps=spec.eps, softcap=spec.softcap,
-                      device=device)
+    dec = MoeDecoder(w["embed"], layers, w["final_norm"], w["lm_head"], inv_freq=inv_freq,
+                     attention_factor=attn_factor, scaling_type=scaling_type, eps=spec.eps, softcap=spec.softcap,
+                     device=device)
+    dec.kv_dtype = kv_dtype
+    return dec

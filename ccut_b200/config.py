@@ -8,7 +8,8 @@
   weight codes, activations in 16 bits); ``w8a8`` is accepted and computed the same way, as
   the reference computes it (its ``_w8a8`` dequantizes the weights and multiplies the
   unquantized activations, ``ccut/quant/method.py:131-139``).  ``kv_cache_dtype``: ``auto`` /
-  ``bf16`` (the decoder's caches are bf16); ``fp8`` is refused.  ``quant_ignore`` applies to
+  ``bf16``, or this path's own ``int4`` (4-bit caches, ``ccut_b200.blocks.attn_kv4``; GQA models);
+  ``fp8`` is refused.  ``quant_ignore`` applies to
   online quantization only.
 - ``[experts]``: the reference streams experts from disk (``expert_residency = "zero"`` or
   ``"page_cache_only"``, a ring of ``expert_ring_slots``); here every expert is packed into HBM
@@ -56,10 +57,11 @@ def quant_settings(app_config, checkpoint_config: dict) -> dict:
         raise ValueError(f"[quant] fp8_compute_mode = {mode!r} is not one of w8a16, w8a8")
     kv = str(q.get("kv_cache_dtype", "auto"))
     if kv == "fp8":
-        raise NotImplementedError("kv_cache_dtype = \"fp8\": the decoder's kv caches are bf16")
-    if kv not in ("auto", "bf16"):
-        raise ValueError(f"[quant] kv_cache_dtype = {kv!r} is not one of auto, bf16, fp8")
-    return {"format": quant_format(checkpoint_config), "fp8_compute_mode": mode, "kv_cache_dtype": "bf16"}
+        raise NotImplementedError("kv_cache_dtype = \"fp8\": the decoder's kv caches are bf16 or int4")
+    if kv not in ("auto", "bf16", "int4"):
+        raise ValueError(f"[quant] kv_cache_dtype = {kv!r} is not one of auto, bf16, int4, fp8")
+    return {"format": quant_format(checkpoint_config), "fp8_compute_mode": mode,
+            "kv_cache_dtype": "bf16" if kv == "auto" else kv}
 
 
 def expert_settings(app_config) -> dict:

@@ -31,7 +31,11 @@ The step ends with ``logits = rms_norm(h, final_norm) @ lm_head^T`` in fp32 (``l
 is kept as an fp32 copy).  ``forward_batch`` runs several sequences in one pass: their tokens
 are stacked for the projections, norms, RoPE (each token at its own position) and the FFN, so
 a MoE block reads its experts once for the whole batch; attention runs per sequence over its
-own cache.  Every block gets its documented layout; the reference's layer
+own cache.  With 4-bit caches (``blocks.attn_kv4``: ``new_cache`` / ``new_pool`` with ``kv_dtype="int4"``)
+the cache writes are one ``kv4_append`` per pool and attention is ``kv4_attention``, one call for sequences of
+one pool that run the same number of tokens.  A layer made with ``adapters`` adds each request's low-rank
+adapter (``adapters.LoraBank``) to its q / k / v and output projections; ``forward_batch`` takes the adapter of
+each sequence.  Every block gets its documented layout; the reference's layer
 passes q as ``[1, seq, heads, d]`` to blocks that take ``[batch, heads, seq, d]``, which is
 the same computation for one token and one kv head only.
 
@@ -46,6 +50,8 @@ import torch
 import torch.nn.functional as F
 
 from ccut_b200 import _lib
+from ccut_b200.adapters import LoraBank
+from ccut_b200.blocks.attn_kv4 import Kv4Cache, Kv4Pool, kv4_append, kv4_attention
 from ccut_b200.blocks.attn_mla import _latent_attention as _mla_attend
 from ccut_b200.blocks.norm import rms_norm
 from ccut_b200.blocks.rope import apply_rope
@@ -184,6 +190,45 @@ def _attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, start_pos: int, s
     return out
 
 
+class _Kv4Step:
+    """What every layer of one ``forward_batch`` over 4-bit caches needs, uploaded once: the rows that the
+    step's tokens go to, and the attention calls (one for all spans when they share a pool and run the same
+    number of tokens, else one per span)."""
+
+    def __init__(self, spans: list, device):
+        pools = {id(s.cache.pool) for s in spans}
+        tok_slots = np.concatenate([np.full(s.n, s.cache.slot, np.int32) for s in spans])
+        tok_pos = np.concatenate([np.arange(s.start, s.start + s.n, dtype=np.int32) for s in spans])
+        slots = np.array([s.cache.slot for s in spans], np.int32)
+        starts = np.array([s.start for s in spans], np.int32)
+        N, B = len(tok_slots), len(spans)
+        up = torch.from_numpy(np.concatenate([tok_slots, tok_pos, slots, starts])).to(device)
+        self.slots_of, self.positions = up[:N], up[N: 2 * N]
+        self.slots, self.starts = up[2 * N: 2 * N + B], up[2 * N + B:]
+        one = len(pools) == 1
+        # (pool, first token, tokens) of every append
+        self.appends = [(spans[0].cache.pool, 0, N)] if one else [(s.cache.pool, s.off, s.n) for s in spans]
+        # (pool, first span, spans, first token, tokens per span, longest length) of every attention call
+        if one and len({s.n for s in spans}) == 1:
+            self.calls = [(spans[0].cache.pool, 0, B, 0, spans[0].n, max(s.start + s.n for s in spans))]
+        else:
+            self.calls = [(s.cache.pool, j, 1, s.off, s.n, s.start + s.n) for j, s in enumerate(spans)]
+
+    def attend(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layer: int, softcap) -> torch.Tensor:
+        """q [heads, N, d] bf16 and k, v [N, kv_heads, d] of the step's tokens: k and v into the caches, then
+        attention -> [N, heads * d] bf16."""
+        for pool, off, n in self.appends:
+            kv4_append(pool, layer, k[off: off + n], v[off: off + n], self.slots_of[off: off + n],
+                       self.positions[off: off + n])
+        H, _, d = q.shape
+        outs = []
+        for pool, j, b, off, n, kv_len in self.calls:
+            qb = q[:, off: off + b * n].reshape(H, b, n, d).transpose(0, 1)
+            o = kv4_attention(qb, pool, layer, self.slots[j: j + b], self.starts[j: j + b], kv_len=kv_len, softcap=softcap)
+            outs.append(o.transpose(1, 2).reshape(b * n, H * d))
+        return outs[0] if len(outs) == 1 else torch.cat(outs)
+
+
 class DecoderLayer:
     """One ``full_attn`` decoder layer.
 
@@ -193,10 +238,11 @@ class DecoderLayer:
     ``ccut_quant_linear``; three of them for q / k / v are fused into one); ``q_norm`` / ``k_norm``
     None, ``[heads * d]`` / ``[kv_heads * d]`` (over the whole projection, the reference's
     ``rms_norm(q.reshape(seq, -1), w)``) or ``[d]`` (per head); ``ffn`` any object with
-    ``forward(x_bf16 [T, H], out_dtype) -> [T, H]`` (``MoeLayer``, ``DenseFfn``)."""
+    ``forward(x_bf16 [T, H], out_dtype) -> [T, H]`` (``MoeLayer``, ``DenseFfn``).  ``adapters``: None, or a dict
+    with a ``LoraBank`` for ``"qkv"`` (widths of q, k and v) and / or ``"o"``."""
 
     def __init__(self, ln1, wq, wk, wv, wo, ln2, ffn, q_norm=None, k_norm=None, *, heads: int, kv_heads: int,
-                 head_dim: int, device="cuda"):
+                 head_dim: int, device="cuda", adapters: dict | None = None):
         dev = torch.device(device)
         if head_dim not in (64, 128):
             raise NotImplementedError(f"head dim {head_dim} (have 64, 128)")
@@ -234,6 +280,17 @@ class DecoderLayer:
         self.k_norm = self._norm_w(k_norm, kv_heads, dev, "k_norm")
         self.ffn = ffn
         self.device = dev
+        self.adapters = self._check_adapters(adapters)
+
+    def _check_adapters(self, adapters: dict | None) -> dict:
+        H, q, kv = self.hidden, self.heads * self.head_dim, self.kv_heads * self.head_dim
+        fits = {"qkv": (H, [q, kv, kv]), "o": (q, [H])}
+        for name, bank in (adapters or {}).items():
+            if name not in fits or not isinstance(bank, LoraBank):
+                raise ValueError(f"adapters take a LoraBank for 'qkv' and 'o', got {name!r}")
+            if (bank.inputs, bank.widths) != fits[name]:
+                raise ValueError(f"adapters[{name!r}] must map {fits[name][0]} features to widths {fits[name][1]}")
+        return dict(adapters or {})
 
     @property
     def cache_layout(self) -> tuple:
@@ -261,16 +318,24 @@ class DecoderLayer:
             return rms_norm(x.contiguous(), w, eps).reshape(seq, n, d)
         return rms_norm(x.reshape(seq, n, d).contiguous(), w, eps)
 
-    def forward(self, h: torch.Tensor, spans: list, layer: int, rope: "_Rope", pooled=None) -> torch.Tensor:
+    def _adapted(self, name: str, y: torch.Tensor, x: torch.Tensor, ids) -> torch.Tensor:
+        """y, a projection's output for x, plus each token's adapter (in place)."""
+        bank = self.adapters.get(name) if ids is not None else None
+        return y if bank is None else bank.add(y, x, ids, out=y)
+
+    def forward(self, h: torch.Tensor, spans: list, layer: int, rope: "_Rope", pooled=None,
+                adapter_ids=None) -> torch.Tensor:
         """h [N, H] fp32 (the residual stream of every span's tokens, one after the other) ->
         [N, H] fp32.  Each ``_Span`` writes its sequence's cache at ``start .. start + n - 1`` of
         ``layer`` and attends over it; the projections, norms, RoPE and the FFN run once over
         all N tokens.  ``pooled`` = ``(pool, slots, starts)`` when every span is one token of a
-        cache in the same ``KvPool``: attention is then one launch for all of them."""
+        cache in the same ``KvPool``: attention is then one launch for all of them.  Over 4-bit caches
+        ``pooled`` is the step's ``_Kv4Step``.  ``adapter_ids``: each token's adapter (int32 [N], -1: none)
+        or None."""
         N = h.shape[0]
         H, Hkv, d = self.heads, self.kv_heads, self.head_dim
         x = rms_norm(h, self.ln1, rope.eps).to(torch.bfloat16)
-        qkv = _project(self.wqkv, x)
+        qkv = self._adapted("qkv", _project(self.wqkv, x), x, adapter_ids)
         q = self._qk_norm(qkv[:, : H * d], self.q_norm, H, rope.eps)
         k = self._qk_norm(qkv[:, H * d: (H + Hkv) * d], self.k_norm, Hkv, rope.eps)
         vt = qkv[:, (H + Hkv) * d:].reshape(N, Hkv, d).transpose(0, 1)
@@ -282,6 +347,9 @@ class DecoderLayer:
         qr, kr = apply_rope(q.transpose(0, 1).unsqueeze(0), k.transpose(0, 1).unsqueeze(0), rope.inv_freq,
                             pos.reshape(1, N), rope.attn_factor, rope.scaling_type)
         qr = qr.to(torch.bfloat16)
+        if isinstance(pooled, _Kv4Step):
+            o2 = pooled.attend(qr[0], kr[0].transpose(0, 1), qkv[:, (H + Hkv) * d:].reshape(N, Hkv, d), layer, rope.softcap)
+            return self._finish(h, o2, rope, adapter_ids)
         for s in spans:
             s.cache.k[layer, :, s.start: s.start + s.n] = kr[0, :, s.off: s.off + s.n]
             s.cache.v[layer, :, s.start: s.start + s.n] = vt[:, s.off: s.off + s.n]
@@ -295,7 +363,10 @@ class DecoderLayer:
                             rope.softcap) for s in spans]
             o = outs[0] if len(outs) == 1 else torch.cat(outs, dim=2)
             o2 = o[0].transpose(0, 1).reshape(N, H * d)
-        h = h + _project(self.wo, o2).float()
+        return self._finish(h, o2, rope, adapter_ids)
+
+    def _finish(self, h: torch.Tensor, o2: torch.Tensor, rope: "_Rope", adapter_ids) -> torch.Tensor:
+        h = h + self._adapted("o", _project(self.wo, o2), o2, adapter_ids).float()
         x2 = rms_norm(h, self.ln2, rope.eps).to(torch.bfloat16)
         return h + self.ffn.forward(x2, out_dtype=torch.float32)
 
@@ -489,36 +560,82 @@ class MoeDecoder:
             raise NotImplementedError("attention logit soft-capping in MLA layers")
         self.rope = _Rope(ft, attention_factor, scaling_type, eps, softcap)
         self.device = dev
+        self.kv_dtype = "bf16"  # of new_cache / new_pool when they are given none
+        self.num_adapters = self._count_adapters([getattr(lay, "adapters", {}) for lay in self.layers])
 
-    def new_cache(self, max_len: int) -> KvCache:
+    @staticmethod
+    def _count_adapters(per_layer: list) -> int:
+        counts = {b.adapters for banks in per_layer for b in banks.values()}
+        if len(counts) > 1:
+            raise ValueError(f"the layers' adapter banks differ in size: {sorted(counts)}")
+        return counts.pop() if counts else 0
+
+    def set_adapters(self, per_layer: list) -> None:
+        """The low-rank adapters of the layers (as ``DecoderLayer``'s ``adapters``, one dict or None per
+        layer), in place of those they have: for a decoder that ``load_decoder`` made."""
+        if len(per_layer) != len(self.layers):
+            raise ValueError(f"{len(per_layer)} entries for {len(self.layers)} layers")
+        if any(not isinstance(lay, DecoderLayer) for lay in self.layers):
+            raise NotImplementedError("low-rank adapters of MLA layers")
+        checked = [lay._check_adapters(banks) for lay, banks in zip(self.layers, per_layer)]
+        self.num_adapters = self._count_adapters(checked)
+        for lay, banks in zip(self.layers, checked):
+            lay.adapters = banks
+
+    def _kv4(self, kv_dtype: str | None) -> bool:
+        kv_dtype = self.kv_dtype if kv_dtype is None else kv_dtype
+        if kv_dtype not in ("bf16", "int4"):
+            raise ValueError(f"kv_dtype {kv_dtype!r} is not one of bf16, int4")
+        if kv_dtype == "int4" and self.layout[0] != "gqa":
+            raise NotImplementedError("4-bit caches of MLA layers")
+        return kv_dtype == "int4"
+
+    def new_cache(self, max_len: int, kv_dtype: str | None = None):
+        """An empty cache of ``max_len`` positions: ``KvCache``, or ``Kv4Cache`` with ``kv_dtype="int4"``."""
         kind, kvh, width = self.layout
+        if self._kv4(kv_dtype):
+            return Kv4Cache(len(self.layers), kvh, max_len, width, self.device)
         return KvCache(len(self.layers), kvh, max_len, width, self.device, values=kind == "gqa")
 
-    def new_pool(self, slots: int, max_len: int) -> KvPool:
+    def new_pool(self, slots: int, max_len: int, kv_dtype: str | None = None):
+        """A pool of ``slots`` such caches: ``KvPool``, or ``Kv4Pool`` with ``kv_dtype="int4"``."""
         kind, kvh, width = self.layout
+        if self._kv4(kv_dtype):
+            return Kv4Pool(slots, len(self.layers), kvh, max_len, width, self.device)
         return KvPool(slots, len(self.layers), kvh, max_len, width, self.device, values=kind == "gqa")
+
+    def _adapter(self, adapter) -> int:
+        if adapter is None:
+            return -1
+        if isinstance(adapter, bool) or not isinstance(adapter, (int, np.integer)) or not 0 <= adapter < self.num_adapters:
+            raise ValueError(f"adapter {adapter!r} is not one of the model's {self.num_adapters}")
+        return int(adapter)
 
     def _ids(self, tokens) -> torch.Tensor:
         if isinstance(tokens, torch.Tensor):
             return tokens.to(device=self.device, dtype=torch.int64).reshape(-1)
         return torch.as_tensor(np.asarray(tokens, dtype=np.int64).reshape(-1)).to(self.device)
 
-    def forward(self, tokens, cache: KvCache, start_pos: int | None = None, all_logits: bool = False) -> torch.Tensor:
+    def forward(self, tokens, cache: KvCache, start_pos: int | None = None, all_logits: bool = False,
+                adapter: int | None = None) -> torch.Tensor:
         """Run ``tokens`` at positions ``start_pos ..`` (default: after the cached ones) and return
         the fp32 logits of the last token ``[vocab]`` (``all_logits``: of every token
-        ``[seq, vocab]``).  Positions from ``start_pos`` on are replaced in ``cache``."""
-        return self.forward_batch([(tokens, cache, start_pos)], all_logits)[0]
+        ``[seq, vocab]``).  Positions from ``start_pos`` on are replaced in ``cache``.  ``adapter``: the
+        low-rank adapter of the layers' banks to add, or None."""
+        return self.forward_batch([(tokens, cache, start_pos, adapter)], all_logits)[0]
 
     def forward_batch(self, items: list, all_logits: bool = False) -> list:
         """Several sequences in one pass: ``items`` = ``[(tokens, cache, start_pos or None), ...]``
-        with a different cache each.  The projections and the FFN run once over all tokens (the
+        with a different cache each (all of one kind), and optionally the sequence's adapter (or None) as
+        a fourth entry.  The projections and the FFN run once over all tokens (the
         MoE block sees every sequence's tokens together); attention runs per sequence over its
         own cache.  Returns per item the logits of its last token ``[vocab]`` (``all_logits``:
         ``[n, vocab]``)."""
         if not items:
             return []
-        spans, ids_all, off = [], [], 0
-        for tokens, cache, start_pos in items:
+        spans, ids_all, adapters, off = [], [], [], 0
+        for tokens, cache, start_pos, *rest in items:
+            adapters.append(self._adapter(rest[0] if rest else None))
             ids = self._ids(tokens)
             n = ids.numel()
             p = cache.length if start_pos is None else int(start_pos)
@@ -539,13 +656,22 @@ class MoeDecoder:
             raise ValueError(f"token ids must be in [0, {self.vocab})")
         pool = spans[0].cache.pool
         pooled = None
-        if len(spans) > 1 and pool is not None and all(s.n == 1 and s.cache.pool is pool for s in spans):
+        kv4 = isinstance(spans[0].cache, Kv4Cache)
+        if any(isinstance(s.cache, Kv4Cache) != kv4 for s in spans):
+            raise ValueError("the caches of a batch must all be bf16 or all 4-bit")
+        extra = {}
+        if any(a >= 0 for a in adapters):
+            per = np.repeat(np.array(adapters, np.int32), [s.n for s in spans])
+            extra["adapter_ids"] = torch.from_numpy(per).to(self.device)
+        if kv4:
+            pooled = _Kv4Step(spans, self.device)
+        elif len(spans) > 1 and pool is not None and all(s.n == 1 and s.cache.pool is pool for s in spans):
             slots = torch.tensor([s.cache.slot for s in spans], dtype=torch.int32).to(self.device)
             starts = torch.tensor([s.start for s in spans], dtype=torch.int32).to(self.device)
             pooled = (pool, slots, starts)
         h = self.embed.index_select(0, ids).float()
         for i, lay in enumerate(self.layers):
-            h = lay.forward(h, spans, i, self.rope, pooled)
+            h = lay.forward(h, spans, i, self.rope, pooled, **extra)
         for s in spans:
             s.cache.length = s.start + s.n
         if all_logits:
