@@ -15,6 +15,7 @@ import numpy as np
 import torch
 
 from ccut_b200 import _lib
+from ccut_b200.layer import _run
 
 __all__ = ["LoraBank"]
 
@@ -106,20 +107,17 @@ class LoraBank:
         if not base.device == x.device == ids.device == self.device:
             raise ValueError(f"base, x and ids must be on {self.device}")
         if out is None:
-            out = torch.empty((n, self.outputs), dtype=base.dtype, device=self.device)
+            out = torch.empty_like(base, memory_format=torch.contiguous_format)
         elif out.dtype != base.dtype or out.shape != base.shape or out.device != base.device or not _rows_ok(out):
             raise ValueError("out must be like base, its rows contiguous and 16-byte aligned")
         base = base if _rows_ok(base) else base.contiguous()
         x = x if x.is_contiguous() and x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
         ids = ids if ids.is_contiguous() else ids.contiguous()
-        lib = _lib.load()
-        with torch.cuda.device(self.device):
-            nbytes = lib.ccut_lora_workspace_bytes(n, self.inputs, self.rank, len(self.widths), self.adapters)
-            ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=self.device)
-            _lib.call("ccut_lora_add", x.data_ptr(), self.a.data_ptr(), self.b.data_ptr(), self.scales.data_ptr(),
-                      ids.data_ptr(), n, self.inputs, self.rank, self.adapters, len(self.widths), self._widths,
-                      base.data_ptr(), base.stride(0), out.data_ptr(), out.stride(0), _DTYPES[base.dtype],
-                      ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream)
+        nbytes = _lib.load().ccut_lora_workspace_bytes(n, self.inputs, self.rank, len(self.widths), self.adapters)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        _run(self.device, "ccut_lora_add", x.data_ptr(), self.a.data_ptr(), self.b.data_ptr(), self.scales.data_ptr(),
+             ids.data_ptr(), n, self.inputs, self.rank, self.adapters, len(self.widths), self._widths, base.data_ptr(),
+             base.stride(0), out.data_ptr(), out.stride(0), _DTYPES[base.dtype], ws.data_ptr(), nbytes)
         return out
 
 

@@ -21,6 +21,7 @@ from __future__ import annotations
 import torch
 
 from ccut_b200 import _lib
+from ccut_b200.layer import _run
 
 __all__ = ["GROUP", "Kv4Cache", "Kv4Pool", "kv4_append", "kv4_attention", "kv4_read"]
 
@@ -71,6 +72,7 @@ class Kv4Pool:
         self.head_dim = 2 * half
         self.device = self.k.device
         self.slot_rows = self.layers * self.kv_heads * self.max_len
+        self._base = (self.k.data_ptr(), self.k_par.data_ptr(), self.v.data_ptr(), self.v_par.data_ptr())
 
     def _pointers(self, layer: int):
         """Device addresses of layer ``layer`` of slot 0: k codes, k params, v codes, v params."""
@@ -78,7 +80,8 @@ class Kv4Pool:
             raise ValueError(f"layer {layer} outside the pool's {self.layers}")
         rows = layer * self.kv_heads * self.max_len
         c, p = rows * (self.head_dim // 2), rows * (self.head_dim // GROUP) * 4
-        return (self.k.data_ptr() + c, self.k_par.data_ptr() + p, self.v.data_ptr() + c, self.v_par.data_ptr() + p)
+        k, kp, v, vp = self._base
+        return k + c, kp + p, v + c, vp + p
 
     def cache(self, slot: int) -> "Kv4Cache":
         return Kv4Cache.in_pool(self, slot)
@@ -115,10 +118,10 @@ class Kv4Cache:
 def _check_pool(pool, device) -> None:
     if not isinstance(pool, Kv4Pool):
         raise ValueError("pool must be a Kv4Pool")
-    if not pool.k.is_cuda:
-        raise ValueError("the 4-bit cache runs on CUDA tensors only")
     if device != pool.device:
         raise ValueError(f"tensors on {device} for a pool on {pool.device}")
+    if device.type != "cuda":
+        raise ValueError("the 4-bit cache runs on CUDA tensors only")
 
 
 def _index(t: torch.Tensor, n: int, pool: Kv4Pool, name: str) -> torch.Tensor:
@@ -152,11 +155,9 @@ def kv4_append(pool: Kv4Pool, layer: int, k: torch.Tensor, v: torch.Tensor, slot
         raise ValueError("k and v must have the same tokens on the same device")
     slots, positions = _index(slots, n, pool, "slots"), _index(positions, n, pool, "positions")
     kc, kp, vc, vp = pool._pointers(layer)
-    with torch.cuda.device(pool.device):
-        _lib.call("ccut_kv4_append", k.data_ptr(), _DTYPES[k.dtype], k.stride(0), k.stride(1), v.data_ptr(),
-                  _DTYPES[v.dtype], v.stride(0), v.stride(1), n, pool.kv_heads, pool.head_dim, slots.data_ptr(),
-                  positions.data_ptr(), kc, kp, vc, vp, pool.max_len, pool.slot_rows, pool.slots,
-                  torch.cuda.current_stream().cuda_stream)
+    _run(pool.device, "ccut_kv4_append", k.data_ptr(), _DTYPES[k.dtype], k.stride(0), k.stride(1), v.data_ptr(),
+         _DTYPES[v.dtype], v.stride(0), v.stride(1), n, pool.kv_heads, pool.head_dim, slots.data_ptr(),
+         positions.data_ptr(), kc, kp, vc, vp, pool.max_len, pool.slot_rows, pool.slots)
 
 
 def kv4_read(pool: Kv4Pool, layer: int, slots: torch.Tensor, positions: torch.Tensor,
@@ -168,14 +169,10 @@ def kv4_read(pool: Kv4Pool, layer: int, slots: torch.Tensor, positions: torch.Te
     slots, positions = _index(slots, n, pool, "slots"), _index(positions, n, pool, "positions")
     if out_dtype not in _DTYPES:
         raise ValueError("out_dtype must be bf16 or fp32")
-    shape = (n, pool.kv_heads, pool.head_dim)
-    k = torch.empty(shape, dtype=out_dtype, device=pool.device)
-    v = torch.empty(shape, dtype=out_dtype, device=pool.device)
+    k, v = torch.empty((2, n, pool.kv_heads, pool.head_dim), dtype=out_dtype, device=pool.device).unbind()
     kc, kp, vc, vp = pool._pointers(layer)
-    with torch.cuda.device(pool.device):
-        _lib.call("ccut_kv4_read", kc, kp, vc, vp, slots.data_ptr(), positions.data_ptr(), n, pool.kv_heads,
-                  pool.head_dim, pool.max_len, pool.slot_rows, pool.slots, k.data_ptr(), v.data_ptr(),
-                  _DTYPES[out_dtype], torch.cuda.current_stream().cuda_stream)
+    _run(pool.device, "ccut_kv4_read", kc, kp, vc, vp, slots.data_ptr(), positions.data_ptr(), n, pool.kv_heads,
+         pool.head_dim, pool.max_len, pool.slot_rows, pool.slots, k.data_ptr(), v.data_ptr(), _DTYPES[out_dtype])
     return k, v
 
 
@@ -201,14 +198,11 @@ def kv4_attention(q: torch.Tensor, pool: Kv4Pool, layer: int, slots: torch.Tenso
     q = q if q.is_contiguous() else q.contiguous()
     if q.data_ptr() % 16:
         q = q.clone()
-    out = torch.empty((b, h, s, d), dtype=out_dtype, device=q.device)
-    lib = _lib.load()
+    out = torch.empty_like(q) if out_dtype == torch.bfloat16 else torch.empty_like(q, dtype=out_dtype)
     kc, kp, vc, vp = pool._pointers(layer)
-    with torch.cuda.device(pool.device):
-        nbytes = lib.ccut_kv4_attention_workspace_bytes(b, h, pool.kv_heads, s, n, d)
-        ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=q.device)
-        _lib.call("ccut_kv4_attention", q.data_ptr(), kc, kp, vc, vp, slots.data_ptr(), starts.data_ptr(), b, h,
-                  pool.kv_heads, s, d, pool.max_len, n, pool.slot_rows, pool.slots, float(scale or 0.0),
-                  float(softcap or 0.0), out.data_ptr(), _DTYPES[out_dtype], ws.data_ptr(), ws.numel(),
-                  torch.cuda.current_stream().cuda_stream)
+    nbytes = _lib.load().ccut_kv4_attention_workspace_bytes(b, h, pool.kv_heads, s, n, d)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 256 else None  # 256: none is used
+    _run(pool.device, "ccut_kv4_attention", q.data_ptr(), kc, kp, vc, vp, slots.data_ptr(), starts.data_ptr(), b, h,
+         pool.kv_heads, s, d, pool.max_len, n, pool.slot_rows, pool.slots, float(scale or 0.0), float(softcap or 0.0),
+         out.data_ptr(), _DTYPES[out_dtype], ws.data_ptr() if ws is not None else None, nbytes)
     return out

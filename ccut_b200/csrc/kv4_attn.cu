@@ -55,6 +55,7 @@ struct Kv4AttnArgs {
   void* out;
   int batch, row_tiles;  // row_tiles: tiles of 8 or 16 query rows per kv head
   int ctas;              // grid of the attention kernel
+  int block;             // positions per block of work, a multiple of kKv4Block
   float2* ml;            // [ctas][2][rows of a tile] running maximum (log2 units) and sum of a partial unit
   float* acc;            // [ctas][2][rows of a tile][d] its unnormalised output
 };
@@ -148,25 +149,20 @@ CCUT_DEVICE int kv4_seen(const Kv4AttnArgs& a, int b) {  // positions its last q
   const int slot = a.slots[b], start = a.starts[b];
   return slot >= 0 && slot < a.num_slots && start >= 0 ? min(a.kv_len, min(start, a.kv_len) + a.seq) : 0;
 }
-template <int NT>
-CCUT_DEVICE int kv4_blocks(int seen) {
-  return max(1, (seen + kKv4Block<NT> - 1) / kKv4Block<NT>);
-}
+CCUT_DEVICE int kv4_blocks(const Kv4AttnArgs& a, int seen) { return max(1, (seen + a.block - 1) / a.block); }
 // Whole warp.  Length of the line.  `mine`: blocks of sequence `lane`, for kv4_find.
-template <int NT>
 CCUT_DEVICE int kv4_total(const Kv4AttnArgs& a, int lane, int& mine) {
-  mine = lane < a.batch ? kv4_blocks<NT>(kv4_seen(a, lane)) : 0;
+  mine = lane < a.batch ? kv4_blocks(a, kv4_seen(a, lane)) : 0;
   unsigned n = mine;  // no overflow: the line is bounded at launch
-  for (int b = lane + 32; b < a.batch; b += 32) n += kv4_blocks<NT>(kv4_seen(a, b));
+  for (int b = lane + 32; b < a.batch; b += 32) n += kv4_blocks(a, kv4_seen(a, b));
   return (int)__reduce_add_sync(0xffffffffu, n) * a.kv_heads * a.row_tiles;
 }
 // Whole warp.  The sequence at place `at` of the line, and the place of its first block.
-template <int NT>
 CCUT_DEVICE int kv4_find(const Kv4AttnArgs& a, int lane, int mine, int at, int& first) {
   const int units = a.kv_heads * a.row_tiles;
   int base = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 32) {
-    const int n = b0 == 0 ? mine : b0 + lane < a.batch ? kv4_blocks<NT>(kv4_seen(a, b0 + lane)) : 0;
+    const int n = b0 == 0 ? mine : b0 + lane < a.batch ? kv4_blocks(a, kv4_seen(a, b0 + lane)) : 0;
     int sum = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -210,14 +206,14 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int grp = a.heads / a.kv_heads, nrows = grp * a.seq;
   int mine, first;
-  const int total = kv4_total<NT>(a, lane, mine), spans = min(a.ctas, total);
+  const int total = kv4_total(a, lane, mine), spans = min(a.ctas, total);
   if ((int)blockIdx.x >= spans) return;
   const int begin = kv4_span(total, spans, blockIdx.x), end = kv4_span(total, spans, blockIdx.x + 1);
-  int b = kv4_find<NT>(a, lane, mine, begin, first);
+  int b = kv4_find(a, lane, mine, begin, first);
   int at = begin;
 
   while (at < end) {
-  const int seen = kv4_seen(a, b), nblocks = kv4_blocks<NT>(seen);
+  const int seen = kv4_seen(a, b), nblocks = kv4_blocks(a, seen);
   const int unit = (at - first) / nblocks, block0 = (at - first) % nblocks;
   const int block1 = min(nblocks, block0 + (end - at));
   const bool whole_unit = block0 == 0 && block1 == nblocks;
@@ -225,9 +221,9 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
   const int kvh = unit % a.kv_heads, r0 = unit / a.kv_heads * kRows;
   const int start = min(a.starts[b], a.kv_len);
   const int last_row = min(nrows, r0 + kRows) - 1;
-  const int k0 = block0 * kBlock;
+  const int k0 = block0 * a.block;
   // positions any row of this tile sees in this segment
-  const int k1 = seen > 0 ? min(min(seen, block1 * kBlock), start + last_row / grp + 1) : 0;
+  const int k1 = seen > 0 ? min(min(seen, block1 * a.block), start + last_row / grp + 1) : 0;
   const size_t row_base = seen > 0 ? (size_t)a.slots[b] * (size_t)a.slot_rows + (size_t)kvh * a.max_len : 0;
 
   // ---- the query rows as B fragments (row n = g of n-tile nt; features t * 16 .. of each group) ----
@@ -622,13 +618,13 @@ __global__ void __launch_bounds__(W > 8 ? W * 32 : 256) kv4_merge_kernel(Kv4Attn
   const int grp = a.heads / a.kv_heads, r = i * grp + h % grp;
   unsigned all = 0, before = 0;
   for (int j = lane; j < a.batch; j += 32) {
-    const int n = kv4_blocks<NT>(kv4_seen(a, j));
+    const int n = kv4_blocks(a, kv4_seen(a, j));
     all += n;
     before += j < b ? n : 0;
   }
   const int units = a.kv_heads * a.row_tiles;
   const int total = (int)__reduce_add_sync(0xffffffffu, all) * units;
-  const int nblocks = kv4_blocks<NT>(kv4_seen(a, b));
+  const int nblocks = kv4_blocks(a, kv4_seen(a, b));
   const int first = (int)__reduce_add_sync(0xffffffffu, before) * units + (r / kRows * a.kv_heads + h / grp) * nblocks;
   const int spans = min(a.ctas, total);
   const int c0 = kv4_span_of(total, spans, first), c1 = kv4_span_of(total, spans, first + nblocks - 1);
@@ -687,7 +683,13 @@ __global__ void __launch_bounds__(W > 8 ? W * 32 : 256) kv4_merge_kernel(Kv4Attn
 
 // Query rows per tile: 8 where a kv head has no more, else 16.
 static int kv4_rows(int heads, int kv_heads, int seq) { return (long)(heads / kv_heads) * seq <= 8 ? 8 : 16; }
-static int kv4_block(int rows) { return rows == 8 ? kKv4Block<1> : kKv4Block<2>; }
+// Positions per block of work: a step of every warp, or all positions where they are few, so that no unit is
+// cut and nothing is left to join (one sequence of 513: 6.5 us uncut, 6.9 cut; of 769: 8.1 and 7.6).
+constexpr int kKv4Uncut = 640;
+static int kv4_block(int rows, int kv_len) {
+  const int step = rows == 8 ? kKv4Block<1> : kKv4Block<2>;
+  return kv_len <= kKv4Uncut ? (kv_len > 0 ? (kv_len + step - 1) / step * step : step) : step;
+}
 static long long kv4_row_tiles(int heads, int kv_heads, int seq) {
   const long long rows = (long long)(heads / kv_heads) * seq, per = kv4_rows(heads, kv_heads, seq);
   return (rows + per - 1) / per;
@@ -699,7 +701,7 @@ static int kv4_ctas(int batch, int heads, int kv_heads, int seq, int kv_len, int
   const bool one = kv4_rows(heads, kv_heads, seq) == 8;
   const int most = 148 * (head_dim == 64 ? (one ? kKv4Resident<64, 1> : kKv4Resident<64, 2>)
                                          : (one ? kKv4Resident<128, 1> : kKv4Resident<128, 2>));
-  const int block = kv4_block(one ? 8 : 16);
+  const int block = kv4_block(one ? 8 : 16, kv_len);
   const long long blocks = kv_len > 0 ? (kv_len + block - 1) / block : 1;
   const long long n = kv4_row_tiles(heads, kv_heads, seq) * kv_heads * batch;
   const long long ctas = n * (blocks < kKv4Parts ? blocks : kKv4Parts);
@@ -712,7 +714,7 @@ static int run_kv4_attention(const Kv4AttnArgs& a, cudaStream_t st) {
   int rc = ensure_smem_limit(kv4_attn_kernel<D, NT, OB>, kKv4Smem<D, NT>, smem_set);
   if (rc) return rc;
   rc = launch_k(kv4_attn_kernel<D, NT, OB>, dim3(a.ctas), dim3(kKv4Warps * 32), kKv4Smem<D, NT>, st, a);
-  if (rc || a.kv_len <= kKv4Block<NT>) return rc;  // one block a unit: no unit is cut
+  if (rc || a.kv_len <= a.block) return rc;  // one block a unit: no unit is cut
   // a warp per row where few spans share a unit, else a CTA
   const long long rows = (long long)a.batch * a.heads * a.seq, units = (long long)a.batch * a.kv_heads * a.row_tiles;
   if (a.ctas <= 8 * units)
@@ -730,7 +732,7 @@ size_t ccut_kv4_attention_workspace_bytes(int batch, int heads, int kv_heads, in
   if (batch < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || seq < 0 || kv_len < 0 ||
       (head_dim != 64 && head_dim != 128))
     return 0;
-  if (batch == 0 || seq == 0 || kv_len <= kv4_block(kv4_rows(heads, kv_heads, seq))) return 256;
+  if (batch == 0 || seq == 0 || kv_len <= kv4_block(kv4_rows(heads, kv_heads, seq), kv_len)) return 256;
   return 256 + (size_t)kv4_ctas(batch, heads, kv_heads, seq, kv_len, head_dim) * 2 * kv4_rows(heads, kv_heads, seq) *
                    (head_dim + 2) * sizeof(float);
 }
@@ -761,7 +763,8 @@ int ccut_kv4_attention(const uint16_t* q, const uint8_t* k_codes, const uint16_t
   Kv4AttnArgs a{q, k_codes, reinterpret_cast<const __half2*>(k_params), v_codes,
                 reinterpret_cast<const __half2*>(v_params), slots, starts, heads, kv_heads, seq, max_len, kv_len,
                 num_slots, slot_rows, scale, softcap, out, batch, (int)kv4_row_tiles(heads, kv_heads, seq),
-                kv4_ctas(batch, heads, kv_heads, seq, kv_len, head_dim), nullptr, nullptr};
+                kv4_ctas(batch, heads, kv_heads, seq, kv_len, head_dim),
+                kv4_block(kv4_rows(heads, kv_heads, seq), kv_len), nullptr, nullptr};
   const int rows = kv4_rows(heads, kv_heads, seq);
   if (need > 256) {
     a.ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + 256);

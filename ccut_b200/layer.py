@@ -53,6 +53,18 @@ def _stream() -> C.c_void_p:
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def _run(device: torch.device, name: str, *args) -> None:
+    """``_lib.call(name, *args, stream)`` with ``device`` current and its current stream: the raw stream handle
+    and no device switch where ``device`` is current already (a switch and a ``Stream`` object cost several
+    microseconds of a decode step's calls)."""
+    i = device.index
+    if i is None or torch._C._cuda_getDevice() != i:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+    else:
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(i))
+
+
 def _ptr(t: torch.Tensor | None) -> C.c_void_p:
     return C.c_void_p(t.data_ptr() if t is not None else 0)
 
