@@ -29,4 +29,23 @@ inline bool kv4_shape_ok(int kv_heads, int head_dim, int max_len, long long slot
 }
 inline bool misaligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a != 0; }
 
+// A cache as the attention kernels read it.
+struct Kv4Cache {
+  const uint8_t* kc;
+  const __half2* kp;
+  const uint8_t* vc;
+  const __half2* vp;
+  int max_len;
+  long long slot_rows;
+};
+
+// kv4_prefill.cu: query blocks of at least this many rows per kv head.  Unpacking the cache costs what about 70 rows
+// take on the short-block kernel.
+constexpr int kKv4LongRows = 97;
+bool kv4_prefill_fits(int batch, int heads, int kv_heads, int seq, int kv_len);
+size_t kv4_prefill_workspace(int batch, int heads, int kv_heads, int seq, int kv_len, int head_dim);
+int launch_kv4_prefill(const Kv4Cache& c, const uint16_t* q, const int32_t* slots, const int32_t* starts, int batch,
+                       int heads, int kv_heads, int seq, int head_dim, int kv_len, int num_slots, float scale,
+                       float softcap, void* out, bool out_bf16, void* workspace, cudaStream_t st);
+
 }  // namespace ccut

@@ -1,4 +1,5 @@
-// kv4_attn.cu -- grouped-query attention over the 4-bit kv cache (format: kv4.cuh).
+// kv4_attn.cu -- grouped-query attention over the 4-bit kv cache (format: kv4.cuh); long query blocks:
+// kv4_prefill.cu.
 //
 // q bf16 [batch, heads, seq, d]; batch row b reads slot slots[b], its query i sees positions
 // <= starts[b] + i (and < kv_len); query head h reads kv head h / (heads / kv_heads).
@@ -732,6 +733,8 @@ size_t ccut_kv4_attention_workspace_bytes(int batch, int heads, int kv_heads, in
   if (batch < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || seq < 0 || kv_len < 0 ||
       (head_dim != 64 && head_dim != 128))
     return 0;
+  if (batch > 0 && seq > 0 && kv4_prefill_fits(batch, heads, kv_heads, seq, kv_len))
+    return kv4_prefill_workspace(batch, heads, kv_heads, seq, kv_len, head_dim);
   if (batch == 0 || seq == 0 || kv_len <= kv4_block(kv4_rows(heads, kv_heads, seq), kv_len)) return 256;
   return 256 + (size_t)kv4_ctas(batch, heads, kv_heads, seq, kv_len, head_dim) * 2 * kv4_rows(heads, kv_heads, seq) *
                    (head_dim + 2) * sizeof(float);
@@ -760,6 +763,12 @@ int ccut_kv4_attention(const uint16_t* q, const uint8_t* k_codes, const uint16_t
   const size_t need = ccut_kv4_attention_workspace_bytes(batch, heads, kv_heads, seq, kv_len, head_dim);
   if (need > 256 && (!workspace || ws_bytes < need)) return CCUT_ERR_WORKSPACE;
   if (!(scale > 0.f)) scale = 1.f / sqrtf((float)head_dim);
+  if (kv4_prefill_fits(batch, heads, kv_heads, seq, kv_len)) {
+    const Kv4Cache c{k_codes, reinterpret_cast<const __half2*>(k_params), v_codes,
+                     reinterpret_cast<const __half2*>(v_params), max_len, slot_rows};
+    return launch_kv4_prefill(c, q, slots, starts, batch, heads, kv_heads, seq, head_dim, kv_len, num_slots, scale,
+                              softcap, out, out_dtype == CCUT_OUT_BF16, workspace, stream);
+  }
   Kv4AttnArgs a{q, k_codes, reinterpret_cast<const __half2*>(k_params), v_codes,
                 reinterpret_cast<const __half2*>(v_params), slots, starts, heads, kv_heads, seq, max_len, kv_len,
                 num_slots, slot_rows, scale, softcap, out, batch, (int)kv4_row_tiles(heads, kv_heads, seq),

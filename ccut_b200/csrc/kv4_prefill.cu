@@ -1,0 +1,496 @@
+// kv4_prefill.cu -- attention of long query blocks (prompt chunks) over the 4-bit kv cache, on tcgen05.
+//
+// The same function as kv4_attn.cu.  Bound: tensor cores and the exponentials (4 x rows x positions x d flop
+// against rows x positions exponentials: at d = 128 a tile's products and its exponentials take the same time).
+//
+// kv4_unpack_kernel turns the cache's rows that any query sees into fp16 once per call (value q s + m, one
+// rounding to 11 bits), 2 x d x 2 bytes per position: about 3% of the products' time at 4096 rows, where
+// unpacking in every CTA would repeat it per 256 rows.  A position that holds a NaN gets a NaN key and a zero
+// value: the key makes every row that sees it NaN, and a masked row multiplies a zero.
+// kv4_prefill_kernel: a CTA takes 256 query rows of one kv head (row r = query r / group, head r % group), two
+// tiles of 128, and streams tiles of 128 positions:
+// - warp 0 loads k and v tiles by TMA into a ring; warp 1 issues the MMAs (M = 128, fp32 in tensor memory):
+//   S_i = Q_i K^T, then O_i += P_i V with P_i read from tensor memory, where it takes the place of S_i.
+// - two warpgroups of softmax threads, one row a thread: S to registers, running maximum, exponentials, P
+//   back as fp16.  While one tile's scores are worked on, the tensor cores run the other's products.
+// - The maximum moves only when a score passes it by 2^8, so O is rescaled a few times per row and not every
+//   tile (probabilities up to 2^8 fit fp16); when it moves, the O of the earlier tiles is complete, since
+//   S_i of a tile is issued behind P_i V of the one before.
+// Roundings: q to fp16 after scaling its row's largest element to [1/2, 1) (11 bits of it, 2^-25 of the
+// largest), k and v above, P 11 bits; scores, maximum, sums and O are fp32.
+#include <math.h>
+
+#include "kv4.cuh"
+#include "tc.cuh"
+
+namespace ccut {
+
+constexpr int kPfRows = 128;       // query rows per tile; two tiles per CTA
+constexpr int kPfTile = 128;       // positions per tile
+constexpr int kPfThreads = 384;    // warps: producer, issuer, two idle, then two warpgroups of softmax
+constexpr float kPfLog2e = 1.4426950408889634f;
+
+struct PrefillArgs {
+  const uint16_t* q;
+  const int32_t* slots;
+  const int32_t* starts;
+  int heads, kv_heads, seq, kv_len, num_slots, padded;  // padded: rows per (batch row, kv head) of the unpacked cache
+  float scale, softcap;
+  void* out;
+  int* status;
+  float* part;  // [splits][rows][d + 2]: maximum, sum, output of a split
+  int splits;
+  long long rows;
+};
+
+template <int D>
+struct PfSmem {
+  static constexpr int kTileBytes = kPfTile * D * 2;  // q, k or v
+  static constexpr int kStages = D == 128 ? 4 : 6;
+  static constexpr int kBytes = 1024 + (2 + kStages) * kTileBytes;
+};
+
+struct PfBars {
+  uint64_t q_full[2], kv_full[6], kv_empty[6], s_full[2], p_full[2], o_full[2];
+  uint32_t tmem;
+  int failed;
+};
+
+CCUT_DEVICE void pf_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// B operand stored [k][n], 64 n to a row of 128 bytes: 8-row groups of k 1024 bytes apart (stride offset), the next
+// 64 n one sub-tile of 128 rows further (leading offset).
+CCUT_DEVICE uint64_t pf_desc_mn(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFF);
+  d |= (uint64_t)(kPfTile * 128 >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+CCUT_DEVICE float pf_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Unpacked rows: [batch][kv_heads][padded][d] fp16 of k and of v; zeros past what the batch row sees.
+template <int D>
+__global__ void __launch_bounds__(256) kv4_unpack_kernel(const uint8_t* __restrict__ kc, const __half2* __restrict__ kp,
+                                                         const uint8_t* __restrict__ vc, const __half2* __restrict__ vp,
+                                                         const int32_t* __restrict__ slots,
+                                                         const int32_t* __restrict__ starts, int kv_heads, int seq,
+                                                         int kv_len, int max_len, long long slot_rows, int num_slots,
+                                                         int padded, uint4* __restrict__ k16, uint4* __restrict__ v16,
+                                                         int* status) {
+  pdl_wait();
+  pdl_trigger();
+  constexpr int W = D / 8, G = D / kKv4Group;
+  const int b = blockIdx.z, h = blockIdx.y;
+  if (blockIdx.x == 0 && b == 0 && h == 0 && threadIdx.x == 0) *status = 0;
+  const int slot = slots[b], start = starts[b];
+  const int seen = slot >= 0 && slot < num_slots && start >= 0 ? min(kv_len, min(start, kv_len) + seq) : 0;
+  const int idx = blockIdx.x * 256 + threadIdx.x, pos = idx / W, w = idx % W;
+  if (pos >= padded || pos >= (seen + kPfTile - 1) / kPfTile * kPfTile) return;  // tiles past the last are not read
+  uint32_t k[4] = {0, 0, 0, 0}, v[4] = {0, 0, 0, 0};
+  if (pos < seen) {
+    const size_t row = (size_t)slot * (size_t)slot_rows + (size_t)h * max_len + pos;
+    bool bad = false;
+    float2 pk{}, pv{};
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const float2 a = __half22float2(kp[row * G + g]), c = __half22float2(vp[row * G + g]);
+      bad |= !(fabsf(a.x) + fabsf(a.y) + fabsf(c.x) + fabsf(c.y) < INFINITY);
+      if (g == w / 8) pk = a, pv = c;
+    }
+    const uint32_t wk = reinterpret_cast<const uint32_t*>(kc)[row * W + w], wv = reinterpret_cast<const uint32_t*>(vc)[row * W + w];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 hk = __floats2half2_rn(kv4_value((wk >> (8 * i)) & 15, pk.x, pk.y), kv4_value((wk >> (8 * i + 4)) & 15, pk.x, pk.y));
+      const __half2 hv = __floats2half2_rn(kv4_value((wv >> (8 * i)) & 15, pv.x, pv.y), kv4_value((wv >> (8 * i + 4)) & 15, pv.x, pv.y));
+      k[i] = bad ? 0x7FFF7FFFu : *reinterpret_cast<const uint32_t*>(&hk);
+      v[i] = bad ? 0u : *reinterpret_cast<const uint32_t*>(&hv);
+    }
+  }
+  const size_t at = (((size_t)b * kv_heads + h) * padded + pos) * W + w;
+  k16[at] = make_uint4(k[0], k[1], k[2], k[3]);
+  v16[at] = make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+template <int D, bool OUT_BF16>
+__global__ void __launch_bounds__(kPfThreads, 1)
+    kv4_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                       const __grid_constant__ PrefillArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  using SM = PfSmem<D>;
+  constexpr int kChunks = D / 64;  // sub-tiles of 64 features, 128 rows of 128 bytes each
+  constexpr int kSub = kPfTile * 128;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+  __shared__ PfBars bars;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int grp = a.heads / a.kv_heads, nrows = grp * a.seq;
+  const int b = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads;
+  const int r0 = (gridDim.x - 1 - blockIdx.x) * 2 * kPfRows;  // the longest first
+  const int slot = a.slots[b], start0 = a.starts[b];
+  const bool valid = slot >= 0 && slot < a.num_slots && start0 >= 0;
+  const int start = min(start0, a.kv_len);
+  const int last_row = min(nrows, r0 + 2 * kPfRows) - 1;
+  const int seen = valid ? min(a.kv_len, start + last_row / grp + 1) : 0;  // by any row of this CTA
+  const int all = (seen + kPfTile - 1) / kPfTile;
+  const int tile0 = (int)((long long)all * blockIdx.z / a.splits), tile1 = (int)((long long)all * (blockIdx.z + 1) / a.splits);
+  const int n = tile1 - tile0;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.q_full[i], kPfRows);
+      mbar_init(&bars.s_full[i], 1);
+      mbar_init(&bars.p_full[i], kPfRows);
+      mbar_init(&bars.o_full[i], 1);
+    }
+    for (int i = 0; i < SM::kStages; ++i) {
+      mbar_init(&bars.kv_full[i], 1);
+      mbar_init(&bars.kv_empty[i], 1);
+    }
+    bars.failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(&bars.tmem, 512);
+    tc::tmem_relinquish();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = bars.tmem;
+  volatile int* failed = &bars.failed;
+  // columns: S_0 (P_0 in its first half), S_1, O_0, O_1
+  auto s_col = [&](int i) { return tmem + i * kPfTile; };
+  auto o_col = [&](int i) { return tmem + 2 * kPfTile + i * D; };
+  uint8_t* q_s = smem;
+  uint8_t* ring = smem + 2 * SM::kTileBytes;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    const bool ok = mbar_wait(bar, parity, a.status);
+    if (!ok) *failed = 1;
+    return ok && !*failed;
+  };
+
+  // 256 x 208 + 128 x 80 registers of the 384 x 168 of the launch; one instruction per warpgroup
+  if (warp < 4) {
+  tc::setmaxnreg_dec<80>();
+  if (warp == 0) {
+    if (lane == 0 && n > 0) {
+      asm volatile("fence.proxy.async;" ::: "memory");  // the unpacked cache was written through the generic proxy
+      tc::prefetch_tmap(&kmap);
+      tc::prefetch_tmap(&vmap);
+      const int row = (int)(((long long)b * a.kv_heads + kvh) * a.padded) + tile0 * kPfTile;
+      for (int t = 0; t < 2 * n; ++t) {  // k and v tiles in turn
+        const int st = t % SM::kStages, use = t / SM::kStages;
+        if (use > 0 && !wait(&bars.kv_empty[st], (use - 1) & 1)) break;
+        mbar_arrive_expect_tx(&bars.kv_full[st], SM::kTileBytes);
+        for (int c = 0; c < kChunks; ++c)
+          tc::tma_load_2d(ring + st * SM::kTileBytes + c * kSub, t & 1 ? &vmap : &kmap, c * 64, row + t / 2 * kPfTile,
+                          &bars.kv_full[st]);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && n > 0) {
+      const uint32_t idesc_s = tc::idesc_f16_m128(kPfTile);
+      const uint32_t idesc_o = tc::idesc_f16_m128(D) | (1u << 16);  // B is [k][n]
+      auto scores = [&](int i, int t) {  // S_i = Q_i K^T, K the ring's tile t
+        const uint32_t q0 = smem_u32(q_s) + i * SM::kTileBytes, k0 = smem_u32(ring) + t % SM::kStages * SM::kTileBytes;
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t off = (ks >> 2) * kSub + (ks & 3) * 32;
+          pf_mma_ss(s_col(i), tc::sdesc_sw128(q0 + off), tc::sdesc_sw128(k0 + off), idesc_s, ks > 0);
+        }
+        tc::commit(&bars.s_full[i]);
+      };
+      bool ok = wait(&bars.q_full[0], 0) && wait(&bars.kv_full[0], 0);
+      tc::fence_after_sync();
+      if (ok) scores(0, 0);
+      ok = ok && wait(&bars.q_full[1], 0);
+      tc::fence_after_sync();
+      if (ok) {
+        scores(1, 0);
+        tc::commit(&bars.kv_empty[0]);
+      }
+      for (int j = 0; ok && j < n; ++j) {
+        const int tv = 2 * j + 1, tk = 2 * j + 2;
+        for (int i = 0; i < 2; ++i) {
+          if (i == 0 && !(ok = wait(&bars.kv_full[tv % SM::kStages], tv / SM::kStages & 1))) break;
+          if (!(ok = wait(&bars.p_full[i], j & 1))) break;
+          tc::fence_after_sync();
+          const uint32_t v0 = smem_u32(ring) + tv % SM::kStages * SM::kTileBytes;
+          for (int ks = 0; ks < kPfTile / 16; ++ks)
+            tc::mma_ts(o_col(i), s_col(i) + ks * 8, pf_desc_mn(v0 + ks * 2048), idesc_o, j > 0 || ks > 0);
+          if (i == 1) tc::commit(&bars.kv_empty[tv % SM::kStages]);
+          if (j + 1 < n) {
+            if (i == 0 && !(ok = wait(&bars.kv_full[tk % SM::kStages], tk / SM::kStages & 1))) break;
+            tc::fence_after_sync();
+            scores(i, tk);
+            if (i == 1) tc::commit(&bars.kv_empty[tk % SM::kStages]);
+          } else {
+            tc::commit(&bars.o_full[i]);
+          }
+        }
+      }
+    }
+  }
+  } else {
+    tc::setmaxnreg_inc<208>();
+    const int i = (warp - 4) >> 2, tr = (warp & 3) * 32 + lane, r = r0 + i * kPfRows + tr;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_addr = s_col(i) + lanes, o_addr = o_col(i) + lanes;
+    const bool live = r < nrows;
+    const int s = r / grp;
+    const long long row = ((long long)b * a.heads + kvh * grp + r % grp) * a.seq + s;
+    const int lim = live ? start + s : a.kv_len;  // last visible position
+    // the row of q as fp16, scaled by a power of two, into the swizzled tile
+    float fr = 0.f;
+    if (n > 0) {
+      uint4 u[D / 8];
+      float mx = 0.f;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        u[c] = live ? *reinterpret_cast<const uint4*>(a.q + row * D + c * 8) : make_uint4(0, 0, 0, 0);
+        const uint32_t w[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(w[e] << 16)), fabsf(__uint_as_float(w[e] & 0xFFFF0000u))));
+      }
+      const int ex = min(max((int)((__float_as_uint(mx) >> 23) & 255) - 126, -90), 90);  // |q| 2^-ex in [1/2, 1)
+      const float f = __int_as_float((127 - ex) << 23);
+      fr = __int_as_float((127 + ex) << 23) * (a.scale * kPfLog2e);
+      uint8_t* dst = q_s + i * SM::kTileBytes + tr * 128;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        const uint32_t w[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
+        uint32_t o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const __half2 h = __floats2half2_rn(__uint_as_float(w[e] << 16) * f, __uint_as_float(w[e] & 0xFFFF0000u) * f);
+          o[e] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        *reinterpret_cast<uint4*>(dst + (c >> 3) * kSub + (((c & 7) ^ (tr & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+      tc::fence_proxy_async_smem();
+      mbar_arrive(&bars.q_full[i]);
+    }
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; ok && j < n; ++j) {
+      ok = wait(&bars.s_full[i], j & 1);
+      ok = !__any_sync(0xffffffffu, !ok);
+      if (!ok) break;
+      tc::fence_after_sync();
+      uint32_t x[4][32];
+      __syncwarp();
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tc::ld_32x32b_x32(s_addr + c * 32, x[c]);
+      tc::wait_ld();
+      const int p0 = (tile0 + j) * kPfTile;
+      float f = fr;
+      if (a.softcap > 0.f) {
+        f = 1.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            x[c][e] = __float_as_uint(tanhf(__uint_as_float(x[c][e]) * (fr / kPfLog2e) / a.softcap) * (a.softcap * kPfLog2e));
+      }
+      if (__any_sync(0xffffffffu, p0 + kPfTile - 1 > min(lim, seen - 1))) {
+        const int vis = min(lim, seen - 1) - p0;  // columns up to this one
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (c * 32 + e > vis) x[c][e] = 0xFF800000u;
+      }
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) top[c] = fmaxf(top[c], __uint_as_float(x[c][e]));
+      const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f;
+      if (__any_sync(0xffffffffu, mt > m + 8.f)) {
+        const float mn = fmaxf(m, mt), al = mn == -INFINITY ? 1.f : pf_ex2(m - mn);
+        m = mn;
+        l *= al;
+        __syncwarp();
+        if (j > 0) {  // O of the tiles before is complete: S_i was issued behind its last product
+#pragma unroll
+          for (int c = 0; c < D; c += 32) {
+            uint32_t y[32];
+            tc::ld_32x32b_x32(o_addr + c, y);
+            tc::wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * al);
+            tc::st_32x32b_x32(o_addr + c, y);
+          }
+        }
+      }
+      const float mu = m == -INFINITY ? 0.f : m;
+      __syncwarp();
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 4; c += 2) {
+        uint32_t p[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const uint32_t* xe = &x[c + (e >> 4)][(e & 15) * 2];
+          const float y0 = pf_ex2(fmaf(__uint_as_float(xe[0]), f, -mu)), y1 = pf_ex2(fmaf(__uint_as_float(xe[1]), f, -mu));
+          sum[0] += y0, sum[1] += y1;
+          const __half2 h = __floats2half2_rn(y0, y1);
+          p[e] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        tc::st_32x32b_x32(s_addr + c * 16, p);
+      }
+      l += sum[0] + sum[1];
+      tc::wait_st();
+      tc::fence_before_sync();
+      mbar_arrive(&bars.p_full[i]);
+    }
+    if (n > 0 && ok) ok = wait(&bars.o_full[i], 0);
+    ok = !__any_sync(0xffffffffu, !ok);
+    tc::fence_after_sync();
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int c = 0; c < D; c += 32) {
+      uint32_t y[32];
+      __syncwarp();
+      if (n > 0 && ok) {
+        tc::ld_32x32b_x32(o_addr + c, y);
+        tc::wait_ld();
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) y[e] = 0;
+      }
+      if (!live) {
+        // a row past the last is not written
+      } else if (a.splits > 1) {
+        float* p = a.part + ((size_t)blockIdx.z * a.rows + row) * (D + 4);
+        if (c == 0) p[0] = m, p[1] = l;
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(p + 4 + c + e) = make_uint4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+      } else if constexpr (OUT_BF16) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+          uint32_t o[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(y[e + 2 * q]) * inv, __uint_as_float(y[e + 2 * q + 1]) * inv);
+            o[q] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row * D + c + e) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; e += 4)
+          *reinterpret_cast<float4*>(static_cast<float*>(a.out) + row * D + c + e) =
+              make_float4(__uint_as_float(y[e]) * inv, __uint_as_float(y[e + 1]) * inv, __uint_as_float(y[e + 2]) * inv,
+                          __uint_as_float(y[e + 3]) * inv);
+      }
+    }
+    tc::fence_before_sync();
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the splits of a row, one warp each, in split order.
+template <int D, bool OUT_BF16>
+__global__ void __launch_bounds__(256) kv4_prefill_merge_kernel(PrefillArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  constexpr int E = D / 32;
+  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= a.rows) return;
+  float M = -INFINITY, L = 0.f, v[E] = {};
+  for (int s = 0; s < a.splits; ++s) {
+    const float* p = a.part + ((size_t)s * a.rows + row) * (D + 4);
+    const float m = p[0], top = fmaxf(M, m), base = top == -INFINITY ? 0.f : top;
+    const float f = pf_ex2(M - base), g = pf_ex2(m - base);
+    M = top;
+    L = fmaf(L, f, p[1] * g);
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = fmaf(v[e], f, p[4 + lane + 32 * e] * g);
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if constexpr (OUT_BF16) static_cast<__nv_bfloat16*>(a.out)[row * D + lane + 32 * e] = __float2bfloat16_rn(v[e] * inv);
+    else static_cast<float*>(a.out)[row * D + lane + 32 * e] = v[e] * inv;
+  }
+}
+
+static long long pf_padded(int kv_len) { return ((long long)kv_len + kPfTile - 1) / kPfTile * kPfTile; }
+static long long pf_row_tiles(int heads, int kv_heads, int seq) {
+  return ((long long)(heads / kv_heads) * seq + 2 * kPfRows - 1) / (2 * kPfRows);
+}
+// Splits of the positions: one CTA an SM, at least four tiles each.
+static int pf_splits(int batch, int heads, int kv_heads, int seq, int kv_len) {
+  const long long units = pf_row_tiles(heads, kv_heads, seq) * kv_heads * batch, tiles = pf_padded(kv_len) / kPfTile;
+  long long sp = units > 0 ? 148 / units : 1;
+  if (sp > tiles / 4) sp = tiles / 4;
+  return sp < 1 ? 1 : sp > 16 ? 16 : (int)sp;
+}
+
+bool kv4_prefill_fits(int batch, int heads, int kv_heads, int seq, int kv_len) {
+  const long long rows = (long long)(heads / kv_heads) * seq;
+  return rows >= kKv4LongRows && kv_len > 0 && (double)batch * kv_heads * pf_padded(kv_len) < 2147483647.0 &&
+         (long long)batch * kv_heads <= 65535 && batch <= 65535 && kv_heads <= 65535 &&
+         pf_padded(kv_len) <= 2147483647LL / 16;
+}
+size_t kv4_prefill_workspace(int batch, int heads, int kv_heads, int seq, int kv_len, int head_dim) {
+  const int sp = pf_splits(batch, heads, kv_heads, seq, kv_len);
+  const size_t cache = (size_t)batch * kv_heads * pf_padded(kv_len) * head_dim * 2 * 2;
+  return 256 + cache + (sp > 1 ? (size_t)sp * batch * heads * seq * (head_dim + 4) * sizeof(float) : 0);
+}
+
+template <int D, bool OB>
+static int run_prefill(const Kv4Cache& c, PrefillArgs a, int batch, void* workspace, cudaStream_t st) {
+  const size_t rows = (size_t)batch * a.kv_heads * a.padded;
+  uint8_t* k16 = static_cast<uint8_t*>(workspace) + 256;
+  uint8_t* v16 = k16 + rows * D * 2;
+  a.status = static_cast<int*>(workspace);
+  a.part = reinterpret_cast<float*>(v16 + rows * D * 2);
+  CUtensorMap kmap, vmap;
+  int rc = encode_rows_map(&kmap, k16, (int)rows, D, kPfTile);
+  if (!rc) rc = encode_rows_map(&vmap, v16, (int)rows, D, kPfTile);
+  if (rc) return rc;
+  rc = launch_k(kv4_unpack_kernel<D>, dim3((unsigned)(((long long)a.padded * (D / 8) + 255) / 256), a.kv_heads, batch),
+                dim3(256), 0, st, c.kc, c.kp, c.vc, c.vp, a.slots, a.starts, a.kv_heads, a.seq, a.kv_len, c.max_len,
+                c.slot_rows, a.num_slots, a.padded, reinterpret_cast<uint4*>(k16), reinterpret_cast<uint4*>(v16), a.status);
+  if (rc) return rc;
+  static std::atomic<uint64_t> smem_set{0};  // devices with the limit raised
+  rc = ensure_smem_limit(kv4_prefill_kernel<D, OB>, PfSmem<D>::kBytes, smem_set);
+  if (rc) return rc;
+  const dim3 grid((unsigned)pf_row_tiles(a.heads, a.kv_heads, a.seq), batch * a.kv_heads, a.splits);
+  rc = launch_k(kv4_prefill_kernel<D, OB>, grid, dim3(kPfThreads), PfSmem<D>::kBytes, st, kmap, vmap, a);
+  if (rc || a.splits == 1) return rc;
+  return launch_k(kv4_prefill_merge_kernel<D, OB>, dim3((unsigned)((a.rows + 7) / 8)), dim3(256), 0, st, a);
+}
+
+int launch_kv4_prefill(const Kv4Cache& c, const uint16_t* q, const int32_t* slots, const int32_t* starts, int batch,
+                       int heads, int kv_heads, int seq, int head_dim, int kv_len, int num_slots, float scale,
+                       float softcap, void* out, bool out_bf16, void* workspace, cudaStream_t st) {
+  PrefillArgs a{q, slots, starts, heads, kv_heads, seq, kv_len, num_slots, (int)pf_padded(kv_len), scale, softcap, out,
+                nullptr, nullptr, pf_splits(batch, heads, kv_heads, seq, kv_len), (long long)batch * heads * seq};
+  if (head_dim == 128)
+    return out_bf16 ? run_prefill<128, true>(c, a, batch, workspace, st) : run_prefill<128, false>(c, a, batch, workspace, st);
+  return out_bf16 ? run_prefill<64, true>(c, a, batch, workspace, st) : run_prefill<64, false>(c, a, batch, workspace, st);
+}
+
+}  // namespace ccut
