@@ -21,7 +21,7 @@
 // - Each warp streams its own tiles of 16 positions through a four-deep cp.async ring, with no barrier
 //   between warps; 32-byte units are placed so that the reads of both operands touch every bank once.
 //   (Prefetching into registers instead took 168 of them, three CTAs an SM, and 67 us where this takes
-//   TIME_RING.)
+//   50.)
 // - The running maximum moves only when a score passes it by 2^8 (one vote a tile instead of
 //   six shuffles a row pair): probabilities stay below 2^8, and fp16's range has room for that.
 // - Tiles that every row sees in whole run without mask tests; the few others (the last tile, the diagonal
@@ -33,8 +33,8 @@
 //   Equal chunks per sequence cost a prologue, a reduction and a partial result every chunk instead
 //   (64 sequences of 3001..8191 positions: 66 us at the best chunk).
 // Roundings to fp16: q, scaled to its row's largest element (2^-35 of it is kept), and sum q_g (2^-15
-// of the largest element); p s_v, scaled by the power of two R that brings the largest v scale seen so
-// far to [1/2, 1) (11 bits, and 2^-25 of the largest absolutely; with fp32 output a second fp16 part
+// of the largest element); p s_v, scaled by the row's power of two R that brings the largest v scale it has
+// seen to [1/2, 1) (11 bits, and 2^-25 of the largest absolutely; with fp32 output a second fp16 part
 // keeps 22).  Everything else, running maximum, sums and outputs, is fp32.
 #include <math.h>
 
@@ -283,13 +283,13 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
     }
   }
 
-  float m[NT][2], l[NT][2], am[NT][G][2], o[NT][D / 16][4], R = 1.f;
-  __half r_inv = __ushort_as_half(0);  // 1 / R; 0 before the first tile
+  float m[NT][2], l[NT][2], am[NT][G][2], o[NT][D / 16][4], R[NT][2];
+  __half r_inv = __ushort_as_half(0);  // the smallest 1 / R; 0 before the first tile
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      m[nt][c] = -INFINITY, l[nt][c] = 0.f;
+      m[nt][c] = -INFINITY, l[nt][c] = 0.f, R[nt][c] = pow2f(30);  // 2^-30: below every scale
 #pragma unroll
       for (int gr = 0; gr < G; ++gr) am[nt][gr][c] = 0.f;
     }
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
       if constexpr (G == 2)
         top = __hmax2(top, __hmax2(as_half2(vpw[U - 1][0][G - 1]), as_half2(vpw[U - 1][1][G - 1])));
     }
-    need |= __hgt(__low2half(top), r_inv);
+    need |= __hge(__low2half(top), r_inv);
     if (__any_sync(0xffffffffu, need)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -424,8 +424,8 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
           if constexpr (U == 2) v = fmaxf(v, fmaxf(sc[U - 1][nt][c], sc[U - 1][nt][c + 2]));
 #pragma unroll
           for (int s = 4; s < 32; s <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, s));
-          v = fmaxf(v, m[nt][c]);
-          const float al = v == -INFINITY ? 1.f : ex2(m[nt][c] - v);
+          v = v > m[nt][c] + 8.f ? v : m[nt][c];  // by the row's own scores: its bits depend on no other row
+          const float al = v == m[nt][c] ? 1.f : ex2(m[nt][c] - v);
           m[nt][c] = v;
           l[nt][c] *= al;
 #pragma unroll
@@ -433,25 +433,37 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
 #pragma unroll
           for (int mt = 0; mt < D / 16; ++mt) o[nt][mt][c] *= al, o[nt][mt][c + 2] *= al;
         }
-      float v = __low2float(top);
+      float low = INFINITY;
 #pragma unroll
-      for (int s = 4; s < 32; s <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, s));
-      v = fminf(v, 65504.f);
-      if (v > __half2float(r_inv)) {
-        const float r = pow2f(-exponent_of(v) - 1), f = r / R;
-        R = r;
-        r_inv = __float2half_rn(1.f / r);
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int c = 0; c < 2; ++c) {
+          float v = __low2float(top);
+          if constexpr (kMasked) {  // of the positions that the row sees
+            v = 0.f;
 #pragma unroll
-          for (int mt = 0; mt < D / 16; ++mt)
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[nt][mt][i] *= f;
-      }
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) v = fmaxf(v, vis[u][nt][c + 2 * h] ? low_f16(vpw[u][h][gr]) : 0.f);
+          }
+#pragma unroll
+          for (int s = 4; s < 32; s <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, s));
+          v = fminf(v, 65504.f);
+          if (v * R[nt][c] >= 1.f) {
+            const float r = pow2f(-exponent_of(v) - 1), f = r / R[nt][c];
+            R[nt][c] = r;
+#pragma unroll
+            for (int mt = 0; mt < D / 16; ++mt) o[nt][mt][c] *= f, o[nt][mt][c + 2] *= f;
+          }
+          low = fminf(low, 1.f / R[nt][c]);
+        }
+      r_inv = __float2half_rn(low);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      float p[NT][4];
+      float p[NT][4], pr[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -459,10 +471,11 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
           p[nt][i] = ex2(sc[u][nt][i] - m[nt][i & 1]);
           if constexpr (kMasked) p[nt][i] = vis[u][nt][i] ? p[nt][i] : 0.f;  // a row that saw nothing yet has m = -inf
           l[nt][i & 1] += p[nt][i];
+          pr[nt][i] = p[nt][i] * R[nt][i & 1];
         }
 #pragma unroll
       for (int gr = 0; gr < G; ++gr) {
-        const float sr[2] = {low_f16(vpw[u][0][gr]) * R, low_f16(vpw[u][1][gr]) * R};
+        const float sv[2] = {low_f16(vpw[u][0][gr]), low_f16(vpw[u][1][gr])};
         const float mv[2] = {high_f16(vpw[u][0][gr]), high_f16(vpw[u][1][gr])};
         uint32_t wb[NT][2], wl[NT][2];  // p s_v R as the B operand: high part, and the rest
 #pragma unroll
@@ -470,7 +483,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
           float w[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            w[i] = p[nt][i] * sr[i >> 1];
+            w[i] = pr[nt][i] * sv[i >> 1];
             if constexpr (kMasked) {  // 0 * NaN stays out
               w[i] = vis[u][nt][i] ? w[i] : 0.f;
               am[nt][gr][i & 1] += vis[u][nt][i] ? p[nt][i] * mv[i >> 1] : 0.f;
@@ -548,7 +561,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
       if (g == 0) sm_m[warp][n] = m[nt][c], sm_l[warp][n] = l[nt][c];
 #pragma unroll
       for (int gr = 0; gr < G; ++gr) {
-        const float u = pow2f(20) / R;
+        const float u = pow2f(20) / R[nt][c];
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) {
           float* d = &sm_o[warp][n][gr * kKv4Group + g * 8 + mt * 2];

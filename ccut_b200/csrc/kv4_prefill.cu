@@ -51,17 +51,32 @@ struct PfSmem {
 };
 
 struct PfBars {
-  uint64_t q_full[2], kv_full[6], kv_empty[6], s_full[2], p_full[2], o_full[2];
+  uint64_t q_full[2], kv_full[6], kv_empty[6], s_full[2], p_half[2], p_full[2], o_full[2];
   uint32_t tmem;
   int failed;
 };
 
+// One thread of the (converged) warp; code behind it keeps its operands in uniform registers.
+CCUT_DEVICE bool pf_elect() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+// D[tmem] (+)= A[smem] B[smem], and with A in tensor memory.
 CCUT_DEVICE void pf_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+CCUT_DEVICE void pf_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 // B operand stored [k][n], 64 n to a row of 128 bytes: 8-row groups of k 1024 bytes apart (stride offset), the next
@@ -79,6 +94,29 @@ CCUT_DEVICE float pf_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+typedef unsigned long long u64;
+CCUT_DEVICE u64 pf_pair(float a, float b) {
+  u64 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+CCUT_DEVICE void pf_unpair(u64 p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+CCUT_DEVICE u64 pf_add2(u64 a, u64 b) {
+  u64 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+CCUT_DEVICE u64 pf_fma2(u64 a, u64 b, u64 c) {
+  u64 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// To fp16, finite: a scale that was rounded up takes an appended group's top to 65536 at most, half a step above 65504.
+CCUT_DEVICE __half2 pf_half2(float a, float b) {
+  return __floats2half2_rn(fminf(fmaxf(a, -65504.f), 65504.f), fminf(fmaxf(b, -65504.f), 65504.f));
 }
 
 // Unpacked rows: [batch][kv_heads][padded][d] fp16 of k and of v; zeros past what the batch row sees.
@@ -113,8 +151,8 @@ __global__ void __launch_bounds__(256) kv4_unpack_kernel(const uint8_t* __restri
     const uint32_t wk = reinterpret_cast<const uint32_t*>(kc)[row * W + w], wv = reinterpret_cast<const uint32_t*>(vc)[row * W + w];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const __half2 hk = __floats2half2_rn(kv4_value((wk >> (8 * i)) & 15, pk.x, pk.y), kv4_value((wk >> (8 * i + 4)) & 15, pk.x, pk.y));
-      const __half2 hv = __floats2half2_rn(kv4_value((wv >> (8 * i)) & 15, pv.x, pv.y), kv4_value((wv >> (8 * i + 4)) & 15, pv.x, pv.y));
+      const __half2 hk = pf_half2(kv4_value((wk >> (8 * i)) & 15, pk.x, pk.y), kv4_value((wk >> (8 * i + 4)) & 15, pk.x, pk.y));
+      const __half2 hv = pf_half2(kv4_value((wv >> (8 * i)) & 15, pv.x, pv.y), kv4_value((wv >> (8 * i + 4)) & 15, pv.x, pv.y));
       k[i] = bad ? 0x7FFF7FFFu : *reinterpret_cast<const uint32_t*>(&hk);
       v[i] = bad ? 0u : *reinterpret_cast<const uint32_t*>(&hv);
     }
@@ -153,6 +191,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.q_full[i], kPfRows);
       mbar_init(&bars.s_full[i], 1);
+      mbar_init(&bars.p_half[i], kPfRows);
       mbar_init(&bars.p_full[i], kPfRows);
       mbar_init(&bars.o_full[i], 1);
     }
@@ -170,7 +209,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  const uint32_t tmem = bars.tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, bars.tmem, 0);
   volatile int* failed = &bars.failed;
   // columns: S_0 (P_0 in its first half), S_1, O_0, O_1
   auto s_col = [&](int i) { return tmem + i * kPfTile; };
@@ -201,47 +240,71 @@ __global__ void __launch_bounds__(kPfThreads, 1)
                           &bars.kv_full[st]);
       }
     }
-  } else if (warp == 1) {
-    if (lane == 0 && n > 0) {
-      const uint32_t idesc_s = tc::idesc_f16_m128(kPfTile);
-      const uint32_t idesc_o = tc::idesc_f16_m128(D) | (1u << 16);  // B is [k][n]
-      auto scores = [&](int i, int t) {  // S_i = Q_i K^T, K the ring's tile t
-        const uint32_t q0 = smem_u32(q_s) + i * SM::kTileBytes, k0 = smem_u32(ring) + t % SM::kStages * SM::kTileBytes;
+  } else if (warp == 1 && n > 0) {
+    // The whole warp walks through the steps and one lane issues: a divergent lane could not use the uniform
+    // registers that the MMAs take their operands from, and moving them there took longer than the MMAs.
+    const uint32_t idesc_s = tc::idesc_f16_m128(kPfTile);
+    const uint32_t idesc_o = tc::idesc_f16_m128(D) | (1u << 16);  // B is [k][n]
+    auto spin = [&](uint64_t* bar, uint32_t parity) {  // its wake-up is on the critical path
+      const bool ok = mbar_spin(bar, parity, a.status);
+      if (!ok) *failed = 1;
+      return __all_sync(0xffffffffu, ok && !*failed) != 0;
+    };
+    const uint64_t q_desc = tc::sdesc_sw128(smem_u32(q_s));
+    const uint64_t k_desc = tc::sdesc_sw128(smem_u32(ring)), v_desc = pf_desc_mn(smem_u32(ring));
+    auto scores = [&](int i, int st, bool free_k) {  // S_i = Q_i K^T, K in the ring's stage st
+      const uint64_t q0 = q_desc + (uint64_t)(i * (SM::kTileBytes >> 4)), k0 = k_desc + (uint64_t)(st * (SM::kTileBytes >> 4));
+      if (pf_elect()) {
+#pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * kSub + (ks & 3) * 32;
-          pf_mma_ss(s_col(i), tc::sdesc_sw128(q0 + off), tc::sdesc_sw128(k0 + off), idesc_s, ks > 0);
+          const uint64_t off = (ks >> 2) * (kSub >> 4) + (ks & 3) * (32 >> 4);
+          pf_mma_ss(s_col(i), q0 + off, k0 + off, idesc_s, ks > 0);
         }
         tc::commit(&bars.s_full[i]);
-      };
-      bool ok = wait(&bars.q_full[0], 0) && wait(&bars.kv_full[0], 0);
-      tc::fence_after_sync();
-      if (ok) scores(0, 0);
-      ok = ok && wait(&bars.q_full[1], 0);
-      tc::fence_after_sync();
-      if (ok) {
-        scores(1, 0);
-        tc::commit(&bars.kv_empty[0]);
+        if (free_k) tc::commit(&bars.kv_empty[st]);
       }
-      for (int j = 0; ok && j < n; ++j) {
-        const int tv = 2 * j + 1, tk = 2 * j + 2;
-        for (int i = 0; i < 2; ++i) {
-          if (i == 0 && !(ok = wait(&bars.kv_full[tv % SM::kStages], tv / SM::kStages & 1))) break;
-          if (!(ok = wait(&bars.p_full[i], j & 1))) break;
+      __syncwarp();
+    };
+    bool ok = spin(&bars.q_full[0], 0) && spin(&bars.kv_full[0], 0);
+    tc::fence_after_sync();
+    if (ok) scores(0, 0, false);
+    ok = ok && spin(&bars.q_full[1], 0);
+    tc::fence_after_sync();
+    if (ok) scores(1, 0, true);
+    int sv = 1, pv = 0;  // stage of the next v tile, and the parity of its use
+    for (int j = 0; ok && j < n; ++j) {
+      int sk = sv + 1, pk = pv;  // of the k tile after it
+      if (sk == SM::kStages) sk = 0, pk ^= 1;
+      const uint64_t v0 = v_desc + (uint64_t)(sv * (SM::kTileBytes >> 4));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (i == 0 && !(ok = spin(&bars.kv_full[sv], pv))) break;
+        if (!(ok = spin(&bars.p_half[i], j & 1))) break;
+        tc::fence_after_sync();
+        if (pf_elect()) {
+#pragma unroll
+          for (int ks = 0; ks < kPfTile / 32; ++ks)
+            pf_mma_ts(o_col(i), s_col(i) + ks * 8, v0 + ks * (2048 >> 4), idesc_o, ks > 0 || j > 0);
+        }
+        __syncwarp();
+        if (!(ok = spin(&bars.p_full[i], j & 1))) break;
+        tc::fence_after_sync();
+        if (pf_elect()) {
+#pragma unroll
+          for (int ks = kPfTile / 32; ks < kPfTile / 16; ++ks)
+            pf_mma_ts(o_col(i), s_col(i) + ks * 8, v0 + ks * (2048 >> 4), idesc_o, 1);
+          if (i == 1) tc::commit(&bars.kv_empty[sv]);
+          if (j + 1 == n) tc::commit(&bars.o_full[i]);
+        }
+        __syncwarp();
+        if (j + 1 < n) {
+          if (i == 0 && !(ok = spin(&bars.kv_full[sk], pk))) break;
           tc::fence_after_sync();
-          const uint32_t v0 = smem_u32(ring) + tv % SM::kStages * SM::kTileBytes;
-          for (int ks = 0; ks < kPfTile / 16; ++ks)
-            tc::mma_ts(o_col(i), s_col(i) + ks * 8, pf_desc_mn(v0 + ks * 2048), idesc_o, j > 0 || ks > 0);
-          if (i == 1) tc::commit(&bars.kv_empty[tv % SM::kStages]);
-          if (j + 1 < n) {
-            if (i == 0 && !(ok = wait(&bars.kv_full[tk % SM::kStages], tk / SM::kStages & 1))) break;
-            tc::fence_after_sync();
-            scores(i, tk);
-            if (i == 1) tc::commit(&bars.kv_empty[tk % SM::kStages]);
-          } else {
-            tc::commit(&bars.o_full[i]);
-          }
+          scores(i, sk, i == 1);
         }
       }
+      sv = sk + 1, pv = pk;
+      if (sv == SM::kStages) sv = 0, pv ^= 1;
     }
   }
   } else {
@@ -321,7 +384,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         for (int c = 0; c < 4; ++c) top[c] = fmaxf(top[c], __uint_as_float(x[c][e]));
       const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f;
       if (__any_sync(0xffffffffu, mt > m + 8.f)) {
-        const float mn = fmaxf(m, mt), al = mn == -INFINITY ? 1.f : pf_ex2(m - mn);
+        const float mn = mt > m + 8.f ? mt : m, al = mn == m ? 1.f : pf_ex2(m - mn);  // by the row's own scores
         m = mn;
         l *= al;
         __syncwarp();
@@ -339,24 +402,30 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       }
       const float mu = m == -INFINITY ? 0.f : m;
       __syncwarp();
-      float sum[2] = {0.f, 0.f};
+      const u64 f2 = pf_pair(f, f), mu2 = pf_pair(-mu, -mu);
+      u64 sum[2] = {0, 0};
 #pragma unroll
       for (int c = 0; c < 4; c += 2) {
         uint32_t p[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
           const uint32_t* xe = &x[c + (e >> 4)][(e & 15) * 2];
-          const float y0 = pf_ex2(fmaf(__uint_as_float(xe[0]), f, -mu)), y1 = pf_ex2(fmaf(__uint_as_float(xe[1]), f, -mu));
-          sum[0] += y0, sum[1] += y1;
+          const u64 t = pf_fma2(pf_pair(__uint_as_float(xe[0]), __uint_as_float(xe[1])), f2, mu2);
+          float y0, y1;
+          pf_unpair(t, y0, y1);
+          y0 = pf_ex2(y0), y1 = pf_ex2(y1);
+          sum[e & 1] = pf_add2(sum[e & 1], pf_pair(y0, y1));
           const __half2 h = __floats2half2_rn(y0, y1);
           p[e] = *reinterpret_cast<const uint32_t*>(&h);
         }
         tc::st_32x32b_x32(s_addr + c * 16, p);
+        tc::wait_st();
+        tc::fence_before_sync();
+        mbar_arrive(c == 0 ? &bars.p_half[i] : &bars.p_full[i]);  // the product of the first half can begin
       }
-      l += sum[0] + sum[1];
-      tc::wait_st();
-      tc::fence_before_sync();
-      mbar_arrive(&bars.p_full[i]);
+      float l0, l1;
+      pf_unpair(pf_add2(sum[0], sum[1]), l0, l1);
+      l += l0 + l1;
     }
     if (n > 0 && ok) ok = wait(&bars.o_full[i], 0);
     ok = !__any_sync(0xffffffffu, !ok);

@@ -287,3 +287,26 @@ def test_captured_call_replays_on_new_inputs(seq):
     b = [kv4_attention(q, other, 0, slots, starts) for _ in range(20)]
     torch.cuda.synchronize()
     assert all(torch.equal(x, want[0]) for x in a) and all(torch.equal(x, want[1]) for x in b)
+
+
+@pytest.mark.parametrize("seq", [1, 3, 70])
+def test_values_at_the_top_of_the_range(seq):
+    """A group of +-1e5 is held as +-65504, its top up to half a step of fp16 more.  The row that
+    sees it gets it; the rows before it, whose mask hides it, keep their bits."""
+    from ccut_b200.blocks.attn_kv4 import kv4_append, kv4_attention
+
+    rng = np.random.default_rng(seq + 50)
+    n, d = 100 + seq, 128
+    pool, host = _pool(rng, 1, 1, 1, 200, d)
+    q = _bf16(rng.standard_normal((1, 4, seq, d)))
+    at = (torch.zeros(1, dtype=torch.int32, device="cuda"), torch.full((1,), n - seq, dtype=torch.int32, device="cuda"))
+    clean = kv4_attention(_dev(q, torch.bfloat16), pool, 0, *at)
+    k = host["k"]
+    row = serving.kv4_values(*k)[0, 0, :, n - 1][None].astype(np.float32)
+    big = np.where(np.arange(d) % 3 == 0, -1e5, 1e5).astype(np.float32)[None, None]
+    kv4_append(pool, 0, _dev(row), _dev(big), at[0], torch.full_like(at[0], n - 1))
+    host["k"], host["v"] = ((pool.k.cpu().numpy(), pool.k_par.cpu().numpy()), (pool.v.cpu().numpy(), pool.v_par.cpu().numpy()))
+    got = kv4_attention(_dev(q, torch.bfloat16), pool, 0, *at)
+    assert torch.equal(got[:, :, :-1], clean[:, :, :-1])
+    assert np.abs(serving.kv4_values(*host["v"])[0, 0, 0, n - 1]).max() >= 65504
+    _check(pool, host, 0, q, [0], [n - seq])
