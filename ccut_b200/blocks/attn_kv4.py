@@ -169,7 +169,8 @@ def kv4_read(pool: Kv4Pool, layer: int, slots: torch.Tensor, positions: torch.Te
     slots, positions = _index(slots, n, pool, "slots"), _index(positions, n, pool, "positions")
     if out_dtype not in _DTYPES:
         raise ValueError("out_dtype must be bf16 or fp32")
-    k, v = torch.empty((2, n, pool.kv_heads, pool.head_dim), dtype=out_dtype, device=pool.device).unbind()
+    k = torch.empty((n, pool.kv_heads, pool.head_dim), dtype=out_dtype, device=pool.device)
+    v = torch.empty_like(k)
     kc, kp, vc, vp = pool._pointers(layer)
     _run(pool.device, "ccut_kv4_read", kc, kp, vc, vp, slots.data_ptr(), positions.data_ptr(), n, pool.kv_heads,
          pool.head_dim, pool.max_len, pool.slot_rows, pool.slots, k.data_ptr(), v.data_ptr(), _DTYPES[out_dtype])

@@ -90,6 +90,11 @@ CCUT_DEVICE uint64_t pf_desc_mn(uint32_t saddr) {
   d |= (uint64_t)2 << 61;
   return d;
 }
+CCUT_DEVICE float pf_max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
 CCUT_DEVICE float pf_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -379,9 +384,9 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       }
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int e = 0; e < 32; ++e)
+      for (int e = 0; e < 32; e += 2)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) top[c] = fmaxf(top[c], __uint_as_float(x[c][e]));
+        for (int c = 0; c < 4; ++c) top[c] = pf_max3(top[c], __uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1]));
       const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f;
       if (__any_sync(0xffffffffu, mt > m + 8.f)) {
         const float mn = mt > m + 8.f ? mt : m, al = mn == m ? 1.f : pf_ex2(m - mn);  // by the row's own scores

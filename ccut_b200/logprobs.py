@@ -45,13 +45,13 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_n: int = 0) -
         logits = logits.contiguous()
     tokens = tokens if tokens.is_contiguous() else tokens.contiguous()
     dev = logits.device
-    f = torch.empty((2 + top_n, rows), dtype=torch.float32, device=dev)  # logprob, entropy, top log probabilities
-    i = torch.empty((1 + top_n, rows), dtype=torch.int32, device=dev)  # rank, top ids
+    logprob = torch.empty(rows, dtype=torch.float32, device=dev)
+    entropy, rank = torch.empty_like(logprob), torch.empty_like(tokens)
+    ids = torch.empty((rows, top_n), dtype=torch.int32, device=dev)
+    top = torch.empty((rows, top_n), dtype=torch.float32, device=dev)
     nbytes = _lib.load().ccut_token_logprobs_workspace_bytes(rows, vocab, top_n)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    fp, ip = f.data_ptr(), i.data_ptr()
     _run(dev, "ccut_token_logprobs", logits.data_ptr(), _DTYPES[logits.dtype], rows, vocab,
-         logits.stride(0) if rows > 1 else vocab, tokens.data_ptr(), top_n, fp, fp + 4 * rows, ip, ip + 4 * rows,
-         fp + 8 * rows, ws.data_ptr(), nbytes)
-    shape = (rows, top_n)
-    return TokenLogprobs(f[0], f[1], i[0], i[1:].view(shape), f[2:].view(shape))
+         logits.stride(0) if rows > 1 else vocab, tokens.data_ptr(), top_n, logprob.data_ptr(), entropy.data_ptr(),
+         rank.data_ptr(), ids.data_ptr(), top.data_ptr(), ws.data_ptr(), nbytes)
+    return TokenLogprobs(logprob, entropy, rank, ids, top)
