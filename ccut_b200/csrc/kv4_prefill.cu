@@ -183,6 +183,14 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   const int grp = a.heads / a.kv_heads, nrows = grp * a.seq;
   const int b = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads;
   const int r0 = (gridDim.x - 1 - blockIdx.x) * 2 * kPfRows;  // the longest first
+  const int tr = threadIdx.x & 127, my_r = r0 + (warp >= 8 ? kPfRows : 0) + tr;  // a softmax thread's query row
+  const bool live = warp >= 4 && my_r < nrows;
+  const int my_s = my_r / grp;
+  const int row = (b * a.heads + kvh * grp + my_r % grp) * a.seq + my_s;  // of q and out; rows fit 31 bits
+  if (live) {
+#pragma unroll
+    for (int c = 0; c < D; c += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.q + (size_t)row * D + c));
+  }
   const int slot = a.slots[b], start0 = a.starts[b];
   const bool valid = slot >= 0 && slot < a.num_slots && start0 >= 0;
   const int start = min(start0, a.kv_len);
@@ -227,9 +235,9 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     return ok && !*failed;
   };
 
-  // 256 x 208 + 128 x 80 registers of the 384 x 168 of the launch; one instruction per warpgroup
+  // 256 x 208 + 128 x 88 registers of the 384 x 168 of the launch; one instruction per warpgroup
   if (warp < 4) {
-  tc::setmaxnreg_dec<80>();
+  tc::setmaxnreg_dec<88>();
   if (warp == 0) {
     if (lane == 0 && n > 0) {
       asm volatile("fence.proxy.async;" ::: "memory");  // the unpacked cache was written through the generic proxy
@@ -314,13 +322,10 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   }
   } else {
     tc::setmaxnreg_inc<208>();
-    const int i = (warp - 4) >> 2, tr = (warp & 3) * 32 + lane, r = r0 + i * kPfRows + tr;
+    const int i = (warp - 4) >> 2;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_addr = s_col(i) + lanes, o_addr = o_col(i) + lanes;
-    const bool live = r < nrows;
-    const int s = r / grp;
-    const long long row = ((long long)b * a.heads + kvh * grp + r % grp) * a.seq + s;
-    const int lim = live ? start + s : a.kv_len;  // last visible position
+    const int lim = live ? start + my_s : a.kv_len;  // last visible position
     // the row of q as fp16, scaled by a power of two, into the swizzled tile
     float fr = 0.f;
     if (n > 0) {
@@ -328,7 +333,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       float mx = 0.f;
 #pragma unroll
       for (int c = 0; c < D / 8; ++c) {
-        u[c] = live ? *reinterpret_cast<const uint4*>(a.q + row * D + c * 8) : make_uint4(0, 0, 0, 0);
+        u[c] = live ? *reinterpret_cast<const uint4*>(a.q + (size_t)row * D + c * 8) : make_uint4(0, 0, 0, 0);
         const uint32_t w[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -395,13 +400,13 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         __syncwarp();
         if (j > 0) {  // O of the tiles before is complete: S_i was issued behind its last product
 #pragma unroll
-          for (int c = 0; c < D; c += 32) {
-            uint32_t y[32];
-            tc::ld_32x32b_x32(o_addr + c, y);
+          for (int c = 0; c < D; c += 16) {
+            uint32_t y[16];
+            tc::ld_32x32b_x16(o_addr + c, y);
             tc::wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * al);
-            tc::st_32x32b_x32(o_addr + c, y);
+            for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * al);
+            tc::st_32x32b_x16(o_addr + c, y);
           }
         }
       }
@@ -463,12 +468,12 @@ __global__ void __launch_bounds__(kPfThreads, 1)
             const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(y[e + 2 * q]) * inv, __uint_as_float(y[e + 2 * q + 1]) * inv);
             o[q] = *reinterpret_cast<const uint32_t*>(&h);
           }
-          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row * D + c + e) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (size_t)row * D + c + e) = make_uint4(o[0], o[1], o[2], o[3]);
         }
       } else {
 #pragma unroll
         for (int e = 0; e < 32; e += 4)
-          *reinterpret_cast<float4*>(static_cast<float*>(a.out) + row * D + c + e) =
+          *reinterpret_cast<float4*>(static_cast<float*>(a.out) + (size_t)row * D + c + e) =
               make_float4(__uint_as_float(y[e]) * inv, __uint_as_float(y[e + 1]) * inv, __uint_as_float(y[e + 2]) * inv,
                           __uint_as_float(y[e + 3]) * inv);
       }
