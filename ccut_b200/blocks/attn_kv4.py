@@ -50,11 +50,11 @@ class Kv4Pool:
     @classmethod
     def wrap(cls, k: torch.Tensor, k_par: torch.Tensor, v: torch.Tensor, v_par: torch.Tensor) -> "Kv4Pool":
         """A pool over existing tensors of the layout above (contiguous, nothing copied)."""
-        if k.dim() != 5 or k.dtype != torch.uint8 or k.shape[4] not in (32, 64):
+        shape = tuple(k.shape)
+        if len(shape) != 5 or k.dtype != torch.uint8 or shape[4] not in (32, 64):
             raise ValueError("k must be uint8 [slots, layers, kv_heads, max_len, 32 or 64]")
-        rows = k.shape[:4]
-        par = rows + (k.shape[4] // 32, 2)
-        if v.dtype != torch.uint8 or v.shape != k.shape or k_par.shape != par or v_par.shape != par:
+        par = shape[:4] + (shape[4] // 32, 2)
+        if v.dtype != torch.uint8 or v.shape != shape or k_par.shape != par or v_par.shape != par:
             raise ValueError("k, v, k_par and v_par must share slots, layers, kv_heads, max_len and head_dim")
         if k_par.dtype != torch.float16 or v_par.dtype != torch.float16:
             raise ValueError("k_par and v_par must be fp16")
@@ -125,22 +125,24 @@ def _check_pool(pool, device) -> None:
 
 
 def _index(t: torch.Tensor, n: int, pool: Kv4Pool, name: str) -> torch.Tensor:
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.device != pool.device:
+    if t.dtype != torch.int32 or t.shape != (n,) or t.device != pool.device:
         raise ValueError(f"{name} must be int32 [{n}] on {pool.device}")
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _rows(x: torch.Tensor, pool: Kv4Pool, name: str) -> torch.Tensor:
-    """x ``[tokens, kv_heads, head_dim]`` bf16 or fp32 with strides the kernel reads in place."""
-    if x.dim() != 3 or x.shape[1] != pool.kv_heads or x.shape[2] != pool.head_dim:
-        raise ValueError(f"{name} must be [tokens, {pool.kv_heads}, {pool.head_dim}], got {tuple(x.shape)}")
-    if x.dtype not in _DTYPES:
+def _rows(x: torch.Tensor, pool: Kv4Pool, name: str) -> tuple:
+    """x ``[tokens, kv_heads, head_dim]`` bf16 or fp32 with strides the kernel reads in place: (x, tokens,
+    address, dtype code, token stride, head stride)."""
+    shape, dt = x.shape, _DTYPES.get(x.dtype)
+    if len(shape) != 3 or shape[1] != pool.kv_heads or shape[2] != pool.head_dim:
+        raise ValueError(f"{name} must be [tokens, {pool.kv_heads}, {pool.head_dim}], got {tuple(shape)}")
+    if dt is None:
         raise ValueError(f"{name} must be bf16 or fp32")
-    if x.stride(2) != 1 or (x.stride(0) | x.stride(1)) % 8 or x.data_ptr() % 16:
-        x = x.contiguous()
-        if x.data_ptr() % 16:
-            x = x.clone()
-    return x
+    (st, sh, sd), p = x.stride(), x.data_ptr()
+    if sd != 1 or (st | sh) % 8 or p % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+        (st, sh, _), p = x.stride(), x.data_ptr()
+    return x, shape[0], p, dt, st, sh
 
 
 def kv4_append(pool: Kv4Pool, layer: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
@@ -149,15 +151,14 @@ def kv4_append(pool: Kv4Pool, layer: int, k: torch.Tensor, v: torch.Tensor, slot
     ``(slots[t], positions[t])`` (int32) of ``layer``.  Pairs outside the pool are skipped; the
     pairs of one call must differ."""
     _check_pool(pool, k.device)
-    k, v = _rows(k, pool, "k"), _rows(v, pool, "v")
-    n = k.shape[0]
-    if v.shape[0] != n or v.device != k.device:
+    k, n, kx, k_dt, k_st, k_sh = _rows(k, pool, "k")
+    v, nv, vx, v_dt, v_st, v_sh = _rows(v, pool, "v")
+    if nv != n or v.device != pool.device:
         raise ValueError("k and v must have the same tokens on the same device")
     slots, positions = _index(slots, n, pool, "slots"), _index(positions, n, pool, "positions")
     kc, kp, vc, vp = pool._pointers(layer)
-    _run(pool.device, "ccut_kv4_append", k.data_ptr(), _DTYPES[k.dtype], k.stride(0), k.stride(1), v.data_ptr(),
-         _DTYPES[v.dtype], v.stride(0), v.stride(1), n, pool.kv_heads, pool.head_dim, slots.data_ptr(),
-         positions.data_ptr(), kc, kp, vc, vp, pool.max_len, pool.slot_rows, pool.slots)
+    _run(pool.device, "ccut_kv4_append", kx, k_dt, k_st, k_sh, vx, v_dt, v_st, v_sh, n, pool.kv_heads, pool.head_dim,
+         slots.data_ptr(), positions.data_ptr(), kc, kp, vc, vp, pool.max_len, pool.slot_rows, pool.slots)
 
 
 def kv4_read(pool: Kv4Pool, layer: int, slots: torch.Tensor, positions: torch.Tensor,
@@ -185,9 +186,10 @@ def kv4_attention(q: torch.Tensor, pool: Kv4Pool, layer: int, slots: torch.Tenso
     head_dim]`` (bf16 or fp32).  ``kv_len``: an upper bound of ``starts[b] + seq`` when the host
     knows one (positions at or past it are not read); default: the pool's ``max_len``."""
     _check_pool(pool, q.device)
-    if q.dtype != torch.bfloat16 or q.dim() != 4 or q.shape[3] != pool.head_dim:
+    shape = q.shape
+    if q.dtype != torch.bfloat16 or len(shape) != 4 or shape[3] != pool.head_dim:
         raise ValueError(f"q must be bf16 [batch, heads, seq, {pool.head_dim}]")
-    b, h, s, d = q.shape
+    b, h, s, d = shape
     if h == 0 or h % pool.kv_heads:
         raise ValueError(f"heads ({h}) must be a positive multiple of kv_heads ({pool.kv_heads})")
     if out_dtype not in _DTYPES:

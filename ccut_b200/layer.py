@@ -57,12 +57,14 @@ def _run(device: torch.device, name: str, *args) -> None:
     """``_lib.call(name, *args, stream)`` with ``device`` current and its current stream: the raw stream handle
     and no device switch where ``device`` is current already (a switch and a ``Stream`` object cost several
     microseconds of a decode step's calls)."""
-    i = device.index
+    i, fn = device.index, getattr(_lib.load(), name)
     if i is None or torch._C._cuda_getDevice() != i:
         with torch.cuda.device(device):
-            _lib.call(name, *args, torch.cuda.current_stream().cuda_stream)
+            code = fn(*args, torch.cuda.current_stream().cuda_stream)
     else:
-        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(i))
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if code:
+        _lib.check(code, name)
 
 
 def _ptr(t: torch.Tensor | None) -> C.c_void_p:
