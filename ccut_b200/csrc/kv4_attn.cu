@@ -20,8 +20,7 @@
 //   by movmatrix.
 // - Each warp streams its own tiles of 16 positions through a four-deep cp.async ring, with no barrier
 //   between warps; 32-byte units are placed so that the reads of both operands touch every bank once.
-//   (Prefetching into registers instead took 168 of them, three CTAs an SM, and 67 us where this takes
-//   50.)
+//   (Prefetching into registers instead took 168 of them and left three CTAs an SM.)
 // - The running maximum moves only when a score passes it by 2^8 (one vote a tile instead of
 //   six shuffles a row pair): probabilities stay below 2^8, and fp16's range has room for that.
 // - Tiles that every row sees in whole run without mask tests; the few others (the last tile, the diagonal
@@ -30,8 +29,11 @@
 //   rows, kv head) units form one line, found from starts on the device, and each CTA of one resident
 //   round takes an equal span of it.  A unit inside one span is finished there; of the others a span
 //   leaves at most two partial results (the first and the last of its units), which a second kernel joins.
-//   Equal chunks per sequence cost a prologue, a reduction and a partial result every chunk instead
-//   (64 sequences of 3001..8191 positions: 66 us at the best chunk).
+//   Equal chunks per sequence cost a prologue, a reduction and a partial result every chunk instead (one
+//   sequence of 131071 positions, when this was changed: 54 us in chunks, 22 in spans).
+// Measured (8 query heads per kv head, d = 128): 64 sequences of 3001..8191 positions 50 us, 4.1 TB/s of codes
+// and params (0.64 of a copy's rate); what is left is the instructions, 0.8 issued of 1 a cycle.  One
+// sequence of 131071: 13 us in two launches.  One of 513: 8.5 us, latency.
 // Roundings to fp16: q, scaled to its row's largest element (2^-35 of it is kept), and sum q_g (2^-15
 // of the largest element); p s_v, scaled by the row's power of two R that brings the largest v scale it has
 // seen to [1/2, 1) (11 bits, and 2^-25 of the largest absolutely; with fp32 output a second fp16 part

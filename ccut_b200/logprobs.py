@@ -49,9 +49,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_n: int = 0) -
     entropy, rank = torch.empty_like(logprob), torch.empty_like(tokens)
     ids = torch.empty((rows, top_n), dtype=torch.int32, device=dev)
     top = torch.empty((rows, top_n), dtype=torch.float32, device=dev)
-    nbytes = _lib.load().ccut_token_logprobs_workspace_bytes(rows, vocab, top_n)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _run(dev, "ccut_token_logprobs", logits.data_ptr(), _DTYPES[logits.dtype], rows, vocab,
          logits.stride(0) if rows > 1 else vocab, tokens.data_ptr(), top_n, logprob.data_ptr(), entropy.data_ptr(),
-         rank.data_ptr(), ids.data_ptr(), top.data_ptr(), ws.data_ptr(), nbytes)
+         rank.data_ptr(), ids.data_ptr(), top.data_ptr())
     return TokenLogprobs(logprob, entropy, rank, ids, top)

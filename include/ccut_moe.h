@@ -380,11 +380,9 @@ CCUT_API int ccut_kv4_attention(const uint16_t* q, const uint8_t* k_codes, const
  * has NaN log probabilities and entropy; in the order a NaN comes after -inf.
  * top_n <= min(vocab, CCUT_MAX_TOP_LOGPROBS). */
 #define CCUT_MAX_TOP_LOGPROBS 32
-CCUT_API size_t ccut_token_logprobs_workspace_bytes(int rows, int vocab, int top_n);
 CCUT_API int ccut_token_logprobs(const void* logits, int dtype, int rows, int vocab, long long ld,
                                  const int32_t* tokens, int top_n, float* logprob, float* entropy, int32_t* rank,
-                                 int32_t* top_ids, float* top_logprobs, void* workspace, size_t ws_bytes,
-                                 ccut_stream_t stream);
+                                 int32_t* top_ids, float* top_logprobs, ccut_stream_t stream);
 
 /* ---- low-rank adapters (no reference counterpart) -------------------------------------------- */
 /* out[t] = base[t] + scales[i] * B_i A_i x[t] with i = ids[t] (int32, device), for a projection

@@ -68,16 +68,14 @@ def test_kv4_attention_checks(lib):
 
 
 def test_logprobs_checks(lib):
-    def call(*, x=FAKE, dt=F32, rows=2, vocab=100, ld=100, tok=FAKE, top=5, ids=FAKE, lp=FAKE, ws=FAKE, nb=1 << 30):
-        return lib.ccut_token_logprobs(x, dt, rows, vocab, ld, tok, top, lp, FAKE, FAKE, ids, FAKE, ws, nb, NULL)
+    def call(*, x=FAKE, dt=F32, rows=2, vocab=100, ld=100, tok=FAKE, top=5, ids=FAKE, lp=FAKE):
+        return lib.ccut_token_logprobs(x, dt, rows, vocab, ld, tok, top, lp, FAKE, FAKE, ids, FAKE, NULL)
 
     for kw in ({"dt": 9}, {"rows": -1}, {"vocab": 0}, {"ld": 99}, {"top": -1}, {"top": 101, "vocab": 100}, {"x": NULL},
                {"tok": NULL}, {"ids": NULL}, {"lp": NULL}):
         assert call(**kw) == _lib.ERR_INVALID, kw
     assert call(top=33) == _lib.ERR_UNSUPPORTED
     assert call(rows=0, x=NULL) == _lib.OK
-    need = lib.ccut_token_logprobs_workspace_bytes(2, 100, 5)
-    assert need >= 256 and call(nb=need - 1) == _lib.ERR_WORKSPACE and call(ws=NULL) == _lib.ERR_WORKSPACE
 
 
 def test_lora_checks(lib):
