@@ -700,8 +700,9 @@ __global__ void __launch_bounds__(W > 8 ? W * 32 : 256) kv4_merge_kernel(Kv4Attn
 // Query rows per tile: 8 where a kv head has no more, else 16.
 static int kv4_rows(int heads, int kv_heads, int seq) { return (long)(heads / kv_heads) * seq <= 8 ? 8 : 16; }
 // Positions per block of work: a step of every warp, or all positions where they are few, so that no unit is
-// cut and nothing is left to join (one sequence of 513: 6.5 us uncut, 6.9 cut; of 769: 8.1 and 7.6).
-constexpr int kKv4Uncut = 640;
+// cut and nothing is left to join (64 sequences of up to 1000: 17.6 us uncut, 19.5 cut; 8 of up to 690: 9.5 and
+// 9.4; one of 1024: 11.0 and 7.7, but the second launch costs the host 5 us of a call's 20).
+constexpr int kKv4Uncut = 1024;
 static int kv4_block(int rows, int kv_len) {
   const int step = rows == 8 ? kKv4Block<1> : kKv4Block<2>;
   return kv_len <= kKv4Uncut ? (kv_len > 0 ? (kv_len + step - 1) / step * step : step) : step;
