@@ -310,3 +310,26 @@ def test_values_at_the_top_of_the_range(seq):
     assert torch.equal(got[:, :, :-1], clean[:, :, :-1])
     assert np.abs(serving.kv4_values(*host["v"])[0, 0, 0, n - 1]).max() >= 65504
     _check(pool, host, 0, q, [0], [n - seq])
+
+
+@pytest.mark.parametrize("d, heads, kvh, seq, lens, dt", [
+    (128, 32, 4, 1, [1, 1025, 3000, 64, 1, 2047], torch.bfloat16),
+    (128, 8, 1, 1, [1100] * 40, torch.float32),
+    (128, 4, 2, 5, [5, 1300, 2500], torch.float32),
+    (64, 16, 2, 2, [1500, 40, 2001], torch.bfloat16),
+    (64, 8, 1, 1, [20011], torch.bfloat16),
+    (64, 12, 1, 1, [9000, 3], torch.float32),
+    (128, 16, 2, 40, [1401, 2600], torch.bfloat16),
+    (64, 16, 1, 20, [6007], torch.float32),
+])
+def test_long_caches(d, heads, kvh, seq, lens, dt):
+    """Lengths at which a sequence is cut into parts that are joined, beside ones that are not; with
+    the pool's length as the bound and with the longest sequence's."""
+    rng = np.random.default_rng(d + heads + seq + 1)
+    B, L = len(lens), max(max(lens), 1100) + 70
+    pool, host = _pool(rng, B, 1, kvh, L, d)
+    slots = rng.permutation(B)
+    qh = _bf16(rng.standard_normal((B, heads, seq, d)))
+    starts = [n - seq for n in lens]
+    _check(pool, host, 0, qh, slots, starts, out_dtype=dt)
+    _check(pool, host, 0, qh, slots, starts, kv_len=max(lens), out_dtype=dt, softcap=20.0)
