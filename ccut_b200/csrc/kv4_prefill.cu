@@ -46,12 +46,14 @@ struct PrefillArgs {
 template <int D>
 struct PfSmem {
   static constexpr int kTileBytes = kPfTile * D * 2;  // q, k or v
-  static constexpr int kStages = D == 128 ? 4 : 6;
+  static constexpr int kStages = D == 128 ? 4 : 8;
+  // Room in tensor memory for P beside S: S of the next tile is computed while the softmax of this one runs.
+  static constexpr bool kAhead = D == 64;
   static constexpr int kBytes = 1024 + (2 + kStages) * kTileBytes;
 };
 
 struct PfBars {
-  uint64_t q_full[2], kv_full[6], kv_empty[6], s_full[2], p_half[2], p_full[2], o_full[2];
+  uint64_t q_full[2], kv_full[8], kv_empty[8], s_full[2], s_free[2], p_half[2], p_full[2], o_full[2];
   uint32_t tmem;
   int failed;
 };
@@ -204,6 +206,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.q_full[i], kPfRows);
       mbar_init(&bars.s_full[i], 1);
+      mbar_init(&bars.s_free[i], kPfRows);
       mbar_init(&bars.p_half[i], kPfRows);
       mbar_init(&bars.p_full[i], kPfRows);
       mbar_init(&bars.o_full[i], 1);
@@ -224,9 +227,10 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   tc::fence_after_sync();
   const uint32_t tmem = __shfl_sync(0xffffffffu, bars.tmem, 0);
   volatile int* failed = &bars.failed;
-  // columns: S_0 (P_0 in its first half), S_1, O_0, O_1
+  // columns: S_0, S_1, O_0, O_1, P_0, P_1 (P_i in the first half of S_i where there is no room)
   auto s_col = [&](int i) { return tmem + i * kPfTile; };
   auto o_col = [&](int i) { return tmem + 2 * kPfTile + i * D; };
+  auto p_col = [&](int i) { return SM::kAhead ? tmem + 2 * kPfTile + 2 * D + i * (kPfTile / 2) : s_col(i); };
   uint8_t* q_s = smem;
   uint8_t* ring = smem + 2 * SM::kTileBytes;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -244,13 +248,19 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       tc::prefetch_tmap(&kmap);
       tc::prefetch_tmap(&vmap);
       const int row = (int)(((long long)b * a.kv_heads + kvh) * a.padded) + tile0 * kPfTile;
-      for (int t = 0; t < 2 * n; ++t) {  // k and v tiles in turn
-        const int st = t % SM::kStages, use = t / SM::kStages;
-        if (use > 0 && !wait(&bars.kv_empty[st], (use - 1) & 1)) break;
+      int st = 0, ph = 1;  // the ring's next stage; its first use finds it empty
+      auto load = [&](const CUtensorMap* map, int j) {
+        if (!wait(&bars.kv_empty[st], ph)) return false;
         mbar_arrive_expect_tx(&bars.kv_full[st], SM::kTileBytes);
         for (int c = 0; c < kChunks; ++c)
-          tc::tma_load_2d(ring + st * SM::kTileBytes + c * kSub, t & 1 ? &vmap : &kmap, c * 64, row + t / 2 * kPfTile,
-                          &bars.kv_full[st]);
+          tc::tma_load_2d(ring + st * SM::kTileBytes + c * kSub, map, c * 64, row + j * kPfTile, &bars.kv_full[st]);
+        if (++st == SM::kStages) st = 0, ph ^= 1;
+        return true;
+      };
+      bool ok = !SM::kAhead || load(&kmap, 0);  // k j + 1 before v j where S runs ahead, else k j
+      for (int j = 0; ok && j < n; ++j) {
+        const int k = SM::kAhead ? j + 1 : j;
+        ok = (k >= n || load(&kmap, k)) && load(&vmap, j);
       }
     }
   } else if (warp == 1 && n > 0) {
@@ -278,53 +288,94 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       }
       __syncwarp();
     };
+    auto products = [&](int i, int k0, int k1, int sv, bool first) {  // O_i (+)= P_i V over k16 steps k0 ..
+      const uint64_t v0 = v_desc + (uint64_t)(sv * (SM::kTileBytes >> 4));
+      if (pf_elect()) {
+#pragma unroll
+        for (int ks = k0; ks < k1; ++ks)
+          pf_mma_ts(o_col(i), p_col(i) + ks * 8, v0 + ks * (2048 >> 4), idesc_o, ks > 0 || !first);
+      }
+    };
+    auto advance = [](int& st, int& ph) {
+      if (++st == SM::kStages) st = 0, ph ^= 1;
+    };
     bool ok = spin(&bars.q_full[0], 0) && spin(&bars.kv_full[0], 0);
     tc::fence_after_sync();
     if (ok) scores(0, 0, false);
     ok = ok && spin(&bars.q_full[1], 0);
     tc::fence_after_sync();
     if (ok) scores(1, 0, true);
-    int sv = 1, pv = 0;  // stage of the next v tile, and the parity of its use
-    for (int j = 0; ok && j < n; ++j) {
-      int sk = sv + 1, pk = pv;  // of the k tile after it
-      if (sk == SM::kStages) sk = 0, pk ^= 1;
-      const uint64_t v0 = v_desc + (uint64_t)(sv * (SM::kTileBytes >> 4));
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (i == 0 && !(ok = spin(&bars.kv_full[sv], pv))) break;
-        if (!(ok = spin(&bars.p_half[i], j & 1))) break;
+    int st = 1, ph = 0;  // the ring's next stage and the parity of its use
+    if constexpr (SM::kAhead) {
+      // S_0 of tile j + 1, P_1 V of j - 1, S_1 of j + 1, P_0 V of j: what two tiles half a step apart ask for in turn
+      auto join = [&](int i, int j, int sv) {
+        if (!spin(&bars.p_full[i], j & 1)) return false;
         tc::fence_after_sync();
+        products(i, 0, kPfTile / 16, sv, j == 0);
         if (pf_elect()) {
-#pragma unroll
-          for (int ks = 0; ks < kPfTile / 32; ++ks)
-            pf_mma_ts(o_col(i), s_col(i) + ks * 8, v0 + ks * (2048 >> 4), idesc_o, ks > 0 || j > 0);
-        }
-        __syncwarp();
-        if (!(ok = spin(&bars.p_full[i], j & 1))) break;
-        tc::fence_after_sync();
-        if (pf_elect()) {
-#pragma unroll
-          for (int ks = kPfTile / 32; ks < kPfTile / 16; ++ks)
-            pf_mma_ts(o_col(i), s_col(i) + ks * 8, v0 + ks * (2048 >> 4), idesc_o, 1);
+          tc::commit(&bars.o_full[i]);
           if (i == 1) tc::commit(&bars.kv_empty[sv]);
-          if (j + 1 == n) tc::commit(&bars.o_full[i]);
         }
         __syncwarp();
+        return true;
+      };
+      int sv = 0;  // of v tile j - 1
+      for (int j = 0; ok && j < n; ++j) {
+        int sk = 0;
         if (j + 1 < n) {
-          if (i == 0 && !(ok = spin(&bars.kv_full[sk], pk))) break;
+          sk = st;
+          if (!(ok = spin(&bars.kv_full[sk], ph) && spin(&bars.s_free[0], j & 1))) break;
+          advance(st, ph);
           tc::fence_after_sync();
-          scores(i, sk, i == 1);
+          scores(0, sk, false);
         }
+        if (j > 0 && !(ok = join(1, j - 1, sv))) break;
+        if (j + 1 < n) {
+          if (!(ok = spin(&bars.s_free[1], j & 1))) break;
+          tc::fence_after_sync();
+          scores(1, sk, true);
+        }
+        sv = st;
+        if (!(ok = spin(&bars.kv_full[sv], ph))) break;
+        advance(st, ph);
+        if (!(ok = join(0, j, sv))) break;
       }
-      sv = sk + 1, pv = pk;
-      if (sv == SM::kStages) sv = 0, pv ^= 1;
+      if (ok) join(1, n - 1, sv);
+    } else {
+      for (int j = 0; ok && j < n; ++j) {
+        const int sv = st;
+        if (!(ok = spin(&bars.kv_full[sv], ph))) break;
+        advance(st, ph);
+        const int sk = st;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (!(ok = spin(&bars.p_half[i], j & 1))) break;
+          tc::fence_after_sync();
+          products(i, 0, kPfTile / 32, sv, j == 0);
+          __syncwarp();
+          if (!(ok = spin(&bars.p_full[i], j & 1))) break;
+          tc::fence_after_sync();
+          products(i, kPfTile / 32, kPfTile / 16, sv, false);
+          if (pf_elect()) {
+            if (i == 1) tc::commit(&bars.kv_empty[sv]);
+            if (j + 1 == n) tc::commit(&bars.o_full[i]);
+          }
+          __syncwarp();
+          if (j + 1 < n) {
+            if (i == 0 && !(ok = spin(&bars.kv_full[sk], ph))) break;
+            tc::fence_after_sync();
+            scores(i, sk, i == 1);
+          }
+        }
+        if (j + 1 < n) advance(st, ph);
+      }
     }
   }
   } else {
     tc::setmaxnreg_inc<208>();
     const int i = (warp - 4) >> 2;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = s_col(i) + lanes, o_addr = o_col(i) + lanes;
+    const uint32_t s_addr = s_col(i) + lanes, p_addr = p_col(i) + lanes, o_addr = o_col(i) + lanes;
     const int lim = live ? start + my_s : a.kv_len;  // last visible position
     // the row of q as fp16, scaled by a power of two, into the swizzled tile
     float fr = 0.f;
@@ -369,6 +420,10 @@ __global__ void __launch_bounds__(kPfThreads, 1)
 #pragma unroll
       for (int c = 0; c < 4; ++c) tc::ld_32x32b_x32(s_addr + c * 32, x[c]);
       tc::wait_ld();
+      if constexpr (SM::kAhead) {
+        tc::fence_before_sync();
+        mbar_arrive(&bars.s_free[i]);
+      }
       const int p0 = (tile0 + j) * kPfTile;
       float f = fr;
       if (a.softcap > 0.f) {
@@ -393,12 +448,19 @@ __global__ void __launch_bounds__(kPfThreads, 1)
 #pragma unroll
         for (int c = 0; c < 4; ++c) top[c] = pf_max3(top[c], __uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1]));
       const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f;
+      if constexpr (SM::kAhead) {  // P and O are free: the product of the tile before is done
+        if (j > 0) {
+          ok = wait(&bars.o_full[i], (j - 1) & 1);
+          ok = !__any_sync(0xffffffffu, !ok);
+          tc::fence_after_sync();
+        }
+      }
       if (__any_sync(0xffffffffu, mt > m + 8.f)) {
         const float mn = mt > m + 8.f ? mt : m, al = mn == m ? 1.f : pf_ex2(m - mn);  // by the row's own scores
         m = mn;
         l *= al;
         __syncwarp();
-        if (j > 0) {  // O of the tiles before is complete: S_i was issued behind its last product
+        if (j > 0) {  // O of the tiles before is complete (else than above: S_i was issued behind its last product)
 #pragma unroll
           for (int c = 0; c < D; c += 16) {
             uint32_t y[16];
@@ -428,16 +490,17 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           const __half2 h = __floats2half2_rn(y0, y1);
           p[e] = *reinterpret_cast<const uint32_t*>(&h);
         }
-        tc::st_32x32b_x32(s_addr + c * 16, p);
+        tc::st_32x32b_x32(p_addr + c * 16, p);
         tc::wait_st();
         tc::fence_before_sync();
-        mbar_arrive(c == 0 ? &bars.p_half[i] : &bars.p_full[i]);  // the product of the first half can begin
+        if (c > 0) mbar_arrive(&bars.p_full[i]);
+        else if (!SM::kAhead) mbar_arrive(&bars.p_half[i]);  // the product of the first half can begin
       }
       float l0, l1;
       pf_unpair(pf_add2(sum[0], sum[1]), l0, l1);
       l += l0 + l1;
     }
-    if (n > 0 && ok) ok = wait(&bars.o_full[i], 0);
+    if (n > 0 && ok) ok = wait(&bars.o_full[i], SM::kAhead ? (n - 1) & 1 : 0);
     ok = !__any_sync(0xffffffffu, !ok);
     tc::fence_after_sync();
     const float inv = l == 0.f ? 0.f : 1.f / l;
