@@ -526,8 +526,9 @@ __global__ void __launch_bounds__(kLoraWarps * 32, OUT_BF16 ? 4 : 3)
   const int R = p.slices * p.rank, ld = lora_ld(R), steps = KR ? KR : p.rank / 16;
   const int bld = lora_ld(p.rank) * 2;  // bytes per row of B
   const size_t plane = (size_t)kLoraRows * ld;
-  uint16_t* hs = reinterpret_cast<uint16_t*>(smem);  // [parts][64][lora_ld(R)]
-  uint8_t* bs = smem + kParts * plane * 2;           // [128][rank] bf16
+  constexpr bool kRegs = KR > 0;  // h of a slice fits registers, as operands; else planes in shared memory
+  uint16_t* hs = reinterpret_cast<uint16_t*>(smem);             // [parts][64][lora_ld(R)]
+  uint8_t* bs = smem + (kRegs ? 0 : kParts * plane * 2);        // [128][rank] bf16
   // base, then out: [64][128], moved 16 bytes a lane, whole lines at a time
   constexpr int kSize = OUT_BF16 ? 2 : 4, kOld = kLoraOutputs * kSize + 16 * kSize, kChunks = kLoraOutputs * kSize / 16;
   uint8_t* os = bs + kLoraOutputs * bld;
@@ -535,7 +536,7 @@ __global__ void __launch_bounds__(kLoraWarps * 32, OUT_BF16 ? 4 : 3)
   const int row0 = t0 + warp * kLoraTile + g, row1 = row0 + 8;
   const bool in0 = row0 < p.tokens, in1 = row1 < p.tokens;
   // h of rows g and g + 8, columns 4 t + 16 c .. + 3 (rows without an adapter are zeros there)
-  constexpr int kBatch = 4;
+  constexpr int kBatch = kRegs ? KR : 4;
   float4 h[2][kBatch];
   auto load_h = [&](int c0) {
 #pragma unroll
@@ -546,7 +547,8 @@ __global__ void __launch_bounds__(kLoraWarps * 32, OUT_BF16 ? 4 : 3)
                       ? *reinterpret_cast<const float4*>(p.part + (size_t)(i ? row1 : row0) * R + (c0 + c) * 16 + 4 * t)
                       : make_float4(0.f, 0.f, 0.f, 0.f);
   };
-  load_h(0);
+  int slice = kRegs ? lora_slice(p, o0) : 0;  // whose h is in registers
+  load_h(slice * KR);
   constexpr int kHop = kLoraWarps * 32 / kChunks;  // rows that the CTA moves at a time
   const int mr = threadIdx.x / kChunks, mc = threadIdx.x % kChunks;
   const bool mine = mc < width * kSize / 16;  // widths are multiples of 8: whole chunks
@@ -574,7 +576,23 @@ __global__ void __launch_bounds__(kLoraWarps * 32, OUT_BF16 ? 4 : 3)
   if (rows.n > 0) fetch_b(rows.uniq[0]);
   const int id0 = rows.ids[warp * kLoraTile + g], id1 = rows.ids[warp * kLoraTile + g + 8];
   const float f0 = id0 >= 0 ? p.scales[id0] : 0.f, f1 = id1 >= 0 ? p.scales[id1] : 0.f;
-  for (int c0 = 0; c0 * 16 < R; c0 += kBatch) {
+  uint32_t hf[kRegs ? KR : 1][kParts][4];
+  auto keep_h = [&]() {  // scaled, in parts
+#pragma unroll
+    for (int c = 0; c < kBatch; ++c)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float f = i ? f1 : f0;
+        float4 v = make_float4(h[i][c].x * f, h[i][c].y * f, h[i][c].z * f, h[i][c].w * f);
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
+          hf[c][part][i] = take_bf16x2(v.x, v.y);
+          hf[c][part][i + 2] = take_bf16x2(v.z, v.w);
+        }
+      }
+  };
+  if constexpr (kRegs) keep_h();
+  for (int c0 = 0; !kRegs && c0 * 16 < R; c0 += kBatch) {
     if (c0 > 0) load_h(c0);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -601,10 +619,24 @@ __global__ void __launch_bounds__(kLoraWarps * 32, OUT_BF16 ? 4 : 3)
         for (int j = j0; j <= j1; ++j) {
           float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
           const uint16_t* hr = hs + (warp * kLoraTile + g) * ld + j * p.rank + 4 * t;
+          if constexpr (kRegs) {
+            if (j != slice) {
+              slice = j;
+              load_h(j * KR);
+              keep_h();
+            }
+          }
 #pragma unroll KR ? KR : 1
           for (int k = 0; k < steps; ++k) {
             uint32_t f[kParts][4];
-            lora_operands<kParts>(hr + 16 * k, plane, ld, f);
+            if constexpr (kRegs) {
+#pragma unroll
+              for (int part = 0; part < kParts; ++part)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[part][e] = hf[k][part][e];
+            } else {
+              lora_operands<kParts>(hr + 16 * k, plane, ld, f);
+            }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {  // a column past the last output is not written, whatever it holds
               const uint2 b = *reinterpret_cast<const uint2*>(br + i * 8 * bld + 32 * k);
@@ -706,7 +738,8 @@ static int run_lora_prompt(const LoraArgs& p, cudaStream_t st) {
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, lora_shrink_kernel, p) != cudaSuccess) return CCUT_ERR_CUDA;
   auto smem = [](size_t R, size_t rank) {
-    return (size_t)(OB ? 2 : 3) * kLoraRows * lora_ld((int)R) * 2 + kLoraOutputs * lora_ld((int)rank) * 2 +
+    const bool regs = rank == 16 || rank == 32 || rank == 64;
+    return (regs ? 0 : (size_t)(OB ? 2 : 3) * kLoraRows * lora_ld((int)R) * 2) + kLoraOutputs * lora_ld((int)rank) * 2 +
            kLoraRows * (kLoraOutputs + 16) * (OB ? 2 : 4);
   };
   auto kern = p.rank == 16   ? lora_expand_kernel<1, OB>
