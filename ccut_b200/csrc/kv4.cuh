@@ -9,8 +9,8 @@
 //
 // Rounding: m = fp16(min) and s = fp16(fl32(max - m) * fl32(1/15)) to the nearest (two roundings of
 // 2^-11; the codes are chosen with the rounded pair, so they only move the grid), q = the nearest of
-// 0..15, ties to even.  Values beyond +-65504 saturate there, so s <= 8734 and q s + m stays in fp16's
-// range.  A group that holds a NaN or an infinity gets s = m = NaN and reads back NaN.
+// 0..15, ties to even.  Values beyond +-65504 saturate there, so s <= 8736 and q s + m <= 65536.
+// A group that holds a NaN or an infinity gets s = m = NaN and reads back NaN.
 #pragma once
 
 #include "host.cuh"
