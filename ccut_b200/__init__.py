@@ -23,13 +23,17 @@ Public entry points
 ``blocks.norm``              drop-in for ``ccut.blocks.norm.rms_norm``
 ``blocks.rope``              drop-in for ``ccut.blocks.rope.apply_rope``
 ``blocks.attn_mla``          drop-ins for ``ccut.blocks.attn_mla`` (MLA latent attention)
+``blocks.attn_kv4``          4-bit kv caches: ``Kv4Pool``, ``kv4_append``, ``kv4_attention``, ``kv4_read``
+``logprobs``                 ``token_logprobs``: log probability, entropy, rank and top alternatives
+``adapters``                 ``LoraBank``: low-rank adapters, a different one per token
 ``model``                    ``MoeDecoder``: embedding, decoder layers (``DecoderLayer``: GQA
                              attention, ``MlaDecoderLayer``: multi-head latent attention; norms,
                              RoPE, bf16 caches in HBM, MoE or dense FFN), final norm, ``lm_head``
                              -- the reference's generic layer forward on the GPU
 ``rope_tables``              RoPE tables: the reference's ``build_rope`` cases, YaRN
 ``backend.GenericBackend``   the ``generate_step`` backend the reference's ``Engine`` calls, over
-                             a ``MoeDecoder`` (prefix-reusing sequence caches, on-device sampling)
+                             a ``MoeDecoder`` (prefix-reusing sequence caches, on-device sampling;
+                             ``kv_dtype="int4"``, ``adapter=``, ``logprobs=``, ``score``)
 ``sampling``                 the reference's temperature / top-k / min-p / top-p transform in torch
 """
 

@@ -353,7 +353,8 @@ CCUT_API int ccut_kv4_read(const uint8_t* k_codes, const uint16_t* k_params, con
                            const uint16_t* v_params, const int32_t* slots, const int32_t* positions, int tokens,
                            int kv_heads, int head_dim, int max_len, long long slot_rows, int num_slots, void* k_out,
                            void* v_out, int out_dtype, ccut_stream_t stream);
-/* ccut_gqa_attention_pool over a 4-bit pool: q bf16 [batch, heads, seq, head_dim], out the same
+/* ccut_gqa_attention_pool over a 4-bit pool (a long block of query rows unpacks what it reads to
+ * fp16 in the workspace first; a workspace needs no zero-fill): q bf16 [batch, heads, seq, head_dim], out the same
  * shape in out_dtype; batch row b reads slot slots[b], its query i sees positions <= starts[b] + i
  * and < kv_len (kv_len <= max_len bounds what any row sees: pass the longest length when the host
  * knows it, else max_len).  A slot outside [0, num_slots) or a negative start gives zero rows;
@@ -395,7 +396,7 @@ CCUT_API int ccut_token_logprobs(const void* logits, int dtype, int rows, int vo
  * rank <= 256, inputs a multiple of 8; x, a, b, base, out and workspace 16-byte aligned.  The sums
  * over the inputs and the ranks are fp32, added to base before the one rounding to dtype.  Up to
  * 256 tokens, an adapter's weights are read once per 16 of its tokens; above that, tokens of one
- * adapter are best next to each other (the weights are read once per 16 neighbours). */
+ * adapter are best next to each other (the weights are read once per 64 neighbours). */
 #define CCUT_LORA_MAX_SLICES 4
 CCUT_API size_t ccut_lora_workspace_bytes(int tokens, int inputs, int rank, int slices, int adapters);
 CCUT_API int ccut_lora_add(const uint16_t* x, const uint16_t* a, const uint16_t* b, const float* scales,
