@@ -61,7 +61,7 @@ class _Seq:
     def __init__(self, cache: KvCache):
         self.cache = cache
         self.ids: list[int] = []
-        self.adapter: int | None = None  # the adapter the cached positions were computed with
+        self.adapter = None  # what the cached positions were computed with: (adapter, of which set), None for none
 
 
 class GenericBackend:
@@ -91,8 +91,9 @@ class GenericBackend:
         """The cache to run ``ids`` in (not one of ``taken``) and how many of its positions stay: those
         of a common prefix computed with the same adapter."""
         best, best_p = None, 0
+        key = None if adapter is None else (adapter, self.model.adapters_set)
         for s in self._seqs:
-            if any(s is t for t in taken) or s.adapter != adapter:
+            if any(s is t for t in taken) or s.adapter != key:
                 continue
             p = common_prefix(s.ids, ids)
             if p > best_p:
@@ -112,7 +113,7 @@ class GenericBackend:
         if any(best is s for s in self._seqs):
             self._seqs.remove(best)
         self._seqs.append(best)
-        best.adapter = adapter
+        best.adapter = key
         return best, reuse
 
     def _check(self, input_ids) -> list[int]:

@@ -562,6 +562,7 @@ class MoeDecoder:
         self.device = dev
         self.kv_dtype = "bf16"  # of new_cache / new_pool when they are given none
         self.num_adapters = self._count_adapters([getattr(lay, "adapters", {}) for lay in self.layers])
+        self.adapters_set = 0  # times that set_adapters changed what an index stands for
 
     @staticmethod
     def _count_adapters(per_layer: list) -> int:
@@ -579,6 +580,7 @@ class MoeDecoder:
             raise NotImplementedError("low-rank adapters of MLA layers")
         checked = [lay._check_adapters(banks) for lay, banks in zip(self.layers, per_layer)]
         self.num_adapters = self._count_adapters(checked)
+        self.adapters_set += 1
         for lay, banks in zip(self.layers, checked):
             lay.adapters = banks
 

@@ -174,6 +174,25 @@ def test_backend_keeps_adapters_apart(ops):
     assert be.score(prompt[:1]) == []
 
 
+def test_new_adapters_take_no_old_cache(ops):
+    """After ``set_adapters`` a cache of the old bank's adapter is not reused; one without an adapter is."""
+    from ccut_b200.backend import GenericBackend
+
+    t = make_tiny(8, kv_heads=2)
+    dec = _build(ops, t)
+    dec.set_adapters(banks(t, 2, 8, 2, "cpu"))
+    prompt = _prompts(t, (6,))[0]
+    be = GenericBackend(dec, max_seqs=3, max_len=16)
+    for a in (None, 0):
+        be.logits_for(prompt, a)
+    assert be.tokens_run == 12
+    dec.set_adapters(banks(t, 2, 8, 3, "cpu"))
+    got = be.logits_for(prompt, 0)
+    assert be.tokens_run == 18 and torch.equal(got, GenericBackend(dec, max_seqs=1, max_len=16).logits_for(prompt, 0))
+    be.logits_for(prompt)
+    assert be.tokens_run == 19
+
+
 def test_config_kv_cache_dtype():
     from ccut_b200 import config
     from tests.test_config import AWQ
