@@ -110,7 +110,7 @@ class LoraBank:
             out = torch.empty_like(base, memory_format=torch.contiguous_format)
         elif out.dtype != base.dtype or out.shape != base.shape or out.device != base.device or not _rows_ok(out):
             raise ValueError("out must be like base, its rows contiguous and 16-byte aligned")
-        base = base if _rows_ok(base) else base.contiguous()
+        base = base if _rows_ok(base) else base.clone(memory_format=torch.contiguous_format)
         x = x if x.is_contiguous() and x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
         ids = ids if ids.is_contiguous() else ids.contiguous()
         nbytes = _lib.load().ccut_lora_workspace_bytes(n, self.inputs, self.rank, len(self.widths), self.adapters)

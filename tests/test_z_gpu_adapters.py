@@ -147,3 +147,38 @@ def test_bank_from_checkpoint_matrices():
                 A, B = (m.astype(np.float64) for m in mats[i][j])
                 ref[t, at: at + widths[j]] += scale * (B @ (A @ x[t]))
     np.testing.assert_allclose(got, ref, rtol=1e-5, atol=1e-4)
+
+
+@pytest.mark.parametrize("tokens, inputs, rank, widths, adapters, dtype", [
+    (300, 200, 64, [264, 72], 3, torch.float32), (513, 128, 32, [136, 40, 88], 4, torch.bfloat16),
+    (700, 512, 64, [520], 2, torch.bfloat16), (259, 64, 96, [200, 8], 2, torch.float32),
+    (321, 1032, 32, [8, 24, 16, 200], 1, torch.float32), (400, 256, 64, [24, 104, 8, 248], 5, torch.bfloat16),
+])
+def test_prompts_match_oracle(tokens, inputs, rank, widths, adapters, dtype):
+    """More tokens than a decode step: every rank class, blocks of outputs that hold several parts."""
+    rng = np.random.default_rng(tokens + rank)
+    x, a, b, s, base = _inputs(rng, tokens, inputs, rank, widths, adapters, dtype)
+    bank = _bank(a, b, s, widths)
+    xd, bd = torch.from_numpy(x).cuda().bfloat16(), torch.from_numpy(base).cuda().to(dtype)
+    for ids in (rng.integers(-1, adapters, tokens), np.sort(rng.integers(0, adapters, tokens)), np.full(tokens, -1)):
+        ids = ids.astype(np.int32)
+        ref = serving.lora_add(base, x, a, b, s, ids, widths)
+        got = bank.add(bd, xd, torch.from_numpy(ids).cuda()).float().cpu().numpy()
+        assert (np.abs(got - ref) <= _tol(ref, x, a, b, s, ids, widths, dtype)).all()
+
+
+def test_misaligned_inputs():
+    """Contiguous tensors that begin off a 16-byte boundary are taken all the same."""
+    rng = np.random.default_rng(8)
+    x, a, b, s, base = _inputs(rng, 5, 64, 16, [24], 2, torch.bfloat16)
+    bank, ids = _bank(a, b, s, [24]), torch.tensor([0, 1, -1, 1, 0], dtype=torch.int32, device="cuda")
+    xd, bd = torch.from_numpy(x).cuda().bfloat16(), torch.from_numpy(base).cuda().bfloat16()
+
+    def shifted(t):
+        flat = torch.zeros(t.numel() + 8, dtype=t.dtype, device="cuda")
+        flat[1: 1 + t.numel()] = t.reshape(-1)
+        return flat[1: 1 + t.numel()].view(t.shape)
+
+    assert torch.equal(bank.add(shifted(bd), shifted(xd), shifted(ids)), bank.add(bd, xd, ids))
+    with pytest.raises(ValueError):
+        bank.add(bd, xd, ids, out=shifted(bd))
