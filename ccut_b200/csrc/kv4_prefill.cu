@@ -53,7 +53,7 @@ struct PfSmem {
 };
 
 struct PfBars {
-  uint64_t q_full[2], kv_full[8], kv_empty[8], s_full[2], s_free[2], p_half[2], p_full[2], o_full[2];
+  uint64_t q_raw[2], q_full[2], kv_full[8], kv_empty[8], s_full[2], s_free[2], p_half[2], p_full[2], o_full[2];
   uint32_t tmem;
   int failed;
 };
@@ -204,6 +204,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.q_raw[i], kPfRows);
       mbar_init(&bars.q_full[i], kPfRows);
       mbar_init(&bars.s_full[i], 1);
       mbar_init(&bars.s_free[i], kPfRows);
@@ -377,14 +378,28 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_addr = s_col(i) + lanes, p_addr = p_col(i) + lanes, o_addr = o_col(i) + lanes;
     const int lim = live ? start + my_s : a.kv_len;  // last visible position
-    // the row of q as fp16, scaled by a power of two, into the swizzled tile
+    // The row of q comes by a bulk copy (16-byte loads, each lane in its own row, took 3000 cycles more) and goes back
+    // as fp16, scaled by a power of two, into the swizzled tile.  The thread's 16-byte pieces are taken in an order
+    // c ^ turn, in which eight threads meet every bank once both in the plain rows and in the swizzled ones: turn is
+    // a linear map of tr & 7 over GF(2) (times x in GF(8)) for which turn and turn ^ tr are both one to one.
     float fr = 0.f;
+    bool ok = true;
     if (n > 0) {
+      uint8_t* const tile = q_s + i * SM::kTileBytes;
+      if (live) {
+        mbar_arrive_expect_tx(&bars.q_raw[i], D * 2);
+        bulk_g2s(tile + tr * (D * 2), a.q + (size_t)row * D, D * 2, &bars.q_raw[i]);
+      } else {
+        mbar_arrive(&bars.q_raw[i]);
+      }
+      ok = wait(&bars.q_raw[i], 0);
+      ok = !__any_sync(0xffffffffu, !ok);
+      const int turn = ((tr << 1) & 7) ^ (tr & 4 ? 3 : 0);
       uint4 u[D / 8];
       float mx = 0.f;
 #pragma unroll
       for (int c = 0; c < D / 8; ++c) {
-        u[c] = live ? *reinterpret_cast<const uint4*>(a.q + (size_t)row * D + c * 8) : make_uint4(0, 0, 0, 0);
+        u[c] = live ? *reinterpret_cast<const uint4*>(tile + tr * (D * 2) + ((c ^ turn) << 4)) : make_uint4(0, 0, 0, 0);
         const uint32_t w[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -393,7 +408,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       const int ex = min(max((int)((__float_as_uint(mx) >> 23) & 255) - 126, -90), 90);  // |q| 2^-ex in [1/2, 1)
       const float f = __int_as_float((127 - ex) << 23);
       fr = __int_as_float((127 + ex) << 23) * (a.scale * kPfLog2e);
-      uint8_t* dst = q_s + i * SM::kTileBytes + tr * 128;
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");  // the tile's rows are all in registers
 #pragma unroll
       for (int c = 0; c < D / 8; ++c) {
         const uint32_t w[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
@@ -403,13 +418,13 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           const __half2 h = __floats2half2_rn(__uint_as_float(w[e] << 16) * f, __uint_as_float(w[e] & 0xFFFF0000u) * f);
           o[e] = *reinterpret_cast<const uint32_t*>(&h);
         }
-        *reinterpret_cast<uint4*>(dst + (c >> 3) * kSub + (((c & 7) ^ (tr & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+        const int k = c ^ turn;
+        *reinterpret_cast<uint4*>(tile + (k >> 3) * kSub + tr * 128 + (((k ^ tr) & 7) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
       }
       tc::fence_proxy_async_smem();
       mbar_arrive(&bars.q_full[i]);
     }
     float m = -INFINITY, l = 0.f;
-    bool ok = true;
     for (int j = 0; ok && j < n; ++j) {
       ok = wait(&bars.s_full[i], j & 1);
       ok = !__any_sync(0xffffffffu, !ok);
@@ -504,6 +519,9 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     ok = !__any_sync(0xffffffffu, !ok);
     tc::fence_after_sync();
     const float inv = l == 0.f ? 0.f : 1.f / l;
+    // a row of bf16 outputs, rows 16 bytes more than their size apart: tile 0's in the place of the query tiles (every S
+    // was issued before its last product), tile 1's behind them, where nothing is left to be read
+    uint8_t* const mine = q_s + (i * kPfRows + tr) * (D * 2 + 16);
 #pragma unroll
     for (int c = 0; c < D; c += 32) {
       uint32_t y[32];
@@ -522,7 +540,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         if (c == 0) p[0] = m, p[1] = l;
 #pragma unroll
         for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(p + 4 + c + e) = make_uint4(y[e], y[e + 1], y[e + 2], y[e + 3]);
-      } else if constexpr (OUT_BF16) {
+      } else if constexpr (OUT_BF16) {  // by a bulk copy of the row from shared memory, as above
 #pragma unroll
         for (int e = 0; e < 32; e += 8) {
           uint32_t o[4];
@@ -531,7 +549,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
             const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(y[e + 2 * q]) * inv, __uint_as_float(y[e + 2 * q + 1]) * inv);
             o[q] = *reinterpret_cast<const uint32_t*>(&h);
           }
-          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (size_t)row * D + c + e) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(mine + (c + e) * 2) = make_uint4(o[0], o[1], o[2], o[3]);
         }
       } else {
 #pragma unroll
@@ -539,6 +557,15 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           *reinterpret_cast<float4*>(static_cast<float*>(a.out) + (size_t)row * D + c + e) =
               make_float4(__uint_as_float(y[e]) * inv, __uint_as_float(y[e + 1]) * inv, __uint_as_float(y[e + 2]) * inv,
                           __uint_as_float(y[e + 3]) * inv);
+      }
+    }
+    if constexpr (OUT_BF16) {
+      if (live && a.splits == 1) {
+        tc::fence_proxy_async_smem();
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n\tcp.async.bulk.commit_group;\n\t"
+                     "cp.async.bulk.wait_group.read 0;" ::"l"(static_cast<uint16_t*>(a.out) + (size_t)row * D),
+                     "r"(smem_u32(mine)), "r"(D * 2)
+                     : "memory");
       }
     }
     tc::fence_before_sync();
