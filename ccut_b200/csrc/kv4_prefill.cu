@@ -378,20 +378,24 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_addr = s_col(i) + lanes, p_addr = p_col(i) + lanes, o_addr = o_col(i) + lanes;
     const int lim = live ? start + my_s : a.kv_len;  // last visible position
-    // The row of q comes by a bulk copy (16-byte loads, each lane in its own row, took 3000 cycles more) and goes back
-    // as fp16, scaled by a power of two, into the swizzled tile.  The thread's 16-byte pieces are taken in an order
-    // c ^ turn, in which eight threads meet every bank once both in the plain rows and in the swizzled ones: turn is
-    // a linear map of tr & 7 over GF(2) (times x in GF(8)) for which turn and turn ^ tr are both one to one.
+    // The tile's rows of q come by one bulk copy per head, whose rows are neighbours (16-byte loads, each lane in its
+    // own row, took 2000 cycles a CTA more); the heads follow one another from the first row's.  A thread takes its row
+    // and writes it back as fp16, scaled by a power of two, into the swizzled tile, its 16-byte pieces in an order c ^
+    // turn in which eight threads meet every bank once both in the plain rows and in the swizzled ones: turn is a
+    // linear map of tr & 7 over GF(2) (times x in GF(8)) for which turn and turn ^ tr are both one to one.
     float fr = 0.f;
     bool ok = true;
     if (n > 0) {
       uint8_t* const tile = q_s + i * SM::kTileBytes;
-      if (live) {
-        mbar_arrive_expect_tx(&bars.q_raw[i], D * 2);
-        bulk_g2s(tile + tr * (D * 2), a.q + (size_t)row * D, D * 2, &bars.q_raw[i]);
+      const int have = min(kPfRows, nrows - (r0 + i * kPfRows)), each = have / grp, more = have % grp;
+      if (tr < min(grp, have)) {  // my_r is the first row of its head
+        const int bytes = ((have - 1 - tr) / grp + 1) * D * 2;
+        mbar_arrive_expect_tx(&bars.q_raw[i], bytes);
+        bulk_g2s(tile + (tr * each + min(tr, more)) * (D * 2), a.q + (size_t)row * D, bytes, &bars.q_raw[i]);
       } else {
         mbar_arrive(&bars.q_raw[i]);
       }
+      const uint8_t* const mine = tile + (tr % grp * each + min(tr % grp, more) + tr / grp) * (D * 2);
       ok = wait(&bars.q_raw[i], 0);
       ok = !__any_sync(0xffffffffu, !ok);
       const int turn = ((tr << 1) & 7) ^ (tr & 4 ? 3 : 0);
@@ -399,7 +403,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       float mx = 0.f;
 #pragma unroll
       for (int c = 0; c < D / 8; ++c) {
-        u[c] = live ? *reinterpret_cast<const uint4*>(tile + tr * (D * 2) + ((c ^ turn) << 4)) : make_uint4(0, 0, 0, 0);
+        u[c] = live ? *reinterpret_cast<const uint4*>(mine + ((c ^ turn) << 4)) : make_uint4(0, 0, 0, 0);
         const uint32_t w[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e)
