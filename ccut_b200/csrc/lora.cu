@@ -240,9 +240,8 @@ __global__ void __launch_bounds__(kLoraWarps * 32) lora_shrink_kernel(const __gr
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int R = p.slices * p.rank, r0 = blockIdx.z * kLoraRankTiles * 8;
   const int nz = min(kLoraRankTiles, (R - r0) / 8), t0 = blockIdx.x * kLoraRows;
-  lora_neighbours(p, t0, rows);
   const int k0 = blockIdx.y * p.k_per_split, k1 = min(p.inputs, k0 + p.k_per_split);
-  const int steps = k1 > k0 ? (k1 - k0 + kLoraStep - 1) / kLoraStep : 0, total = steps * rows.n;
+  const int steps = k1 > k0 ? (k1 - k0 + kLoraStep - 1) / kLoraStep : 0;
   // copies of a stage: thread -> 16-byte chunk tid % 8 of rows tid / 8, + 16, + 32, + 48 of x and of A; the
   // addresses move from stage to stage and back at the next adapter
   const int cr = threadIdx.x >> 3, cc = threadIdx.x & 7;
@@ -253,20 +252,30 @@ __global__ void __launch_bounds__(kLoraWarps * 32) lora_shrink_kernel(const __gr
   const uint16_t* wa = nullptr;
   const int xrows = (p.tokens - t0 - cr + 15) / 16, wrows = (nz * 8 - cr + 15) / 16;  // of the four, those that exist
   const uint32_t to = smem_u32(ring) + lora_chunk(cr, cc);  // rows 16 apart: the same place, 2048 bytes on
-  auto issue = [&]() {
-    if (fetch_step == 0) wa = p.a + ((size_t)rows.uniq[fetch_adapter] * R + r0 + min(cr, nz * 8 - 1)) * p.inputs;
-    const bool in = fetch_k < k1;
-    const uint32_t st = to + fetch_stage * kLoraStageBytes;
+  auto issue_x = [&](int stage, int k) {
 #pragma unroll
     for (int i = 0; i < kLoraRows / 16; ++i) {
-      const bool xin = in && i < xrows, win = in && i < wrows;
-      lora_copy(st + i * 2048, xin ? xa + i * hop + fetch_k : p.x, xin);
-      lora_copy(st + kLoraRows * 128 + i * 2048, win ? wa + i * hop + fetch_k : p.x, win);
+      const bool in = k < k1 && i < xrows;
+      lora_copy(to + stage * kLoraStageBytes + i * 2048, in ? xa + i * hop + k : p.x, in);
+    }
+  };
+  auto issue = [&](bool with_x) {
+    if (fetch_step == 0) wa = p.a + ((size_t)rows.uniq[fetch_adapter] * R + r0 + min(cr, nz * 8 - 1)) * p.inputs;
+    if (with_x) issue_x(fetch_stage, fetch_k);
+#pragma unroll
+    for (int i = 0; i < kLoraRows / 16; ++i) {
+      const bool in = fetch_k < k1 && i < wrows;
+      lora_copy(to + fetch_stage * kLoraStageBytes + kLoraRows * 128 + i * 2048, in ? wa + i * hop + fetch_k : p.x, in);
     }
     fetch_k += kLoraStep;
     if (++fetch_stage == kLoraStages) fetch_stage = 0;
     if (++fetch_step == steps) fetch_step = 0, ++fetch_adapter, fetch_k = first_k;
   };
+#pragma unroll
+  for (int i = 0; i < kLoraStages - 1; ++i)
+    if (i < steps) issue_x(i, first_k + i * kLoraStep);  // on its way during the lookup
+  lora_neighbours(p, t0, rows);
+  const int total = steps * rows.n;
   float keep[kLoraRankTiles][4], acc[kLoraRankTiles][4];
 #pragma unroll
   for (int n = 0; n < kLoraRankTiles; ++n)
@@ -275,14 +284,14 @@ __global__ void __launch_bounds__(kLoraWarps * 32) lora_shrink_kernel(const __gr
   const int id0 = rows.ids[warp * kLoraTile + g], id1 = rows.ids[warp * kLoraTile + g + 8];
 #pragma unroll
   for (int i = 0; i < kLoraStages - 1; ++i) {
-    if (i < total) issue();
+    if (i < total) issue(i >= steps);
     cp_async_commit();
   }
   int step = 0, adapter = 0, stage = 0;
   for (int s = 0; s < total; ++s) {
     cp_async_wait<kLoraStages - 2>();
     __syncthreads();  // everyone's copies of this stage have landed, everyone is done with the stage before
-    if (s + kLoraStages - 1 < total) issue();
+    if (s + kLoraStages - 1 < total) issue(true);
     cp_async_commit();
     const uint8_t* st = ring + stage * kLoraStageBytes;
     if (++stage == kLoraStages) stage = 0;
@@ -510,14 +519,12 @@ __global__ void __launch_bounds__(kLoraWarps * 32) lora_expand_group_kernel(cons
 // Where output r of a block lies in shared memory: column n of n-tile i at 16-block + 8 i + n.
 CCUT_DEVICE int lora_place(int r) { return (r & ~15) + ((r >> 1) & 1) * 8 + ((r >> 2) & 3) * 2 + (r & 1); }
 
-// Prompts.  Grid (tiles of 64 tokens, blocks of 128 outputs): base and h are on their way while the adapters are
-// looked up, the adapter's rows of B next; warp w has tokens 16 w .. and all the outputs.  KR: rank / 16, or
+// Prompts.  Grid (tiles of 64 tokens, blocks of 128 outputs): base is on its way while the adapters are looked up,
+// the adapter's rows of B next, all before the wait for h; warp w has tokens 16 w .. and all the outputs.  KR: rank / 16, or
 // 0 for any.
 template <int KR, bool OUT_BF16>
 __global__ void __launch_bounds__(kLoraWarps * 32, OUT_BF16 ? 4 : 3)
     lora_expand_kernel(const __grid_constant__ LoraArgs p) {
-  pdl_wait();
-  pdl_trigger();
   constexpr int kParts = OUT_BF16 ? 2 : 3, kBlocks = kLoraOutputs / 16;
   using Four = LoraFour<OUT_BF16>;
   __shared__ LoraRows rows;
@@ -548,7 +555,6 @@ __global__ void __launch_bounds__(kLoraWarps * 32, OUT_BF16 ? 4 : 3)
                       : make_float4(0.f, 0.f, 0.f, 0.f);
   };
   int slice = kRegs ? lora_slice(p, o0) : 0;  // whose h is in registers
-  load_h(slice * KR);
   constexpr int kHop = kLoraWarps * 32 / kChunks;  // rows that the CTA moves at a time
   const int mr = threadIdx.x / kChunks, mc = threadIdx.x % kChunks;
   const bool mine = mc < width * kSize / 16;  // widths are multiples of 8: whole chunks
@@ -574,6 +580,9 @@ __global__ void __launch_bounds__(kLoraWarps * 32, OUT_BF16 ? 4 : 3)
     cp_async_commit();
   };
   if (rows.n > 0) fetch_b(rows.uniq[0]);
+  pdl_wait();  // base, ids and B were there before the shrink kernel began; h is what it makes
+  pdl_trigger();
+  load_h(slice * KR);
   const int id0 = rows.ids[warp * kLoraTile + g], id1 = rows.ids[warp * kLoraTile + g + 8];
   const float f0 = id0 >= 0 ? p.scales[id0] : 0.f, f1 = id1 >= 0 ? p.scales[id1] : 0.f;
   uint32_t hf[kRegs ? KR : 1][kParts][4];
@@ -749,8 +758,14 @@ static int run_lora_prompt(const LoraArgs& p, cudaStream_t st) {
   rc = ensure_smem_limit(kern, smem(kLoraMaxRanks, kLoraMaxRanks),
                          expand_set[p.rank == 16 ? 0 : p.rank == 32 ? 1 : p.rank == 64 ? 2 : 3]);
   if (rc) return rc;
-  return launch_k(kern, dim3(tiles, (p.outputs + kLoraOutputs - 1) / kLoraOutputs), dim3(kLoraWarps * 32),
-                  smem(R, p.rank), st, p);
+  // begun while the shrink kernel runs, whatever the call's size: that was launched without the attribute, so all that
+  // is read before the wait is complete
+  const bool on = g_pdl_on;
+  g_pdl_on = pdl_enabled();
+  rc = launch_k(kern, dim3(tiles, (p.outputs + kLoraOutputs - 1) / kLoraOutputs), dim3(kLoraWarps * 32),
+                smem(R, p.rank), st, p);
+  g_pdl_on = on;
+  return rc;
 }
 
 }  // namespace ccut
