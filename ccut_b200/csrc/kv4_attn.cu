@@ -32,8 +32,9 @@
 //   Equal chunks per sequence cost a prologue, a reduction and a partial result every chunk instead (one
 //   sequence of 131071 positions, when this was changed: 54 us in chunks, 22 in spans).
 // Measured (8 query heads per kv head, d = 128): 64 sequences of 3001..8191 positions 50 us, 4.1 TB/s of codes
-// and params (0.64 of a copy's rate); what is left is the instructions, 0.8 issued of 1 a cycle.  One
-// sequence of 131071: 13 us in two launches.  One of 513: 8.5 us, latency.
+// and params (0.64 of a copy's rate); the schedulers issue in 0.55 of the cycles, three warps each in chains of
+// dependent instructions (four, at 128 registers: 53 us).  One sequence of 131071: 13 us in two launches.
+// One of 513: 8.5 us, latency.
 // Roundings to fp16: q, scaled to its row's largest element (2^-35 of it is kept), and sum q_g (2^-15
 // of the largest element); p s_v, scaled by the row's power of two R that brings the largest v scale it has
 // seen to [1/2, 1) (11 bits, and 2^-25 of the largest absolutely; with fp32 output a second fp16 part

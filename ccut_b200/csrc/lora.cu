@@ -18,8 +18,8 @@
 //   prompt).  A row takes the result of its own adapter by selection, so nothing of another request's
 //   adapter (a NaN weight, say) reaches it.  x and A stream through a cp.async ring; the inputs are split
 //   over a cluster of up to 8 CTAs whose sums meet in distributed shared memory, in rank order.  Bound: HBM (x, base
-//   and out).  4093 tokens, rank 64, 4096 inputs, 2048 bf16 outputs: 46 us, 1.5 TB/s
-//   (18 + 25: a CTA's few stages are mostly their latency, three CTAs an SM for its tiles in shared memory).
+//   and out).  4093 tokens, rank 64, 4096 inputs, 2048 bf16 outputs: 38 us, 1.8 TB/s
+//   (18 + 20: a CTA's few stages are mostly their latency).
 // The outputs of two n-tiles interleave so that a lane holds four neighbours.
 #include <type_traits>
 
