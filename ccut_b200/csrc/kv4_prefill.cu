@@ -13,9 +13,15 @@
 //   S_i = Q_i K^T, then O_i += P_i V with P_i read from tensor memory, where it takes the place of S_i.
 // - two warpgroups of softmax threads, one row a thread: S to registers, running maximum, exponentials, P
 //   back as fp16.  While one tile's scores are worked on, the tensor cores run the other's products.
-// - The maximum moves only when a score passes it by 2^8, so O is rescaled a few times per row and not every
-//   tile (probabilities up to 2^8 fit fp16); when it moves, the O of the earlier tiles is complete, since
+// - The maximum moves only when a score of the row passes it by 2^8, so O is rescaled a few times per row and not
+//   every tile (probabilities up to 2^8 fit fp16); when it moves, the O of the earlier tiles is complete, since
 //   S_i of a tile is issued behind P_i V of the one before.
+// - With 64 features P has columns of its own: S_i of the next tile is computed while the softmax of this one
+//   runs (4096 rows: 118 us, 134 in turn).  With 128 tensor memory is full, and a softmax warp waits 1400 of
+//   the 3300 cycles of a step; tiles of 64 positions with two score buffers took 185 us for 158, since the
+//   query operand is then read twice as often.
+// Measured, 32 heads on 4 kv heads: 4096 rows from position 0, d = 128, 145 us (0.95 PFLOP/s of visible
+// products), 8192 rows 494 us (1.11); d = 64 118 us.
 // Roundings: q to fp16 after scaling its row's largest element to [1/2, 1) (11 bits of it, 2^-25 of the
 // largest), k and v above, P 11 bits; scores, maximum, sums and O are fp32.
 #include <math.h>
