@@ -114,10 +114,10 @@ class LoraBank:
         x = x if x.is_contiguous() and x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
         ids = ids if ids.is_contiguous() else ids.contiguous()
         nbytes = _lib.load().ccut_lora_workspace_bytes(n, self.inputs, self.rank, len(self.widths), self.adapters)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
         _run(self.device, "ccut_lora_add", x.data_ptr(), self.a.data_ptr(), self.b.data_ptr(), self.scales.data_ptr(),
              ids.data_ptr(), n, self.inputs, self.rank, self.adapters, len(self.widths), self._widths, base.data_ptr(),
-             base.stride(0), out.data_ptr(), out.stride(0), _DTYPES[base.dtype], ws.data_ptr(), nbytes)
+             base.stride(0), out.data_ptr(), out.stride(0), _DTYPES[base.dtype], ws.data_ptr() if nbytes else None, nbytes)
         return out
 
 

@@ -461,19 +461,7 @@ static int run_logprobs(const LpArgs& a, cudaStream_t st) {
   static std::atomic<uint64_t> wide_set{0};  // devices on which clusters of more than 8 are allowed
   int rc = ensure_attribute(logprobs_kernel<BF16, TOP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1, wide_set);
   if (rc) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = a.ctas;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = g_pdl_on ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, logprobs_kernel<BF16, TOP>, a) == cudaSuccess ? CCUT_OK : CCUT_ERR_CUDA;
+  return launch_cluster(logprobs_kernel<BF16, TOP>, grid, block, 0, st, a.ctas, a);
 }
 
 }  // namespace ccut

@@ -4,18 +4,17 @@
 // where j(o) is the slice (q, k or v of a fused projection, say) that output o belongs to; a row whose
 // id is outside [0, adapters) keeps its base.
 //
-// Two launches: a shrink kernel gives h[t, slices * rank] = A x of the rows with their adapters (in parts over
-// the inputs), lora_expand_* scales h, multiplies by B and adds the base.  Products are m16n8k16 bf16 MMAs
-// with 16 tokens as the M, in one of two ways:
-// - Up to kLoraGroupTokens tokens (a decode step), a CTA takes up to 16 tokens of ONE adapter, wherever they
-//   are in the batch: every CTA sorts the few ids itself (each token's rank among its own), so that an
-//   adapter's weights are read once however the requests mix, and all adapters at the same time.  Bound:
-//   latency.  The four warps split the inputs; operands come straight from global memory (the order of
-//   the k index of an MMA is free: a lane's operand registers are 16 consecutive bytes of a row of x or A).
-//   The expand kernel looks its unit up and fetches B and base before it waits for the shrink kernel.
-//   64 tokens, 16 adapters of rank 16, 2048 inputs, 5120 outputs: 15 us.
-// - More tokens (prompts): a CTA takes 64 neighbours and loops over their distinct adapters (one, inside a
-//   prompt).  A row takes the result of its own adapter by selection, so nothing of another request's
+// Products are m16n8k16 bf16 MMAs with 16 tokens as the M, in one of two ways:
+// - Up to kLoraGroupTokens tokens (a decode step), one launch: a cluster takes up to 16 tokens of ONE adapter,
+//   wherever they are in the batch: every CTA sorts the few ids itself (each token's rank among its own), so that
+//   an adapter's weights are read once however the requests mix, and all adapters at the same time.  Bound:
+//   latency.  The CTAs and warps split the inputs, add up h through distributed shared memory and then split
+//   the outputs; operands come straight from global memory (the order of the k index of an MMA is free: a
+//   lane's operand registers are 16 consecutive bytes of a row of x or A).
+//   64 tokens, 16 adapters of rank 16, 2048 inputs, 5120 outputs: TIME_STEP (15 us in two kernels).
+// - More tokens (prompts), two launches: a shrink kernel gives h[t, slices * rank] = A x, the expand kernel scales it,
+//   multiplies by B and adds the base.  A CTA takes 64 neighbours and loops over their distinct adapters (one,
+//   inside a prompt).  A row takes the result of its own adapter by selection, so nothing of another request's
 //   adapter (a NaN weight, say) reaches it.  x and A stream through a cp.async ring; the inputs are split
 //   over a cluster of up to 8 CTAs whose sums meet in distributed shared memory, in rank order.  Bound: HBM (x, base
 //   and out).  4093 tokens, rank 64, 4096 inputs, 2048 bf16 outputs: 38 us, 1.8 TB/s
@@ -150,79 +149,14 @@ CCUT_DEVICE void lora_neighbours(const LoraArgs& p, int t0, LoraRows& rows) {
   __syncthreads();
 }
 
-// Decode steps.  Grid (units, splits, blocks of 64 rank rows).
-__global__ void __launch_bounds__(kLoraWarps * 32) lora_shrink_group_kernel(const __grid_constant__ LoraArgs p) {
-  pdl_wait();
-  pdl_trigger();
-  __shared__ LoraTile tile;
-  __shared__ __align__(16) int ids[kLoraGroupTokens];
-  __shared__ int counts[kLoraGroupTokens / 32];
-  __shared__ float red[kLoraWarps - 1][32][kLoraRankTiles * 4 + 1];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int R = p.slices * p.rank, r0 = blockIdx.z * kLoraRankTiles * 8;
-  const int nz = min(kLoraRankTiles, (R - r0) / 8);
-  if (!lora_group(p, blockIdx.x, tile, ids, counts)) return;
-  const int a = tile.uniq[0];
-  if (a < 0) return;
-  const int per = p.k_per_split / kLoraWarps;  // a multiple of 32
-  const int k0 = blockIdx.y * p.k_per_split + warp * per, k1 = min(p.inputs, k0 + per);
-  const int row0 = tile.rows[g], row1 = tile.rows[g + 8];
-  const uint16_t* x0 = p.x + (size_t)max(row0, 0) * p.inputs;
-  const uint16_t* x1 = p.x + (size_t)max(row1, 0) * p.inputs;
-  const uint16_t* ar = p.a + ((size_t)a * R + r0 + g) * p.inputs;
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  float acc[kLoraRankTiles][4];
-#pragma unroll
-  for (int n = 0; n < kLoraRankTiles; ++n)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
-  // 32 inputs a step: lane t holds inputs k + 8 t .. + 7 of its rows
-#pragma unroll 2
-  for (int k = k0; k < k1; k += 32) {
-    const int kk = k + 8 * t;
-    const bool in = kk < k1;
-    const uint4 v0 = in && row0 >= 0 ? __ldg(reinterpret_cast<const uint4*>(x0 + kk)) : zero;
-    const uint4 v1 = in && row1 >= 0 ? __ldg(reinterpret_cast<const uint4*>(x1 + kk)) : zero;
-    uint4 w[kLoraRankTiles];
-#pragma unroll
-    for (int n = 0; n < kLoraRankTiles; ++n)
-      w[n] = in && n < nz ? __ldg(reinterpret_cast<const uint4*>(ar + (size_t)n * 8 * p.inputs + kk)) : zero;
-    const uint32_t f0[4] = {v0.x, v1.x, v0.y, v1.y}, f1[4] = {v0.z, v1.z, v0.w, v1.w};
-#pragma unroll
-    for (int n = 0; n < kLoraRankTiles; ++n)
-      if (n < nz) {
-        mma_16816<true>(acc[n], f0, w[n].x, w[n].y);
-        mma_16816<true>(acc[n], f1, w[n].z, w[n].w);
-      }
-  }
-  if (warp > 0) {  // the warps' sums, in warp order
-#pragma unroll
-    for (int n = 0; n < kLoraRankTiles; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) red[warp - 1][lane][n * 4 + i] = acc[n][i];
-  }
-  __syncthreads();
-  if (warp > 0) return;
-#pragma unroll
-  for (int w = 0; w < kLoraWarps - 1; ++w)
-#pragma unroll
-    for (int n = 0; n < kLoraRankTiles; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[n][i] += red[w][lane][n * 4 + i];
-  float* h = p.part + (size_t)blockIdx.y * p.tokens * R + r0 + 2 * t;
-#pragma unroll
-  for (int n = 0; n < kLoraRankTiles; ++n)
-    if (n < nz) {
-      if (row0 >= 0) *reinterpret_cast<float2*>(h + (size_t)row0 * R + n * 8) = make_float2(acc[n][0], acc[n][1]);
-      if (row1 >= 0) *reinterpret_cast<float2*>(h + (size_t)row1 * R + n * 8) = make_float2(acc[n][2], acc[n][3]);
-    }
-}
-
 // Byte offset of 16-byte chunk c of row r in a tile of 128-byte rows: ldmatrix reads 8 rows of one chunk without
 // meeting a bank twice.
 CCUT_DEVICE int lora_chunk(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
 CCUT_DEVICE void lora_copy(uint32_t to, const void* from, bool in) {  // 16 bytes, zeros when !in
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(in ? 16 : 0) : "memory");
+}
+CCUT_DEVICE void st_cluster(uint32_t addr, const float4& v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 CCUT_DEVICE float4 ld_cluster(uint32_t addr) {
   float4 v;
@@ -414,104 +348,190 @@ CCUT_DEVICE int lora_slice(const LoraArgs& p, int o) {
   return j;
 }
 
-// Decode steps.  Grid (units, blocks of 128 outputs): warp w takes 32 outputs, in blocks of 8 x 2 (columns n of
-// n-tile i: output 4 (n / 2) + 2 i + n % 2 of 16; slices end at multiples of 8, so a block of 16 has one or two).
+// Decode steps.  Grid (C, units), a cluster of C = p.splits CTAs per unit.  The CTAs split the inputs; their sums of h
+// meet in every CTA through distributed shared memory, in rank order, and the warps of the cluster then take the
+// outputs in turn, in blocks of 8 x 2 (column n of n-tile i: output 4 (n / 2) + 2 i + n % 2 of 16; slices end at
+// multiples of 8, so a block of 16 has one or two).
+__host__ __device__ constexpr int lora_hp_ld(int R) { return R + 4; }
+__host__ __device__ constexpr size_t lora_group_smem(int R, int parts) {
+  const size_t planes = (size_t)parts * kLoraTile * lora_ld(R) * 2, red = (size_t)(kLoraWarps - 1) * 32 * (kLoraRankTiles * 4 + 1) * 4;
+  return (size_t)kLoraTile * lora_hp_ld(R) * 4 + (planes > red ? planes : red);
+}
 template <bool OUT_BF16>
-__global__ void __launch_bounds__(kLoraWarps * 32) lora_expand_group_kernel(const __grid_constant__ LoraArgs p) {
-  constexpr int kParts = OUT_BF16 ? 2 : 3, kBlocks = kLoraOutputs / kLoraWarps / 16, kFetch = 2;
+__global__ void __launch_bounds__(kLoraWarps * 32) lora_group_kernel(const __grid_constant__ LoraArgs p) {
+  pdl_wait();
+  pdl_trigger();
+  constexpr int kParts = OUT_BF16 ? 2 : 3, kBlocks = 2, kFetch = 4;
   using Four = LoraFour<OUT_BF16>;
   __shared__ LoraTile tile;
   __shared__ __align__(16) int ids[kLoraGroupTokens];
   __shared__ int counts[kLoraGroupTokens / 32];
-  extern __shared__ __align__(16) uint16_t hs[];  // [parts][16][lora_ld(R)]
+  extern __shared__ __align__(16) float hp[];  // [16][R + 4] this CTA's sums; then the warps' sums, later the planes of h
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int R = p.slices * p.rank, ld = lora_ld(R);
+  const int R = p.slices * p.rank, ld = lora_ld(R), hld = lora_hp_ld(R), part = blockIdx.x;
   const size_t plane = (size_t)kLoraTile * ld;
-  const int o0 = blockIdx.y * kLoraOutputs + warp * (kLoraOutputs / kLoraWarps);
-  const bool unit = lora_group(p, blockIdx.x, tile, ids, counts);
-  const int a = unit ? tile.uniq[0] : -1;
-  const int row0 = unit ? tile.rows[g] : -1, row1 = unit ? tile.rows[g + 8] : -1;
-  // base, and the first two k steps of B, while the shrink kernel still runs
+  float(*red)[32][kLoraRankTiles * 4 + 1] = reinterpret_cast<float(*)[32][kLoraRankTiles * 4 + 1]>(hp + kLoraTile * hld);
+  uint16_t* hs = reinterpret_cast<uint16_t*>(hp + kLoraTile * hld);  // [parts][16][lora_ld(R)]
+  if (!lora_group(p, blockIdx.y, tile, ids, counts)) return;  // the same for the whole cluster, as the next
+  const int a = tile.uniq[0];
+  if (a < 0 && p.base == p.out) return;  // in place: rows without an adapter stay
+  const int row0 = tile.rows[g], row1 = tile.rows[g + 8];
+
+  if (a >= 0) {  // h of this CTA's inputs
+    const int per = p.k_per_split / kLoraWarps;  // a multiple of 32
+    const int k0 = part * p.k_per_split + warp * per, k1 = min(p.inputs, k0 + per);
+    const uint16_t* x0 = p.x + (size_t)max(row0, 0) * p.inputs;
+    const uint16_t* x1 = p.x + (size_t)max(row1, 0) * p.inputs;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    for (int r0 = 0; r0 < R; r0 += kLoraRankTiles * 8) {
+      const int nz = min(kLoraRankTiles, (R - r0) / 8);
+      const uint16_t* ar = p.a + ((size_t)a * R + r0 + g) * p.inputs;
+      float acc[kLoraRankTiles][4];
+#pragma unroll
+      for (int n = 0; n < kLoraRankTiles; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+      // 32 inputs a step: lane t holds inputs k + 8 t .. + 7 of its rows
+#pragma unroll 2
+      for (int k = k0; k < k1; k += 32) {
+        const int kk = k + 8 * t;
+        const bool in = kk < k1;
+        const uint4 v0 = in && row0 >= 0 ? __ldg(reinterpret_cast<const uint4*>(x0 + kk)) : zero;
+        const uint4 v1 = in && row1 >= 0 ? __ldg(reinterpret_cast<const uint4*>(x1 + kk)) : zero;
+        uint4 w[kLoraRankTiles];
+#pragma unroll
+        for (int n = 0; n < kLoraRankTiles; ++n)
+          w[n] = in && n < nz ? __ldg(reinterpret_cast<const uint4*>(ar + (size_t)n * 8 * p.inputs + kk)) : zero;
+        const uint32_t f0[4] = {v0.x, v1.x, v0.y, v1.y}, f1[4] = {v0.z, v1.z, v0.w, v1.w};
+#pragma unroll
+        for (int n = 0; n < kLoraRankTiles; ++n)
+          if (n < nz) {
+            mma_16816<true>(acc[n], f0, w[n].x, w[n].y);
+            mma_16816<true>(acc[n], f1, w[n].z, w[n].w);
+          }
+      }
+      if (r0 > 0) __syncthreads();  // warp 0 has read the block before
+      if (warp > 0) {               // the warps' sums, in warp order
+#pragma unroll
+        for (int n = 0; n < kLoraRankTiles; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) red[warp - 1][lane][n * 4 + i] = acc[n][i];
+      }
+      __syncthreads();
+      if (warp == 0) {
+#pragma unroll
+        for (int n = 0; n < kLoraRankTiles; ++n)
+          if (n < nz) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int w = 0; w < kLoraWarps - 1; ++w) acc[n][i] += red[w][lane][n * 4 + i];
+            float* h = hp + r0 + n * 8 + 2 * t;
+            *reinterpret_cast<float2*>(h + g * hld) = make_float2(acc[n][0], acc[n][1]);
+            *reinterpret_cast<float2*>(h + (g + 8) * hld) = make_float2(acc[n][2], acc[n][3]);
+          }
+      }
+    }
+  }
+
+  // this warp's blocks of 16 outputs, two at a time: base and four k steps of B on their way before they are needed
+  const int blocks = (p.outputs + 15) / 16, stride = p.splits * kLoraWarps, steps = p.rank / 16;
   typename Four::Raw base[kBlocks][2];
   uint2 w[kBlocks][2][kFetch];
-  const int steps = p.rank / 16;
+  auto fetch = [&](int block) {
 #pragma unroll
-  for (int q = 0; q < kBlocks; ++q) {
-    const int o = o0 + q * 16 + 4 * t, oc = o0 + q * 16 + (g >> 1) * 4 + (g & 1);
-    if (o < p.outputs) {
-      if (row0 >= 0) base[q][0] = Four::load(p.base, (size_t)row0 * p.base_ld + o);
-      if (row1 >= 0) base[q][1] = Four::load(p.base, (size_t)row1 * p.base_ld + o);
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int k = 0; k < kFetch; ++k)
-        w[q][i][k] = a >= 0 && oc + 2 * i < p.outputs && k < steps
-                         ? __ldg(reinterpret_cast<const uint2*>(p.b + ((size_t)a * p.outputs + oc + 2 * i) * p.rank + 16 * k + 4 * t))
-                         : make_uint2(0, 0);
-  }
-  pdl_wait();
-  pdl_trigger();
-  if (!unit) return;
-  if (a >= 0) {
-    const float scale = p.scales[a];
-    for (int i = threadIdx.x; i < kLoraTile * R / 4; i += kLoraWarps * 32) {
-      const int r = i / (R / 4), c = i % (R / 4) * 4, row = tile.rows[r];
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (row >= 0) {
-#pragma unroll 8
-        for (int s = 0; s < p.splits; ++s) {
-          const float4 y = *reinterpret_cast<const float4*>(p.part + ((size_t)s * p.tokens + row) * R + c);
-          v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
-        }
-        v.x *= scale, v.y *= scale, v.z *= scale, v.w *= scale;
+    for (int q = 0; q < kBlocks; ++q) {
+      const int o16 = (block + q * stride) * 16, o = o16 + 4 * t, oc = o16 + (g >> 1) * 4 + (g & 1);
+      if (o < p.outputs) {
+        if (row0 >= 0) base[q][0] = Four::load(p.base, (size_t)row0 * p.base_ld + o);
+        if (row1 >= 0) base[q][1] = Four::load(p.base, (size_t)row1 * p.base_ld + o);
       }
-      lora_keep<kParts>(hs, plane, r * ld + c, v);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int k = 0; k < kFetch; ++k)
+          w[q][i][k] = a >= 0 && oc + 2 * i < p.outputs && k < steps
+                           ? __ldg(reinterpret_cast<const uint2*>(p.b + ((size_t)a * p.outputs + oc + 2 * i) * p.rank + 16 * k + 4 * t))
+                           : make_uint2(0, 0);
+    }
+  };
+  const int block0 = part * kLoraWarps + warp;
+  fetch(block0);
+  if (a >= 0) {
+    // each CTA adds up its share of h and puts the sums in their place in all (every CTA adding up all of h took 9000
+    // cycles with 16 of them)
+    const int all = kLoraTile * R / 4, share = (all + p.splits - 1) / p.splits, end = min(all, (part + 1) * share);
+    tc::cluster_sync();
+    for (int i = part * share + threadIdx.x; i < end; i += kLoraWarps * 32) {
+      const float* at = hp + i / (R / 4) * hld + i % (R / 4) * 4;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+      for (int s = 0; s < p.splits; ++s) {
+        const float4 y = ld_cluster(tc::mapa(at, s));
+        v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
+      }
+      for (int s = 0; s < p.splits; ++s) st_cluster(tc::mapa(at, s), v);
+    }
+    tc::cluster_sync();
+    const float scale = p.scales[a];
+    for (int i = threadIdx.x; i < all; i += kLoraWarps * 32) {
+      const int r = i / (R / 4), c = i % (R / 4) * 4;
+      const float4 v = *reinterpret_cast<const float4*>(hp + r * hld + c);
+      lora_keep<kParts>(hs, plane, r * ld + c, make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale));
     }
     __syncthreads();
-  } else if (p.base == p.out) {
-    return;  // in place: rows without an adapter stay
   }
+  for (int block = block0; block < blocks; block += kBlocks * stride) {
+    if (block > block0) fetch(block);
 #pragma unroll
-  for (int q = 0; q < kBlocks; ++q) {
-    const int o = o0 + q * 16;
-    if (o >= p.outputs) break;
-    float d[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    if (a >= 0) {
-      // both halves of the block (8 outputs, lanes t < 2 and t >= 2) share a slice, or each has its own
-      const int j0 = lora_slice(p, o), j1 = o + 8 < p.outputs ? lora_slice(p, o + 8) : j0;
-      const int oc = o + (g >> 1) * 4 + (g & 1);
-      for (int j = j0; j <= j1; ++j) {
-        float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-        for (int k = 0; k < steps; ++k) {
-          uint32_t f[kParts][4];
-          lora_operands<kParts>(hs + g * ld + j * p.rank + 16 * k + 4 * t, plane, ld, f);
+    for (int q = 0; q < kBlocks; ++q) {
+      const int o = (block + q * stride) * 16;
+      if (o >= p.outputs) break;
+      float d[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      if (a >= 0) {
+        // both halves of the block (8 outputs, lanes t < 2 and t >= 2) share a slice, or each has its own
+        const int j0 = lora_slice(p, o), j1 = o + 8 < p.outputs ? lora_slice(p, o + 8) : j0;
+        const int oc = o + (g >> 1) * 4 + (g & 1);
+        for (int j = j0; j <= j1; ++j) {
+          float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+          const uint16_t* h = hs + g * ld + j * p.rank + 4 * t;
+          auto step = [&](int k, uint2 b0, uint2 b1) {
+            uint32_t f[kParts][4];
+            lora_operands<kParts>(h + 16 * k, plane, ld, f);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            uint2 b = make_uint2(0, 0);
-            if (k == 0) b = w[q][i][0];
-            else if (k == 1) b = w[q][i][1];
-            else if (oc + 2 * i < p.outputs)
-              b = __ldg(reinterpret_cast<const uint2*>(p.b + ((size_t)a * p.outputs + oc + 2 * i) * p.rank + 16 * k + 4 * t));
+            for (int part = 0; part < kParts; ++part) {
+              mma_16816<true>(acc[0], f[part], b0.x, b0.y);
+              mma_16816<true>(acc[1], f[part], b1.x, b1.y);
+            }
+          };
 #pragma unroll
-            for (int part = 0; part < kParts; ++part) mma_16816<true>(acc[i], f[part], b.x, b.y);
+          for (int k = 0; k < kFetch; ++k)
+            if (k < steps) step(k, w[q][0][k], w[q][1][k]);
+          for (int k = kFetch; k < steps; ++k) {
+            uint2 b[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              b[i] = oc + 2 * i < p.outputs
+                         ? __ldg(reinterpret_cast<const uint2*>(p.b + ((size_t)a * p.outputs + oc + 2 * i) * p.rank + 16 * k + 4 * t))
+                         : make_uint2(0, 0);
+            step(k, b[0], b[1]);
           }
+          const bool mine = (t < 2 ? j0 : j1) == j;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[i][e] = mine ? acc[i][e] : d[i][e];
         }
-        const bool mine = (t < 2 ? j0 : j1) == j;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) d[i][e] = mine ? acc[i][e] : d[i][e];
       }
-    }
-    if (o + 4 * t < p.outputs) {
-      const bool has = a >= 0;
-      if (row0 >= 0)
-        Four::store(p.out, (size_t)row0 * p.out_ld + o + 4 * t,
-                    has ? Four::add(base[q][0], d[0][0], d[0][1], d[1][0], d[1][1]) : base[q][0]);
-      if (row1 >= 0)
-        Four::store(p.out, (size_t)row1 * p.out_ld + o + 4 * t,
-                    has ? Four::add(base[q][1], d[0][2], d[0][3], d[1][2], d[1][3]) : base[q][1]);
+      if (o + 4 * t < p.outputs) {
+        const bool has = a >= 0;
+        if (row0 >= 0)
+          Four::store(p.out, (size_t)row0 * p.out_ld + o + 4 * t,
+                      has ? Four::add(base[q][0], d[0][0], d[0][1], d[1][0], d[1][1]) : base[q][0]);
+        if (row1 >= 0)
+          Four::store(p.out, (size_t)row1 * p.out_ld + o + 4 * t,
+                      has ? Four::add(base[q][1], d[0][2], d[0][3], d[1][2], d[1][3]) : base[q][1]);
+      }
     }
   }
 }
@@ -693,35 +713,26 @@ static int lora_per_split(int inputs, int splits, bool group) {
   const int step = group ? 32 * kLoraWarps : kLoraStep;
   return ((inputs + splits - 1) / splits + step - 1) / step * step;
 }
-// Splits of the inputs: two CTAs an SM for a decode step (at most 16, at least 128 inputs each); for prompts a
-// cluster of 1, 2, 4 or 8 (at least one stage each).
+// Splits of the inputs, a cluster: for a decode step 1 to 16 CTAs (four an SM at most, one step of its warps each or
+// more), for prompts 1 to 8 (one stage each or more).
 static int lora_splits(int tokens, int inputs, int ranks, int adapters) {
   const bool group = tokens <= kLoraGroupTokens;
-  const long z = (ranks + 8 * kLoraRankTiles - 1) / (8 * kLoraRankTiles);
+  const long z = group ? 1 : (ranks + 8 * kLoraRankTiles - 1) / (8 * kLoraRankTiles);
   const long base = (group ? lora_units(tokens, adapters) : (tokens + kLoraRows - 1) / kLoraRows) * z;
-  if (!group) {
-    int sp = 8;
-    while (sp > 1 && (base * sp > 4 * 148 || inputs < sp * kLoraStep)) sp /= 2;
-    return sp;
-  }
-  long sp = base > 0 ? (2L * 148 + base - 1) / base : 1;
-  if (sp > 16) sp = 16;
-  const int per = lora_per_split(inputs, (int)(sp < 1 ? 1 : sp), true);
-  return (inputs + per - 1) / per;
-}
-// Parts of h that the workspace holds.
-static int lora_parts(int tokens, int inputs, int ranks, int adapters) {
-  return tokens <= kLoraGroupTokens ? lora_splits(tokens, inputs, ranks, adapters) : 1;
+  const int step = group ? 32 * kLoraWarps : kLoraStep;
+  int sp = group ? 16 : 8;
+  while (sp > 1 && (base * sp > 4 * 148 || inputs < sp * step)) sp /= 2;
+  return sp;
 }
 
 template <bool OB>
 static int run_lora_group(const LoraArgs& p, cudaStream_t st) {
-  const int R = p.rank * p.slices;
-  const unsigned units = lora_units(p.tokens, p.adapters), z = (R + 8 * kLoraRankTiles - 1) / (8 * kLoraRankTiles);
-  int rc = launch_k(lora_shrink_group_kernel, dim3(units, p.splits, z), dim3(kLoraWarps * 32), 0, st, p);
+  static_assert(lora_group_smem(kLoraMaxRanks, 3) <= 45 * 1024, "no raised limit needed");
+  static std::atomic<uint64_t> wide_set{0};  // devices on which clusters of more than 8 are allowed
+  int rc = ensure_attribute(lora_group_kernel<OB>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1, wide_set);
   if (rc) return rc;
-  return launch_k(lora_expand_group_kernel<OB>, dim3(units, (p.outputs + kLoraOutputs - 1) / kLoraOutputs),
-                  dim3(kLoraWarps * 32), (size_t)(OB ? 2 : 3) * kLoraTile * lora_ld(R) * 2, st, p);
+  return launch_cluster(lora_group_kernel<OB>, dim3(p.splits, lora_units(p.tokens, p.adapters)), dim3(kLoraWarps * 32),
+                        lora_group_smem(p.rank * p.slices, OB ? 2 : 3), st, p.splits, p);
 }
 
 template <bool OB>
@@ -777,7 +788,7 @@ extern "C" {
 size_t ccut_lora_workspace_bytes(int tokens, int inputs, int rank, int slices, int adapters) {
   if (tokens < 0 || inputs <= 0 || rank <= 0 || slices <= 0 || adapters < 0 || (long)rank * slices > kLoraMaxRanks)
     return 0;
-  return 256 + (size_t)lora_parts(tokens, inputs, rank * slices, adapters) * tokens * rank * slices * sizeof(float);
+  return tokens <= kLoraGroupTokens ? 0 : 256 + (size_t)tokens * rank * slices * sizeof(float);
 }
 
 int ccut_lora_add(const uint16_t* x, const uint16_t* a, const uint16_t* b, const float* scales, const int32_t* ids,
@@ -803,14 +814,13 @@ int ccut_lora_add(const uint16_t* x, const uint16_t* a, const uint16_t* b, const
   if (!x || !ids || !base || !out || (adapters > 0 && (!a || !b || !scales))) return CCUT_ERR_INVALID;
   for (const void* q : {(const void*)x, (const void*)a, (const void*)b, base, (const void*)out})
     if (reinterpret_cast<uintptr_t>(q) % 16) return CCUT_ERR_INVALID;
-  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 ||
-      ws_bytes < ccut_lora_workspace_bytes(tokens, inputs, rank, slices, adapters))
-    return CCUT_ERR_WORKSPACE;
+  const size_t need = ccut_lora_workspace_bytes(tokens, inputs, rank, slices, adapters);
+  if (need > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || ws_bytes < need)) return CCUT_ERR_WORKSPACE;
   const int R = rank * slices;
   p.x = x, p.a = a, p.b = b, p.scales = scales, p.ids = ids;
   p.tokens = tokens, p.inputs = inputs, p.outputs = (int)o, p.rank = rank, p.slices = slices, p.adapters = adapters;
   p.base = base, p.base_ld = base_ld, p.out = out, p.out_ld = out_ld;
-  p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 256);
+  if (need > 0) p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 256);
   p.splits = lora_splits(tokens, inputs, R, adapters);
   p.k_per_split = lora_per_split(inputs, p.splits, tokens <= kLoraGroupTokens);
   if ((o + kLoraOutputs - 1) / kLoraOutputs > 65535) return CCUT_ERR_UNSUPPORTED;

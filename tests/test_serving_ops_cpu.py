@@ -94,8 +94,10 @@ def test_lora_checks(lib):
     assert call(rank=144) == _lib.ERR_UNSUPPORTED  # 2 * 144 > 256
     assert call(slices=5, widths=(C.c_int * 5)(8, 8, 8, 8, 8)) == _lib.ERR_UNSUPPORTED
     assert call(tokens=0, x=NULL) == _lib.OK
-    need = lib.ccut_lora_workspace_bytes(3, 128, 16, 2, 2)
-    assert need > 256 and call(nb=need - 1) == _lib.ERR_WORKSPACE and call(ws=ODD) == _lib.ERR_WORKSPACE
+    assert lib.ccut_lora_workspace_bytes(256, 128, 16, 2, 2) == 0  # a decode step takes none
+    need = lib.ccut_lora_workspace_bytes(300, 128, 16, 2, 2)
+    assert need > 256 and call(tokens=300, nb=need - 1) == _lib.ERR_WORKSPACE
+    assert call(tokens=300, ws=ODD) == _lib.ERR_WORKSPACE and call(tokens=300, ws=NULL) == _lib.ERR_WORKSPACE
 
 
 def test_python_checks():
