@@ -11,7 +11,7 @@
 //   latency.  The CTAs and warps split the inputs, add up h through distributed shared memory and then split
 //   the outputs; operands come straight from global memory (the order of the k index of an MMA is free: a
 //   lane's operand registers are 16 consecutive bytes of a row of x or A).
-//   64 tokens, 16 adapters of rank 16, 2048 inputs, 5120 outputs: TIME_STEP (15 us in two kernels).
+//   64 tokens, 16 adapters of rank 16, 2048 inputs, 5120 outputs: 10.5 us (14.8 in two kernels).
 // - More tokens (prompts), two launches: a shrink kernel gives h[t, slices * rank] = A x, the expand kernel scales it,
 //   multiplies by B and adds the base.  A CTA takes 64 neighbours and loops over their distinct adapters (one,
 //   inside a prompt).  A row takes the result of its own adapter by selection, so nothing of another request's
@@ -82,6 +82,7 @@ CCUT_DEVICE bool lora_group(const LoraArgs& p, int u, LoraTile& tile, int* ids, 
     rank[k] = 0;
   }
   const int4* ids4 = reinterpret_cast<const int4*>(ids);
+#pragma unroll 4
   for (int q = 0; q < (p.tokens + 3) / 4; ++q) {  // every token's rank among the tokens of its id
     const int4 v = ids4[q];
 #pragma unroll
@@ -100,7 +101,8 @@ CCUT_DEVICE bool lora_group(const LoraArgs& p, int u, LoraTile& tile, int* ids, 
 #pragma unroll
   for (int k = 0; k < kPer; ++k) {
     int first = 0;
-    for (int w = 0; w < k * kLoraWarps + warp; ++w) first += counts[w];
+#pragma unroll
+    for (int w = 0; w < kLoraGroupTokens / 32; ++w) first += w < k * kLoraWarps + warp ? counts[w] : 0;
     if ((leaders[k] >> lane & 1) && first + __popc(leaders[k] & ((1u << lane) - 1)) == u) {
       tile.uniq[0] = mine[k];
       tile.uniq[1] = rank[k];
@@ -361,7 +363,7 @@ template <bool OUT_BF16>
 __global__ void __launch_bounds__(kLoraWarps * 32) lora_group_kernel(const __grid_constant__ LoraArgs p) {
   pdl_wait();
   pdl_trigger();
-  constexpr int kParts = OUT_BF16 ? 2 : 3, kBlocks = 2, kFetch = 4;
+  constexpr int kParts = OUT_BF16 ? 2 : 3, kBlocks = 5, kFetch = 2;
   using Four = LoraFour<OUT_BF16>;
   __shared__ LoraTile tile;
   __shared__ __align__(16) int ids[kLoraGroupTokens];
@@ -434,7 +436,7 @@ __global__ void __launch_bounds__(kLoraWarps * 32) lora_group_kernel(const __gri
     }
   }
 
-  // this warp's blocks of 16 outputs, two at a time: base and four k steps of B on their way before they are needed
+  // this warp's blocks of 16 outputs, five at a time: base and two k steps of B on their way before they are needed
   const int blocks = (p.outputs + 15) / 16, stride = p.splits * kLoraWarps, steps = p.rank / 16;
   typename Four::Raw base[kBlocks][2];
   uint2 w[kBlocks][2][kFetch];
