@@ -11,7 +11,8 @@
 //   latency.  The CTAs and warps split the inputs, add up h through distributed shared memory and then split
 //   the outputs; operands come straight from global memory (the order of the k index of an MMA is free: a
 //   lane's operand registers are 16 consecutive bytes of a row of x or A).
-//   64 tokens, 16 adapters of rank 16, 2048 inputs, 5120 outputs: 10.5 us (14.8 in two kernels).
+//   64 tokens, 16 adapters of rank 16, 2048 inputs, 5120 outputs: 10.3 us (14.8 in two kernels that
+//   passed h through memory; one token alone: 7.7 and 5.8, but a launch less is 4 us less of host time).
 // - More tokens (prompts), two launches: a shrink kernel gives h[t, slices * rank] = A x, the expand kernel scales it,
 //   multiplies by B and adds the base.  A CTA takes 64 neighbours and loops over their distinct adapters (one,
 //   inside a prompt).  A row takes the result of its own adapter by selection, so nothing of another request's
