@@ -182,3 +182,39 @@ def test_misaligned_inputs():
     assert torch.equal(bank.add(shifted(bd), shifted(xd), shifted(ids)), bank.add(bd, xd, ids))
     with pytest.raises(ValueError):
         bank.add(bd, xd, ids, out=shifted(bd))
+
+
+@pytest.mark.parametrize("tokens", [37, 300])
+def test_captured_calls_and_two_streams(tokens):
+    """A captured call replayed after its inputs changed gives the eager answer, the same bits twice; calls on
+    two streams at once do not disturb each other."""
+    rng = np.random.default_rng(tokens + 9)
+    x, a, b, s, base = _inputs(rng, tokens, 520, 32, [72, 16], 5, torch.bfloat16)
+    bank = _bank(a, b, s, [72, 16])
+    xd, bd = torch.from_numpy(x).cuda().bfloat16(), torch.from_numpy(base).cuda().bfloat16()
+    ids = [torch.from_numpy(rng.integers(-1, 5, tokens).astype(np.int32)).cuda() for _ in range(3)]
+    want = [bank.add(bd, xd, i) for i in ids]
+    held = ids[0].clone()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        bank.add(bd, xd, held)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = bank.add(bd, xd, held)
+    for i, w in zip(ids + ids, want + want):
+        held.copy_(i)
+        graph.replay()
+        assert torch.equal(out, w)
+    streams = [torch.cuda.Stream() for _ in ids]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    got = [[] for _ in ids]
+    for _ in range(4):
+        for st, i, g in zip(streams, ids, got):
+            with torch.cuda.stream(st):
+                g.append(bank.add(bd, xd, i))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(y, w) for y in g)
