@@ -4,9 +4,10 @@
 // params at (slots[t], positions[t]) of the pool.  Eight lanes hold a group's 64 features (8 each, one
 // or two 16-byte loads), find its minimum and maximum with three shuffles and write one 32-bit word of
 // codes each: 32 contiguous bytes per group.  Each input byte is read once, 36 bytes per group are written;
-// bound for long prompts: the instructions of the codes (about 20 a feature) before HBM, and latency for a decode step.
+// bound for long prompts: the instructions (about 15 a feature) before HBM, and latency for a decode step.
 // kv4_read_kernel: the fp32 / bf16 values of given rows, four features a lane.
-// Append and read of 8190 x 4 rows of 128 (fp32): 25 us together, 2.9 TB/s; of 64 tokens 3.9 us.
+// Append and read of 8190 x 4 rows of 128 (fp32): 23 us together, 3.1 TB/s; of 64 tokens 3.7 us
+// (four groups a thread of the read kernel: 22.5 and 5.1).
 #include "kv4.cuh"
 
 namespace ccut {
@@ -35,19 +36,36 @@ struct Kv4In {
   __half2* params;
 };
 
+CCUT_DEVICE float kv4_max3(float a, float b, float c) {  // NaN when one is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+CCUT_DEVICE float kv4_min3(float a, float b, float c) {
+  float r;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // A code before the clamp to 0..15 is rint(fl32(d / s)).  d (1 / s) is within 2^-17 of that quotient where the clamp
 // leaves anything, so where it is further than 2^-15 from the middle of two integers it rounds to the same one;
-// the rest take the division (for every code it took 19 us of 8190 x 4 fp32 rows of 128, cold, where this takes 16).
+// the rest take the division (for every code it took 19 us of 8190 x 4 fp32 rows of 128, cold, where this takes 14).
 CCUT_DEVICE uint32_t kv4_codes(const float (&x)[8], float m, float s) {
   const float r = __frcp_rn(s), magic = 12582912.f;  // 1.5 2^23: y + magic has the rounded y in its low bits
+  const u64 m2 = pf_pair(-m, -m), r2 = pf_pair(r, r), up = pf_pair(magic, magic), down = pf_pair(-magic, -magic);
   uint32_t w = 0;
   float worst = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float y = fminf(fmaxf(__fsub_rn(x[i], m) * r, 0.f), 15.f), u = __fadd_rn(y, magic);
-    worst = fmaxf(worst, fabsf(y - __fsub_rn(u, magic)));
-    w |= (__float_as_uint(u) & 15u) << (4 * i);
+  for (int i = 0; i < 8; i += 2) {
+    float y0, y1, u0, u1, d0, d1;
+    pf_unpair(pf_mul2(pf_add2(pf_pair(x[i], x[i + 1]), m2), r2), y0, y1);
+    const u64 y = pf_pair(fminf(fmaxf(y0, 0.f), 15.f), fminf(fmaxf(y1, 0.f), 15.f)), u = pf_add2(y, up);
+    pf_unpair(u, u0, u1);
+    pf_unpair(pf_fma2(pf_add2(u, down), pf_pair(-1.f, -1.f), y), d0, d1);  // y - its integer, exact
+    worst = pf_max3(worst, fabsf(d0), fabsf(d1));
+    w += (__float_as_uint(u0) << (4 * i)) + (__float_as_uint(u1) << (4 * i + 4));
   }
+  w -= 0x4B400000u * 0x11111111u;  // the exponents
   if (worst > 0.5f - 0x1p-15f) {
     w = 0;
 #pragma unroll
@@ -79,20 +97,16 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4In k, Kv4In v, int t
   const long long off = t * in.token_stride + h * in.head_stride + g * kKv4Group + lane8 * 8;
   if (blockIdx.y) load8<V_BF16>(in.x, off, x);
   else load8<K_BF16>(in.x, off, x);
-  float lo = x[0], hi = x[0];
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-    bad |= !(fabsf(x[i]) <= 3.402823466e38f);
-  }
+  // the least and the largest, NaN if one is there
+  float lo = kv4_min3(kv4_min3(x[0], x[1], x[2]), kv4_min3(x[3], x[4], x[5]), fminf(x[6], x[7]));
+  float hi = kv4_max3(kv4_max3(x[0], x[1], x[2]), kv4_max3(x[3], x[4], x[5]), kv4_max3(x[6], x[7], x[7]));
 #pragma unroll
   for (int o = 4; o > 0; o >>= 1) {
+    const float h = __shfl_xor_sync(mask, hi, o);
     lo = fminf(lo, __shfl_xor_sync(mask, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(mask, hi, o));
+    hi = kv4_max3(hi, h, h);
   }
-  bad = (__ballot_sync(mask, bad) & mask) != 0;
+  const bool bad = !(hi <= 3.402823466e38f && lo >= -3.402823466e38f);
   lo = fminf(fmaxf(lo, -65504.f), 65504.f);
   hi = fminf(fmaxf(hi, -65504.f), 65504.f);
   __half m = __float2half_rn(lo);

@@ -22,6 +22,35 @@ constexpr int kKv4Group = 64;
 // The value of code q under the pair (s, m): q * s has at most 15 significant bits, so the fma rounds once.
 CCUT_DEVICE float kv4_value(uint32_t q, float s, float m) { return fmaf((float)q, s, m); }
 
+// Two floats in a register pair, and the three-operand maximum.
+typedef unsigned long long u64;
+CCUT_DEVICE u64 pf_pair(float a, float b) {
+  u64 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+CCUT_DEVICE void pf_unpair(u64 p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+CCUT_DEVICE u64 pf_add2(u64 a, u64 b) {
+  u64 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+CCUT_DEVICE u64 pf_fma2(u64 a, u64 b, u64 c) {
+  u64 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+CCUT_DEVICE u64 pf_mul2(u64 a, u64 b) {
+  u64 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+CCUT_DEVICE float pf_max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
 // Host-side shape checks shared by the entry points.
 inline bool kv4_shape_ok(int kv_heads, int head_dim, int max_len, long long slot_rows, int num_slots) {
   return kv_heads > 0 && (head_dim == 64 || head_dim == 128) && max_len > 0 && num_slots >= 0 &&

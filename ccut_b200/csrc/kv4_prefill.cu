@@ -98,33 +98,10 @@ CCUT_DEVICE uint64_t pf_desc_mn(uint32_t saddr) {
   d |= (uint64_t)2 << 61;
   return d;
 }
-CCUT_DEVICE float pf_max3(float a, float b, float c) {
-  float y;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-  return y;
-}
 CCUT_DEVICE float pf_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-
-typedef unsigned long long u64;
-CCUT_DEVICE u64 pf_pair(float a, float b) {
-  u64 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-CCUT_DEVICE void pf_unpair(u64 p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
-CCUT_DEVICE u64 pf_add2(u64 a, u64 b) {
-  u64 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-CCUT_DEVICE u64 pf_fma2(u64 a, u64 b, u64 c) {
-  u64 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
 }
 
 // To fp16, finite: a scale that was rounded up takes an appended group's top to 65536 at most, half a step above 65504.
