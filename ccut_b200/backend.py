@@ -40,7 +40,7 @@ from typing import Any, Callable
 import numpy as np
 import torch
 
-from ccut_b200.logprobs import token_logprobs
+from ccut_b200.logprobs import MAX_TOP, token_logprobs
 from ccut_b200.model import KvCache, MoeDecoder
 from ccut_b200.sampling import sample
 
@@ -178,13 +178,21 @@ class GenericBackend:
         and ``rank``, the distribution's ``entropy`` (nats) and the n best ``top`` as ``(id,
         logprob)``, from the logits before temperature and filters."""
         requests = list(requests)
+        top_n = None if logprobs is None else self._alternatives(logprobs)
         logits = self.logits_batch([r[0] for r in requests], [(r[1] or {}).get("adapter") for r in requests])
         tokens = [sample(lg, r[1], self._gen) for lg, r in zip(logits, requests)]
         if logprobs is None:
             return tokens
         if not requests:
             return []
-        return list(zip(tokens, self._answers(torch.stack([lg.reshape(-1) for lg in logits]), tokens, int(logprobs))))
+        return list(zip(tokens, self._answers(torch.stack([lg.reshape(-1) for lg in logits]), tokens, top_n)))
+
+    def _alternatives(self, n) -> int:  # refused before anything runs
+        if isinstance(n, bool) or not isinstance(n, (int, np.integer)) or not 0 <= n <= self.model.vocab:
+            raise ValueError(f"alternatives must be an int in [0, {self.model.vocab}], got {n!r}")
+        if n > MAX_TOP:
+            raise NotImplementedError(f"{n} alternatives (have up to {MAX_TOP})")
+        return int(n)
 
     @staticmethod
     def _answers(logits: torch.Tensor, tokens, top_n: int) -> list:
@@ -198,7 +206,7 @@ class GenericBackend:
         """The answers (as ``generate_batch``) for ``input_ids[1:]``, each given the ids before it.  Runs in
         a cache of its own, ``min(prefill_chunk, 1024)`` positions at a time (the logits of one chunk are
         held at once)."""
-        ids = self._check(input_ids)
+        ids, top_n = self._check(input_ids), self._alternatives(top_n)
         out: list = []
         if len(ids) < 2:
             return out
@@ -209,7 +217,7 @@ class GenericBackend:
             extra = {} if adapter is None else {"adapter": adapter}
             logits = self.model.forward(ids[c0:c1], cache, c0, all_logits=True, **extra)
             self.tokens_run += c1 - c0
-            out += self._answers(logits, ids[c0 + 1: c1 + 1], int(top_n))
+            out += self._answers(logits, ids[c0 + 1: c1 + 1], top_n)
         return out
 
     # ---- L1Backend interface -------------------------------------------------------------

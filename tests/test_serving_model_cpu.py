@@ -174,6 +174,27 @@ def test_backend_keeps_adapters_apart(ops):
     assert be.score(prompt[:1]) == []
 
 
+def test_alternatives_are_checked_before_anything_runs(ops):
+    """A number of alternatives that no answer can hold is refused with no position computed, no cache taken."""
+    from ccut_b200.backend import GenericBackend
+
+    t = make_tiny(8, kv_heads=2)
+    be = GenericBackend(_build(ops, t), max_seqs=2, max_len=16)
+    prompt = _prompts(t, (6,))[0]
+    for n, err in ((-1, ValueError), (1.5, ValueError), (True, ValueError), ("2", ValueError), (t.vocab + 1, ValueError),
+                   (33, NotImplementedError)):
+        if n == 33 and t.vocab < 33:
+            err = ValueError
+        for call in (lambda: be.generate_step(prompt, {"temperature": 0.0}, logprobs=n),
+                     lambda: be.generate_batch([(prompt, None)], logprobs=n), lambda: be.score(prompt, top_n=n)):
+            with pytest.raises(err):
+                call()
+    assert be.tokens_run == 0 and not be._seqs
+    with pytest.raises(ValueError):
+        be.score(prompt, adapter=0)
+    assert be.tokens_run == 0
+
+
 def test_new_adapters_take_no_old_cache(ops):
     """After ``set_adapters`` a cache of the old bank's adapter is not reused; one without an adapter is."""
     from ccut_b200.backend import GenericBackend
