@@ -333,3 +333,13 @@ def test_long_caches(d, heads, kvh, seq, lens, dt):
     starts = [n - seq for n in lens]
     _check(pool, host, 0, qh, slots, starts, out_dtype=dt)
     _check(pool, host, 0, qh, slots, starts, kv_len=max(lens), out_dtype=dt, softcap=20.0)
+
+
+@pytest.mark.parametrize("d, seq, dt", [(128, 40, torch.bfloat16), (64, 33, torch.float32), (64, 1, torch.float32)])
+def test_short_rows_beside_long_ones(d, seq, dt):
+    """In a call whose positions are split over several CTAs: rows that see one tile, rows of no slot and rows
+    with a negative start."""
+    rng = np.random.default_rng(d + seq)
+    pool, host = _pool(rng, 4, 1, 2, 2700, d)
+    qh = _bf16(rng.standard_normal((6, 16, seq, d)))
+    _check(pool, host, 0, qh, [2, 0, 4, 1, 3, -1], [0, 2600, 7, 100, -3, 50], out_dtype=dt)
