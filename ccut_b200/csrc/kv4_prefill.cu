@@ -156,8 +156,6 @@ template <int D, bool OUT_BF16>
 __global__ void __launch_bounds__(kPfThreads, 1)
     kv4_prefill_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                        const __grid_constant__ PrefillArgs a) {
-  pdl_wait();
-  pdl_trigger();
   using SM = PfSmem<D>;
   constexpr int kChunks = D / 64;  // sub-tiles of 64 features, 128 rows of 128 bytes each
   constexpr int kSub = kPfTile * 128;
@@ -165,26 +163,6 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
   __shared__ PfBars bars;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int grp = a.heads / a.kv_heads, nrows = grp * a.seq;
-  const int b = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads;
-  const int r0 = (gridDim.x - 1 - blockIdx.x) * 2 * kPfRows;  // the longest first
-  const int tr = threadIdx.x & 127, my_r = r0 + (warp >= 8 ? kPfRows : 0) + tr;  // a softmax thread's query row
-  const bool live = warp >= 4 && my_r < nrows;
-  const int my_s = my_r / grp;
-  const int row = (b * a.heads + kvh * grp + my_r % grp) * a.seq + my_s;  // of q and out; rows fit 31 bits
-  if (live) {
-#pragma unroll
-    for (int c = 0; c < D; c += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.q + (size_t)row * D + c));
-  }
-  const int slot = a.slots[b], start0 = a.starts[b];
-  const bool valid = slot >= 0 && slot < a.num_slots && start0 >= 0;
-  const int start = min(start0, a.kv_len);
-  const int last_row = min(nrows, r0 + 2 * kPfRows) - 1;
-  const int seen = valid ? min(a.kv_len, start + last_row / grp + 1) : 0;  // by any row of this CTA
-  const int all = (seen + kPfTile - 1) / kPfTile;
-  const int tile0 = (int)((long long)all * blockIdx.z / a.splits), tile1 = (int)((long long)all * (blockIdx.z + 1) / a.splits);
-  const int n = tile1 - tile0;
-
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.q_raw[i], kPfRows);
@@ -206,16 +184,46 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     tc::tmem_alloc(&bars.tmem, 512);
     tc::tmem_relinquish();
   }
+  const int grp = a.heads / a.kv_heads, nrows = grp * a.seq;
+  const int b = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads;
+  const int r0 = (gridDim.x - 1 - blockIdx.x) * 2 * kPfRows;  // the longest first
+  const int tr = threadIdx.x & 127, my_tile = warp >= 8, my_r = r0 + my_tile * kPfRows + tr;  // a softmax thread's query row
+  const bool live = warp >= 4 && my_r < nrows;
+  const int my_s = my_r / grp;
+  const int row = (b * a.heads + kvh * grp + my_r % grp) * a.seq + my_s;  // of q and out; rows fit 31 bits
+  uint8_t* q_s = smem;
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
+  pdl_wait();
+  pdl_trigger();
+  // A tile's rows of q come by one bulk copy per head, whose rows are neighbours (16-byte loads, each lane in its own
+  // row, took 2000 cycles a CTA more); the heads follow one another from the first row's.
+  const int have = min(kPfRows, nrows - (r0 + my_tile * kPfRows)), each = have / grp, more = have % grp;
+  if (warp >= 4) {
+    if (tr < min(grp, have)) {  // my_r is the first row of its head
+      const int bytes = ((have - 1 - tr) / grp + 1) * D * 2;
+      mbar_arrive_expect_tx(&bars.q_raw[my_tile], bytes);
+      bulk_g2s(q_s + my_tile * SM::kTileBytes + (tr * each + min(tr, more)) * (D * 2), a.q + (size_t)row * D, bytes,
+               &bars.q_raw[my_tile]);
+    } else {
+      mbar_arrive(&bars.q_raw[my_tile]);
+    }
+  }
+  const int slot = a.slots[b], start0 = a.starts[b];
+  const bool valid = slot >= 0 && slot < a.num_slots && start0 >= 0;
+  const int start = min(start0, a.kv_len);
+  const int last_row = min(nrows, r0 + 2 * kPfRows) - 1;
+  const int seen = valid ? min(a.kv_len, start + last_row / grp + 1) : 0;  // by any row of this CTA
+  const int all = (seen + kPfTile - 1) / kPfTile;
+  const int tile0 = (int)((long long)all * blockIdx.z / a.splits), tile1 = (int)((long long)all * (blockIdx.z + 1) / a.splits);
+  const int n = tile1 - tile0;
   const uint32_t tmem = __shfl_sync(0xffffffffu, bars.tmem, 0);
   volatile int* failed = &bars.failed;
   // columns: S_0, S_1, O_0, O_1, P_0, P_1 (P_i in the first half of S_i where there is no room)
   auto s_col = [&](int i) { return tmem + i * kPfTile; };
   auto o_col = [&](int i) { return tmem + 2 * kPfTile + i * D; };
   auto p_col = [&](int i) { return SM::kAhead ? tmem + 2 * kPfTile + 2 * D + i * (kPfTile / 2) : s_col(i); };
-  uint8_t* q_s = smem;
   uint8_t* ring = smem + 2 * SM::kTileBytes;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     const bool ok = mbar_wait(bar, parity, a.status);
@@ -361,26 +369,16 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_addr = s_col(i) + lanes, p_addr = p_col(i) + lanes, o_addr = o_col(i) + lanes;
     const int lim = live ? start + my_s : a.kv_len;  // last visible position
-    // The tile's rows of q come by one bulk copy per head, whose rows are neighbours (16-byte loads, each lane in its
-    // own row, took 2000 cycles a CTA more); the heads follow one another from the first row's.  A thread takes its row
-    // and writes it back as fp16, scaled by a power of two, into the swizzled tile, its 16-byte pieces in an order c ^
-    // turn in which eight threads meet every bank once both in the plain rows and in the swizzled ones: turn is a
-    // linear map of tr & 7 over GF(2) (times x in GF(8)) for which turn and turn ^ tr are both one to one.
+    // The thread takes its row of q and writes it back as fp16, scaled by a power of two, into the swizzled tile, its
+    // 16-byte pieces in an order c ^ turn in which eight threads meet every bank once both in the plain rows and in
+    // the swizzled ones: turn is a linear map of tr & 7 over GF(2) (times x in GF(8)) for which turn and turn ^ tr
+    // are both one to one.
     float fr = 0.f;
-    bool ok = true;
+    bool ok = wait(&bars.q_raw[i], 0);  // also where there is nothing to see: the copy must have landed
+    ok = !__any_sync(0xffffffffu, !ok);
     if (n > 0) {
       uint8_t* const tile = q_s + i * SM::kTileBytes;
-      const int have = min(kPfRows, nrows - (r0 + i * kPfRows)), each = have / grp, more = have % grp;
-      if (tr < min(grp, have)) {  // my_r is the first row of its head
-        const int bytes = ((have - 1 - tr) / grp + 1) * D * 2;
-        mbar_arrive_expect_tx(&bars.q_raw[i], bytes);
-        bulk_g2s(tile + (tr * each + min(tr, more)) * (D * 2), a.q + (size_t)row * D, bytes, &bars.q_raw[i]);
-      } else {
-        mbar_arrive(&bars.q_raw[i]);
-      }
       const uint8_t* const mine = tile + (tr % grp * each + min(tr % grp, more) + tr / grp) * (D * 2);
-      ok = wait(&bars.q_raw[i], 0);
-      ok = !__any_sync(0xffffffffu, !ok);
       const int turn = ((tr << 1) & 7) ^ (tr & 4 ? 3 : 0);
       uint4 u[D / 8];
       float mx = 0.f;
