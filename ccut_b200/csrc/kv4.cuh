@@ -68,9 +68,10 @@ struct Kv4Cache {
   long long slot_rows;
 };
 
-// kv4_prefill.cu: query blocks of at least this many rows per kv head.  Unpacking the cache costs what about 70 rows
-// take on the short-block kernel.
-constexpr int kKv4LongRows = 97;
+// kv4_prefill.cu: query blocks of at least this many rows per kv head.  Short-block / long-block kernel, 4 kv heads, d =
+// 128: 128 rows on one sequence of 8000 27.9 / 30.8 us, on eight of 4000 55 / 51; 160 rows 28 / 31 and 70 / 52
+// (d = 64, four of 4000: 27.0 / 26.6 and 30.7 / 26.9).
+constexpr int kKv4LongRows = 129;
 bool kv4_prefill_fits(int batch, int heads, int kv_heads, int seq, int kv_len);
 size_t kv4_prefill_workspace(int batch, int heads, int kv_heads, int seq, int kv_len, int head_dim);
 int launch_kv4_prefill(const Kv4Cache& c, const uint16_t* q, const int32_t* slots, const int32_t* starts, int batch,
