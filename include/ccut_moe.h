@@ -354,7 +354,8 @@ CCUT_API int ccut_kv4_read(const uint8_t* k_codes, const uint16_t* k_params, con
                            int kv_heads, int head_dim, int max_len, long long slot_rows, int num_slots, void* k_out,
                            void* v_out, int out_dtype, ccut_stream_t stream);
 /* ccut_gqa_attention_pool over a 4-bit pool (a long block of query rows unpacks what it reads to
- * fp16 in the workspace first; a workspace needs no zero-fill): q bf16 [batch, heads, seq, head_dim], out the same
+ * fp16 in the workspace first; a workspace needs no zero-fill, and its status word is written by
+ * long blocks alone): q bf16 [batch, heads, seq, head_dim], out the same
  * shape in out_dtype; batch row b reads slot slots[b], its query i sees positions <= starts[b] + i
  * and < kv_len (kv_len <= max_len bounds what any row sees: pass the longest length when the host
  * knows it, else max_len).  A slot outside [0, num_slots) or a negative start gives zero rows;
