@@ -505,13 +505,16 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     tc::fence_after_sync();
     const float inv = l == 0.f ? 0.f : 1.f / l;
     // a row of bf16 outputs, rows 16 bytes more than their size apart: tile 0's in the place of the query tiles (every S
-    // was issued before its last product), tile 1's behind them, where nothing is left to be read
+    // was issued before its last product), tile 1's behind them, where nothing is left to be read.  Tile 0's last rows pass
+    // the end of its query tile: it is the products that order them behind the copy of tile 1's, so rows that come
+    // without products (zeros) go straight to memory.
+    const bool staged = n > 0 && ok;
     uint8_t* const mine = q_s + (i * kPfRows + tr) * (D * 2 + 16);
 #pragma unroll
     for (int c = 0; c < D; c += 32) {
       uint32_t y[32];
       __syncwarp();
-      if (n > 0 && ok) {
+      if (staged) {
         tc::ld_32x32b_x32(o_addr + c, y);
         tc::wait_ld();
       } else {
@@ -534,7 +537,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
             const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(y[e + 2 * q]) * inv, __uint_as_float(y[e + 2 * q + 1]) * inv);
             o[q] = *reinterpret_cast<const uint32_t*>(&h);
           }
-          *reinterpret_cast<uint4*>(mine + (c + e) * 2) = make_uint4(o[0], o[1], o[2], o[3]);
+          if (staged) *reinterpret_cast<uint4*>(mine + (c + e) * 2) = make_uint4(o[0], o[1], o[2], o[3]);
+          else *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (size_t)row * D + c + e) = make_uint4(0, 0, 0, 0);
         }
       } else {
 #pragma unroll
@@ -545,7 +549,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       }
     }
     if constexpr (OUT_BF16) {
-      if (live && a.splits == 1) {
+      if (live && a.splits == 1 && staged) {
         tc::fence_proxy_async_smem();
         asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n\tcp.async.bulk.commit_group;\n\t"
                      "cp.async.bulk.wait_group.read 0;" ::"l"(static_cast<uint16_t*>(a.out) + (size_t)row * D),
