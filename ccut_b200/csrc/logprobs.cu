@@ -207,7 +207,10 @@ struct LpWarp {  // a warp's state
       bar = nth;
       bar_value = entry_value(nth);
     }
-    if (lane == share - 1 && list) mine[0] = entry_value(list);
+    if (lane == share - 1 && list) {
+      const float v = entry_value(list);
+      mine[0] = isnan(v) ? -INFINITY : v;  // NaN comes last in the order: it bars nothing, nor does its warp
+    }
   }
   // At least `share` logits of each of the row's `wpr` warps here reach its published value: at least top_n reach
   // the least of them.

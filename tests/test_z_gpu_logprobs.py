@@ -131,3 +131,37 @@ def test_captured_and_repeated_calls_agree():
         g.replay()
         for a, b in zip(out, token_logprobs(x, tok, top_n=8)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows, vocab, top, dtype", [
+    (2400, 8192, 20, torch.float32), (1200, 8200, 20, torch.float32), (40, 100001, 8, torch.float32),
+    (4, 100000, 32, torch.bfloat16), (300, 50000, 32, torch.float32), (5000, 2500, 20, torch.bfloat16),
+])
+def test_runs_of_nan_are_last_in_the_order(rows, vocab, top, dtype):
+    """NaN in whole stretches of a row, at its begin, in its middle, at its end, or nearly everywhere: the
+    alternatives and the rank are the first of the rest, the same in every call."""
+    from ccut_b200.logprobs import token_logprobs
+
+    rng = np.random.default_rng(rows + vocab)
+    x = rng.standard_normal((rows, vocab)).astype(np.float32)
+    x = np.sort(x, 1) if rows == 1200 else x  # the best come last
+    if dtype == torch.bfloat16:
+        x = formats.bf16_bits_to_f32(formats.bf16_bits_from_f32(x))
+    for r in range(rows):
+        kind = r % 6
+        if kind < 4:
+            n = (600, vocab // 2, vocab // 8, vocab - 10)[kind]
+            at = (0, 0, vocab // 8 * 3, 7)[kind]
+            x[r, at: at + n] = np.nan
+        elif kind == 4:
+            x[r, vocab // 4:] = np.nan
+    tok = rng.integers(0, vocab, rows).astype(np.int32)
+    xd, td = torch.from_numpy(x).cuda().to(dtype), torch.from_numpy(tok).cuda()
+    order = np.lexsort((np.broadcast_to(np.arange(vocab), x.shape), -x, np.isnan(x)))  # NaN last, then by value, then by index
+    rank = np.argsort(order, 1)[np.arange(rows), tok] + 1
+    for _ in range(5):
+        r = token_logprobs(xd, td, top_n=top)
+        np.testing.assert_array_equal(r.top_ids.cpu().numpy(), order[:, :top])
+        np.testing.assert_array_equal(r.rank.cpu().numpy(), rank)
+        nan = torch.from_numpy(np.isnan(x).any(1)).cuda()
+        assert torch.equal(torch.isnan(r.logprob), nan) and torch.equal(torch.isnan(r.entropy), nan)
