@@ -109,6 +109,7 @@ SIGNATURES: dict[str, tuple] = {
                                  _i, _vp, _sz, _vp]),
     "ccut_workspace_status": (_i, [_vp, _vp]),
     "ccut_debug_wait_expiry": (_i, [_vp, C.c_longlong, _vp]),
+    "ccut_debug_kv4_wait_budget": (_i, [_ll, C.POINTER(_ll)]),
 }
 
 _lib = None

@@ -757,6 +757,12 @@ size_t ccut_kv4_attention_workspace_bytes(int batch, int heads, int kv_heads, in
                    (head_dim + 2) * sizeof(float);
 }
 
+int ccut_debug_kv4_wait_budget(long long cycles, long long* before) {
+  if (cycles < 0 || cycles > kWaitBudgetCycles || !before) return CCUT_ERR_INVALID;
+  *before = kv4_wait_budget(cycles);
+  return CCUT_OK;
+}
+
 int ccut_kv4_attention(const uint16_t* q, const uint8_t* k_codes, const uint16_t* k_params, const uint8_t* v_codes,
                        const uint16_t* v_params, const int32_t* slots, const int32_t* starts, int batch, int heads,
                        int kv_heads, int seq, int head_dim, int max_len, int kv_len, long long slot_rows,

@@ -47,6 +47,7 @@ struct PrefillArgs {
   float* part;  // [splits][rows][d + 2]: maximum, sum, output of a split
   int splits;
   long long rows;
+  long long budget;  // of every wait, in cycles
 };
 
 template <int D>
@@ -59,9 +60,9 @@ struct PfSmem {
 };
 
 struct PfBars {
-  uint64_t q_raw[2], q_full[2], kv_full[8], kv_empty[8], s_full[2], s_free[2], p_half[2], p_full[2], o_full[2];
+  uint64_t q_raw[2], q_full[2], kv_full[8], kv_empty[8], s_full[2], s_free[2], p_half[2], p_full[2], o_full[2], drain;
   uint32_t tmem;
-  int failed;
+  int failed, loads;  // a wait ran out; k and v tiles that were sent for
 };
 
 // One thread of the (converged) warp; code behind it keeps its operands in uniform registers.
@@ -177,7 +178,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       mbar_init(&bars.kv_full[i], 1);
       mbar_init(&bars.kv_empty[i], 1);
     }
-    bars.failed = 0;
+    mbar_init(&bars.drain, 1);
+    bars.failed = bars.loads = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -226,7 +228,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   auto p_col = [&](int i) { return SM::kAhead ? tmem + 2 * kPfTile + 2 * D + i * (kPfTile / 2) : s_col(i); };
   uint8_t* ring = smem + 2 * SM::kTileBytes;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    const bool ok = mbar_wait(bar, parity, a.status);
+    const bool ok = mbar_wait(bar, parity, a.status, a.budget);
     if (!ok) *failed = 1;
     return ok && !*failed;
   };
@@ -240,12 +242,13 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       tc::prefetch_tmap(&kmap);
       tc::prefetch_tmap(&vmap);
       const int row = (int)(((long long)b * a.kv_heads + kvh) * a.padded) + tile0 * kPfTile;
-      int st = 0, ph = 1;  // the ring's next stage; its first use finds it empty
+      int st = 0, ph = 1, loads = 0;  // the ring's next stage; its first use finds it empty
       auto load = [&](const CUtensorMap* map, int j) {
         if (!wait(&bars.kv_empty[st], ph)) return false;
         mbar_arrive_expect_tx(&bars.kv_full[st], SM::kTileBytes);
         for (int c = 0; c < kChunks; ++c)
           tc::tma_load_2d(ring + st * SM::kTileBytes + c * kSub, map, c * 64, row + j * kPfTile, &bars.kv_full[st]);
+        ++loads;
         if (++st == SM::kStages) st = 0, ph ^= 1;
         return true;
       };
@@ -254,6 +257,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         const int k = SM::kAhead ? j + 1 : j;
         ok = (k >= n || load(&kmap, k)) && load(&vmap, j);
       }
+      bars.loads = loads;
     }
   } else if (warp == 1 && n > 0) {
     // The whole warp walks through the steps and one lane issues: a divergent lane could not use the uniform
@@ -261,7 +265,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     const uint32_t idesc_s = tc::idesc_f16_m128(kPfTile);
     const uint32_t idesc_o = tc::idesc_f16_m128(D) | (1u << 16);  // B is [k][n]
     auto spin = [&](uint64_t* bar, uint32_t parity) {  // its wake-up is on the critical path
-      const bool ok = mbar_spin(bar, parity, a.status);
+      const bool ok = mbar_spin(bar, parity, a.status, a.budget);
       if (!ok) *failed = 1;
       return __all_sync(0xffffffffu, ok && !*failed) != 0;
     };
@@ -305,8 +309,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         tc::fence_after_sync();
         products(i, 0, kPfTile / 16, sv, j == 0);
         if (pf_elect()) {
-          tc::commit(&bars.o_full[i]);
           if (i == 1) tc::commit(&bars.kv_empty[sv]);
+          tc::commit(&bars.o_full[i]);
         }
         __syncwarp();
         return true;
@@ -560,6 +564,19 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     tc::fence_before_sync();
   }
   __syncthreads();
+  if (*failed) {  // copies and products that nobody waited for end before shared and tensor memory go, or a second passes
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < 2; ++i) mbar_wait(&bars.q_raw[i], 0, a.status);
+      for (int u = max(0, bars.loads - SM::kStages); u < bars.loads; ++u)
+        mbar_wait(&bars.kv_full[u % SM::kStages], u / SM::kStages & 1, a.status);
+    }
+    if (warp == 1) {
+      if (pf_elect()) tc::commit(&bars.drain);
+      __syncwarp();
+      mbar_wait(&bars.drain, 0, a.status);
+    }
+    __syncthreads();
+  }
   if (warp == 1) {
     tc::fence_after_sync();
     tc::tmem_dealloc(tmem, 512);
@@ -617,6 +634,13 @@ size_t kv4_prefill_workspace(int batch, int heads, int kv_heads, int seq, int kv
   return 256 + cache + (sp > 1 ? (size_t)sp * batch * heads * seq * (head_dim + 4) * sizeof(float) : 0);
 }
 
+static thread_local long long g_pf_budget = kWaitBudgetCycles;
+long long kv4_wait_budget(long long cycles) {
+  const long long was = g_pf_budget;
+  g_pf_budget = cycles;
+  return was;
+}
+
 template <int D, bool OB>
 static int run_prefill(const Kv4Cache& c, PrefillArgs a, int batch, void* workspace, cudaStream_t st) {
   const size_t rows = (size_t)batch * a.kv_heads * a.padded;
@@ -645,7 +669,8 @@ int launch_kv4_prefill(const Kv4Cache& c, const uint16_t* q, const int32_t* slot
                        int heads, int kv_heads, int seq, int head_dim, int kv_len, int num_slots, float scale,
                        float softcap, void* out, bool out_bf16, void* workspace, cudaStream_t st) {
   PrefillArgs a{q, slots, starts, heads, kv_heads, seq, kv_len, num_slots, (int)pf_padded(kv_len), scale, softcap, out,
-                nullptr, nullptr, pf_splits(batch, heads, kv_heads, seq, kv_len), (long long)batch * heads * seq};
+                nullptr, nullptr, pf_splits(batch, heads, kv_heads, seq, kv_len), (long long)batch * heads * seq,
+                g_pf_budget};
   if (head_dim == 128)
     return out_bf16 ? run_prefill<128, true>(c, a, batch, workspace, st) : run_prefill<128, false>(c, a, batch, workspace, st);
   return out_bf16 ? run_prefill<64, true>(c, a, batch, workspace, st) : run_prefill<64, false>(c, a, batch, workspace, st);

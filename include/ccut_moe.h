@@ -420,6 +420,11 @@ CCUT_API int ccut_workspace_status(void* workspace, ccut_stream_t stream);
  * the idle barrier succeeded, which they must not).  Read the status with
  * ccut_workspace_status. */
 CCUT_API int ccut_debug_wait_expiry(void* workspace, long long budget_cycles, ccut_stream_t stream);
+/* The limit, in SM clocks (at most the kernels' own ~1 s, the default), of the waits inside the long
+ * query blocks of ccut_kv4_attention that this host thread launches from now on; *before receives the
+ * one until now.  With a limit of 0 waits run out in an ordinary call: its outputs are then
+ * not to be used, its status word says so, and the next call is not affected. */
+CCUT_API int ccut_debug_kv4_wait_budget(long long cycles, long long* before);
 
 /* ---- expert parallelism over NCCL (no reference counterpart: the reference runs a
  * layer's experts in one process, ccut/models/generic.py:364-385,

@@ -170,3 +170,18 @@ def test_oracle_format_rounds_within_a_step():
     m = np.abs(p[..., 1].astype(np.float64)).repeat(64, -1)
     # half a step; the top end may be cut by 15 half-ulps of s, the bottom by half an ulp of m
     assert (np.abs(serving.kv4_values(c, p) - x) <= s * (0.5 + 15 * 2.0 ** -11) + m * 2.0 ** -11).all()
+
+
+def test_wait_budget_checks():
+    import ctypes as C
+
+    from ccut_b200 import _lib, build
+
+    build.build()
+    lib, was = _lib.load(), C.c_longlong(-1)
+    assert lib.ccut_debug_kv4_wait_budget(-1, C.byref(was)) == _lib.ERR_INVALID
+    assert lib.ccut_debug_kv4_wait_budget(1 << 40, C.byref(was)) == _lib.ERR_INVALID  # above the kernels' own limit
+    assert lib.ccut_debug_kv4_wait_budget(0, None) == _lib.ERR_INVALID and was.value == -1
+    assert lib.ccut_debug_kv4_wait_budget(5, C.byref(was)) == 0 and was.value > 5
+    default = was.value
+    assert lib.ccut_debug_kv4_wait_budget(default, C.byref(was)) == 0 and was.value == 5
