@@ -21,8 +21,8 @@
 // - Each warp streams its own tiles of 16 positions through a four-deep cp.async ring, with no barrier
 //   between warps; 32-byte units are placed so that the reads of both operands touch every bank once.
 //   (Prefetching into registers instead took 168 of them and left three CTAs an SM.)
-// - The running maximum moves only when a score passes it by 2^8 (one vote a tile instead of
-//   six shuffles a row pair): probabilities stay below 2^8, and fp16's range has room for that.
+// - The running maximum moves only when a score passes it by 2^4 (one vote a tile instead of
+//   six shuffles a row pair): probabilities stay below 2^4, and fp16's range has room for that (kKv4Room).
 // - Tiles that every row sees in whole run without mask tests; the few others (the last tile, the diagonal
 //   of a query block) run a masked copy.
 // - Work is cut evenly whatever the lengths: the blocks of 128 or 64 positions of all (sequence, tile of query
@@ -37,8 +37,12 @@
 // One of 513: 8.5 us, latency.
 // Roundings to fp16: q, scaled to its row's largest element (2^-35 of it is kept), and sum q_g (2^-15
 // of the largest element); p s_v, scaled by the row's power of two R that brings the largest v scale it has
-// seen to [1/2, 1) (11 bits, and 2^-25 of the largest absolutely; with fp32 output a second fp16 part
-// keeps 22).  Everything else, running maximum, sums and outputs, is fp32.
+// seen to [2^10, 2^11) (11 bits, and 2^-35 of that scale absolutely; with fp32 output a second fp16 part
+// keeps 22 bits, and 2^-35).  Everything else, running maximum, sums and outputs, is fp32.
+// The codes are not centred, so the sums of p s c and of p m cancel and the rounding of p s_v counts two to three
+// times: 64 ragged caches' outputs are 1.74e-3 off (relative norm), where the rounding to bf16 alone makes 1.66e-3.  Two
+// parts for bf16 output too take 56 us for 50 (1.66e-3); what the part leaves, times the middle of the
+// codes, added to the sum of p m 53 us (1.67e-3).
 #include <math.h>
 
 #include "kv4.cuh"
@@ -287,12 +291,12 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
   }
 
   float m[NT][2], l[NT][2], am[NT][G][2], o[NT][D / 16][4], R[NT][2];
-  __half r_inv = __ushort_as_half(0);  // the smallest 1 / R; 0 before the first tile
+  __half r_inv = __ushort_as_half(0);  // the least scale that needs a smaller R; 0 before the first tile
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      m[nt][c] = -INFINITY, l[nt][c] = 0.f, R[nt][c] = pow2f(30);  // 2^-30: below every scale
+      m[nt][c] = -INFINITY, l[nt][c] = 0.f, R[nt][c] = pow2f(30 + kKv4Room);  // 2^-30: below every scale
 #pragma unroll
       for (int gr = 0; gr < G; ++gr) am[nt][gr][c] = 0.f;
     }
@@ -407,7 +411,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
             vis[u][nt][i] = p < k1 && p <= lim[nt][i & 1];
             if (!vis[u][nt][i]) x = -INFINITY;
           }
-          need |= x > m[nt][i & 1] + 8.f;
+          need |= x > m[nt][i & 1] + kKv4Lag;
         }
     }
     __half2 top = __hmax2(as_half2(vpw[0][0][0]), as_half2(vpw[0][1][0]));
@@ -427,7 +431,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
           if constexpr (U == 2) v = fmaxf(v, fmaxf(sc[U - 1][nt][c], sc[U - 1][nt][c + 2]));
 #pragma unroll
           for (int s = 4; s < 32; s <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, s));
-          v = v > m[nt][c] + 8.f ? v : m[nt][c];  // by the row's own scores: its bits depend on no other row
+          v = v > m[nt][c] + kKv4Lag ? v : m[nt][c];  // by the row's own scores: its bits depend on no other row
           const float al = v == m[nt][c] ? 1.f : ex2(m[nt][c] - v);
           m[nt][c] = v;
           l[nt][c] *= al;
@@ -454,13 +458,13 @@ __global__ void __launch_bounds__(kKv4Warps * 32, kKv4Resident<D, NT>) kv4_attn_
 #pragma unroll
           for (int s = 4; s < 32; s <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, s));
           v = fminf(v, 65504.f);
-          if (v * R[nt][c] >= 1.f) {
-            const float r = pow2f(-exponent_of(v) - 1), f = r / R[nt][c];
+          if (v * R[nt][c] >= pow2f(kKv4Room)) {
+            const float r = pow2f(kKv4Room - 1 - exponent_of(v)), f = r / R[nt][c];
             R[nt][c] = r;
 #pragma unroll
             for (int mt = 0; mt < D / 16; ++mt) o[nt][mt][c] *= f, o[nt][mt][c + 2] *= f;
           }
-          low = fminf(low, 1.f / R[nt][c]);
+          low = fminf(low, pow2f(kKv4Room) / R[nt][c]);
         }
       r_inv = __float2half_rn(low);
     }

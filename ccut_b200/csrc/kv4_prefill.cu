@@ -13,8 +13,8 @@
 //   S_i = Q_i K^T, then O_i += P_i V with P_i read from tensor memory, where it takes the place of S_i.
 // - two warpgroups of softmax threads, one row a thread: S to registers, running maximum, exponentials, P
 //   back as fp16.  While one tile's scores are worked on, the tensor cores run the other's products.
-// - The maximum moves only when a score of the row passes it by 2^8, so O is rescaled a few times per row and not
-//   every tile (probabilities up to 2^8 fit fp16); when it moves, the O of the earlier tiles is complete, since
+// - The maximum moves only when a score of the row passes it by 2^4, so O is rescaled a few times per row and not
+//   every tile (probabilities up to 2^4 fit fp16, scaled as they are by kKv4Room); when it moves, the O of the earlier tiles is complete, since
 //   S_i of a tile is issued behind P_i V of the one before.
 // - With 64 features P has columns of its own: S_i of the next tile is computed while the softmax of this one
 //   runs (4096 rows: 118 us, 134 in turn).  With 128 tensor memory is full, and a softmax warp waits 1400 of
@@ -23,7 +23,8 @@
 // Measured, 32 heads on 4 kv heads: 4096 rows from position 0, d = 128, 145 us (0.95 PFLOP/s of visible
 // products), 8192 rows 494 us (1.11); d = 64 118 us.
 // Roundings: q to fp16 after scaling its row's largest element to [1/2, 1) (11 bits of it, 2^-25 of the
-// largest), k and v above, P 11 bits; scores, maximum, sums and O are fp32.
+// largest), k and v above, P to 11 bits down to 2^-25 of the maximum and 2^-36 of it absolutely, whatever the type
+// of the output; scores, maximum, sums and O are fp32.
 #include <math.h>
 
 #include "kv4.cuh"
@@ -413,7 +414,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       tc::fence_proxy_async_smem();
       mbar_arrive(&bars.q_full[i]);
     }
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f;  // the maximum less kKv4Room: l and O are 2^kKv4Room larger, and so are P's
     for (int j = 0; ok && j < n; ++j) {
       ok = wait(&bars.s_full[i], j & 1);
       ok = !__any_sync(0xffffffffu, !ok);
@@ -459,8 +460,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           tc::fence_after_sync();
         }
       }
-      if (__any_sync(0xffffffffu, mt > m + 8.f)) {
-        const float mn = mt > m + 8.f ? mt : m, al = mn == m ? 1.f : pf_ex2(m - mn);  // by the row's own scores
+      if (__any_sync(0xffffffffu, mt > m + (kKv4Room + kKv4Lag))) {
+        const float mn = mt > m + (kKv4Room + kKv4Lag) ? mt - kKv4Room : m, al = mn == m ? 1.f : pf_ex2(m - mn);  // by the row's own scores
         m = mn;
         l *= al;
         __syncwarp();
