@@ -102,6 +102,7 @@ SIGNATURES: dict[str, tuple] = {
     "ccut_kv4_read": (_i, [_vp] * 6 + [_i, _i, _i, _i, _ll, _i, _vp, _vp, _i, _vp]),
     "ccut_kv4_attention_workspace_bytes": (_sz, [_i] * 6),
     "ccut_kv4_attention": (_i, [_vp] * 7 + [_i] * 7 + [_ll, _i, _f, _f, _vp, _i, _vp, _sz, _vp]),
+    "ccut_kv4_attention_reported": (_i, [_vp] * 7 + [_i] * 7 + [_ll, _i, _f, _f, _vp, _i, _vp, _sz, _vp, _vp]),
     "ccut_token_logprobs": (_i, [_vp, _i, _i, _i, _ll, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
     "ccut_lora_workspace_bytes": (_sz, [_i] * 5),
     "ccut_lora_add": (_i, [_vp] * 5 + [_i] * 5 + [C.POINTER(_i), _vp, _ll, _vp, _ll, _i, _vp, _sz, _vp]),

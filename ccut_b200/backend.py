@@ -26,6 +26,10 @@ absent: none); a cache serves only requests of the adapter it was computed with.
 ``n`` best alternatives (``ccut_b200.logprobs``, on the logits before temperature and filters); ``score``
 answers them for the tokens of a given text.
 
+Over 4-bit caches a step whose attention ran out of one of its bounded waits raises ``TimeoutError``
+(the reference's class for a stalled wait, ccut/experts/reader.py:327); the caches are emptied, so the next
+call of the request computes its prompt again.
+
 ``generate`` and ``forward_step`` give the interface of the reference's fallback backend
 (``L1Backend``, ``ccut/models/backend_transformers.py:31-124``), which the engine uses when a
 backend has no ``generate_step``: ``forward_step(input_ids, past)`` returns the logits of the
@@ -40,6 +44,7 @@ from typing import Any, Callable
 import numpy as np
 import torch
 
+from ccut_b200 import _lib
 from ccut_b200.logprobs import MAX_TOP, token_logprobs
 from ccut_b200.model import KvCache, MoeDecoder
 from ccut_b200.sampling import sample
@@ -124,11 +129,26 @@ class GenericBackend:
             raise ValueError(f"{len(ids)} ids exceed the backend's max_len of {self.max_len}")
         return ids
 
+    def _check_waits(self) -> None:
+        """Raises when a bounded wait of the attention over 4-bit caches ran out since the last check; no
+        cache is reused then."""
+        code = self.model.kv_status()
+        if code:
+            for s in self._seqs:
+                s.cache.truncate(0)
+                s.ids = []
+            _lib.check(code, "attention over 4-bit caches")
+
     def logits_batch(self, id_lists, adapters=None) -> list:
         """fp32 logits ``[vocab]`` of the last id of every list, the lists run together: each
         call of the decoder takes the next ``prefill_chunk`` ids (at most) of every list that
         has ids left, so decoding sequences share their MoE passes.  ``adapters``: the adapter of
         every list (or None), default none."""
+        out = self._logits(id_lists, adapters)
+        self._check_waits()
+        return out
+
+    def _logits(self, id_lists, adapters) -> list:
         lists = [self._check(ids) for ids in id_lists]
         adapters = [None] * len(lists) if adapters is None else list(adapters)
         if len(adapters) != len(lists):
@@ -169,7 +189,7 @@ class GenericBackend:
         """The next token id; with ``logprobs`` = n, ``(id, answer)`` as ``generate_batch``."""
         if logprobs is not None:
             return self.generate_batch([(input_ids, sampling_params)], logprobs)[0]
-        return sample(self.logits_for(input_ids, (sampling_params or {}).get("adapter")), sampling_params, self._gen)
+        return self.generate_batch([(input_ids, sampling_params)])[0]
 
     def generate_batch(self, requests, logprobs: int | None = None) -> list:
         """``requests`` = ``[(input_ids, sampling_params), ...]``, one per scheduled request of an
@@ -179,8 +199,9 @@ class GenericBackend:
         logprob)``, from the logits before temperature and filters."""
         requests = list(requests)
         top_n = None if logprobs is None else self._alternatives(logprobs)
-        logits = self.logits_batch([r[0] for r in requests], [(r[1] or {}).get("adapter") for r in requests])
+        logits = self._logits([r[0] for r in requests], [(r[1] or {}).get("adapter") for r in requests])
         tokens = [sample(lg, r[1], self._gen) for lg, r in zip(logits, requests)]
+        self._check_waits()  # the tokens were waited for
         if logprobs is None:
             return tokens
         if not requests:
@@ -218,6 +239,7 @@ class GenericBackend:
             logits = self.model.forward(ids[c0:c1], cache, c0, all_logits=True, **extra)
             self.tokens_run += c1 - c0
             out += self._answers(logits, ids[c0 + 1: c1 + 1], top_n)
+            self._check_waits()
         return out
 
     # ---- L1Backend interface -------------------------------------------------------------
@@ -238,6 +260,11 @@ class GenericBackend:
             c1 = min(len(ids), c0 + self.prefill_chunk)
             logits = self.model.forward(ids[c0:c1], cache, c0)
             self.tokens_run += c1 - c0
+        try:
+            self._check_waits()
+        except TimeoutError:
+            cache.truncate(start)
+            raise
         return logits.reshape(1, -1), cache
 
     def generate(self, token_ids, max_tokens: int, on_token: Callable[[int], None] | None = None,

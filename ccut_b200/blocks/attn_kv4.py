@@ -28,14 +28,39 @@ __all__ = ["GROUP", "Kv4Cache", "Kv4Pool", "kv4_append", "kv4_attention", "kv4_r
 GROUP = 64  # features per (scale, minimum) pair
 
 _DTYPES = {torch.bfloat16: _lib.OUT_BF16, torch.float32: _lib.OUT_F32}
+_words: dict = {}  # device -> the status word of its wrapped pools, and its address
+
+
+def _device_word(device: torch.device) -> tuple:
+    """One status word for all wrapped pools of a device that were given none: wrapping launches nothing."""
+    word = _words.get(device)
+    if word is None:
+        t = torch.zeros(1, dtype=torch.int32, device=device)
+        word = (t, t.data_ptr())
+        if device.type != "cuda" or not torch.cuda.is_current_stream_capturing():  # a graph's memory is the graph's
+            _words[device] = word
+    return word
+
+
+def read_status(word: torch.Tensor) -> int:
+    """The code in a status word (0 = ok), which is cleared; waits for the current stream."""
+    if word.device.type != "cuda":
+        code = int(word)
+        word.zero_()
+        return code
+    with torch.cuda.device(word.device):
+        return _lib.load().ccut_workspace_status(word.data_ptr(), torch.cuda.current_stream().cuda_stream)
 
 
 class Kv4Pool:
     """The 4-bit caches of up to ``slots`` sequences in one allocation: ``k`` / ``v`` codes
     ``[slots, layers, kv_heads, max_len, head_dim / 2]`` uint8 and ``k_par`` / ``v_par``
-    ``[slots, layers, kv_heads, max_len, head_dim / 64, 2]`` fp16."""
+    ``[slots, layers, kv_heads, max_len, head_dim / 64, 2]`` fp16.  ``status`` (int32 ``[1]``, by default one of
+    its own; pools may share one) keeps the error of an attention call whose bounded waits ran out
+    until ``workspace_status`` reads it."""
 
-    def __init__(self, slots: int, layers: int, kv_heads: int, max_len: int, head_dim: int, device="cuda"):
+    def __init__(self, slots: int, layers: int, kv_heads: int, max_len: int, head_dim: int, device="cuda",
+                 status: torch.Tensor | None = None):
         if slots <= 0 or layers <= 0 or kv_heads <= 0 or max_len <= 0:
             raise ValueError("slots, layers, kv_heads and max_len must be positive")
         if head_dim not in (64, 128):
@@ -46,10 +71,13 @@ class Kv4Pool:
         self.k_par = torch.zeros(rows + (head_dim // GROUP, 2), dtype=torch.float16, device=device)
         self.v_par = torch.zeros_like(self.k_par)
         self._shape()
+        self._report_to(torch.zeros(1, dtype=torch.int32, device=device) if status is None else status)
 
     @classmethod
-    def wrap(cls, k: torch.Tensor, k_par: torch.Tensor, v: torch.Tensor, v_par: torch.Tensor) -> "Kv4Pool":
-        """A pool over existing tensors of the layout above (contiguous, nothing copied)."""
+    def wrap(cls, k: torch.Tensor, k_par: torch.Tensor, v: torch.Tensor, v_par: torch.Tensor,
+             status: torch.Tensor | None = None) -> "Kv4Pool":
+        """A pool over existing tensors of the layout above (contiguous, nothing copied); without a
+        ``status`` of its own it shares one with the device's other such pools."""
         shape = tuple(k.shape)
         if len(shape) != 5 or k.dtype != torch.uint8 or shape[4] not in (32, 64):
             raise ValueError("k must be uint8 [slots, layers, kv_heads, max_len, 32 or 64]")
@@ -65,7 +93,20 @@ class Kv4Pool:
         p = cls.__new__(cls)
         p.k, p.k_par, p.v, p.v_par = k, k_par, v, v_par
         p._shape()
+        if status is None:
+            p.status, p._status = _device_word(p.device)
+        else:
+            p._report_to(status)
         return p
+
+    def workspace_status(self) -> int:
+        """Device status word of the attention calls over this pool (0 = ok); clears it."""
+        return read_status(self.status)
+
+    def _report_to(self, status: torch.Tensor) -> None:
+        if status.dtype != torch.int32 or status.shape != (1,) or status.device != self.device:
+            raise ValueError(f"status must be int32 [1] on {self.device}")
+        self.status, self._status = status, status.data_ptr()
 
     def _shape(self) -> None:
         self.slots, self.layers, self.kv_heads, self.max_len, half = self.k.shape
@@ -94,8 +135,9 @@ class Kv4Cache:
     """One sequence's 4-bit cache: slot ``slot`` of ``pool`` (a pool of one slot of its own when
     made directly), ``length`` positions valid."""
 
-    def __init__(self, layers: int, kv_heads: int, max_len: int, head_dim: int, device="cuda"):
-        self._take(Kv4Pool(1, layers, kv_heads, max_len, head_dim, device), 0)
+    def __init__(self, layers: int, kv_heads: int, max_len: int, head_dim: int, device="cuda",
+                 status: torch.Tensor | None = None):
+        self._take(Kv4Pool(1, layers, kv_heads, max_len, head_dim, device, status), 0)
 
     @classmethod
     def in_pool(cls, pool: Kv4Pool, slot: int) -> "Kv4Cache":
@@ -184,7 +226,8 @@ def kv4_attention(q: torch.Tensor, pool: Kv4Pool, layer: int, slots: torch.Tenso
     """q ``[batch, heads, seq, head_dim]`` bf16; batch row b attends over slot ``slots[b]`` of
     ``layer``, its query i over positions ``<= starts[b] + i`` (int32) -> ``[batch, heads, seq,
     head_dim]`` (bf16 or fp32).  ``kv_len``: an upper bound of ``starts[b] + seq`` when the host
-    knows one (positions at or past it are not read); default: the pool's ``max_len``."""
+    knows one (positions at or past it are not read); default: the pool's ``max_len``.  A call whose
+    bounded waits ran out leaves zero rows and an error for ``pool.workspace_status()``."""
     _check_pool(pool, q.device)
     shape = q.shape
     if q.dtype != torch.bfloat16 or len(shape) != 4 or shape[3] != pool.head_dim:
@@ -205,7 +248,7 @@ def kv4_attention(q: torch.Tensor, pool: Kv4Pool, layer: int, slots: torch.Tenso
     kc, kp, vc, vp = pool._pointers(layer)
     nbytes = _lib.load().ccut_kv4_attention_workspace_bytes(b, h, pool.kv_heads, s, n, d)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 256 else None  # 256: none is used
-    _run(pool.device, "ccut_kv4_attention", q.data_ptr(), kc, kp, vc, vp, slots.data_ptr(), starts.data_ptr(), b, h,
+    _run(pool.device, "ccut_kv4_attention_reported", q.data_ptr(), kc, kp, vc, vp, slots.data_ptr(), starts.data_ptr(), b, h,
          pool.kv_heads, s, d, pool.max_len, n, pool.slot_rows, pool.slots, float(scale or 0.0), float(softcap or 0.0),
-         out.data_ptr(), _DTYPES[out_dtype], ws.data_ptr() if ws is not None else None, nbytes)
+         out.data_ptr(), _DTYPES[out_dtype], ws.data_ptr() if ws is not None else None, nbytes, pool._status)
     return out

@@ -83,7 +83,7 @@ bool kv4_prefill_fits(int batch, int heads, int kv_heads, int seq, int kv_len);
 size_t kv4_prefill_workspace(int batch, int heads, int kv_heads, int seq, int kv_len, int head_dim);
 int launch_kv4_prefill(const Kv4Cache& c, const uint16_t* q, const int32_t* slots, const int32_t* starts, int batch,
                        int heads, int kv_heads, int seq, int head_dim, int kv_len, int num_slots, float scale,
-                       float softcap, void* out, bool out_bf16, void* workspace, cudaStream_t st);
+                       float softcap, void* out, bool out_bf16, void* workspace, int* status, cudaStream_t st);
 long long kv4_wait_budget(long long cycles);  // of this thread's later launches; returns the one before
 
 }  // namespace ccut

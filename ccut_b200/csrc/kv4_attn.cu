@@ -772,6 +772,17 @@ int ccut_kv4_attention(const uint16_t* q, const uint8_t* k_codes, const uint16_t
                        int kv_heads, int seq, int head_dim, int max_len, int kv_len, long long slot_rows,
                        int num_slots, float scale, float softcap, void* out, int out_dtype, void* workspace,
                        size_t ws_bytes, ccut_stream_t stream) {
+  return ccut_kv4_attention_reported(q, k_codes, k_params, v_codes, v_params, slots, starts, batch, heads, kv_heads, seq,
+                                     head_dim, max_len, kv_len, slot_rows, num_slots, scale, softcap, out, out_dtype,
+                                     workspace, ws_bytes, nullptr, stream);
+}
+
+int ccut_kv4_attention_reported(const uint16_t* q, const uint8_t* k_codes, const uint16_t* k_params,
+                                const uint8_t* v_codes, const uint16_t* v_params, const int32_t* slots,
+                                const int32_t* starts, int batch, int heads, int kv_heads, int seq, int head_dim,
+                                int max_len, int kv_len, long long slot_rows, int num_slots, float scale, float softcap,
+                                void* out, int out_dtype, void* workspace, size_t ws_bytes, int32_t* status,
+                                ccut_stream_t stream) {
   PdlScope pdl_scope((long)batch * seq);
   if (head_dim != 64 && head_dim != 128) return CCUT_ERR_UNSUPPORTED;
   if (batch < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || seq < 0 || kv_len < 0 || kv_len > max_len ||
@@ -782,7 +793,7 @@ int ccut_kv4_attention(const uint16_t* q, const uint8_t* k_codes, const uint16_t
   if (!q || !out || !slots || !starts || (num_slots > 0 && (!k_codes || !k_params || !v_codes || !v_params)))
     return CCUT_ERR_INVALID;
   if (misaligned(q, 16) || misaligned(k_codes, 16) || misaligned(v_codes, 16) || misaligned(k_params, head_dim / 16) ||
-      misaligned(v_params, head_dim / 16) || misaligned(out, 16) || misaligned(workspace, 16))
+      misaligned(v_params, head_dim / 16) || misaligned(out, 16) || misaligned(workspace, 16) || misaligned(status, 4))
     return CCUT_ERR_INVALID;
   // rows in a grid; the line of work in 32 bits
   const double line = (double)batch * kv_heads * kv4_row_tiles(heads, kv_heads, seq) * (kv_len / kKv4Block<2> + 1);
@@ -794,7 +805,7 @@ int ccut_kv4_attention(const uint16_t* q, const uint8_t* k_codes, const uint16_t
     const Kv4Cache c{k_codes, reinterpret_cast<const __half2*>(k_params), v_codes,
                      reinterpret_cast<const __half2*>(v_params), max_len, slot_rows};
     return launch_kv4_prefill(c, q, slots, starts, batch, heads, kv_heads, seq, head_dim, kv_len, num_slots, scale,
-                              softcap, out, out_dtype == CCUT_OUT_BF16, workspace, stream);
+                              softcap, out, out_dtype == CCUT_OUT_BF16, workspace, status, stream);
   }
   Kv4AttnArgs a{q, k_codes, reinterpret_cast<const __half2*>(k_params), v_codes,
                 reinterpret_cast<const __half2*>(v_params), slots, starts, heads, kv_heads, seq, max_len, kv_len,

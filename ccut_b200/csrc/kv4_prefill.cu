@@ -643,11 +643,12 @@ long long kv4_wait_budget(long long cycles) {
 }
 
 template <int D, bool OB>
-static int run_prefill(const Kv4Cache& c, PrefillArgs a, int batch, void* workspace, cudaStream_t st) {
+static int run_prefill(const Kv4Cache& c, PrefillArgs a, int batch, void* workspace, int* status, cudaStream_t st) {
   const size_t rows = (size_t)batch * a.kv_heads * a.padded;
   uint8_t* k16 = static_cast<uint8_t*>(workspace) + 256;
   uint8_t* v16 = k16 + rows * D * 2;
-  a.status = static_cast<int*>(workspace);
+  int* const word = static_cast<int*>(workspace);
+  a.status = status ? status : word;
   a.part = reinterpret_cast<float*>(v16 + rows * D * 2);
   CUtensorMap kmap, vmap;
   int rc = encode_rows_map(&kmap, k16, (int)rows, D, kPfTile);
@@ -655,7 +656,7 @@ static int run_prefill(const Kv4Cache& c, PrefillArgs a, int batch, void* worksp
   if (rc) return rc;
   rc = launch_k(kv4_unpack_kernel<D>, dim3((unsigned)(((long long)a.padded * (D / 8) + 255) / 256), a.kv_heads, batch),
                 dim3(256), 0, st, c.kc, c.kp, c.vc, c.vp, a.slots, a.starts, a.kv_heads, a.seq, a.kv_len, c.max_len,
-                c.slot_rows, a.num_slots, a.padded, reinterpret_cast<uint4*>(k16), reinterpret_cast<uint4*>(v16), a.status);
+                c.slot_rows, a.num_slots, a.padded, reinterpret_cast<uint4*>(k16), reinterpret_cast<uint4*>(v16), word);
   if (rc) return rc;
   static std::atomic<uint64_t> smem_set{0};  // devices with the limit raised
   rc = ensure_smem_limit(kv4_prefill_kernel<D, OB>, PfSmem<D>::kBytes, smem_set);
@@ -668,13 +669,15 @@ static int run_prefill(const Kv4Cache& c, PrefillArgs a, int batch, void* worksp
 
 int launch_kv4_prefill(const Kv4Cache& c, const uint16_t* q, const int32_t* slots, const int32_t* starts, int batch,
                        int heads, int kv_heads, int seq, int head_dim, int kv_len, int num_slots, float scale,
-                       float softcap, void* out, bool out_bf16, void* workspace, cudaStream_t st) {
+                       float softcap, void* out, bool out_bf16, void* workspace, int* status, cudaStream_t st) {
   PrefillArgs a{q, slots, starts, heads, kv_heads, seq, kv_len, num_slots, (int)pf_padded(kv_len), scale, softcap, out,
                 nullptr, nullptr, pf_splits(batch, heads, kv_heads, seq, kv_len), (long long)batch * heads * seq,
                 g_pf_budget};
   if (head_dim == 128)
-    return out_bf16 ? run_prefill<128, true>(c, a, batch, workspace, st) : run_prefill<128, false>(c, a, batch, workspace, st);
-  return out_bf16 ? run_prefill<64, true>(c, a, batch, workspace, st) : run_prefill<64, false>(c, a, batch, workspace, st);
+    return out_bf16 ? run_prefill<128, true>(c, a, batch, workspace, status, st)
+                    : run_prefill<128, false>(c, a, batch, workspace, status, st);
+  return out_bf16 ? run_prefill<64, true>(c, a, batch, workspace, status, st)
+                  : run_prefill<64, false>(c, a, batch, workspace, status, st);
 }
 
 }  // namespace ccut

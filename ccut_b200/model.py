@@ -51,7 +51,7 @@ import torch.nn.functional as F
 
 from ccut_b200 import _lib
 from ccut_b200.adapters import LoraBank
-from ccut_b200.blocks.attn_kv4 import Kv4Cache, Kv4Pool, kv4_append, kv4_attention
+from ccut_b200.blocks.attn_kv4 import Kv4Cache, Kv4Pool, kv4_append, kv4_attention, read_status
 from ccut_b200.blocks.attn_mla import _latent_attention as _mla_attend
 from ccut_b200.blocks.norm import rms_norm
 from ccut_b200.blocks.rope import apply_rope
@@ -561,6 +561,7 @@ class MoeDecoder:
         self.rope = _Rope(ft, attention_factor, scaling_type, eps, softcap)
         self.device = dev
         self.kv_dtype = "bf16"  # of new_cache / new_pool when they are given none
+        self._kv_word: torch.Tensor | None = None  # status word of the 4-bit caches made here
         self.num_adapters = self._count_adapters([getattr(lay, "adapters", {}) for lay in self.layers])
         self.adapters_set = 0  # times that set_adapters changed what an index stands for
 
@@ -590,20 +591,26 @@ class MoeDecoder:
             raise ValueError(f"kv_dtype {kv_dtype!r} is not one of bf16, int4")
         if kv_dtype == "int4" and self.layout[0] != "gqa":
             raise NotImplementedError("4-bit caches of MLA layers")
+        if kv_dtype == "int4" and self._kv_word is None:
+            self._kv_word = torch.zeros(1, dtype=torch.int32, device=self.device)
         return kv_dtype == "int4"
+
+    def kv_status(self) -> int:
+        """Device status word of the attention over the 4-bit caches made here (0 = ok); clears it."""
+        return 0 if self._kv_word is None else read_status(self._kv_word)
 
     def new_cache(self, max_len: int, kv_dtype: str | None = None):
         """An empty cache of ``max_len`` positions: ``KvCache``, or ``Kv4Cache`` with ``kv_dtype="int4"``."""
         kind, kvh, width = self.layout
         if self._kv4(kv_dtype):
-            return Kv4Cache(len(self.layers), kvh, max_len, width, self.device)
+            return Kv4Cache(len(self.layers), kvh, max_len, width, self.device, self._kv_word)
         return KvCache(len(self.layers), kvh, max_len, width, self.device, values=kind == "gqa")
 
     def new_pool(self, slots: int, max_len: int, kv_dtype: str | None = None):
         """A pool of ``slots`` such caches: ``KvPool``, or ``Kv4Pool`` with ``kv_dtype="int4"``."""
         kind, kvh, width = self.layout
         if self._kv4(kv_dtype):
-            return Kv4Pool(slots, len(self.layers), kvh, max_len, width, self.device)
+            return Kv4Pool(slots, len(self.layers), kvh, max_len, width, self.device, self._kv_word)
         return KvPool(slots, len(self.layers), kvh, max_len, width, self.device, values=kind == "gqa")
 
     def _adapter(self, adapter) -> int:

@@ -370,6 +370,15 @@ CCUT_API int ccut_kv4_attention(const uint16_t* q, const uint8_t* k_codes, const
                                 int max_len, int kv_len, long long slot_rows, int num_slots, float scale,
                                 float softcap, void* out, int out_dtype, void* workspace, size_t ws_bytes,
                                 ccut_stream_t stream);
+/* The same with a status word of the caller's (device int32, zero before its first use; NULL: the
+ * workspace's): a wait that runs out stores CCUT_ERR_TIMEOUT there, and no call clears it, so that one
+ * word can stand for many calls.  ccut_workspace_status reads and clears it. */
+CCUT_API int ccut_kv4_attention_reported(const uint16_t* q, const uint8_t* k_codes, const uint16_t* k_params,
+                                         const uint8_t* v_codes, const uint16_t* v_params, const int32_t* slots,
+                                         const int32_t* starts, int batch, int heads, int kv_heads, int seq,
+                                         int head_dim, int max_len, int kv_len, long long slot_rows, int num_slots,
+                                         float scale, float softcap, void* out, int out_dtype, void* workspace,
+                                         size_t ws_bytes, int32_t* status, ccut_stream_t stream);
 
 /* ---- log probabilities of given tokens (no reference counterpart: the reference's engine answers
  * with token ids only, ccut/engine.py:335-352) ------------------------------------------------ */

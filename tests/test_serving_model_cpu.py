@@ -219,3 +219,63 @@ def test_config_kv_cache_dtype():
     from tests.test_config import AWQ
 
     assert config.quant_settings({"quant": {"kv_cache_dtype": "int4"}}, AWQ)["kv_cache_dtype"] == "int4"
+
+
+def test_an_expired_wait_reaches_the_caller(ops, monkeypatch):
+    """A status in the caches' word (as the attention leaves it when a bounded wait ran out) ends the step with
+    TimeoutError, whichever call the step is; the caches are not reused, and the next call answers as a
+    new backend does.  The bf16 caches have no such word."""
+    from ccut_b200 import _lib
+    from ccut_b200.backend import GenericBackend
+
+    t = make_tiny(9, kv_heads=2)
+    dec = _build(ops, t)
+    prompt = _prompts(t, (6,))[0]
+    assert dec.kv_status() == 0
+    attend, stall = ops.kv4_attention, []
+
+    def stalled(q, pool, *a, **k):
+        if stall:
+            pool.status.fill_(_lib.ERR_TIMEOUT)
+        return attend(q, pool, *a, **k)
+
+    monkeypatch.setattr(ops, "kv4_attention", stalled)
+    greedy = {"temperature": 0.0}
+    for pool in (True, False):
+        be = GenericBackend(dec, max_seqs=3, max_len=16, pool=pool, kv_dtype="int4")
+        want = be.generate_step(prompt, greedy)
+        calls = [lambda: be.generate_step(prompt, greedy), lambda: be.generate_step(prompt, greedy, logprobs=1),
+                 lambda: be.generate_batch([(prompt, greedy), (prompt[:4], None)]), lambda: be.logits_for(prompt),
+                 lambda: be.score(prompt), lambda: be.forward_step(prompt), lambda: be.generate(prompt, 2)]
+        for call in calls:
+            stall.append(1)
+            with pytest.raises(TimeoutError):
+                call()
+            stall.clear()
+            assert all(s.ids == [] and s.cache.length == 0 for s in be._seqs) and dec.kv_status() == 0
+            ran = be.tokens_run
+            assert be.generate_step(prompt, greedy) == want and be.tokens_run == ran + len(prompt)
+        _, past = be.forward_step(prompt[:3])
+        stall.append(1)
+        with pytest.raises(TimeoutError):
+            be.forward_step(prompt, past)
+        stall.clear()
+        assert past.length == 3
+        again = be.forward_step(prompt, be.forward_step(prompt[:3])[1])[0]
+        assert torch.equal(be.forward_step(prompt, past)[0], again)
+
+
+def test_status_words():
+    from ccut_b200 import _lib
+    from ccut_b200.blocks.attn_kv4 import Kv4Cache, Kv4Pool
+
+    a, b = Kv4Pool(1, 1, 1, 8, 64, device="cpu"), Kv4Pool(1, 1, 1, 8, 64, device="cpu")
+    a.status.fill_(_lib.ERR_TIMEOUT)
+    assert b.workspace_status() == 0 and a.workspace_status() == _lib.ERR_TIMEOUT and a.workspace_status() == 0
+    own = torch.zeros(1, dtype=torch.int32)
+    assert Kv4Cache(1, 1, 8, 64, "cpu", own).pool.status is own
+    assert Kv4Pool.wrap(a.k, a.k_par, a.v, a.v_par, own).status is own
+    assert Kv4Pool.wrap(a.k, a.k_par, a.v, a.v_par).status is Kv4Pool.wrap(b.k, b.k_par, b.v, b.v_par).status
+    for bad in (torch.zeros(2, dtype=torch.int32), torch.zeros(1), torch.zeros((), dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            Kv4Pool.wrap(a.k, a.k_par, a.v, a.v_par, bad)

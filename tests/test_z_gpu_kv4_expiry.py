@@ -61,3 +61,45 @@ def test_a_call_whose_waits_run_out_ends(budget, d, seq, L, dt):
         call()
         assert lib.ccut_workspace_status(ws.data_ptr(), s) == 0
         assert torch.equal(out, want)
+
+
+def test_the_pool_keeps_the_status(budget):
+    """The word of a pool keeps the error over later calls until it is read; wrapped pools share one; other pools
+    know nothing of it."""
+    from ccut_b200.blocks.attn_kv4 import Kv4Pool, kv4_attention
+
+    rng = np.random.default_rng(1)
+    wrapped, _ = _pool(rng, 2, 1, 1, 300, 64)
+    own = Kv4Pool(2, 1, 1, 300, 64)
+    q = _dev(_bf16(rng.standard_normal((2, 4, 50, 64))), torch.bfloat16)
+    slots, starts = (_dev(np.array(a, np.int32)) for a in ([1, 0], [200, 9]))
+    for pool, other in ((wrapped, own), (own, wrapped)):
+        want = kv4_attention(q, pool, 0, slots, starts)
+        budget(0)
+        kv4_attention(q, pool, 0, slots, starts)
+        budget(2_000_000_000)
+        assert torch.equal(kv4_attention(q, pool, 0, slots, starts), want)
+        assert other.workspace_status() == 0
+        assert pool.workspace_status() == _lib.ERR_TIMEOUT and pool.workspace_status() == 0
+
+
+@pytest.mark.parametrize("pool", [True, False])
+def test_the_backend_raises(budget, pool):
+    from ccut_b200.backend import GenericBackend
+    from tests.gpu_helpers import gpu_layer
+    from tests.model_helpers import make_tiny, quantized_layers
+    from tests.test_z_gpu_engine import _decoder
+
+    t = make_tiny(53, kv_heads=1, head_dim=64)
+    dec = _decoder(t, [gpu_layer(ol.lw) for ol in quantized_layers(t, "awq_int4_g128", seed=53)])
+    prompt = [int(x) for x in np.random.default_rng(2).integers(0, t.vocab, 200)]
+    greedy = {"temperature": 0.0}
+    be = GenericBackend(dec, max_seqs=2, max_len=256, pool=pool, kv_dtype="int4")
+    want = be.generate_step(prompt, greedy)
+    budget(0)
+    with pytest.raises(TimeoutError):
+        be.generate_step(prompt[:-1][::-1], greedy)
+    with pytest.raises(TimeoutError):
+        be.score(prompt)
+    budget(2_000_000_000)
+    assert be.generate_step(prompt, greedy) == want and dec.kv_status() == 0
