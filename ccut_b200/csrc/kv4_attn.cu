@@ -795,7 +795,8 @@ int ccut_kv4_attention_reported(const uint16_t* q, const uint8_t* k_codes, const
   if (misaligned(q, 16) || misaligned(k_codes, 16) || misaligned(v_codes, 16) || misaligned(k_params, head_dim / 16) ||
       misaligned(v_params, head_dim / 16) || misaligned(out, 16) || misaligned(workspace, 16) || misaligned(status, 4))
     return CCUT_ERR_INVALID;
-  // rows in a grid; the line of work in 32 bits
+  // rows in a grid; positions, the line of work in 32 bits (a start past the cache counts as kv_len; blocks round up)
+  if ((long long)kv_len + seq > 2147483647LL - 4096) return CCUT_ERR_UNSUPPORTED;
   const double line = (double)batch * kv_heads * kv4_row_tiles(heads, kv_heads, seq) * (kv_len / kKv4Block<2> + 1);
   if ((double)batch * heads * seq > 2147483647.0 || line > 2147483647.0) return CCUT_ERR_UNSUPPORTED;
   const size_t need = ccut_kv4_attention_workspace_bytes(batch, heads, kv_heads, seq, kv_len, head_dim);

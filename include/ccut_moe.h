@@ -361,7 +361,7 @@ CCUT_API int ccut_kv4_read(const uint8_t* k_codes, const uint16_t* k_params, con
  * knows it, else max_len).  A slot outside [0, num_slots) or a negative start gives zero rows;
  * what a query does not see never reaches its row, whatever is stored there.  scale <= 0 means
  * 1/sqrt(head_dim); softcap > 0 as in ccut_gqa_attention.  q, out and workspace are 16-byte
- * aligned. */
+ * aligned, kv_len + seq is below 2^31 - 4096. */
 CCUT_API size_t ccut_kv4_attention_workspace_bytes(int batch, int heads, int kv_heads, int seq, int kv_len,
                                                    int head_dim);
 CCUT_API int ccut_kv4_attention(const uint16_t* q, const uint8_t* k_codes, const uint16_t* k_params,

@@ -185,3 +185,15 @@ def test_wait_budget_checks():
     assert lib.ccut_debug_kv4_wait_budget(5, C.byref(was)) == 0 and was.value > 5
     default = was.value
     assert lib.ccut_debug_kv4_wait_budget(default, C.byref(was)) == 0 and was.value == 5
+
+
+def test_positions_that_pass_31_bits(lib):
+    """What a query may see, kv_len + seq, is an int in the kernels: a call past it is refused."""
+    most = 2 ** 31 - 1
+
+    def call(kv_len, seq):
+        return lib.ccut_kv4_attention(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 1, 2, 1, seq, 64, most, kv_len, most, 1,
+                                      0.0, 0.0, FAKE, BF, FAKE, 1 << 40, NULL)
+
+    for kv_len, seq in ((most, 1), (most - 100, 64), (most - 4096 - 63, 64)):
+        assert call(kv_len, seq) == _lib.ERR_UNSUPPORTED
