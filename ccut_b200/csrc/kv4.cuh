@@ -75,9 +75,11 @@ struct Kv4Cache {
   long long slot_rows;
 };
 
-// kv4_prefill.cu: query blocks of at least this many rows per kv head.  Short-block / long-block kernel, 4 kv heads, d =
-// 128: 128 rows on one sequence of 8000 27.9 / 30.8 us, on eight of 4000 55 / 51; 160 rows 28 / 31 and 70 / 52
-// (d = 64, four of 4000: 27.0 / 26.6 and 30.7 / 26.9).
+// kv4_prefill.cu: query blocks of at least this many rows per kv head, whatever else.  Short-block / long-block kernel, 4
+// kv heads, d = 128: 128 rows on one sequence of 8000 27.9 / 30.8 us, on eight of 4000 55 / 51; 160 rows 28 / 31 and
+// 70 / 52 (d = 64, four of 4000: 27.0 / 26.6 and 30.7 / 26.9).  So one sequence would stay with the short blocks
+// beyond 128 rows (10%) and a full machine would leave them before (8%): the limit lies between.  The short blocks
+// also keep exact keys and values, and need no workspace for an unpacked cache.
 constexpr int kKv4LongRows = 129;
 bool kv4_prefill_fits(int batch, int heads, int kv_heads, int seq, int kv_len);
 size_t kv4_prefill_workspace(int batch, int heads, int kv_heads, int seq, int kv_len, int head_dim);

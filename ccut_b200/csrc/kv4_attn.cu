@@ -18,16 +18,17 @@
 //   they would take as the M.  The order of the k index is free, so a lane's operands are the next
 //   bytes of a cache row (no ldmatrix), and the scores' accumulators become the second product's operand
 //   by movmatrix.
-// - Each warp streams its own tiles of 16 positions through a four-deep cp.async ring, with no barrier
-//   between warps; 32-byte units are placed so that the reads of both operands touch every bank once.
+// - Each warp streams its own tiles through a cp.async ring, with no barrier between warps: up to 8 query rows
+//   (one n-tile) tiles of 32 positions, three deep, with more rows (two n-tiles) 16 positions, four deep.
+//   32-byte units are placed so that the reads of both operands touch every bank once.
 //   (Prefetching into registers instead took 168 of them and left three CTAs an SM.)
 // - The running maximum moves only when a score passes it by 2^4 (one vote a tile instead of
 //   six shuffles a row pair): probabilities stay below 2^4, and fp16's range has room for that (kKv4Room).
 // - Tiles that every row sees in whole run without mask tests; the few others (the last tile, the diagonal
 //   of a query block) run a masked copy.
-// - Work is cut evenly whatever the lengths: the blocks of 128 or 64 positions of all (sequence, tile of query
-//   rows, kv head) units form one line, found from starts on the device, and each CTA of one resident
-//   round takes an equal span of it.  A unit inside one span is finished there; of the others a span
+// - Work is cut evenly whatever the lengths: the blocks of 128 (8 rows) or 64 positions of all (sequence, tile of
+//   query rows, kv head) units form one line (a call of up to kKv4Uncut positions has one block a unit), found from
+//   starts on the device, and each CTA of one resident round takes an equal span of it.  A unit inside one span is finished there; of the others a span
 //   leaves at most two partial results (the first and the last of its units), which a second kernel joins.
 //   Equal chunks per sequence cost a prologue, a reduction and a partial result every chunk instead (one
 //   sequence of 131071 positions, when this was changed: 54 us in chunks, 22 in spans).
@@ -705,8 +706,9 @@ __global__ void __launch_bounds__(W > 8 ? W * 32 : 256) kv4_merge_kernel(Kv4Attn
 // Query rows per tile: 8 where a kv head has no more, else 16.
 static int kv4_rows(int heads, int kv_heads, int seq) { return (long)(heads / kv_heads) * seq <= 8 ? 8 : 16; }
 // Positions per block of work: a step of every warp, or all positions where they are few, so that no unit is
-// cut and nothing is left to join (64 sequences of up to 1000: 17.6 us uncut, 19.5 cut; 8 of up to 690: 9.5 and
-// 9.4; one of 1024: 11.0 and 7.7, but the second launch costs the host 5 us of a call's 20).
+// cut and nothing is left to join: 64 sequences of up to 1000 17.6 us uncut, 19.5 cut; 8 of up to 690 9.5 and
+// 9.4.  The limit looks at the positions alone, for calls from the host: one sequence of 1024 takes 11.0 us uncut and
+// 7.7 cut, but the second launch costs the host 5 us of a call's 20.  A captured graph pays the 3 us.
 constexpr int kKv4Uncut = 1024;
 static int kv4_block(int rows, int kv_len) {
   const int step = rows == 8 ? kKv4Block<1> : kKv4Block<2>;

@@ -5,8 +5,8 @@
 //
 // kv4_unpack_kernel turns the cache's rows that any query sees into fp16 once per call (value q s + m, one
 // rounding to 11 bits), 2 x d x 2 bytes per position: about 3% of the products' time at 4096 rows, where
-// unpacking in every CTA would repeat it per 256 rows.  A position that holds a NaN gets a NaN key and a zero
-// value: the key makes every row that sees it NaN, and a masked row multiplies a zero.
+// unpacking in every CTA would repeat it per 256 rows.  A position that holds a NaN, in k or in v, gets a NaN key and
+// a zero value: the key makes every row that sees it NaN, in all its features, and a masked row multiplies a zero.
 // kv4_prefill_kernel: a CTA takes 256 query rows of one kv head (row r = query r / group, head r % group), two
 // tiles of 128, and streams tiles of 128 positions:
 // - warp 0 loads k and v tiles by TMA into a ring; warp 1 issues the MMAs (M = 128, fp32 in tensor memory):
@@ -14,13 +14,13 @@
 // - two warpgroups of softmax threads, one row a thread: S to registers, running maximum, exponentials, P
 //   back as fp16.  While one tile's scores are worked on, the tensor cores run the other's products.
 // - The maximum moves only when a score of the row passes it by 2^4, so O is rescaled a few times per row and not
-//   every tile (probabilities up to 2^4 fit fp16, scaled as they are by kKv4Room); when it moves, the O of the earlier tiles is complete, since
-//   S_i of a tile is issued behind P_i V of the one before.
+//   every tile (probabilities up to 2^4 fit fp16, scaled as they are by kKv4Room); when it moves, the O of the
+//   earlier tiles is complete, since S_i of a tile is issued behind P_i V of the one before.
 // - With 64 features P has columns of its own: S_i of the next tile is computed while the softmax of this one
 //   runs (4096 rows: 118 us, 134 in turn).  With 128 tensor memory is full, and a softmax warp waits 1400 of
 //   the 3300 cycles of a step; tiles of 64 positions with two score buffers took 185 us for 158, since the
 //   query operand is then read twice as often.
-// Measured, 32 heads on 4 kv heads: 4096 rows from position 0, d = 128, 145 us (0.95 PFLOP/s of visible
+// Measured, 32 heads on 4 kv heads: 4096 rows from position 0, d = 128, 148 us (0.93 PFLOP/s of visible
 // products), 8192 rows 494 us (1.11); d = 64 118 us.
 // Roundings: q to fp16 after scaling its row's largest element to [1/2, 1) (11 bits of it, 2^-25 of the
 // largest), k and v above, P to 11 bits down to 2^-25 of the maximum and 2^-36 of it absolutely, whatever the type

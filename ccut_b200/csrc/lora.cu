@@ -833,7 +833,9 @@ int ccut_lora_add(const uint16_t* x, const uint16_t* a, const uint16_t* b, const
   const bool ob = dtype == CCUT_OUT_BF16;
   if (tokens <= kLoraGroupTokens) {
     // what a warp has on its way: more outputs at ranks of up to 32, more of B's k steps above (64 tokens, rank 3 x 64,
-    // 4096 inputs, 6144 outputs: 21.2 us, 21.9 with the other)
+    // 4096 inputs, 6144 outputs: 21.2 us, 21.9 with the other).  As many blocks as three CTAs an SM have registers for
+    // (8 spill: 12.3 us at 5120 outputs); between 2 and 6 it matters little: 5120 outputs 10.2 us with 5, 10.6 to 10.9
+    // with the others, 2560 9.2 (9.1 to 9.5), 2048 8.3 (8.0 to 8.5), 8192 of 4096 inputs 12.7 (12.5 to 12.9)
     if (rank <= 32) return ob ? run_lora_group<true, 5, 2>(p, stream) : run_lora_group<false, 5, 2>(p, stream);
     return ob ? run_lora_group<true, 3, 4>(p, stream) : run_lora_group<false, 3, 4>(p, stream);
   }

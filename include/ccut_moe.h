@@ -359,7 +359,10 @@ CCUT_API int ccut_kv4_read(const uint8_t* k_codes, const uint16_t* k_params, con
  * shape in out_dtype; batch row b reads slot slots[b], its query i sees positions <= starts[b] + i
  * and < kv_len (kv_len <= max_len bounds what any row sees: pass the longest length when the host
  * knows it, else max_len).  A slot outside [0, num_slots) or a negative start gives zero rows;
- * what a query does not see never reaches its row, whatever is stored there.  scale <= 0 means
+ * what a query does not see never reaches its row, whatever is stored there.  A block of up to 128
+ * rows per kv head (heads / kv_heads * seq) multiplies the codes themselves; a longer one rounds k and v
+ * to fp16 and its probabilities to 11 bits, with fp32 output as well, and a NaN that a row sees makes
+ * all its features NaN.  q is below 2^90 in size.  scale <= 0 means
  * 1/sqrt(head_dim); softcap > 0 as in ccut_gqa_attention.  q, out and workspace are 16-byte
  * aligned, kv_len + seq is below 2^31 - 4096. */
 CCUT_API size_t ccut_kv4_attention_workspace_bytes(int batch, int heads, int kv_heads, int seq, int kv_len,
