@@ -228,8 +228,8 @@ def kv4_attention(q: torch.Tensor, pool: Kv4Pool, layer: int, slots: torch.Tenso
     head_dim]`` (bf16 or fp32).  ``kv_len``: an upper bound of ``starts[b] + seq`` when the host
     knows one (positions at or past it are not read); default: the pool's ``max_len``.  ``scale``: None (or 0) for
     ``head_dim ** -0.5``.  Up to 128 query rows per kv head (``heads / kv_heads * seq``) the codes themselves
-    are multiplied, and fp32 output keeps 20 bits; more rows round k, v and the probabilities to fp16 (11
-    bits), whatever ``out_dtype``.  A call whose
+    are multiplied, and fp32 output is off by about 1e-6 of the largest value; more rows round k, v and the
+    probabilities to fp16 (11 bits), whatever ``out_dtype``.  A call whose
     bounded waits ran out leaves zero rows and an error for ``pool.workspace_status()``."""
     _check_pool(pool, q.device)
     shape = q.shape

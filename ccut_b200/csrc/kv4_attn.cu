@@ -39,11 +39,13 @@
 // Roundings to fp16: q, scaled to its row's largest element (2^-35 of it is kept), and sum q_g (2^-15
 // of the largest element); p s_v, scaled by the row's power of two R that brings the largest v scale it has
 // seen to [2^10, 2^11) (11 bits, and 2^-35 of that scale absolutely; with fp32 output a second fp16 part
-// keeps 22 bits, and 2^-35).  Everything else, running maximum, sums and outputs, is fp32.
+// keeps 22 bits, and 2^-35).  Everything else, running maximum, sums and outputs, is fp32; the leading zeros
+// of subnormal operands are bits that the tensor cores' sums do without, which with fp32 output shows as 1e-6
+// of the largest value (decode of 513 to 131071 positions), 1.5e-5 to 2.8e-4 of the output's norm.
 // The codes are not centred, so the sums of p s c and of p m cancel and the rounding of p s_v counts two to three
-// times: 64 ragged caches' outputs are 1.74e-3 off (relative norm), where the rounding to bf16 alone makes 1.66e-3.  Two
-// parts for bf16 output too take 56 us for 50 (1.66e-3); what the part leaves, times the middle of the
-// codes, added to the sum of p m 53 us (1.67e-3).
+// times: 64 ragged caches' bf16 outputs are 1.74e-3 off (relative norm), where the rounding to bf16 alone makes 1.66e-3.
+// What it would cost: two parts 56 us for 50 (1.66e-3); codes centred at 7.5 by the sum of the rounded p s_v, one
+// more product, 52.6 us (1.67e-3).
 #include <math.h>
 
 #include "kv4.cuh"
