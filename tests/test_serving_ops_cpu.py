@@ -187,6 +187,16 @@ def test_wait_budget_checks():
     assert lib.ccut_debug_kv4_wait_budget(default, C.byref(was)) == 0 and was.value == 5
 
 
+def test_status_word_checks(lib):
+    def call(status, q=FAKE, batch=2):
+        return lib.ccut_kv4_attention_reported(q, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, batch, 8, 2, 1, 64, 50, 50, 100, 4, 0.0,
+                                               0.0, FAKE, BF, FAKE, 1 << 20, status, NULL)
+
+    assert call(C.c_void_p(4098)) == _lib.ERR_INVALID
+    assert call(FAKE, q=NULL) == _lib.ERR_INVALID
+    assert call(NULL, batch=0) == _lib.OK and call(FAKE, batch=0) == _lib.OK
+
+
 def test_positions_that_pass_31_bits(lib):
     """What a query may see, kv_len + seq, is an int in the kernels: a call past it is refused."""
     most = 2 ** 31 - 1
